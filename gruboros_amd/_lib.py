@@ -100,6 +100,12 @@ SIGNATURES = {
     "mg_gemm_wgrad_pair": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _fp, _c_i64,
                                     _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _fp, _c_i64, _c_int, _c_int,
                                     _vp, _c_size, _vp]),
+    "mg_delta_fwd_workspace_bytes": (_c_size, [_c_int, _vp, _c_int]),
+    "mg_delta_bwd_workspace_bytes": (_c_size, [_c_int, _vp]),
+    "mg_delta_fwd": (_c_int, [_c_int] + [_vp] * 6 + [ctypes.c_float, _fp, _vp, _fp, _c_int, _vp, _c_size, _vp]),
+    "mg_delta_bwd": (_c_int, [_c_int] + [_vp] * 6 + [ctypes.c_float, _vp, _c_size, _vp, _fp] + [_vp] * 5
+                     + [_fp, _vp, _c_size, _vp]),
+    "mg_delta_step": (_c_int, [_c_int] + [_vp] * 6 + [ctypes.c_float, _fp, _vp, _vp]),
     "mg_gemm_wgrad_pair_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
 }
 

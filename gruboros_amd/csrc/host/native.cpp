@@ -17,6 +17,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <sstream>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -727,6 +728,107 @@ Tensor column_sum(const Tensor& x, int64_t stream) {
   return out;
 }
 
+// ------------------------------------------------------------------ gated delta rule
+
+// a [B, T, H, ...] operand; a dimension of one element has no stride
+mg_rows rows(const Tensor& t) {
+  const auto s = [&](int i) { return t.size(i) == 1 ? int64_t(0) : t.stride(i); };
+  return {ptr(t), s(0), s(1), s(2)};
+}
+// every operand of the type and on the device of the first
+void alike(const Tensor& first, std::initializer_list<const Tensor*> rest) {
+  for (const Tensor* t : rest) {
+    if (t->scalar_type() != first.scalar_type())
+      fail(std::string("expected ") + c10::toString(first.scalar_type()) + " like the first operand, got " + c10::toString(t->scalar_type()));
+    if (t->device() != first.device()) fail("operands on different devices: " + first.device().str() + " and " + t->device().str());
+  }
+}
+void shape(const Tensor& t, at::IntArrayRef want, const char* name) {
+  if (t.sizes() != want) {
+    std::ostringstream m;
+    m << name << ": expected " << want << ", got " << t.sizes();
+    fail(m.str());
+  }
+}
+mg_delta_dims delta_dims(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta) {
+  if (q.dim() != 4 || v.dim() != 4) fail("q and v: expected [B, T, H, D]");
+  alike(q, {&k, &v, &g, &beta});
+  const int64_t B = q.size(0), T = q.size(1), H = v.size(2);
+  shape(k, q.sizes(), "k");
+  shape(v, {B, T, H, v.size(3)}, "v");
+  shape(g, {B, T, H}, "g");
+  shape(beta, {B, T, H}, "beta");
+  for (const Tensor* t : {&q, &k, &v})
+    if (t->stride(3) != 1) fail("q, k and v need a unit inner stride");
+  if (q.numel() == 0 || v.numel() == 0) fail("empty operand");
+  for (int64_t n : {B, T, H, q.size(2), q.size(3), v.size(3)})
+    if (n > INT32_MAX) fail("a dimension is too large");
+  return {int(B), int(T), int(q.size(2)), int(H), int(q.size(3)), int(v.size(3))};
+}
+float* state_ptr(const Opt& t, const mg_delta_dims& d, const Tensor& like, const char* name) {
+  if (!t) return nullptr;
+  shape(*t, {d.B, d.H, d.K, d.V}, name);
+  if (!t->is_contiguous()) fail(std::string(name) + ": expected a contiguous tensor");
+  if (t->device() != like.device()) fail(std::string(name) + ": on another device than the operands");
+  return fp(*t);
+}
+
+// (o, last state or none, what the backward reads or none)
+std::tuple<Tensor, Opt, Opt> delta_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                                       const Opt& h0, double scale, bool want_state, bool keep, int64_t stream) {
+  need_cuda(q);
+  c10::DeviceGuard guard(q.device());
+  const mg_delta_dims d = delta_dims(q, k, v, g, beta);
+  const mg_rows rq = rows(q), rk = rows(k), rv = rows(v), rg = rows(g), rb = rows(beta);
+  Tensor o = make(v.sizes(), v.scalar_type(), v);
+  Opt state;
+  if (want_state) state = make({d.B, d.H, d.K, d.V}, at::kFloat, v);
+  const size_t wsb = mg_delta_fwd_workspace_bytes(code(q), &d, keep);
+  Tensor ws = bytes(wsb, q);
+  check(mg_delta_fwd(code(q), &d, &rq, &rk, &rv, &rg, &rb, scale, state_ptr(h0, d, q, "initial state"), ptr(o), fp(state), keep,
+                     ptr(ws), wsb, st(stream)),
+        "mg_delta_fwd");
+  return {o, state, keep ? Opt(ws) : std::nullopt};
+}
+
+// (dq, dk, dv, dg, dbeta, dh0 or none)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Opt> delta_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                                                  const Tensor& beta, double scale, const Tensor& kept,
+                                                                  const Tensor& dout, const Opt& dstate, bool want_dh0,
+                                                                  int64_t stream) {
+  need_cuda(q);
+  c10::DeviceGuard guard(q.device());
+  const mg_delta_dims d = delta_dims(q, k, v, g, beta);
+  alike(q, {&dout});
+  shape(dout, v.sizes(), "dout");
+  if (dout.stride(3) != 1) fail("dout needs a unit inner stride");
+  const mg_rows rq = rows(q), rk = rows(k), rv = rows(v), rg = rows(g), rb = rows(beta), ro = rows(dout);
+  Tensor dq = make(q.sizes(), q.scalar_type(), q), dk = make(q.sizes(), q.scalar_type(), q);
+  Tensor dv = make(v.sizes(), v.scalar_type(), v), dg = make(g.sizes(), g.scalar_type(), g), db = make(g.sizes(), g.scalar_type(), g);
+  Opt dh0;
+  if (want_dh0) dh0 = make({d.B, d.H, d.K, d.V}, at::kFloat, v);
+  const size_t wsb = mg_delta_bwd_workspace_bytes(code(q), &d);
+  Tensor ws = bytes(wsb, q);
+  check(mg_delta_bwd(code(q), &d, &rq, &rk, &rv, &rg, &rb, scale, ptr(kept), kept.numel(), &ro, state_ptr(dstate, d, q, "state gradient"),
+                     ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(db), fp(dh0), ptr(ws), wsb, st(stream)),
+        "mg_delta_bwd");
+  return {dq, dk, dv, dg, db, dh0};
+}
+
+// q, k [B, Hk, K], v [B, H, V], g, beta [B, H], all dense; state [B, H, K, V] in place. Returns o [B, H, V].
+Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& state,
+                  double scale, int64_t stream) {
+  need_cuda(q);
+  c10::DeviceGuard guard(q.device());
+  const mg_delta_dims d = delta_dims(q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), g.unsqueeze(1), beta.unsqueeze(1));
+  for (const Tensor* t : {&q, &k, &v, &g, &beta})
+    if (!t->is_contiguous()) fail("a step's operands are contiguous");
+  Tensor o = make(v.sizes(), v.scalar_type(), v);
+  check(mg_delta_step(code(q), &d, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), scale, state_ptr(state, d, q, "state"), ptr(o), st(stream)),
+        "mg_delta_step");
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -756,4 +858,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("head_backward", &head_backward, nogil());
   m.def("infer_layer", &infer_layer, nogil());
   m.def("column_sum", &column_sum, nogil());
+  m.def("delta_fwd", &delta_fwd, nogil());
+  m.def("delta_bwd", &delta_bwd, nogil());
+  m.def("delta_step", &delta_step, nogil());
 }

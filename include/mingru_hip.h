@@ -654,6 +654,58 @@ int mg_decode_ff_f16(int B, int D, int F, const float* x, const float* norm_w, c
 int mg_decode_head_f16(int B, int D, int V, const float* x_in, const void* pending, const float* norm_w,
                        const void* w_out, void* logits, float eps, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Gated delta rule: the recurrence of a mixer whose state is a matrix, beside
+ * the minGRU scan. Per (b, h), with S in R^{K x V}:
+ *   S_t = e^{g_t} S_{t-1} + beta_t k_t (v_t - e^{g_t} S_{t-1}^T k_t)^T,
+ *   o_t = scale S_t^T q_t,
+ * S_{-1} = h0 (or 0 when h0 is NULL). No counterpart in the reference.
+ *
+ * dtype (MG_F32 or MG_BF16) is that of q, k, v, g, beta, o and their
+ * gradients; states and their gradients are fp32, dense [B, H, K, V], and are
+ * carried unrounded: matrix operands are split into bf16 limbs whose products
+ * are summed in fp32. Gradients in bf16 are rounded to nearest.
+ * H value heads share Hk query/key heads (H a multiple of Hk; head h reads
+ * q, k of head h / (H / Hk), whose gradient is the sum over its value heads).
+ * g is the logarithm of the decay; below -200 it counts as -200 (e^g is 0 in
+ * fp32 from -104 on, where dg is 0): -inf forgets the state.
+ *
+ * mg_rows: element (b, t, h, d) of an operand at p + b sb + t st + h sh + d
+ * (elements; d contiguous; g and beta have no d). q, k and dout: p and the
+ * strides multiples of 16 bytes. o, dv: dense [B, T, H, V]; dq, dk: dense
+ * [B, T, Hk, K]; dg, dbeta: dense [B, T, H].
+ * K and V multiples of 8, K <= 128, V <= 256; T >= 1;
+ * B H ceil(T / 64) < 2^31; 64 token strides below 2 GiB.
+ *
+ * mg_delta_fwd runs over chunks of 64 tokens. state (nullable) receives the
+ * last state; it must not overlap h0. keep != 0 keeps in `workspace` what
+ * mg_delta_bwd reads (its `kept`; states and updates of every chunk). The
+ * workspace (256-byte aligned, any contents) holds the chunks' small matrices
+ * otherwise. mg_delta_bwd reads the forward's operands and `kept` unchanged;
+ * dstate (nullable): gradient of the last state; dh0 (nullable) receives h0's.
+ *
+ * mg_delta_step: one token. dims->T is 1; q, k dense [B, Hk, K], v, o dense
+ * [B, H, V], g, beta dense [B, H]; v and o aligned to 4 elements; state is
+ * updated in place (16-byte aligned). No workspace. */
+typedef struct {
+  int B, T, Hk, H, K, V;
+} mg_delta_dims;
+typedef struct {
+  const void* p;
+  int64_t sb, st, sh;
+} mg_rows;
+size_t mg_delta_fwd_workspace_bytes(int dtype, const mg_delta_dims* dims, int keep);
+size_t mg_delta_bwd_workspace_bytes(int dtype, const mg_delta_dims* dims);
+int mg_delta_fwd(int dtype, const mg_delta_dims* dims, const mg_rows* q, const mg_rows* k, const mg_rows* v,
+                 const mg_rows* g, const mg_rows* beta, float scale, const float* h0, void* o, float* state,
+                 int keep, void* workspace, size_t workspace_bytes, void* stream);
+int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows* q, const mg_rows* k, const mg_rows* v,
+                 const mg_rows* g, const mg_rows* beta, float scale, const void* kept, size_t kept_bytes,
+                 const mg_rows* dout, const float* dstate, void* dq, void* dk, void* dv, void* dg, void* dbeta,
+                 float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+int mg_delta_step(int dtype, const mg_delta_dims* dims, const void* q, const void* k, const void* v, const void* g,
+                  const void* beta, float scale, float* state, void* o, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
