@@ -106,6 +106,13 @@ SIGNATURES = {
     "mg_delta_bwd": (_c_int, [_c_int] + [_vp] * 6 + [ctypes.c_float, _vp, _c_size, _vp, _fp] + [_vp] * 5
                      + [_fp, _vp, _c_size, _vp]),
     "mg_delta_step": (_c_int, [_c_int] + [_vp] * 6 + [ctypes.c_float, _fp, _vp, _vp]),
+    "mg_layernorm_fwd": (_c_int, [_c_int, _vp, _c_int, _vp, _fp, _fp, _fp, _c_int, _vp, _fp, _fp, _c_i64, _c_int,
+                                  ctypes.c_float, ctypes.c_double, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp]),
+    "mg_layernorm_bwd_workspace_bytes": (_c_size, [_c_i64, _c_int]),
+    "mg_layernorm_bwd": (_c_int, [_c_int, _vp, _fp, _fp, _fp, _c_int, _vp, _fp, _vp, _c_int, _vp, _fp, _fp, _c_i64, _c_int,
+                                  ctypes.c_double, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp, _c_size, _vp]),
+    "mg_dropout": (_c_int, [_c_int, _vp, _c_int, _vp, _vp, _c_i64, ctypes.c_double, ctypes.c_uint64, _vp,
+                            ctypes.c_uint64, _vp]),
     "mg_gemm_wgrad_pair_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
 }
 

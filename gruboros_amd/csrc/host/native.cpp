@@ -829,6 +829,81 @@ Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   return o;
 }
 
+// ------------------------------------------------------------------ layer norm, dropout
+
+// seed: a device int64 scalar read by the kernels, or the number itself
+const int64_t* seed_ptr(const Opt& t, const Tensor& like) {
+  if (!t) return nullptr;
+  if (t->scalar_type() != at::kLong || t->numel() != 1 || t->device() != like.device())
+    fail("seed: expected one int64 on " + like.device().str());
+  return static_cast<const int64_t*>(ptr(*t));
+}
+void dense(const Tensor& t, const Tensor& like, const char* name) {
+  if (!t.is_contiguous() || t.numel() != like.numel() || t.device() != like.device())
+    fail(std::string(name) + ": expected a contiguous tensor of as many values, on " + like.device().str());
+}
+
+// (xn or none, y, mean, rstd); dense operands
+std::tuple<Opt, Tensor, Tensor, Tensor> layernorm_fwd(const Tensor& x, const Opt& delta, const Tensor& w, const Opt& b, bool bf16,
+                                                      double eps, double p, uint64_t seed, const Opt& seed_t, uint64_t offset,
+                                                      int64_t stream) {
+  need_cuda(x);
+  c10::DeviceGuard guard(x.device());
+  const int64_t D = x.size(-1), N = x.numel() / std::max<int64_t>(D, 1);
+  if (D > INT32_MAX) fail("rows are too long");
+  dense(x, x, "x");
+  if (delta) dense(*delta, x, "delta");
+  Opt x_out;
+  if (delta) x_out = make(x.sizes(), at::kFloat, x);
+  Tensor y = make(x.sizes(), bf16 ? at::kBFloat16 : at::kFloat, x), mean = make({N}, at::kFloat, x), rstd = make({N}, at::kFloat, x);
+  check(mg_layernorm_fwd(code(x), ptr(x), delta ? code(*delta) : 0, ptr(delta), vec(w, D, "weight"), b ? vec(*b, D, "bias") : nullptr,
+                         fp(x_out), code(y), ptr(y), fp(mean), fp(rstd), N, D, eps, p, seed, seed_ptr(seed_t, x), offset, st(stream)),
+        "mg_layernorm_fwd");
+  return {x_out, y, mean, rstd};
+}
+
+// (dx, ddelta, dw, db); dy or dres may be none (zero)
+std::tuple<Opt, Opt, Tensor, Opt> layernorm_bwd(const Tensor& xn, const Tensor& w, const Tensor& mean, const Tensor& rstd,
+                                                const Opt& dy_, const Opt& dres_, bool want_dx, int delta_type, bool want_db,
+                                                double p, uint64_t seed, const Opt& seed_t, uint64_t offset, int64_t stream) {
+  need_cuda(xn);
+  c10::DeviceGuard guard(xn.device());
+  const int64_t D = xn.size(-1), N = xn.numel() / std::max<int64_t>(D, 1);
+  Tensor dy = dy_ ? dy_->contiguous() : at::zeros(xn.sizes(), xn.options().dtype(at::kFloat));
+  Opt dres, dx, dd, db;
+  if (dres_) dres = dres_->to(at::kFloat).contiguous();
+  dense(xn, xn, "xn");
+  dense(dy, xn, "dy");
+  if (dres) dense(*dres, xn, "dres");
+  if (want_dx) dx = make(xn.sizes(), xn.scalar_type(), xn);
+  if (delta_type >= 0) dd = make(xn.sizes(), delta_type == MG_BF16 ? at::kBFloat16 : at::kFloat, xn);
+  Tensor dw = make({D}, at::kFloat, xn);
+  if (want_db) db = make({D}, at::kFloat, xn);
+  const size_t wsb = mg_layernorm_bwd_workspace_bytes(N, D);
+  Tensor ws = bytes(wsb, xn);
+  check(mg_layernorm_bwd(code(xn), ptr(xn), vec(w, D, "weight"), vec(mean, N, "mean"), vec(rstd, N, "rstd"), code(dy), ptr(dy),
+                         fp(dres), ptr(dx), std::max(delta_type, 0), ptr(dd), fp(dw), fp(db), N, D, p, seed,
+                         seed_ptr(seed_t, xn), offset, ptr(ws), wsb, st(stream)),
+        "mg_layernorm_bwd");
+  return {dx, dd, dw, db};
+}
+
+// residual + keep(x) x / (1 - p) in out_type (MG_F32, MG_BF16)
+Tensor dropout(const Tensor& x, const Opt& residual, int out_type, double p, uint64_t seed, const Opt& seed_t, uint64_t offset,
+               int64_t stream) {
+  need_cuda(x);
+  c10::DeviceGuard guard(x.device());
+  dense(x, x, "x");
+  Tensor y = make(x.sizes(), out_type == MG_BF16 ? at::kBFloat16 : at::kFloat, x);
+  if (residual) {
+    dense(*residual, x, "residual");
+    if (residual->scalar_type() != y.scalar_type()) fail("residual: expected the output's dtype");
+  }
+  check(mg_dropout(code(x), ptr(x), code(y), ptr(residual), ptr(y), x.numel(), p, seed, seed_ptr(seed_t, x), offset, st(stream)),
+        "mg_dropout");
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -858,6 +933,9 @@ PYBIND11_MODULE(_native, m) {
   m.def("head_backward", &head_backward, nogil());
   m.def("infer_layer", &infer_layer, nogil());
   m.def("column_sum", &column_sum, nogil());
+  m.def("layernorm_fwd", &layernorm_fwd, nogil());
+  m.def("layernorm_bwd", &layernorm_bwd, nogil());
+  m.def("dropout", &dropout, nogil());
   m.def("delta_fwd", &delta_fwd, nogil());
   m.def("delta_bwd", &delta_bwd, nogil());
   m.def("delta_step", &delta_step, nogil());

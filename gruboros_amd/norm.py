@@ -1,5 +1,5 @@
 """Autograd Functions over the fused residual-add + RMSNorm kernels
-(mg_add_rmsnorm_fwd / mg_add_rmsnorm_bwd).
+(mg_add_rmsnorm_fwd / mg_add_rmsnorm_bwd), and layer norm.
 
 Reference semantics: torch.nn.RMSNorm(dim) as used by mingru/minLM.py:67,
 :69, :74 (eps=None -> float32 machine epsilon) and the residual adds at
@@ -7,13 +7,18 @@ mingru/minLM.py:125 and :130. The residual stream is kept in fp32; the
 normalized output is produced in the activation dtype, optionally (bf16) as
 a hi/lo pair [N, 2D] = [bf16(y) | bf16(y - bf16(y))] whose hi half is the
 usual output: the operand of the fp32-accurate products (gemm HILO).
+layer_norm and add_layer_norm are the same pair for the other usual norm
+(mg_layernorm_fwd / mg_layernorm_bwd; no counterpart in the reference), with
+the dropout of the joining branch in the same pass.
 Weights of any floating dtype are accepted (a model cast with
 .to(torch.bfloat16), as reference generate.py:140-142 does); the kernels read
 them as fp32.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import MG_BF16, dtype_code, native, require_cuda, stream_of
+from .dropout import check_drop
 
 FP32_EPS = float(torch.finfo(torch.float32).eps)
 
@@ -133,3 +138,75 @@ def add_rms_norm(x, delta, w, out_dtype=None, with_lo=False):
     w = _check(x, w, delta)
     out_dtype = out_dtype or x.dtype
     return AddRMSNormFn.apply(x.contiguous(), delta.contiguous(), w, out_dtype, _lo_ok(out_dtype, with_lo))
+
+
+class LayerNormFn(torch.autograd.Function):
+    """(xn, y) with xn = x + dropout(delta), or (None, y) without a delta; see add_layer_norm."""
+
+    @staticmethod
+    def forward(ctx, x, delta, w, b, out_dtype, eps, drop):
+        p, seed, seed_t, offset = drop
+        xn, y, mean, rstd = native().layernorm_fwd(x, delta, w, b, dtype_code(out_dtype) == MG_BF16, eps, p, seed, seed_t, offset,
+                                                   stream_of(x))
+        ctx.save_for_backward(x if xn is None else xn, w, mean, rstd, seed_t)
+        ctx.args = p, seed, offset, -1 if delta is None else dtype_code(delta.dtype)
+        ctx.set_materialize_grads(False)
+        return xn, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dx_out, dy):
+        if dx_out is None and dy is None:
+            return (None,) * 7
+        xn, w, mean, rstd, seed_t = ctx.saved_tensors
+        p, seed, offset, delta_type = ctx.args
+        need = ctx.needs_input_grad
+        dx, dd, dw, db = native().layernorm_bwd(xn, w, mean, rstd, dy, dx_out, need[0], delta_type if need[1] else -1, need[3],
+                                                p, seed, seed_t, offset, stream_of(xn))
+        return dx, dd, (dw if need[2] else None), db, None, None, None
+
+
+def _check_layer_norm(x, w, b, delta, out_dtype):
+    require_cuda(x, w, b, delta)
+    D = x.shape[-1] if x.dim() else 0
+    if not 1 <= D <= 16384:
+        raise ValueError(f"layer norm rows hold 1 to 16384 values, got {D}")
+    if x.dtype not in ((torch.float32,) if delta is not None else (torch.float32, torch.bfloat16)):
+        raise ValueError(f"x must be float32{'' if delta is not None else ' or bfloat16'}, got {x.dtype}")
+    dtype_code(out_dtype)
+    for t, name in ((w, "weight"), (b, "bias")):
+        if t is not None and (not t.is_floating_point() or t.shape != (D,)):
+            raise ValueError(f"{name} must be a floating [{D}] vector, got {t.dtype} {tuple(t.shape)}")
+    if delta is not None:
+        dtype_code(delta.dtype)
+        if delta.shape != x.shape:
+            raise ValueError(f"delta {tuple(delta.shape)} must match x {tuple(x.shape)}")
+    for t in (w, b, delta):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"operands on {x.device} and {t.device}")
+    # (casts that autograd differentiates, for models whose parameters are bf16 or fp16)
+    return w.float().contiguous(), None if b is None else b.float().contiguous()
+
+
+def layer_norm(x, w, b=None, out_dtype=None, eps=1e-5):
+    """Layer norm of x (float32 or bfloat16) over its last dim (1 to 16384 values):
+    (x - mean) / sqrt(variance + eps) * w + b, statistics in fp32; output in out_dtype (default x's).
+    Gradients reach x, w and b."""
+    out_dtype = out_dtype or x.dtype
+    w, b = _check_layer_norm(x, w, b, None, out_dtype)
+    if x.numel() == 0:
+        return torch.empty_like(x, dtype=out_dtype)
+    return LayerNormFn.apply(x.contiguous(), None, w, b, out_dtype, eps, (0.0, 0, None, 0))[1]
+
+
+def add_layer_norm(x, delta, w, b=None, out_dtype=None, eps=1e-5, dropout_p=0.0, seed=None, offset=0):
+    """Returns (xn, layer_norm(xn)) with xn = x + dropout(delta): the residual add, the dropout of
+    the branch that joins and the next norm in one pass. x fp32, delta fp32 or bf16; dropout_p,
+    seed and offset as in gruboros_amd.dropout.dropout (whose values are dropped the same), a seed
+    being needed only where dropout_p > 0. Gradients reach x, delta, w and b."""
+    out_dtype = out_dtype or x.dtype
+    w, b = _check_layer_norm(x, w, b, delta, out_dtype)
+    drop = check_drop(dropout_p, 0 if seed is None and dropout_p == 0 else seed, offset, x.device)
+    if x.numel() == 0:
+        return x + delta.float(), torch.empty_like(x, dtype=out_dtype)
+    return LayerNormFn.apply(x.contiguous(), delta.contiguous(), w, b, out_dtype, eps, drop)

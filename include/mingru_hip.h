@@ -47,8 +47,9 @@ extern "C" {
 /* Library version (major*10000 + minor*100 + patch): 206 = 0.2.6, the ABI
  * declared in this file (0.2.1 to 0.2.5 add entry points to 0.2.0 and change
  * none; 0.2.6 changes no signature: mg_gemm also splits small bf16 products
- * along K, see mg_gemm, and mg_gemm_f32, mg_gemm_group, mg_gemm_hilo_cols and
- * mg_scan_fwd_pair are additions under the same number). */
+ * along K, see mg_gemm, and mg_gemm_f32, mg_gemm_group, mg_gemm_hilo_cols,
+ * mg_scan_fwd_pair, mg_delta_*, mg_layernorm_* and mg_dropout are additions
+ * under the same number). */
 int mg_version(void);
 
 /* Message of the last failed call on this thread ("" if none). */
@@ -705,6 +706,39 @@ int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows* q, const m
                  float* dh0, void* workspace, size_t workspace_bytes, void* stream);
 int mg_delta_step(int dtype, const mg_delta_dims* dims, const void* q, const void* k, const void* v, const void* g,
                   const void* beta, float scale, float* state, void* o, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm with the residual add and the dropout of the added branch:
+ *   xn = x + keep(delta) delta / (1 - p)     (delta nullable: xn = x)
+ *   y  = (xn - mean(xn)) / sqrt(var(xn) + eps) * w + b   (b nullable)
+ * over rows of D (1 to 16384) elements, dense [N, D], of any alignment. x is
+ * fp32, or bf16 without a delta; delta and y fp32 or bf16; w, b fp32 [D].
+ * x_out (with a delta) receives xn in fp32; mean and rstd (nullable together)
+ * what the backward reads. No counterpart in the reference, whose norms are
+ * mg_add_rmsnorm's.
+ * mg_layernorm_bwd: dres (nullable) is the gradient of xn from its other use;
+ * dx (x's dtype), ddelta, dw and db (fp32 [D]) are nullable. bf16 gradients
+ * are rounded to nearest. dw and db are summed in a fixed order.
+ *
+ * keep: element e of a call's tensor (row-major index) takes word e % 4 of
+ * Philox4x32-10 at counter (e / 4, offset) under the key `seed`, or *seed_p
+ * when seed_p is not NULL, read on the stream; it is dropped (0 whatever it
+ * was) where the word is below floor(p 2^32). 0 <= p < 1; nothing is drawn
+ * when p is 0. The backward makes the same words again: no mask is stored. */
+int mg_layernorm_fwd(int x_dtype, const void* x, int delta_dtype, const void* delta, const float* w, const float* b,
+                     float* x_out, int y_dtype, void* y, float* mean, float* rstd, int64_t N, int D, float eps,
+                     double p, uint64_t seed, const int64_t* seed_p, uint64_t offset, void* stream);
+size_t mg_layernorm_bwd_workspace_bytes(int64_t N, int D);
+int mg_layernorm_bwd(int x_dtype, const void* xn, const float* w, const float* mean, const float* rstd, int dy_dtype,
+                     const void* dy, const float* dres, void* dx, int ddelta_dtype, void* ddelta, float* dw, float* db,
+                     int64_t N, int D, double p, uint64_t seed, const int64_t* seed_p, uint64_t offset,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Dropout of n values: y = residual + keep(x) x / (1 - p), residual nullable
+ * and of y's dtype; x and y fp32 or bf16 each, all 16-byte aligned. The
+ * backward is the same call on dy without a residual. */
+int mg_dropout(int x_dtype, const void* x, int y_dtype, const void* residual, void* y, int64_t n, double p,
+               uint64_t seed, const int64_t* seed_p, uint64_t offset, void* stream);
 
 #ifdef __cplusplus
 }
