@@ -69,14 +69,14 @@ struct Args {
   // chunk data, index c = (b H + h) NC + n
   char* img;             // [c][Tile::kBytes]: the chunk's operands as they lie in LDS
   double* Gd;            // [c][64]
-  uint32_t* Sw;          // kept for the backward: [(b H + h)(NC + 1) + n][K][VP]
-  uint32_t* dw;          // [c][64][VP]
+  bf16_t* Sw;            // kept for the backward: each chunk's entry state, [c][VP / 32][NW][32][KP]
+  bf16_t* dw;            // d, [c][VP / 32][NW][32][64]
   // backward
   const char* dout;      // [B, T, H, V]
   int64_t do_sb, do_st, do_sh;
   const float* dstate;   // or null
-  uint32_t* dSw;         // [c][K][VP]
-  uint32_t* yw;          // [c][64][VP]
+  bf16_t* dSw;           // the gradients of the exit states, as Sw
+  bf16_t* yw;            // dy, as dw
   char *dq, *dk, *dv, *dg, *db;
   float* dh0;
   float *dqp, *dkp;      // shared heads: [B, T, H, K] before their sum
@@ -113,38 +113,10 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[N]) {
   for (int l = 0; l < N; ++l) out[l] = __builtin_bit_cast(bf16x8, w[l]);
 }
 
-// A value kept for the backward in four bytes: fp32 (fp32 inputs), or the first limb above the
-// second rounded to nearest (bf16 inputs: the operand form of the backward's products, 2^-17).
+// Limbs of what is kept for the backward's products: two of a state or update of bf16 inputs (2^-16,
+// far below the rounding of the gradients they end in), all three of fp32 inputs.
 template <int NI>
-__device__ __forceinline__ uint32_t keep(float x) {
-  if constexpr (NI == 3) return __float_as_uint(x);
-  const uint32_t h = __float_as_uint(x) & 0xffff0000u;
-  return h | f32_to_bf16(x - __uint_as_float(h));
-}
-template <int NI>
-__device__ __forceinline__ float kept(uint32_t w) {
-  if constexpr (NI == 3) return __uint_as_float(w);
-  return __uint_as_float(w & 0xffff0000u) + __uint_as_float(w << 16);
-}
-// 8 kept words as limbs (2 of packed words, 3 of fp32)
-template <int NI>
-struct kept_limbs {
-  static constexpr int N = NI == 3 ? 3 : 2;
-};
-template <int NI>
-__device__ __forceinline__ void unkeep(const u32x4& a, const u32x4& b, bf16x8 (&out)[kept_limbs<NI>::N]) {
-  if constexpr (NI == 3) {
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(a[i]), x[4 + i] = __uint_as_float(b[i]);
-    split<3>(x, out);
-  } else {
-    const u32x4 h = {hi16x2(a[0], a[1]), hi16x2(a[2], a[3]), hi16x2(b[0], b[1]), hi16x2(b[2], b[3])};
-    const u32x4 l = {lo16x2(a[0], a[1]), lo16x2(a[2], a[3]), lo16x2(b[0], b[1]), lo16x2(b[2], b[3])};
-    out[0] = __builtin_bit_cast(bf16x8, h);
-    out[1] = __builtin_bit_cast(bf16x8, l);
-  }
-}
+constexpr int kKept = NI == 3 ? 3 : 2;
 
 // c += a b over the limb products (i, j) with i + j < ORD, the small ones first
 template <int ORD, int NA, int NB>
@@ -166,6 +138,34 @@ __device__ __forceinline__ float ld(const float* p) { return *p; }
 __device__ __forceinline__ float ld(const bf16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ void st(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st(bf16_t* p, float x) { *p = f32_to_bf16(x); }
+
+// Column accesses of the passes over the chunks: a buffer over the chunk's rows of one head, the lane's
+// column and first row in its offset, a scalar offset per register. Rows and columns past the end are
+// out of the buffer's range: they read as zero and are not written.
+constexpr uint32_t kOutOfRange = 0x80000000u;
+template <typename E>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const E* p, int64_t st_, int rows, int cols) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(p), static_cast<short>(0),
+                                           static_cast<int>(((rows - 1) * st_ + cols) * sizeof(E)), 0x00020000);
+}
+template <typename E>
+__device__ __forceinline__ uint32_t load_col(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t row_off) {  // raw
+  if constexpr (sizeof(E) == 2)
+    return __builtin_amdgcn_raw_buffer_load_b16(r, off, row_off, 0);
+  else
+    return __builtin_amdgcn_raw_buffer_load_b32(r, off, row_off, 0);
+}
+template <typename E>
+__device__ __forceinline__ float value(uint32_t raw) {
+  return __uint_as_float(sizeof(E) == 2 ? raw << 16 : raw);
+}
+template <typename E>
+__device__ __forceinline__ void store_col(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t row_off, float x) {
+  if constexpr (sizeof(E) == 2)
+    __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x), r, off, row_off, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, off, row_off, 0);
+}
 
 // 8 consecutive values as limbs; nothing (zero) unless ok
 __device__ __forceinline__ void load8(const bf16_t* p, bool ok, bf16x8 (&out)[1]) {
@@ -232,13 +232,18 @@ struct Tile {
   static constexpr int kStages = 2 * kBytes <= 160 * 1024 ? 2 : 1;
 };
 
-template <int BYTES>
-__device__ __forceinline__ void stage(char* lds, const char* src, int lane, int wave, int waves) {
+template <int BYTES, int WAVES>
+__device__ __forceinline__ void stage(char* lds, const void* src, int lane, int wave) {
   const __amdgpu_buffer_rsrc_t rsrc =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src), static_cast<short>(0), BYTES, 0x00020000);
-  for (int i = wave; i < BYTES / 1024; i += waves)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + i * 1024), 16,
-                                             i * 1024 + lane * 16, 0, 0, 0);
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), static_cast<short>(0), BYTES, 0x00020000);
+  int off = wave * 1024;
+#pragma unroll
+  for (int i = 0; i < (BYTES / 1024 + WAVES - 1) / WAVES; ++i) {
+    asm volatile("" : "+s"(off));  // (one running offset: else every copy's is kept in registers of its own)
+    if ((i + 1) * WAVES <= BYTES / 1024 || i * WAVES + wave < BYTES / 1024)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + off), 16, lane * 16, off, 0, 0);
+    off += WAVES * 1024;
+  }
 }
 
 __device__ __forceinline__ void staged() {
@@ -456,59 +461,94 @@ __device__ __forceinline__ void frags_t(const char* m, int plane, int t, int p, 
   for (int l = 0; l < N; ++l) out[l] = frag_t<U, PERM>(m + l * plane, t, p, lane);
 }
 
-template <int KP, int NI, bool KEEP, int MAXW>
-__global__ __launch_bounds__(64 * MAXW) void state_kernel(Args a, int tiles) {
-  using E = typename elem<NI>::type;
-  using L = Tile<KP, NI>;
-  constexpr int KT = KP / 16, KB = KP / 32, NP = L::NP, U = L::U;
-  __shared__ __attribute__((aligned(16))) char lds[L::kStages * L::kBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, m = lane & 15, g = lane >> 4;
-  int bh, tile;
-  place(blockIdx.x, a.B * a.H, tiles, bh, tile);
-  const int h = bh % a.H, b = bh / a.H, col = (tile * waves + wave) * 16 + m;
-  const bool in = col < a.V;
-  const E* v = reinterpret_cast<const E*>(a.v) + b * a.v_sb + h * a.v_sh + min(col, a.V - 1);
-  E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(b) * a.T * a.H + h) * a.V + col;
-  const int64_t o_st = static_cast<int64_t>(a.H) * a.V;
+// Limbs of an operand (lane = column, 8 rows per register group) to an image of [columns][rows]
+template <int U, int NW, int N>
+__device__ __forceinline__ void keep(bf16_t* img, int plane, int row, int u, const bf16x8 (&x)[N]) {
+#pragma unroll
+  for (int l = 0; l < NW; ++l) *reinterpret_cast<bf16x8*>(reinterpret_cast<char*>(img) + l * plane + at<U>(row, u)) = x[l];
+}
 
-  f32x4 S[KT];
+// What a wave of the passes works on
+template <int KP, int NI, int W>
+struct Place {
+  int lane, wave, m, g, bh, h, b, col;
+  bool in;
+  __device__ __forceinline__ Place(const Args& a, int tiles) {
+    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+    int tile;
+    place(blockIdx.x, a.B * a.H, tiles, bh, tile);
+    h = bh % a.H, b = bh / a.H, col = (tile * W + wave) * 16 + m;
+    in = col < a.V;
+  }
+};
+
+// The state (or its gradient) of a head's columns from dense [K][V] fp32, or zero
+template <int KT, typename P>
+__device__ __forceinline__ void load_state(f32x4 (&S)[KT], const float* s, const Args& a, const P& w) {
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = row_of(t, 4 * g + r);
-      S[t][r] = a.h0 && in && row_of(t, 4 * g) < a.K ? a.h0[(static_cast<int64_t>(bh) * a.K + d) * a.V + col] : 0.0f;
-    }
-  const char* img = a.img + static_cast<int64_t>(bh) * a.NC * L::kBytes;
-  stage<L::kBytes>(lds, img, lane, wave, waves);
-  for (int n = 0; n < a.NC; ++n) {
-    char* cur = lds + (L::kStages == 2 ? (n & 1) * L::kBytes : 0);
-    const int t0 = n * C;
-    const int64_t c = static_cast<int64_t>(bh) * a.NC + n;
-    float vv[4][4];
+    for (int r = 0; r < 4; ++r)
+      S[t][r] = s && w.in && row_of(t, 4 * w.g) < a.K  // (K % 8 == 0)
+                    ? s[(static_cast<int64_t>(w.bh) * a.K + row_of(t, 4 * w.g + r)) * a.V + w.col] : 0.0f;
+}
+template <int KT, typename P>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[KT], float* s, const Args& a, const P& w) {
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (w.in && row_of(t, 4 * w.g) < a.K) s[(static_cast<int64_t>(w.bh) * a.K + row_of(t, 4 * w.g + r)) * a.V + w.col] = S[t][r];
+}
+
+template <int KP, int NI, bool KEEP, int W>
+__global__ __launch_bounds__(512) void state_kernel(Args a, int tiles) {  // (bounds of 8 waves: no accumulator registers apart)
+  using E = typename elem<NI>::type;
+  using L = Tile<KP, NI>;
+  constexpr int KT = KP / 16, KB = KP / 32, NP = L::NP, U = L::U, NW = kKept<NI>;
+  __shared__ __attribute__((aligned(16))) char lds[L::kStages * L::kBytes];
+  const Place<KP, NI, W> w(a, tiles);
+  const int lane = w.lane, g = w.g;
+  const int64_t o_st = static_cast<int64_t>(a.H) * a.V;
+  const E* v = reinterpret_cast<const E*>(a.v) + w.b * a.v_sb + w.h * a.v_sh;
+  E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(w.b) * a.T * a.H + w.h) * a.V;
+  const uint32_t vs = static_cast<uint32_t>(a.v_st * sizeof(E)), os = static_cast<uint32_t>(o_st * sizeof(E));
+  const uint32_t v_off = w.in ? 8 * g * vs + w.col * sizeof(E) : kOutOfRange, o_off = w.in ? 8 * g * os + w.col * sizeof(E) : kOutOfRange;
+  const char* img = a.img + static_cast<int64_t>(w.bh) * a.NC * L::kBytes;
+
+  // v of a chunk, loaded one chunk ahead, and before the copy of its operands: loads come back in order
+  uint32_t next[4][4];
+  const auto load_v = [&](int n) {
+    const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int tok = t0 + row_of(t, 4 * g + r);  // (past the end: the last token's, not used)
-        const float x = ld(v + min(tok, a.T - 1) * a.v_st);
-        vv[t][r] = in && tok < a.T ? x : 0.0f;
-      }
-    if constexpr (KEEP) {
-      uint32_t* sw = a.Sw + (static_cast<int64_t>(bh) * (a.NC + 1) + n) * a.K * a.VP + col;
+      for (int r = 0; r < 4; ++r) next[t][r] = load_col<E>(vr, v_off, row_of(t, r) * vs);
+  };
+  f32x4 S[KT];
+  load_state(S, a.h0, a, w);
+  stage<L::kBytes, W>(lds, img, lane, w.wave);
+  load_v(0);
+  for (int n = 0; n < a.NC; ++n) {
+    char* cur = lds + (L::kStages == 2 ? (n & 1) * L::kBytes : 0);
+    const int t0 = n * C, rows = min(C, a.T - t0);
+    const int64_t c = static_cast<int64_t>(w.bh) * a.NC + n;
+    f32x4 vv[4];
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (row_of(t, 4 * g) < a.K) sw[row_of(t, 4 * g + r) * a.VP] = keep<NI>(S[t][r]);  // (K % 8 == 0)
-        }
-    }
+      for (int r = 0; r < 4; ++r) vv[t][r] = value<E>(next[t][r]);
     bf16x8 sb[KB][3];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) split_pair<3>(S[2 * kb], S[2 * kb + 1], sb[kb]);
+    for (int kb = 0; kb < KB; ++kb) {
+      split_pair<3>(S[2 * kb], S[2 * kb + 1], sb[kb]);
+      if constexpr (KEEP)
+        keep<U, NW>(a.Sw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * KP, 32 * KP * 2, w.col % 32, 4 * kb + g, sb[kb]);
+    }
     staged();
+    if (n + 1 < a.NC) load_v(n + 1);
     if constexpr (L::kStages == 2)
-      if (n + 1 < a.NC) stage<L::kBytes>(lds + ((n + 1) & 1) * L::kBytes, img + static_cast<int64_t>(n + 1) * L::kBytes, lane, wave, waves);
+      if (n + 1 < a.NC) stage<L::kBytes, W>(lds + ((n + 1) & 1) * L::kBytes, img + static_cast<int64_t>(n + 1) * L::kBytes, lane, w.wave);
     const float* gt = reinterpret_cast<const float*>(cur + L::kGate);
     f32x4 y[4], oa[4];
 #pragma unroll
@@ -552,6 +592,8 @@ __global__ __launch_bounds__(64 * MAXW) void state_kernel(Args a, int tiles) {
     for (int p = 0; p < 2; ++p) {
       split_pair<NP>(d[2 * p], d[2 * p + 1], db[p]);
       split_pair<3>(e[2 * p], e[2 * p + 1], eb[p]);
+      if constexpr (KEEP)
+        keep<8, NW>(a.dw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * C, 32 * C * 2, w.col % 32, 4 * p + g, db[p]);
     }
     const float last = gt[63];
 #pragma unroll
@@ -564,6 +606,7 @@ __global__ __launch_bounds__(64 * MAXW) void state_kernel(Args a, int tiles) {
         S[t] = mm<3>(x, eb[p], S[t]);
       }
     }
+    const __amdgpu_buffer_rsrc_t orr = rows_buffer(o + t0 * o_st, o_st, rows, a.V);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -573,83 +616,64 @@ __global__ __launch_bounds__(64 * MAXW) void state_kernel(Args a, int tiles) {
         oa[t] = mm<NP>(x, db[p], oa[t]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = row_of(t, 4 * g + r);
-        if (in && t0 + i < a.T) st(o + (t0 + i) * o_st, oa[t][r]);
-        if constexpr (KEEP) a.dw[(c * C + i) * a.VP + col] = keep<NI>(d[t][r]);
-      }
+      for (int r = 0; r < 4; ++r) store_col<E>(orr, o_off, row_of(t, r) * os, oa[t][r]);
     }
     if constexpr (L::kStages == 1) {
       __syncthreads();
-      if (n + 1 < a.NC) stage<L::kBytes>(lds, img + static_cast<int64_t>(n + 1) * L::kBytes, lane, wave, waves);
+      if (n + 1 < a.NC) stage<L::kBytes, W>(lds, img + static_cast<int64_t>(n + 1) * L::kBytes, lane, w.wave);
     }
   }
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = row_of(t, 4 * g + r);
-      if (row_of(t, 4 * g) < a.K) {
-        if (a.state && in) a.state[(static_cast<int64_t>(bh) * a.K + d) * a.V + col] = S[t][r];
-        if constexpr (KEEP)
-          a.Sw[((static_cast<int64_t>(bh) * (a.NC + 1) + a.NC) * a.K + d) * a.VP + col] = keep<NI>(S[t][r]);
-      }
-    }
+  if (a.state) store_state(S, a.state, a, w);
 }
 
-template <int KP, int NI, int MAXW>
-__global__ __launch_bounds__(64 * MAXW) void dstate_kernel(Args a, int tiles) {
+template <int KP, int NI, int W>
+__global__ __launch_bounds__(512) void dstate_kernel(Args a, int tiles) {
   using E = typename elem<NI>::type;
   using L = Tile<KP, NI>;
-  constexpr int KT = KP / 16, KB = KP / 32, NP = L::NP, U = L::U;
+  constexpr int KT = KP / 16, KB = KP / 32, NP = L::NP, U = L::U, NW = kKept<NI>;
   __shared__ __attribute__((aligned(16))) char lds[L::kStages * L::kBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, m = lane & 15, g = lane >> 4;
-  int bh, tile;
-  place(blockIdx.x, a.B * a.H, tiles, bh, tile);
-  const int h = bh % a.H, b = bh / a.H, col = (tile * waves + wave) * 16 + m;
-  const bool in = col < a.V;
-  const E* dout = reinterpret_cast<const E*>(a.dout) + b * a.do_sb + h * a.do_sh + min(col, a.V - 1);
-  E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(b) * a.T * a.H + h) * a.V + col;
+  const Place<KP, NI, W> w(a, tiles);
+  const int lane = w.lane, g = w.g;
   const int64_t v_st = static_cast<int64_t>(a.H) * a.V;
+  const E* dout = reinterpret_cast<const E*>(a.dout) + w.b * a.do_sb + w.h * a.do_sh;
+  E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(w.b) * a.T * a.H + w.h) * a.V;
+  const uint32_t is = static_cast<uint32_t>(a.do_st * sizeof(E)), os = static_cast<uint32_t>(v_st * sizeof(E));
+  const uint32_t i_off = w.in ? 8 * g * is + w.col * sizeof(E) : kOutOfRange, o_off = w.in ? 8 * g * os + w.col * sizeof(E) : kOutOfRange;
+  const char* img = a.img + static_cast<int64_t>(w.bh) * a.NC * L::kBytes;
 
+  uint32_t next[4][4];
+  const auto load_go = [&](int n) {
+    const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) next[t][r] = load_col<E>(ir, i_off, row_of(t, r) * is);
+  };
   f32x4 S[KT];  // the gradient of the state
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = row_of(t, 4 * g + r);
-      S[t][r] = a.dstate && in && row_of(t, 4 * g) < a.K ? a.dstate[(static_cast<int64_t>(bh) * a.K + d) * a.V + col] : 0.0f;
-    }
-  const char* img = a.img + static_cast<int64_t>(bh) * a.NC * L::kBytes;
-  stage<L::kBytes>(lds + (L::kStages == 2 ? ((a.NC - 1) & 1) * L::kBytes : 0), img + static_cast<int64_t>(a.NC - 1) * L::kBytes, lane, wave, waves);
+  load_state(S, a.dstate, a, w);
+  load_go(a.NC - 1);
+  stage<L::kBytes, W>(lds + (L::kStages == 2 ? ((a.NC - 1) & 1) * L::kBytes : 0), img + static_cast<int64_t>(a.NC - 1) * L::kBytes, lane, w.wave);
   for (int n = a.NC - 1; n >= 0; --n) {
     char* cur = lds + (L::kStages == 2 ? (n & 1) * L::kBytes : 0);
-    const int t0 = n * C;
-    const int64_t c = static_cast<int64_t>(bh) * a.NC + n;
+    const int t0 = n * C, rows = min(C, a.T - t0);
+    const int64_t c = static_cast<int64_t>(w.bh) * a.NC + n;
     f32x4 go[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int tok = t0 + row_of(t, 4 * g + r);  // (past the end: the last token's, not used)
-        const float x = ld(dout + min(tok, a.T - 1) * a.do_st);
-        go[t][r] = in && tok < a.T ? x : 0.0f;
-      }
-    uint32_t* sw = a.dSw + c * a.K * a.VP + col;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (row_of(t, 4 * g) < a.K) sw[row_of(t, 4 * g + r) * a.VP] = keep<NI>(S[t][r]);  // (K % 8 == 0)
-      }
+      for (int r = 0; r < 4; ++r) go[t][r] = value<E>(next[t][r]);
     bf16x8 sb[KB][3], gb[2][NI];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) split_pair<3>(S[2 * kb], S[2 * kb + 1], sb[kb]);
+    for (int kb = 0; kb < KB; ++kb) {
+      split_pair<3>(S[2 * kb], S[2 * kb + 1], sb[kb]);
+      keep<U, NW>(a.dSw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * KP, 32 * KP * 2, w.col % 32, 4 * kb + g, sb[kb]);
+    }
+    staged();
+    if (n > 0) load_go(n - 1);
+    if constexpr (L::kStages == 2)
+      if (n > 0) stage<L::kBytes, W>(lds + ((n - 1) & 1) * L::kBytes, img + static_cast<int64_t>(n - 1) * L::kBytes, lane, w.wave);
 #pragma unroll
     for (int p = 0; p < 2; ++p) split_pair<NI>(go[2 * p], go[2 * p + 1], gb[p]);
-    staged();
-    if constexpr (L::kStages == 2)
-      if (n > 0) stage<L::kBytes>(lds + ((n - 1) & 1) * L::kBytes, img + static_cast<int64_t>(n - 1) * L::kBytes, lane, wave, waves);
     const float* gt = reinterpret_cast<const float*>(cur + L::kGate);
     f32x4 dd[4];
 #pragma unroll
@@ -670,10 +694,11 @@ __global__ __launch_bounds__(64 * MAXW) void dstate_kernel(Args a, int tiles) {
       }
       dd[t] = x;
     }
-    bf16x8 ddb[2][3], xb[2][3], wb[2][3];
+    bf16x8 ddb[2][3], xb[2][3], wb[2][3], yb[2][NW];
 #pragma unroll
     for (int p = 0; p < 2; ++p) split_pair<3>(dd[2 * p], dd[2 * p + 1], ddb[p]);
-    f32x4 dy[4], x[4], w[4];
+    f32x4 dy[4], x[4], u[4];
+    const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       dy[t] = f32x4{0, 0, 0, 0};
@@ -687,18 +712,18 @@ __global__ __launch_bounds__(64 * MAXW) void dstate_kernel(Args a, int tiles) {
       const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row_of(t, 4 * g));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = row_of(t, 4 * g + r);
         const float dvv = be[r] * dy[t][r];
-        if (in && t0 + i < a.T) st(dv + (t0 + i) * v_st, dvv);
-        a.yw[(c * C + i) * a.VP + col] = keep<NI>(dy[t][r]);
+        store_col<E>(orr, o_off, row_of(t, r) * os, dvv);
         x[t][r] = -eg[r] * dvv;
-        w[t][r] = a.scale * eg[r] * go[t][r];
+        u[t][r] = a.scale * eg[r] * go[t][r];
       }
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       split_pair<3>(x[2 * p], x[2 * p + 1], xb[p]);
-      split_pair<3>(w[2 * p], w[2 * p + 1], wb[p]);
+      split_pair<3>(u[2 * p], u[2 * p + 1], wb[p]);
+      split_pair<NW>(dy[2 * p], dy[2 * p + 1], yb[p]);
+      keep<8, NW>(a.yw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * C, 32 * C * 2, w.col % 32, 4 * p + g, yb[p]);
     }
     const float last = gt[63];
 #pragma unroll
@@ -715,272 +740,226 @@ __global__ __launch_bounds__(64 * MAXW) void dstate_kernel(Args a, int tiles) {
     }
     if constexpr (L::kStages == 1) {
       __syncthreads();
-      if (n > 0) stage<L::kBytes>(lds, img + static_cast<int64_t>(n - 1) * L::kBytes, lane, wave, waves);
+      if (n > 0) stage<L::kBytes, W>(lds, img + static_cast<int64_t>(n - 1) * L::kBytes, lane, w.wave);
     }
   }
-  if (a.dh0) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = row_of(t, 4 * g + r);
-        if (in && row_of(t, 4 * g) < a.K) a.dh0[(static_cast<int64_t>(bh) * a.K + d) * a.V + col] = S[t][r];
-      }
-  }
+  if (a.dh0) store_state(S, a.dh0, a, w);
 }
 
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
 
 template <int KP, int NI>
 struct GradTile {
-  static constexpr int NW = kept_limbs<NI>::N;   // limbs of d, dy and of N, F
-  static constexpr int kRow = 64 * 64;           // bytes of one limb of a [64][32] block
-  static constexpr int kK = 0, kQ = NI * C * KP * 2;
-  static constexpr int kF = 2 * kQ, kN = kF + NW * kPlane * 2;  // F, N; before them, the blocks of dy, d, do
-  static constexpr int kY = kF, kD = kY + NW * kRow, kO = kD + NW * kRow;
-  static_assert(kO + NI * kRow <= kN + NW * kPlane * 2, "blocks fit where F and N go");
-  static constexpr int kVec = kN + NW * kPlane * 2;             // floats: sums [2][4][64], dy.v [64], dot [4]
-  static constexpr int kBytes = kVec + (8 * 64 + 64 + 4) * 4;
+  static constexpr int W = KP / 16;                                           // a wave for 16 columns of dq, dk
+  static constexpr int NW = kKept<NI>;
+  static constexpr int kState = NW * 32 * KP * 2, kVec = NW * 32 * C * 2;     // bytes of 32 columns of a state, of d or dy
+  static constexpr int kS = 0, kE = kState, kD = 2 * kState, kY = kD + kVec;  // S, dS', d, dy, 32 columns at a time;
+  static constexpr int kK = 0, kQ = NI * C * KP * 2;                          // then in their place k, q
+  static constexpr int kF = 2 * kQ, kN = kF + NW * kPlane * 2;                // and F, N
+  static constexpr int kSums = kY + kVec > kN + NW * kPlane * 2 ? kY + kVec : kN + NW * kPlane * 2;
+  static constexpr int kBytes = kSums + (2 * W * 64 + 64 + W) * 4;            // floats: q.dq, k.Z [W][64], dy.v [64], [W]
 };
 
 template <int KP, int NI>
-__global__ __launch_bounds__(256) void grad_kernel(Args a) {
+__global__ __launch_bounds__(64 * (KP / 16)) void grad_kernel(Args a) {
   using E = typename elem<NI>::type;
   using L = GradTile<KP, NI>;
-  constexpr int NW = L::NW, U = KP / 8, CT = KP / 64;  // column tiles of 16 per wave
+  constexpr int NW = L::NW, U = KP / 8, W = L::W;
   __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x;
   const int n = static_cast<int>(c % a.NC), bh = static_cast<int>(c / a.NC), h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
   const int hk = h / grp, t0 = n * C, rows = min(C, a.T - t0);
-  const int64_t sid = static_cast<int64_t>(bh) * (a.NC + 1) + n;
-  float* vec = reinterpret_cast<float*>(lds + L::kVec);
-
+  float* vec = reinterpret_cast<float*>(lds + L::kSums);
   const char* img = a.img + c * Tile<KP, NI>::kBytes;
-  stage<2 * L::kQ>(lds, img, lane, wave, 4);  // k and q
-  // <S', dS'>
-  {
-    const uint32_t* s1 = a.Sw + (sid + 1) * a.K * a.VP;
-    const uint32_t* s2 = a.dSw + c * a.K * a.VP;
-    float sum = 0.0f;
-    for (int i = 4 * tid; i < a.K * a.VP; i += 1024) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(s1 + i), y = *reinterpret_cast<const u32x4*>(s2 + i);
+  const float* gt = reinterpret_cast<const float*>(img + Tile<KP, NI>::kGate);
+  const double* Gd = a.Gd + c * 64;
+
+  // Products over the value columns, 32 at a time, in this wave's 16 columns of K: W1 = dy S^T, W2 = do S^T,
+  // W3 = d dS'^T, and a diagonal block of S dS'^T. Of the 64 x 64 products dy d^T and do d^T a wave takes 16 rows of
+  // both (W = 4) or of one (W = 8: waves 0 to 3 the first, 4 to 7 the second); waves 0 to 3 also a diagonal block of dy v^T.
+  f32x4 w1[4], w2[4], w3[4], m1[4], m2[W == 4 ? 4 : 1], ss = {0, 0, 0, 0}, yv = ss;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += kept<NI>(x[j]) * kept<NI>(y[j]);
+  for (int t = 0; t < 4; ++t) w1[t] = w2[t] = w3[t] = m1[t] = m2[W == 4 ? t : 0] = f32x4{0, 0, 0, 0};
+  const int mr = wave & 3;
+  const E* orow = reinterpret_cast<const E*>(a.dout) + b * a.do_sb + t0 * a.do_st + h * a.do_sh + 8 * g;
+  const E* vrow = reinterpret_cast<const E*>(a.v) + b * a.v_sb + (t0 + 16 * mr + m) * a.v_st + h * a.v_sh + 8 * g;
+  for (int vb = 0; vb < a.VP / 32; ++vb) {
+    const int64_t blk = c * (a.VP / 32) + vb;
+    if (vb) __syncthreads();
+    stage<L::kState, W>(lds + L::kS, a.Sw + blk * NW * 32 * KP, lane, wave);
+    stage<L::kState, W>(lds + L::kE, a.dSw + blk * NW * 32 * KP, lane, wave);
+    stage<L::kVec, W>(lds + L::kD, a.dw + blk * NW * 32 * C, lane, wave);
+    stage<L::kVec, W>(lds + L::kY, a.yw + blk * NW * 32 * C, lane, wave);
+    bf16x8 fo[4][NI], fv[NI];
+    const bool cols = 32 * vb + 8 * g < a.V;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) load8(orow + (16 * t + m) * a.do_st + 32 * vb, 16 * t + m < rows && cols, fo[t]);
+    if (wave < 4) {
+      float x[8];  // (v may lie at any alignment)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 16 * mr + m < rows && cols ? ld(vrow + 32 * vb + j) : 0.0f;
+      split<NI>(x, fv);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) vec[9 * 64 + wave] = sum;
-  }
-  // products over the value columns, 32 at a time: W1 = dy S^T, W2 = do S^T, W3 = d dS'^T (this wave's
-  // columns), M1 = dy d^T, M2 = do d^T (this wave's rows)
-  f32x4 w1[4][CT], w2[4][CT], w3[4][CT], m1[4], m2[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    m1[t] = f32x4{0, 0, 0, 0}, m2[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < CT; ++i) w1[t][i] = w2[t][i] = w3[t][i] = f32x4{0, 0, 0, 0};
-  }
-  const int sr = tid >> 2, su = tid & 3;  // the row and 16-byte unit that this thread stages
-  float dyv = 0.0f;
-  const E* vrow = reinterpret_cast<const E*>(a.v) + b * a.v_sb + (t0 + sr) * a.v_st + h * a.v_sh + 8 * su;
-  const E* orow = reinterpret_cast<const E*>(a.dout) + b * a.do_sb + (t0 + sr) * a.do_st + h * a.do_sh + 8 * su;
-  for (int vb = 0; vb < a.VP; vb += 32) {
-    __syncthreads();
-    {
-      const u32x4* yp = reinterpret_cast<const u32x4*>(a.yw + (c * C + sr) * a.VP + vb + 8 * su);
-      const u32x4* dp = reinterpret_cast<const u32x4*>(a.dw + (c * C + sr) * a.VP + vb + 8 * su);
-      const u32x4 y0 = yp[0], y1 = yp[1], d0 = dp[0], d1 = dp[1];
-      const bool ok = sr < rows && vb + 8 * su < a.V;
-      bf16x8 ly[NW], ldl[NW], lo[NI];
-      unkeep<NI>(y0, y1, ly);
-      unkeep<NI>(d0, d1, ldl);
-      load8(orow + vb, ok, lo);
-      const int pos = sr * 64 + ((su ^ ((sr >> 1) & 3)) * 16);
-#pragma unroll
-      for (int l = 0; l < NW; ++l) {
-        *reinterpret_cast<bf16x8*>(lds + L::kY + l * L::kRow + pos) = ly[l];
-        *reinterpret_cast<bf16x8*>(lds + L::kD + l * L::kRow + pos) = ldl[l];
-      }
-#pragma unroll
-      for (int l = 0; l < NI; ++l) *reinterpret_cast<bf16x8*>(lds + L::kO + l * L::kRow + pos) = lo[l];
-      if (ok) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dyv += kept<NI>(y0[j]) * ld(vrow + vb + j) + kept<NI>(y1[j]) * ld(vrow + vb + 4 + j);
-      }
-    }
-    bf16x8 s[CT][NW], ds[CT][NW];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const int d = (wave * CT + i) * 16 + m;
-      u32x4 s0 = {0, 0, 0, 0}, s1 = s0, e0 = s0, e1 = s0;
-      if (d < a.K) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(a.Sw + (sid * a.K + d) * a.VP + vb + 8 * g);
-        const u32x4* e = reinterpret_cast<const u32x4*>(a.dSw + (c * a.K + d) * a.VP + vb + 8 * g);
-        s0 = p[0], s1 = p[1], e0 = e[0], e1 = e[1];
-      }
-      unkeep<NI>(s0, s1, s[i]);
-      unkeep<NI>(e0, e1, ds[i]);
-    }
-    __syncthreads();
-    const auto block = [&](int base, int t, int l) {
-      const int r = 16 * t + m;
-      return *reinterpret_cast<const bf16x8*>(lds + base + l * L::kRow + r * 64 + ((g ^ ((r >> 1) & 3)) * 16));
-    };
+    staged();
+    bf16x8 s[NW], ds[NW];
+    frags_t<U, false>(lds + L::kS, 32 * KP * 2, wave, 0, lane, s);
+    frags_t<U, false>(lds + L::kE, 32 * KP * 2, wave, 0, lane, ds);
+    ss = mm<NW>(s, ds, ss);
     bf16x8 yr[NW], orr[NI];
-#pragma unroll
-    for (int l = 0; l < NW; ++l) yr[l] = block(L::kY, wave, l);
-#pragma unroll
-    for (int l = 0; l < NI; ++l) orr[l] = block(L::kO, wave, l);
+    frags_t<8, false>(lds + L::kY, 32 * C * 2, mr, 0, lane, yr);
+    if (wave < 4) yv = mm<NW>(yr, fv, yv);
+    load8(orow + (16 * mr + m) * a.do_st + 32 * vb, 16 * mr + m < rows && cols, orr);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      bf16x8 fy[NW], fd[NW], fo[NI];
-#pragma unroll
-      for (int l = 0; l < NW; ++l) fy[l] = block(L::kY, t, l), fd[l] = block(L::kD, t, l);
-#pragma unroll
-      for (int l = 0; l < NI; ++l) fo[l] = block(L::kO, t, l);
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        w1[t][i] = mm<NW>(fy, s[i], w1[t][i]);
-        w2[t][i] = mm<NW>(fo, s[i], w2[t][i]);
-        w3[t][i] = mm<NW>(fd, ds[i], w3[t][i]);
-      }
-      if (t <= wave) {
-        m1[t] = mm<NW>(yr, fd, m1[t]);
-        m2[t] = mm<NW>(orr, fd, m2[t]);
+      bf16x8 fy[NW], fd[NW];
+      frags_t<8, false>(lds + L::kY, 32 * C * 2, t, 0, lane, fy);
+      frags_t<8, false>(lds + L::kD, 32 * C * 2, t, 0, lane, fd);
+      w1[t] = mm<NW>(fy, s, w1[t]);
+      w2[t] = mm<NW>(fo[t], s, w2[t]);
+      w3[t] = mm<NW>(fd, ds, w3[t]);
+      if (t <= mr) {
+        if constexpr (W == 4) {
+          m1[t] = mm<NW>(yr, fd, m1[t]);
+          m2[t] = mm<NW>(orr, fd, m2[t]);
+        } else if (wave < 4) {
+          m1[t] = mm<NW>(yr, fd, m1[t]);
+        } else {
+          m1[t] = mm<NW>(orr, fd, m1[t]);
+        }
       }
     }
   }
   __syncthreads();
-  const float* gt = reinterpret_cast<const float*>(img + Tile<KP, NI>::kGate);
-  const double* Gd = a.Gd + c * 64;
+  stage<2 * L::kQ, W>(lds, img, lane, wave);  // k and q
   // F and N, in this wave's rows, to LDS
+  const auto put = [&](int plane, int row, int col, float x) {
+    const int pos = at<8>(row, col >> 3) + (col & 7) * 2;
+#pragma unroll
+    for (int l = 0; l < NW; ++l) {
+      const uint32_t u = __float_as_uint(x);
+      *reinterpret_cast<bf16_t*>(lds + plane + l * kPlane * 2 + pos) = NW == 2 && l == 1 ? f32_to_bf16(x) : static_cast<bf16_t>(u >> 16);
+      x -= __uint_as_float(u & 0xffff0000u);
+    }
+  };
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * wave + 4 * g + r, col = 16 * t + m;
+      const int row = 16 * mr + 4 * g + r, col = 16 * t + m;
       const float dec = col <= row ? expf(static_cast<float>(Gd[row] - Gd[col])) : 0.0f;
-      float f = col < row ? dec * m1[t][r] : 0.0f, nn = col <= row ? a.scale * dec * m2[t][r] : 0.0f;
-      const int pos = at<8>(row, col >> 3) + (col & 7) * 2;
-#pragma unroll
-      for (int l = 0; l < NW; ++l) {
-        const uint32_t fh = __float_as_uint(f), nh = __float_as_uint(nn);
-        const bool round = NW == 2 && l == 1;
-        *reinterpret_cast<bf16_t*>(lds + L::kF + l * kPlane * 2 + pos) = round ? f32_to_bf16(f) : static_cast<bf16_t>(fh >> 16);
-        *reinterpret_cast<bf16_t*>(lds + L::kN + l * kPlane * 2 + pos) = round ? f32_to_bf16(nn) : static_cast<bf16_t>(nh >> 16);
-        f -= __uint_as_float(fh & 0xffff0000u);
-        nn -= __uint_as_float(nh & 0xffff0000u);
-      }
+      if (W == 4 || wave < 4) put(L::kF, row, col, col < row ? dec * m1[t][r] : 0.0f);
+      if (W == 4 || wave >= 4) put(L::kN, row, col, col <= row ? a.scale * dec * (W == 4 ? m2[W == 4 ? t : 0][r] : m1[t][r]) : 0.0f);
     }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int i0 = 16 * t + 4 * g;
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float eg = gt[i0 + r], tail = gt[64 + i0 + r];
-#pragma unroll
-      for (int i = 0; i < CT; ++i) w1[t][i][r] *= eg, w2[t][i][r] *= a.scale * eg, w3[t][i][r] *= tail;
+      const int i = 16 * t + 4 * g + r;
+      w1[t][r] *= gt[i], w2[t][r] *= a.scale * gt[i], w3[t][r] *= gt[64 + i];
     }
+  if (wave < 4) {  // the diagonals' lanes
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * g + r == m) vec[2 * W * 64 + 16 * mr + m] = yv[r];
   }
   staged();
+  // <S', dS'> = e^{G_C} <S, dS'> + sum_j k_j.(e^{G_C - G_j} (d dS'^T)_j): its first part from the diagonals
+  float dot = 0.0f;
 #pragma unroll
-  for (int i = 0; i < CT; ++i) {
-    const int ct = wave * CT + i;
+  for (int r = 0; r < 4; ++r) dot += 4 * g + r == m ? ss[r] : 0.0f;
+  dot *= gt[63];
+  const int d = 16 * wave + m;
+  // k and q where this wave's accumulators are
+  const auto at_acc = [&](int base, int row) {
+    float x = 0.0f;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      bf16x8 kf[NI], qf[NI], bk[NW];
-      frags_t<U, false>(lds + L::kK, C * KP * 2, ct, p, lane, kf);
-      frags_t<U, false>(lds + L::kQ, C * KP * 2, ct, p, lane, qf);
-      {
-        float x[8];
+    for (int l = 0; l < NI; ++l)
+      x += bf16_to_f32(*reinterpret_cast<const bf16_t*>(lds + base + l * C * KP * 2 + at<U>(row, d >> 3) + (d & 7) * 2));
+    return x;
+  };
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float kv = static_cast<float>(kf[0][j]);
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int l = 1; l < NI; ++l) kv += static_cast<float>(kf[l][j]);
-          x[j] = -kv * gt[128 + 32 * p + 8 * g + j];
-        }
-        split<NW>(x, bk);
+    for (int r = 0; r < 4; ++r) dot += at_acc(L::kK, 16 * t + 4 * g + r) * w3[t][r];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    bf16x8 kf[NI], qf[NI], bk[NW];
+    frags_t<U, false>(lds + L::kK, C * KP * 2, wave, p, lane, kf);
+    frags_t<U, false>(lds + L::kQ, C * KP * 2, wave, p, lane, qf);
+    {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float kv = static_cast<float>(kf[0][j]);
+#pragma unroll
+        for (int l = 1; l < NI; ++l) kv += static_cast<float>(kf[l][j]);
+        x[j] = -kv * gt[128 + 32 * p + 8 * g + j];
       }
+      split<NW>(x, bk);
+    }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (p <= t / 2) {
-          bf16x8 f[NW];
+    for (int t = 0; t < 4; ++t) {
+      bf16x8 f[NW];
+      if (p <= t / 2) {
 #pragma unroll
-          for (int l = 0; l < NW; ++l) f[l] = frag_plain<8>(lds + L::kF + l * kPlane * 2, t, p, lane);
-          w1[t][i] = mm<NW>(f, kf, w1[t][i]);
+        for (int l = 0; l < NW; ++l) f[l] = frag_plain<8>(lds + L::kF + l * kPlane * 2, t, p, lane);
+        w1[t] = mm<NW>(f, kf, w1[t]);
 #pragma unroll
-          for (int l = 0; l < NW; ++l) f[l] = frag_plain<8>(lds + L::kN + l * kPlane * 2, t, p, lane);
-          w2[t][i] = mm<NW>(f, kf, w2[t][i]);
-        }
-        if (p >= t / 2) {
-          bf16x8 f[NW];
-          frags_t<8, false>(lds + L::kN, kPlane * 2, t, p, lane, f);
-          w3[t][i] = mm<NW>(f, qf, w3[t][i]);
-          frags_t<8, false>(lds + L::kF, kPlane * 2, t, p, lane, f);
-          w3[t][i] = mm<NW>(f, bk, w3[t][i]);
-        }
+        for (int l = 0; l < NW; ++l) f[l] = frag_plain<8>(lds + L::kN + l * kPlane * 2, t, p, lane);
+        w2[t] = mm<NW>(f, kf, w2[t]);
+      }
+      if (p >= t / 2) {
+        frags_t<8, false>(lds + L::kN, kPlane * 2, t, p, lane, f);
+        w3[t] = mm<NW>(f, qf, w3[t]);
+        frags_t<8, false>(lds + L::kF, kPlane * 2, t, p, lane, f);
+        w3[t] = mm<NW>(f, bk, w3[t]);
       }
     }
   }
   // outputs, and the row sums q.dq and k.Z
+  const int64_t tok0 = static_cast<int64_t>(b) * a.T + t0;
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = 16 * t + 4 * g + r;
-      const float be = gt[128 + row];
-      float qd = 0.0f, kz = 0.0f;
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const int d = (wave * CT + i) * 16 + m;
-        const float dq = w2[t][i][r], z = w1[t][i][r], dk = w3[t][i][r] - be * z;
-        float qv = 0.0f, kv = 0.0f;
-#pragma unroll
-        for (int l = 0; l < NI; ++l) {
-          const int pos = l * C * KP * 2 + at<U>(row, d >> 3) + (d & 7) * 2;
-          qv += bf16_to_f32(*reinterpret_cast<const bf16_t*>(lds + L::kQ + pos));
-          kv += bf16_to_f32(*reinterpret_cast<const bf16_t*>(lds + L::kK + pos));
-        }
-        qd += qv * dq;
-        kz += kv * z;
-        if (row < rows && d < a.K) {
-          const int64_t tok = static_cast<int64_t>(b) * a.T + t0 + row;
-          if (grp == 1) {
-            st(reinterpret_cast<E*>(a.dq) + (tok * a.Hk + hk) * a.K + d, dq);
-            st(reinterpret_cast<E*>(a.dk) + (tok * a.Hk + hk) * a.K + d, dk);
-          } else {
-            a.dqp[(tok * a.H + h) * a.K + d] = dq;
-            a.dkp[(tok * a.H + h) * a.K + d] = dk;
-          }
+      const float dq = w2[t][r], z = w1[t][r], dk = w3[t][r] - gt[128 + row] * z;
+      float qd = at_acc(L::kQ, row) * dq, kz = at_acc(L::kK, row) * z;
+      if (row < rows && d < a.K) {
+        if (grp == 1) {
+          st(reinterpret_cast<E*>(a.dq) + ((tok0 + row) * a.Hk + hk) * a.K + d, dq);
+          st(reinterpret_cast<E*>(a.dk) + ((tok0 + row) * a.Hk + hk) * a.K + d, dk);
+        } else {
+          a.dqp[((tok0 + row) * a.H + h) * a.K + d] = dq;
+          a.dkp[((tok0 + row) * a.H + h) * a.K + d] = dk;
         }
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) qd += __shfl_xor(qd, o, 64), kz += __shfl_xor(kz, o, 64);
-      if (m == 0) vec[wave * 64 + row] = qd, vec[256 + wave * 64 + row] = kz;
+      if (m == 0) vec[wave * 64 + row] = qd, vec[(W + wave) * 64 + row] = kz;
     }
-  dyv += __shfl_xor(dyv, 1, 64);
-  dyv += __shfl_xor(dyv, 2, 64);
-  if (su == 0) vec[512 + sr] = dyv;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+  if (lane == 0) vec[(2 * W + 1) * 64 + wave] = dot;
   __syncthreads();
   if (wave == 0) {
-    float qd = 0.0f, kz = 0.0f, dot = 0.0f;
+    float qd = 0.0f, kz = 0.0f, all = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) qd += vec[w * 64 + lane], kz += vec[256 + w * 64 + lane], dot += vec[9 * 64 + w];
-    const float yv = vec[512 + lane], be = gt[128 + lane];
-    double s = static_cast<double>(qd) - static_cast<double>(be) * yv;
+    for (int w = 0; w < W; ++w) qd += vec[w * 64 + lane], kz += vec[(W + w) * 64 + lane], all += vec[(2 * W + 1) * 64 + w];
+    const float y = vec[2 * W * 64 + lane], be = gt[128 + lane];
+    double s = static_cast<double>(qd) - static_cast<double>(be) * y;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const double x = __shfl_down(s, o, 64);
       if (lane + o < 64) s += x;
     }
     if (lane < rows) {
-      const int64_t tok = (static_cast<int64_t>(b) * a.T + t0 + lane) * a.H + h;
+      const int64_t tok = (tok0 + lane) * a.H + h;
       const float gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
       // a decay that is zero in fp32 passes nothing on
-      st(reinterpret_cast<E*>(a.dg) + tok, gv < -104.0f ? 0.0f : static_cast<float>(s + dot));
-      st(reinterpret_cast<E*>(a.db) + tok, yv - kz);
+      st(reinterpret_cast<E*>(a.dg) + tok, gv < -104.0f ? 0.0f : static_cast<float>(s + all));
+      st(reinterpret_cast<E*>(a.db) + tok, y - kz);
     }
   }
 }
@@ -1093,20 +1072,22 @@ inline Layout layout(int dtype, const mg_delta_dims& s, bool keep_) {
   l.img = 0;
   l.G = c * image;
   l.S = l.G + c * 512;
-  l.d = l.S + (keep_ ? up(bh * (n + 1) * s.K * vp * 4) : 0);
-  l.end = l.d + (keep_ ? c * C * vp * 4 : 0);
+  const size_t nw = dtype == MG_F32 ? 3 : 2;
+  l.d = l.S + (keep_ ? c * vp * nw * (s.K <= 64 ? 64 : 128) * 2 : 0);
+  l.end = l.d + (keep_ ? c * vp * nw * C * 2 : 0);
   return l;
 }
 
 struct BwdLayout {
   size_t dS, y, dqp, dkp, end;
 };
-inline BwdLayout bwd_layout(const mg_delta_dims& s) {
+inline BwdLayout bwd_layout(int dtype, const mg_delta_dims& s) {
   const size_t c = static_cast<size_t>(s.B) * s.H * chunks(s), vp = vpad(s.V);
   BwdLayout l;
   l.dS = 0;
-  l.y = up(c * s.K * vp * 4);
-  l.dqp = l.y + c * C * vp * 4;
+  const size_t nw = dtype == MG_F32 ? 3 : 2;
+  l.y = c * vp * nw * (s.K <= 64 ? 64 : 128) * 2;
+  l.dqp = l.y + c * vp * nw * C * 2;
   l.dkp = l.dqp + (s.H > s.Hk ? up(static_cast<size_t>(s.B) * s.T * s.H * s.K * 4) : 0);
   l.end = l.dkp + (l.dkp - l.dqp);
   return l;
@@ -1154,7 +1135,7 @@ inline void fill(Args& a, const mg_delta_dims& s, float scale, const mg_rows* q,
   a.g = static_cast<const char*>(g->p), a.g_sb = g->sb, a.g_st = g->st, a.g_sh = g->sh;
   a.beta = static_cast<const char*>(beta->p), a.b_sb = beta->sb, a.b_st = beta->st, a.b_sh = beta->sh;
   a.img = ws + l.img, a.Gd = reinterpret_cast<double*>(ws + l.G);
-  a.Sw = reinterpret_cast<uint32_t*>(ws + l.S), a.dw = reinterpret_cast<uint32_t*>(ws + l.d);
+  a.Sw = reinterpret_cast<bf16_t*>(ws + l.S), a.dw = reinterpret_cast<bf16_t*>(ws + l.d);
 }
 
 template <int KP, int NI>
@@ -1163,17 +1144,13 @@ int launch_fwd(const Args& a, bool keep_, hipStream_t st_) {
   hipLaunchKernelGGL((chunk_kernel<KP, NI>), dim3(bh * a.NC), dim3(256), 0, st_, a);
   const int w = waves_for(bh, a.VP), tiles = a.VP / 16 / w;
   const dim3 grid(bh * tiles), block(64 * w);
-  if (keep_) {
-    if (w == 8)
-      hipLaunchKernelGGL((state_kernel<KP, NI, true, 8>), grid, block, 0, st_, a, tiles);
-    else
-      hipLaunchKernelGGL((state_kernel<KP, NI, true, 4>), grid, block, 0, st_, a, tiles);
-  } else {
-    if (w == 8)
-      hipLaunchKernelGGL((state_kernel<KP, NI, false, 8>), grid, block, 0, st_, a, tiles);
-    else
-      hipLaunchKernelGGL((state_kernel<KP, NI, false, 4>), grid, block, 0, st_, a, tiles);
-  }
+#define GO(W)                                                                                         \
+  if (keep_)                                                                                          \
+    hipLaunchKernelGGL((state_kernel<KP, NI, true, W>), grid, block, 0, st_, a, tiles);               \
+  else                                                                                                \
+    hipLaunchKernelGGL((state_kernel<KP, NI, false, W>), grid, block, 0, st_, a, tiles);
+  if (w == 8) { GO(8) } else if (w == 4) { GO(4) } else { GO(2) }
+#undef GO
   return check_launch("mg_delta_fwd");
 }
 
@@ -1182,11 +1159,14 @@ int launch_bwd(const Args& a, hipStream_t st_) {
   using E = typename elem<NI>::type;
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
   const int w = waves_for(bh, a.VP), tiles = a.VP / 16 / w;
+  const dim3 grid(bh * tiles), block(64 * w);
   if (w == 8)
-    hipLaunchKernelGGL((dstate_kernel<KP, NI, 8>), dim3(bh * tiles), dim3(64 * w), 0, st_, a, tiles);
+    hipLaunchKernelGGL((dstate_kernel<KP, NI, 8>), grid, block, 0, st_, a, tiles);
+  else if (w == 4)
+    hipLaunchKernelGGL((dstate_kernel<KP, NI, 4>), grid, block, 0, st_, a, tiles);
   else
-    hipLaunchKernelGGL((dstate_kernel<KP, NI, 4>), dim3(bh * tiles), dim3(64 * w), 0, st_, a, tiles);
-  hipLaunchKernelGGL((grad_kernel<KP, NI>), dim3(bh * a.NC), dim3(256), 0, st_, a);
+    hipLaunchKernelGGL((dstate_kernel<KP, NI, 2>), grid, block, 0, st_, a, tiles);
+  hipLaunchKernelGGL((grad_kernel<KP, NI>), dim3(bh * a.NC), dim3(64 * GradTile<KP, NI>::W), 0, st_, a);
   if (a.H > a.Hk) {
     const int64_t n = static_cast<int64_t>(a.B) * a.T * a.Hk * a.K;
     hipLaunchKernelGGL((sum_heads_kernel<E>), dim3((n / 4 + 255) / 256), dim3(256), 0, st_, a.dqp, a.dkp,
@@ -1223,7 +1203,7 @@ extern "C" size_t mg_delta_fwd_workspace_bytes(int dtype, const mg_delta_dims* d
 
 extern "C" size_t mg_delta_bwd_workspace_bytes(int dtype, const mg_delta_dims* dims) {
   if (delta::check_dims("mg_delta_bwd_workspace_bytes", dtype, dims)) return 0;
-  return delta::bwd_layout(*dims).end;
+  return delta::bwd_layout(dtype, *dims).end;
 }
 
 extern "C" int mg_delta_fwd(int dtype, const mg_delta_dims* dims, const mg_rows* q, const mg_rows* k, const mg_rows* v,
@@ -1269,7 +1249,7 @@ extern "C" int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows*
   const delta::Layout l = delta::layout(dtype, *dims, true);
   if (!kept || kept_bytes < l.end || !aligned(kept, 256))
     return fail(MG_ERR_WORKSPACE, "%s: the forward's buffer has %zu bytes < %zu (or is not 256-byte aligned)", fn, kept_bytes, l.end);
-  const delta::BwdLayout w = delta::bwd_layout(*dims);
+  const delta::BwdLayout w = delta::bwd_layout(dtype, *dims);
   if (!workspace || workspace_bytes < w.end || !aligned(workspace, 256))
     return fail(MG_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu (or not 256-byte aligned)", fn, workspace_bytes, w.end);
   delta::Args a = {};
@@ -1277,7 +1257,7 @@ extern "C" int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows*
   char* ws = static_cast<char*>(workspace);
   a.dout = static_cast<const char*>(dout->p), a.do_sb = dout->sb, a.do_st = dout->st, a.do_sh = dout->sh;
   a.dstate = dstate, a.dh0 = dh0;
-  a.dSw = reinterpret_cast<uint32_t*>(ws + w.dS), a.yw = reinterpret_cast<uint32_t*>(ws + w.y);
+  a.dSw = reinterpret_cast<bf16_t*>(ws + w.dS), a.yw = reinterpret_cast<bf16_t*>(ws + w.y);
   a.dqp = reinterpret_cast<float*>(ws + w.dqp), a.dkp = reinterpret_cast<float*>(ws + w.dkp);
   a.dq = static_cast<char*>(dq), a.dk = static_cast<char*>(dk), a.dv = static_cast<char*>(dv);
   a.dg = static_cast<char*>(dg), a.db = static_cast<char*>(dbeta);
