@@ -87,27 +87,31 @@ struct Args {
 __device__ __forceinline__ uint32_t hi16x2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ uint32_t lo16x2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 
-// 8 fp32 values as N limbs. N = 3: by cutting the mantissa (8 + 8 + 8 bits, exact). N = 2: the second
-// limb rounded to nearest, off by 2^-17 at most.
+// 8 fp32 values as N limbs. N = 3: by cutting the mantissa (8 + 8 + 8 bits, exact). N = 2: both rounded to
+// nearest, off by 2^-18 at most.
+__device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[3]) {
+  w[0] = hi16x2(__float_as_uint(a), __float_as_uint(b));
+  a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+  b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+  w[1] = hi16x2(__float_as_uint(a), __float_as_uint(b));
+  a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+  b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+  w[2] = hi16x2(__float_as_uint(a), __float_as_uint(b));
+}
+__device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[2]) {
+  w[0] = pack_bf16x2(a, b);
+  w[1] = pack_bf16x2(a - __uint_as_float(w[0] << 16), b - __uint_as_float(w[0] & 0xffff0000u));
+}
+__device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[1]) { w[0] = hi16x2(__float_as_uint(a), __float_as_uint(b)); }
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[N]) {
   u32x4 w[N];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float a = x[2 * i], b = x[2 * i + 1];
-    w[0][i] = hi16x2(__float_as_uint(a), __float_as_uint(b));
-    if constexpr (N > 1) {
-      a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-      b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-      if constexpr (N == 2) {
-        w[1][i] = pack_bf16x2(a, b);
-      } else {
-        w[1][i] = hi16x2(__float_as_uint(a), __float_as_uint(b));
-        a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-        b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-        w[2][i] = hi16x2(__float_as_uint(a), __float_as_uint(b));
-      }
-    }
+    uint32_t l[N];
+    pair_limbs(x[2 * i], x[2 * i + 1], l);
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j][i] = l[j];
   }
 #pragma unroll
   for (int l = 0; l < N; ++l) out[l] = __builtin_bit_cast(bf16x8, w[l]);
@@ -229,11 +233,10 @@ struct Tile {
   static constexpr int U = KP / 8;
   static constexpr int kK = 0, kQ = NI * C * KP * 2, kT = 2 * kQ, kP = kT + 3 * kPlane * 2, kGate = kP + NP * kPlane * 2;
   static constexpr int kBytes = kGate + 1024;
-  static constexpr int kStages = 2 * kBytes <= 160 * 1024 ? 2 : 1;
 };
 
 template <int BYTES, int WAVES>
-__device__ __forceinline__ void stage(char* lds, const void* src, int lane, int wave) {
+__device__ __forceinline__ void stage(char* lds, const void* src, int lane, int wave) {  // BYTES / 1024 / WAVES loads a wave, rounded up
   const __amdgpu_buffer_rsrc_t rsrc =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), static_cast<short>(0), BYTES, 0x00020000);
   int off = wave * 1024;
@@ -422,6 +425,18 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- the pass over the chunks
+//
+// A workgroup of four waves owns 16 CT value columns of one head's state and takes the chunks in order.
+// The state never leaves its accumulators: wave w holds rows 32 w ... 32 w + 31 of S and, in each chunk,
+// makes rows 16 w' ... (16 of the 64 tokens) of y, d and o. What the other waves need as a B operand,
+// S for K S and Q S, y for T y, d for K^T d and P d, goes through LDS as limbs, already in the operand's
+// register order (an accumulator's lane is the operand's lane: a fragment is 16 bytes per lane, written and
+// read without conflicts). Three barriers a chunk; its operands arrive by asynchronous copies that
+// are issued as soon as the part of LDS is free that they go to, up to a chunk ahead.
+//
+// Against a wave of its own for each 16 columns (no exchange, no barriers, 4 to 8 times fewer
+// waves): the chain of one chunk, not the work, bounds the pass, and one wave took 4.1 us a chunk
+// for it (B2 T16381 H16 K128 V128, 1053 us).
 
 // Workgroups of one (batch, head) differ by the value columns and read the same chunk operands: ids
 // that are equal modulo the 8 XCDs, so that they share an L2.
@@ -438,18 +453,6 @@ __device__ __forceinline__ void place(int id, int BH, int tiles, int& bh, int& t
   }
 }
 
-// Rows (accumulator order) of two adjacent tiles as 8 values of a B operand
-__device__ __forceinline__ void pair8(const f32x4& a, const f32x4& b, float (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-}
-template <int N>
-__device__ __forceinline__ void split_pair(const f32x4& a, const f32x4& b, bf16x8 (&out)[N]) {
-  float x[8];
-  pair8(a, b, x);
-  split<N>(x, out);
-}
-
 template <int U, int N>
 __device__ __forceinline__ void frags(const char* m, int plane, int t, int kb, int lane, bf16x8 (&out)[N]) {
 #pragma unroll
@@ -461,291 +464,489 @@ __device__ __forceinline__ void frags_t(const char* m, int plane, int t, int p, 
   for (int l = 0; l < N; ++l) out[l] = frag_t<U, PERM>(m + l * plane, t, p, lane);
 }
 
-// Limbs of an operand (lane = column, 8 rows per register group) to an image of [columns][rows]
-template <int U, int NW, int N>
-__device__ __forceinline__ void keep(bf16_t* img, int plane, int row, int u, const bf16x8 (&x)[N]) {
+// 4 values (one accumulator) as N limbs of half a fragment
+template <int N>
+__device__ __forceinline__ void split4(const f32x4& x, uint2 (&out)[N]) {
+  uint32_t a[N], b[N];
+  pair_limbs(x[0], x[1], a);
+  pair_limbs(x[2], x[3], b);
 #pragma unroll
-  for (int l = 0; l < NW; ++l) *reinterpret_cast<bf16x8*>(reinterpret_cast<char*>(img) + l * plane + at<U>(row, u)) = x[l];
+  for (int l = 0; l < N; ++l) out[l] = make_uint2(a[l], b[l]);
 }
 
-// What a wave of the passes works on
-template <int KP, int NI, int W>
-struct Place {
-  int lane, wave, m, g, bh, h, b, col;
-  bool in;
-  __device__ __forceinline__ Place(const Args& a, int tiles) {
-    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-    int tile;
-    place(blockIdx.x, a.B * a.H, tiles, bh, tile);
-    h = bh % a.H, b = bh / a.H, col = (tile * W + wave) * 16 + m;
-    in = col < a.V;
-  }
+// B operands in LDS, kFrag bytes per fragment and limb: fragment f of F, limb l at (l F + f) kFrag. The 16 bytes
+// past 1 KiB keep two halves' writes from being one instruction at distances that the compiler can merge: a merged
+// write is no longer known to miss the copies under way, and waits for all of them.
+constexpr int kFrag = 1040;
+template <int F, int N>
+__device__ __forceinline__ void put_half(char* x, int f, int lane, int half, const uint2 (&v)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) *reinterpret_cast<uint2*>(x + (l * F + f) * kFrag + lane * 16 + half * 8) = v[l];
+}
+template <int F, int N>
+__device__ __forceinline__ void put_full(char* x, int f, int lane, const bf16x8 (&v)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) *reinterpret_cast<bf16x8*>(x + (l * F + f) * kFrag + lane * 16) = v[l];
+}
+template <int F, int N>
+__device__ __forceinline__ void get(const char* x, int f, int lane, bf16x8 (&v)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) v[l] = *reinterpret_cast<const bf16x8*>(x + (l * F + f) * kFrag + lane * 16);
+}
+
+// All waves' LDS accesses so far are done, and all but this wave's last N memory operations
+template <int N>
+__device__ __forceinline__ void sync() {
+  if constexpr (N < 0)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// LDS of a pass, in arrays of their own: the compiler then knows that reading one need not wait for the
+// copies under way to the others. NX: fragments and limbs of the exchange besides the state's.
+template <int KP, int NI, int CT, int NX>
+struct Team {
+  using T_ = Tile<KP, NI>;
+  static constexpr int KB = KP / 32, NP = T_::NP;
+  static constexpr int nK = NI * C * KP * 2, nT = 3 * kPlane * 2, nP = NP * kPlane * 2, nS = CT * KB * 3 * kFrag, nX = CT * NX * kFrag;
+  // k and the vectors twice (they are read to the end of a chunk, and at once in the next), where that fits
+  static constexpr bool kDouble = 3 * nK + nT + nP + 2048 + nS + nX <= 160 * 1024;
+  static constexpr int nK1 = kDouble ? nK : 16, nX1 = kDouble ? nX : 16, nG1 = kDouble ? 256 : 4;  // (else not used)
+  static constexpr int cK = nK / 4096, cT = nT / 4096, cP = nP / 4096;        // copies a wave
+  static_assert(kDouble || 2 * nK + nT + nP + 1024 + 64 + nS <= 160 * 1024, "the pass fits in LDS");
 };
 
-// The state (or its gradient) of a head's columns from dense [K][V] fp32, or zero
-template <int KT, typename P>
-__device__ __forceinline__ void load_state(f32x4 (&S)[KT], const float* s, const Args& a, const P& w) {
+// What a wave of a pass works on
+template <int CT>
+struct Place {
+  int lane, w, m, g, bh, h, b, tile;
+  __device__ __forceinline__ explicit Place(const Args& a) {
+    lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+    place(blockIdx.x, a.B * a.H, a.VP / 16 / CT, bh, tile);
+    h = bh % a.H, b = bh / a.H;
+  }
+  __device__ __forceinline__ int col(int i) const { return (tile * CT + i) * 16 + m; }
+};
+
+// This wave's rows of the state (or its gradient), from dense [K][V] fp32, or zero
+template <int CT, typename P>
+__device__ __forceinline__ void load_state(f32x4 (&S)[CT][2], const float* s, const Args& a, const P& p) {
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
+  for (int i = 0; i < CT; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      S[t][r] = s && w.in && row_of(t, 4 * w.g) < a.K  // (K % 8 == 0)
-                    ? s[(static_cast<int64_t>(w.bh) * a.K + row_of(t, 4 * w.g + r)) * a.V + w.col] : 0.0f;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = row_of(2 * p.w + t, 4 * p.g + r);
+        S[i][t][r] = s && p.col(i) < a.V && d < a.K ? s[(static_cast<int64_t>(p.bh) * a.K + d) * a.V + p.col(i)] : 0.0f;
+      }
 }
-template <int KT, typename P>
-__device__ __forceinline__ void store_state(const f32x4 (&S)[KT], float* s, const Args& a, const P& w) {
+template <int CT, typename P>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[CT][2], float* s, const Args& a, const P& p) {
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
+  for (int i = 0; i < CT; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (w.in && row_of(t, 4 * w.g) < a.K) s[(static_cast<int64_t>(w.bh) * a.K + row_of(t, 4 * w.g + r)) * a.V + w.col] = S[t][r];
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = row_of(2 * p.w + t, 4 * p.g + r);
+        if (p.col(i) < a.V && d < a.K) s[(static_cast<int64_t>(p.bh) * a.K + d) * a.V + p.col(i)] = S[i][t][r];
+      }
 }
 
-template <int KP, int NI, bool KEEP, int W>
-__global__ __launch_bounds__(512) void state_kernel(Args a, int tiles) {  // (bounds of 8 waves: no accumulator registers apart)
+// This wave's rows of the state to the other waves and, where kept, to memory: [columns][rows] images
+template <int KP, int NI, int CT, typename P>
+__device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, bf16_t* kept, int64_t c, const Args& a, const P& p) {
+  constexpr int NW = kKept<NI>, U = KP / 8;
+  if (p.w < KP / 32) {
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      const float x[8] = {S[i][0][0], S[i][0][1], S[i][0][2], S[i][0][3], S[i][1][0], S[i][1][1], S[i][1][2], S[i][1][3]};
+      bf16x8 l[3];
+      split<3>(x, l);
+      put_full<CT * (KP / 32)>(xs, i * (KP / 32) + p.w, p.lane, l);
+      if (kept) {
+        char* img = reinterpret_cast<char*>(kept + (c * (a.VP / 32) + p.col(i) / 32) * NW * 32 * KP) + at<U>(p.col(i) % 32, 4 * p.w + p.g);
+#pragma unroll
+        for (int q = 0; q < NW; ++q) *reinterpret_cast<bf16x8*>(img + q * 32 * KP * 2) = l[q];
+      }
+    }
+  }
+}
+// Half a fragment of d or dy to its image
+template <int NI, typename P>
+__device__ __forceinline__ void keep_half(bf16_t* kept, int64_t c, int col, const uint2 (&l)[kKept<NI>], const Args& a, const P& p) {
+  constexpr int NW = kKept<NI>;
+  char* img = reinterpret_cast<char*>(kept + (c * (a.VP / 32) + col / 32) * NW * 32 * C) + at<8>(col % 32, 4 * (p.w / 2) + p.g) + 8 * (p.w & 1);
+#pragma unroll
+  for (int q = 0; q < NW; ++q) *reinterpret_cast<uint2*>(img + q * 32 * C * 2) = l[q];
+}
+
+// Fragments of the exchange besides the state's: y, e^{G_C - G} d, d; and dd, -e^G beta dy, scale e^G do, do
+template <int NI> constexpr int kStateX = 2 * 3 + 2 * 3 + 2 * (NI == 3 ? 3 : 2);
+template <int NI> constexpr int kGradX = 3 * 2 * 3 + 2 * NI;
+
+template <int KP, int NI, bool KEEP, int CT>
+__global__ __launch_bounds__(256) void state_kernel(Args a) {
   using E = typename elem<NI>::type;
-  using L = Tile<KP, NI>;
-  constexpr int KT = KP / 16, KB = KP / 32, NP = L::NP, U = L::U, NW = kKept<NI>;
-  __shared__ __attribute__((aligned(16))) char lds[L::kStages * L::kBytes];
-  const Place<KP, NI, W> w(a, tiles);
-  const int lane = w.lane, g = w.g;
+  using I = Tile<KP, NI>;
+  using L = Team<KP, NI, CT, kStateX<NI>>;
+  constexpr int KB = KP / 32, NP = L::NP, U = KP / 8, NW = kKept<NI>;
+  __shared__ __attribute__((aligned(16))) char lk0[L::nK], lk1[L::nK1], lq[L::nK], lt[L::nT], lp[L::nP], ls[L::nS], lx[L::nX1];
+  __shared__ __attribute__((aligned(16))) float lg0[256], lg1[L::nG1];
+  const Place<CT> p(a);
+  const int lane = p.lane, g = p.g, w = p.w, pw = w / 2;
+  // (without room of its own the exchange lies over q, which is read before it)
+  char *xs = ls, *xy = L::kDouble ? lx : lq, *xe = xy + CT * 6 * kFrag, *xd = xe + CT * 6 * kFrag;
   const int64_t o_st = static_cast<int64_t>(a.H) * a.V;
-  const E* v = reinterpret_cast<const E*>(a.v) + w.b * a.v_sb + w.h * a.v_sh;
-  E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(w.b) * a.T * a.H + w.h) * a.V;
+  const E* v = reinterpret_cast<const E*>(a.v) + p.b * a.v_sb + p.h * a.v_sh;
+  E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
   const uint32_t vs = static_cast<uint32_t>(a.v_st * sizeof(E)), os = static_cast<uint32_t>(o_st * sizeof(E));
-  const uint32_t v_off = w.in ? 8 * g * vs + w.col * sizeof(E) : kOutOfRange, o_off = w.in ? 8 * g * os + w.col * sizeof(E) : kOutOfRange;
-  const char* img = a.img + static_cast<int64_t>(w.bh) * a.NC * L::kBytes;
+  const int row = row_of(w, 4 * g);  // the lane's first of four tokens
+  const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * I::kBytes;
+  const auto image = [&](int n) { return img + static_cast<int64_t>(n) * I::kBytes; };
 
-  // v of a chunk, loaded one chunk ahead, and before the copy of its operands: loads come back in order
-  uint32_t next[4][4];
+  uint32_t next[CT][4];  // v of a chunk, loaded one chunk ahead
   const auto load_v = [&](int n) {
     const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < CT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) next[t][r] = load_col<E>(vr, v_off, row_of(t, r) * vs);
+      for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(vr, p.col(i) < a.V ? row * vs + p.col(i) * sizeof(E) : kOutOfRange, r * vs);
   };
-  f32x4 S[KT];
-  load_state(S, a.h0, a, w);
-  stage<L::kBytes, W>(lds, img, lane, w.wave);
+  f32x4 S[CT][2];
+  load_state(S, a.h0, a, p);
   load_v(0);
-  for (int n = 0; n < a.NC; ++n) {
-    char* cur = lds + (L::kStages == 2 ? (n & 1) * L::kBytes : 0);
-    const int t0 = n * C, rows = min(C, a.T - t0);
-    const int64_t c = static_cast<int64_t>(w.bh) * a.NC + n;
-    f32x4 vv[4];
+  stage<L::nK, 4>(lk0, image(0) + I::kK, lane, w);
+  stage<L::nK, 4>(lq, image(0) + I::kQ, lane, w);
+  stage<L::nT, 4>(lt, image(0) + I::kT, lane, w);
+  stage<1024, 1>(reinterpret_cast<char*>(lg0), image(0) + I::kGate, lane, 0);
+  if constexpr (!L::kDouble) stage<L::nP, 4>(lp, image(0) + I::kP, lane, w);
+  publish<KP, NI>(S, xs, KEEP ? a.Sw : nullptr, static_cast<int64_t>(p.bh) * a.NC, a, p);
+  sync<0>();
+  // What a wave issues for certain after T's copies and before the next barrier: o's stores, kept d's, the state's
+  // (which not all waves have when KB < 4). A wait leaves the operations of the segments since in flight.
+  constexpr int kLater = 4 * CT + (KEEP ? NW * CT : 0);
+  const auto chunk = [&](int n, char* ck, char* nk, float* gt, float* ng) __attribute__((always_inline)) {
+    const int t0 = n * C, rows = min(C, a.T - t0), n1 = min(n + 1, a.NC - 1);  // (the last chunk's copies bring it once more)
+    const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
+    f32x4 vv[CT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < CT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) vv[t][r] = value<E>(next[t][r]);
-    bf16x8 sb[KB][3];
+      for (int r = 0; r < 4; ++r) vv[i][r] = value<E>(next[i][r]);
+    load_v(n1);
+    if constexpr (L::kDouble) {
+      stage<1024, 1>(reinterpret_cast<char*>(ng), image(n1) + I::kGate, lane, 0);
+      stage<L::nK, 4>(nk, image(n1) + I::kK, lane, w);
+      stage<L::nP, 4>(lp, image(n) + I::kP, lane, w);
+    }
+    const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
+    const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row);
+    const float last = gt[63];
+    // y and the state's part of o: this wave's 16 tokens
+    f32x4 ks[CT], oa[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) ks[i] = oa[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      split_pair<3>(S[2 * kb], S[2 * kb + 1], sb[kb]);
-      if constexpr (KEEP)
-        keep<U, NW>(a.Sw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * KP, 32 * KP * 2, w.col % 32, 4 * kb + g, sb[kb]);
-    }
-    staged();
-    if (n + 1 < a.NC) load_v(n + 1);
-    if constexpr (L::kStages == 2)
-      if (n + 1 < a.NC) stage<L::kBytes, W>(lds + ((n + 1) & 1) * L::kBytes, img + static_cast<int64_t>(n + 1) * L::kBytes, lane, w.wave);
-    const float* gt = reinterpret_cast<const float*>(cur + L::kGate);
-    f32x4 y[4], oa[4];
+      bf16x8 fk[NI], fq[NI];
+      frags<U>(ck, C * KP * 2, w, kb, lane, fk);
+      frags<U>(lq, C * KP * 2, w, kb, lane, fq);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        bf16x8 x[NI];
-        frags<U>(cur + L::kK, C * KP * 2, t, kb, lane, x);
-        ks = mm<3>(x, sb[kb], ks);
-        frags<U>(cur + L::kQ, C * KP * 2, t, kb, lane, x);
-        qs = mm<NP>(x, sb[kb], qs);  // only o, which is rounded to the inputs' type, sees this product
-      }
-      const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row_of(t, 4 * g));
-      const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row_of(t, 4 * g));
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        y[t][r] = be[r] * (vv[t][r] - eg[r] * ks[r]);
-        oa[t][r] = a.scale * eg[r] * qs[r];
+      for (int i = 0; i < CT; ++i) {
+        bf16x8 sb[3];
+        get<CT * KB>(xs, i * KB + kb, lane, sb);
+        ks[i] = mm<3>(fk, sb, ks[i]);
+        oa[i] = mm<NP>(fq, sb, oa[i]);  // (only o, which is rounded to the inputs' type, sees this product)
       }
     }
-    bf16x8 yb[2][3];
+    if constexpr (!L::kDouble) sync<-1>();  // (the exchange lies over q)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) split_pair<3>(y[2 * p], y[2 * p + 1], yb[p]);
-    f32x4 d[4], e[4];
+    for (int i = 0; i < CT; ++i) {
+      uint2 l[3];
+      split4(be * (vv[i] - eg * ks[i]), l);
+      put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
+      oa[i] *= a.scale * eg;
+    }
+    sync<L::kDouble ? 4 * CT + 1 + L::cK + L::cP : -1>();  // y is there, and T
+    if constexpr (L::kDouble) stage<L::nK, 4>(lq, image(n1) + I::kQ, lane, w);
+    f32x4 d[CT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      d[t] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < CT; ++i) d[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int p = 0; p <= t / 2; ++p) {
-        bf16x8 x[3];
-        frags<8>(cur + L::kT, kPlane * 2, t, p, lane, x);
-        d[t] = mm<3>(x, yb[p], d[t]);
+    for (int q = 0; q < 2; ++q) {
+      if (q <= pw) {
+        bf16x8 ft[3];
+        frags<8>(lt, kPlane * 2, w, q, lane, ft);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 yb[3];
+          get<2 * CT>(xy, 2 * i + q, lane, yb);
+          d[i] = mm<3>(ft, yb, d[i]);
+        }
       }
-      const f32x4 tail = *reinterpret_cast<const f32x4*>(gt + 64 + row_of(t, 4 * g));
-#pragma unroll
-      for (int r = 0; r < 4; ++r) e[t][r] = tail[r] * d[t][r];
     }
-    bf16x8 db[2][NP], eb[2][3];
+    uint2 dl[CT][NP];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      split_pair<NP>(d[2 * p], d[2 * p + 1], db[p]);
-      split_pair<3>(e[2 * p], e[2 * p + 1], eb[p]);
-      if constexpr (KEEP)
-        keep<8, NW>(a.dw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * C, 32 * C * 2, w.col % 32, 4 * p + g, db[p]);
+    for (int i = 0; i < CT; ++i) {
+      uint2 l[3];
+      split4(tail * d[i], l);
+      put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
+      split4(d[i], dl[i]);
+      put_half<2 * CT>(xd, 2 * i + pw, lane, w & 1, dl[i]);
     }
-    const float last = gt[63];
+    sync<L::kDouble ? L::cK : -1>();  // d is there, and P
+    if constexpr (L::kDouble) stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      S[t] *= last;
+      for (int i = 0; i < CT; ++i) keep_half<NI>(a.dw, c, p.col(i), dl[i], a, p);
+    }
+    if (w < KB) {
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        bf16x8 x[NI];
-        frags_t<U, true>(cur + L::kK, C * KP * 2, t, p, lane, x);
-        S[t] = mm<3>(x, eb[p], S[t]);
+      for (int i = 0; i < CT; ++i) S[i][0] *= last, S[i][1] *= last;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        bf16x8 f0[NI], f1[NI];
+        frags_t<U, true>(ck, C * KP * 2, 2 * w, q, lane, f0);
+        frags_t<U, true>(ck, C * KP * 2, 2 * w + 1, q, lane, f1);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 eb[3];
+          get<2 * CT>(xe, 2 * i + q, lane, eb);
+          S[i][0] = mm<3>(f0, eb, S[i][0]);
+          S[i][1] = mm<3>(f1, eb, S[i][1]);
+        }
+      }
+    }
+    publish<KP, NI>(S, xs, KEEP && n + 1 < a.NC ? a.Sw : nullptr, c + 1, a, p);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (q <= pw) {
+        bf16x8 fp[NP];
+        frags<8>(lp, kPlane * 2, w, q, lane, fp);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 db[NP];
+          get<2 * CT>(xd, 2 * i + q, lane, db);
+          oa[i] = mm<NP>(fp, db, oa[i]);
+        }
       }
     }
     const __amdgpu_buffer_rsrc_t orr = rows_buffer(o + t0 * o_st, o_st, rows, a.V);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int i = 0; i < CT; ++i)
 #pragma unroll
-      for (int p = 0; p <= t / 2; ++p) {
-        bf16x8 x[NP];
-        frags<8>(cur + L::kP, kPlane * 2, t, p, lane, x);
-        oa[t] = mm<NP>(x, db[p], oa[t]);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) store_col<E>(orr, o_off, row_of(t, r) * os, oa[t][r]);
+      for (int r = 0; r < 4; ++r)
+        store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, oa[i][r]);
+    if constexpr (L::kDouble) {
+      sync<L::cT + kLater>();  // the state is there, and k, q and the vectors
+    } else {
+      sync<-1>();
+      stage<1024, 1>(reinterpret_cast<char*>(gt), image(n1) + I::kGate, lane, 0);
+      stage<L::nK, 4>(ck, image(n1) + I::kK, lane, w);
+      stage<L::nK, 4>(lq, image(n1) + I::kQ, lane, w);
+      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+      stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
+      sync<0>();
     }
-    if constexpr (L::kStages == 1) {
-      __syncthreads();
-      if (n + 1 < a.NC) stage<L::kBytes, W>(lds, img + static_cast<int64_t>(n + 1) * L::kBytes, lane, w.wave);
-    }
+  };
+  for (int n = 0;;) {
+    chunk(n, lk0, L::kDouble ? lk1 : lk0, lg0, L::kDouble ? lg1 : lg0);
+    if (++n >= a.NC) break;
+    chunk(n, L::kDouble ? lk1 : lk0, lk0, L::kDouble ? lg1 : lg0, lg0);
+    if (++n >= a.NC) break;
   }
-  if (a.state) store_state(S, a.state, a, w);
+  if (a.state && w < KB) store_state(S, a.state, a, p);
 }
 
-template <int KP, int NI, int W>
-__global__ __launch_bounds__(512) void dstate_kernel(Args a, int tiles) {
+template <int KP, int NI, int CT>
+__global__ __launch_bounds__(256) void dstate_kernel(Args a) {
   using E = typename elem<NI>::type;
-  using L = Tile<KP, NI>;
-  constexpr int KT = KP / 16, KB = KP / 32, NP = L::NP, U = L::U, NW = kKept<NI>;
-  __shared__ __attribute__((aligned(16))) char lds[L::kStages * L::kBytes];
-  const Place<KP, NI, W> w(a, tiles);
-  const int lane = w.lane, g = w.g;
+  using I = Tile<KP, NI>;
+  using L = Team<KP, NI, CT, kGradX<NI>>;
+  constexpr int KB = KP / 32, NP = L::NP, U = KP / 8, NW = kKept<NI>;
+  __shared__ __attribute__((aligned(16))) char lk0[L::nK], lk1[L::nK1], lq[L::nK], lt[L::nT], lp[L::nP], ls[L::nS], lx[L::nX1];
+  __shared__ __attribute__((aligned(16))) float lg0[256], lg1[L::nG1];
+  const Place<CT> p(a);
+  const int lane = p.lane, g = p.g, w = p.w, pw = w / 2;
+  // without room of its own the exchange lies over P, which is read before it, and do's over q, which comes after it
+  char *xs = ls, *xy = L::kDouble ? lx : lp, *xe = xy + CT * 6 * kFrag, *xu = xe + CT * 6 * kFrag;
+  char* xo = L::kDouble ? xu + CT * 6 * kFrag : lq;
   const int64_t v_st = static_cast<int64_t>(a.H) * a.V;
-  const E* dout = reinterpret_cast<const E*>(a.dout) + w.b * a.do_sb + w.h * a.do_sh;
-  E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(w.b) * a.T * a.H + w.h) * a.V;
+  const E* dout = reinterpret_cast<const E*>(a.dout) + p.b * a.do_sb + p.h * a.do_sh;
+  E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
   const uint32_t is = static_cast<uint32_t>(a.do_st * sizeof(E)), os = static_cast<uint32_t>(v_st * sizeof(E));
-  const uint32_t i_off = w.in ? 8 * g * is + w.col * sizeof(E) : kOutOfRange, o_off = w.in ? 8 * g * os + w.col * sizeof(E) : kOutOfRange;
-  const char* img = a.img + static_cast<int64_t>(w.bh) * a.NC * L::kBytes;
+  const int row = row_of(w, 4 * g);
+  const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * I::kBytes;
+  const auto image = [&](int n) { return img + static_cast<int64_t>(n) * I::kBytes; };
 
-  uint32_t next[4][4];
+  uint32_t next[CT][4];  // do of a chunk, loaded one chunk ahead
+  f32x4 go[CT];
   const auto load_go = [&](int n) {
     const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < CT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) next[t][r] = load_col<E>(ir, i_off, row_of(t, r) * is);
+      for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(ir, p.col(i) < a.V ? row * is + p.col(i) * sizeof(E) : kOutOfRange, r * is);
   };
-  f32x4 S[KT];  // the gradient of the state
-  load_state(S, a.dstate, a, w);
-  load_go(a.NC - 1);
-  stage<L::kBytes, W>(lds + (L::kStages == 2 ? ((a.NC - 1) & 1) * L::kBytes : 0), img + static_cast<int64_t>(a.NC - 1) * L::kBytes, lane, w.wave);
-  for (int n = a.NC - 1; n >= 0; --n) {
-    char* cur = lds + (L::kStages == 2 ? (n & 1) * L::kBytes : 0);
-    const int t0 = n * C, rows = min(C, a.T - t0);
-    const int64_t c = static_cast<int64_t>(w.bh) * a.NC + n;
-    f32x4 go[4];
+  const auto put_go = [&]() {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < CT; ++i) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) go[t][r] = value<E>(next[t][r]);
-    bf16x8 sb[KB][3], gb[2][NI];
+      for (int r = 0; r < 4; ++r) go[i][r] = value<E>(next[i][r]);
+      uint2 l[NI];
+      split4(go[i], l);
+      put_half<2 * CT>(xo, 2 * i + pw, lane, w & 1, l);
+    }
+  };
+  f32x4 S[CT][2];  // the gradient of the state
+  load_state(S, a.dstate, a, p);
+  const int last_n = a.NC - 1;
+  load_go(last_n);
+  stage<L::nK, 4>(lk0, image(last_n) + I::kK, lane, w);
+  stage<1024, 1>(reinterpret_cast<char*>(lg0), image(last_n) + I::kGate, lane, 0);
+  stage<L::nT, 4>(lt, image(last_n) + I::kT, lane, w);
+  stage<L::nP, 4>(lp, image(last_n) + I::kP, lane, w);
+  put_go();
+  publish<KP, NI>(S, xs, a.dSw, static_cast<int64_t>(p.bh) * a.NC + last_n, a, p);
+  sync<0>();
+  const auto chunk = [&](int n, char* ck, char* nk, float* gt, float* ng) __attribute__((always_inline)) {
+    const int t0 = n * C, rows = min(C, a.T - t0), n1 = max(n - 1, 0);  // (the last chunk's copies bring it once more)
+    const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
+    load_go(n1);
+    if constexpr (L::kDouble) {
+      stage<1024, 1>(reinterpret_cast<char*>(ng), image(n1) + I::kGate, lane, 0);
+      stage<L::nK, 4>(nk, image(n1) + I::kK, lane, w);
+      stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
+    }
+    const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
+    const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row);
+    const float last = gt[63];
+    f32x4 dd[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) dd[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      split_pair<3>(S[2 * kb], S[2 * kb + 1], sb[kb]);
-      keep<U, NW>(a.dSw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * KP, 32 * KP * 2, w.col % 32, 4 * kb + g, sb[kb]);
-    }
-    staged();
-    if (n > 0) load_go(n - 1);
-    if constexpr (L::kStages == 2)
-      if (n > 0) stage<L::kBytes, W>(lds + ((n - 1) & 1) * L::kBytes, img + static_cast<int64_t>(n - 1) * L::kBytes, lane, w.wave);
+      bf16x8 f[NI];
+      frags<U>(ck, C * KP * 2, w, kb, lane, f);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) split_pair<NI>(go[2 * p], go[2 * p + 1], gb[p]);
-    const float* gt = reinterpret_cast<const float*>(cur + L::kGate);
-    f32x4 dd[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        bf16x8 f[NI];
-        frags<U>(cur + L::kK, C * KP * 2, t, kb, lane, f);
-        x = mm<3>(f, sb[kb], x);
+      for (int i = 0; i < CT; ++i) {
+        bf16x8 sb[3];
+        get<CT * KB>(xs, i * KB + kb, lane, sb);
+        dd[i] = mm<3>(f, sb, dd[i]);
       }
-      x *= *reinterpret_cast<const f32x4*>(gt + 64 + row_of(t, 4 * g));
+    }
 #pragma unroll
-      for (int p = t / 2; p < 2; ++p) {
+    for (int i = 0; i < CT; ++i) dd[i] *= tail;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (q >= pw) {
         bf16x8 f[NP];
-        frags_t<8, true>(cur + L::kP, kPlane * 2, t, p, lane, f);
-        x = mm<3>(f, gb[p], x);
-      }
-      dd[t] = x;
-    }
-    bf16x8 ddb[2][3], xb[2][3], wb[2][3], yb[2][NW];
+        frags_t<8, true>(lp, kPlane * 2, w, q, lane, f);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) split_pair<3>(dd[2 * p], dd[2 * p + 1], ddb[p]);
-    f32x4 dy[4], x[4], u[4];
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 ob[NI];
+          get<2 * CT>(xo, 2 * i + q, lane, ob);
+          dd[i] = mm<3>(f, ob, dd[i]);
+        }
+      }
+    }
+    if constexpr (!L::kDouble) sync<-1>();
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      uint2 l[3];
+      split4(dd[i], l);
+      put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
+    }
+    sync<L::kDouble ? 4 * CT + 1 + 2 * L::cK : -1>();  // dd is there, and T
+    if constexpr (L::kDouble)
+      stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
+    else
+      stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
+    f32x4 dy[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) dy[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (q >= pw) {
+        bf16x8 f[3];
+        frags_t<8, true>(lt, kPlane * 2, w, q, lane, f);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 b[3];
+          get<2 * CT>(xy, 2 * i + q, lane, b);
+          dy[i] = mm<3>(f, b, dy[i]);
+        }
+      }
+    }
     const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      dy[t] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < CT; ++i) {
+      const f32x4 x = be * dy[i];
 #pragma unroll
-      for (int p = t / 2; p < 2; ++p) {
-        bf16x8 f[3];
-        frags_t<8, true>(cur + L::kT, kPlane * 2, t, p, lane, f);
-        dy[t] = mm<3>(f, ddb[p], dy[t]);
+      for (int r = 0; r < 4; ++r)
+        store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, x[r]);
+      uint2 l[3];
+      split4(-eg * x, l);
+      put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
+      split4(a.scale * eg * go[i], l);
+      put_half<2 * CT>(xu, 2 * i + pw, lane, w & 1, l);
+    }
+    sync<L::kDouble ? L::cP + 4 * CT : 0>();  // they are there, and q
+    if constexpr (L::kDouble) stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      uint2 l[NW];
+      split4(dy[i], l);
+      keep_half<NI>(a.yw, c, p.col(i), l, a, p);
+    }
+    if (w < KB) {
+#pragma unroll
+      for (int i = 0; i < CT; ++i) S[i][0] *= last, S[i][1] *= last;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        bf16x8 k0[NI], k1[NI], q0[NI], q1[NI];
+        frags_t<U, true>(ck, C * KP * 2, 2 * w, q, lane, k0);
+        frags_t<U, true>(ck, C * KP * 2, 2 * w + 1, q, lane, k1);
+        frags_t<U, true>(lq, C * KP * 2, 2 * w, q, lane, q0);
+        frags_t<U, true>(lq, C * KP * 2, 2 * w + 1, q, lane, q1);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 b[3];
+          get<2 * CT>(xe, 2 * i + q, lane, b);
+          S[i][0] = mm<3>(k0, b, S[i][0]);
+          S[i][1] = mm<3>(k1, b, S[i][1]);
+          get<2 * CT>(xu, 2 * i + q, lane, b);
+          S[i][0] = mm<3>(q0, b, S[i][0]);
+          S[i][1] = mm<3>(q1, b, S[i][1]);
+        }
       }
-      const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row_of(t, 4 * g));
-      const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row_of(t, 4 * g));
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float dvv = be[r] * dy[t][r];
-        store_col<E>(orr, o_off, row_of(t, r) * os, dvv);
-        x[t][r] = -eg[r] * dvv;
-        u[t][r] = a.scale * eg[r] * go[t][r];
-      }
     }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      split_pair<3>(x[2 * p], x[2 * p + 1], xb[p]);
-      split_pair<3>(u[2 * p], u[2 * p + 1], wb[p]);
-      split_pair<NW>(dy[2 * p], dy[2 * p + 1], yb[p]);
-      keep<8, NW>(a.yw + (c * (a.VP / 32) + w.col / 32) * NW * 32 * C, 32 * C * 2, w.col % 32, 4 * p + g, yb[p]);
+    if constexpr (L::kDouble) {
+      put_go();
+      publish<KP, NI>(S, xs, n > 0 ? a.dSw : nullptr, c - 1, a, p);
+      sync<L::cT + NW * CT>();  // the state and do are there, and k, P and the vectors
+    } else {
+      sync<-1>();
+      stage<L::nK, 4>(ck, image(n1) + I::kK, lane, w);
+      stage<1024, 1>(reinterpret_cast<char*>(gt), image(n1) + I::kGate, lane, 0);
+      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+      stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
+      put_go();
+      publish<KP, NI>(S, xs, n > 0 ? a.dSw : nullptr, c - 1, a, p);
+      sync<0>();
     }
-    const float last = gt[63];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      S[t] *= last;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        bf16x8 f[NI];
-        frags_t<U, true>(cur + L::kK, C * KP * 2, t, p, lane, f);
-        S[t] = mm<3>(f, xb[p], S[t]);
-        frags_t<U, true>(cur + L::kQ, C * KP * 2, t, p, lane, f);
-        S[t] = mm<3>(f, wb[p], S[t]);
-      }
-    }
-    if constexpr (L::kStages == 1) {
-      __syncthreads();
-      if (n > 0) stage<L::kBytes, W>(lds, img + static_cast<int64_t>(n - 1) * L::kBytes, lane, w.wave);
-    }
+  };
+  for (int n = last_n;;) {
+    chunk(n, lk0, L::kDouble ? lk1 : lk0, lg0, L::kDouble ? lg1 : lg0);
+    if (--n < 0) break;
+    chunk(n, L::kDouble ? lk1 : lk0, lk0, L::kDouble ? lg1 : lg0, lg0);
+    if (--n < 0) break;
   }
-  if (a.dh0) store_state(S, a.dh0, a, w);
+  if (a.dh0 && w < KB) store_state(S, a.dh0, a, p);
 }
-
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
 
 template <int KP, int NI>
@@ -1116,13 +1317,10 @@ inline int check_rows(const char* fn, const char* name, int dtype, const mg_rows
   return MG_OK;
 }
 
-// Waves per workgroup of the passes over the chunks: a workgroup takes a CU's LDS, so as few waves
-// as spread the value columns over all CUs.
-inline int waves_for(int64_t bh, int vp) {
-  const int tiles = vp / 16;
-  int w = 2;
-  while (w < 8 && tiles % (2 * w) == 0 && bh * (tiles / w) > kCUs) w *= 2;
-  return w;
+// Value columns per workgroup of the passes over the chunks, in tiles of 16: two where that still leaves
+// a workgroup for every CU (the chunk's operands are then read for twice the columns), else one. fp32 has LDS for one.
+inline int columns_for(int64_t bh, int vp, int dtype_limbs) {
+  return dtype_limbs == 1 && bh * (vp / 32) >= kCUs ? 2 : 1;
 }
 
 inline void fill(Args& a, const mg_delta_dims& s, float scale, const mg_rows* q, const mg_rows* k, const mg_rows* v,
@@ -1142,15 +1340,21 @@ template <int KP, int NI>
 int launch_fwd(const Args& a, bool keep_, hipStream_t st_) {
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
   hipLaunchKernelGGL((chunk_kernel<KP, NI>), dim3(bh * a.NC), dim3(256), 0, st_, a);
-  const int w = waves_for(bh, a.VP), tiles = a.VP / 16 / w;
-  const dim3 grid(bh * tiles), block(64 * w);
-#define GO(W)                                                                                         \
-  if (keep_)                                                                                          \
-    hipLaunchKernelGGL((state_kernel<KP, NI, true, W>), grid, block, 0, st_, a, tiles);               \
-  else                                                                                                \
-    hipLaunchKernelGGL((state_kernel<KP, NI, false, W>), grid, block, 0, st_, a, tiles);
-  if (w == 8) { GO(8) } else if (w == 4) { GO(4) } else { GO(2) }
-#undef GO
+  const int ct = columns_for(bh, a.VP, NI);
+  const dim3 grid(bh * (a.VP / 16 / ct));
+  if constexpr (NI == 1) {
+    if (ct == 2) {
+      if (keep_)
+        hipLaunchKernelGGL((state_kernel<KP, NI, true, 2>), grid, dim3(256), 0, st_, a);
+      else
+        hipLaunchKernelGGL((state_kernel<KP, NI, false, 2>), grid, dim3(256), 0, st_, a);
+      return check_launch("mg_delta_fwd");
+    }
+  }
+  if (keep_)
+    hipLaunchKernelGGL((state_kernel<KP, NI, true, 1>), grid, dim3(256), 0, st_, a);
+  else
+    hipLaunchKernelGGL((state_kernel<KP, NI, false, 1>), grid, dim3(256), 0, st_, a);
   return check_launch("mg_delta_fwd");
 }
 
@@ -1158,14 +1362,12 @@ template <int KP, int NI>
 int launch_bwd(const Args& a, hipStream_t st_) {
   using E = typename elem<NI>::type;
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
-  const int w = waves_for(bh, a.VP), tiles = a.VP / 16 / w;
-  const dim3 grid(bh * tiles), block(64 * w);
-  if (w == 8)
-    hipLaunchKernelGGL((dstate_kernel<KP, NI, 8>), grid, block, 0, st_, a, tiles);
-  else if (w == 4)
-    hipLaunchKernelGGL((dstate_kernel<KP, NI, 4>), grid, block, 0, st_, a, tiles);
-  else
-    hipLaunchKernelGGL((dstate_kernel<KP, NI, 2>), grid, block, 0, st_, a, tiles);
+  const int ct = columns_for(bh, a.VP, NI);
+  const dim3 grid(bh * (a.VP / 16 / ct));
+  if constexpr (NI == 1) {
+    if (ct == 2) hipLaunchKernelGGL((dstate_kernel<KP, NI, 2>), grid, dim3(256), 0, st_, a);
+  }
+  if (ct == 1) hipLaunchKernelGGL((dstate_kernel<KP, NI, 1>), grid, dim3(256), 0, st_, a);
   hipLaunchKernelGGL((grad_kernel<KP, NI>), dim3(bh * a.NC), dim3(64 * GradTile<KP, NI>::W), 0, st_, a);
   if (a.H > a.Hk) {
     const int64_t n = static_cast<int64_t>(a.B) * a.T * a.Hk * a.K;
