@@ -625,9 +625,9 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
   if constexpr (!L::kDouble) stage<L::nP, 4>(lp, image(0) + I::kP, lane, w);
   publish<KP, NI>(S, xs, KEEP ? a.Sw : nullptr, static_cast<int64_t>(p.bh) * a.NC, a, p);
   sync<0>();
-  // What a wave issues for certain after T's copies and before the next barrier: o's stores, kept d's, the state's
-  // (which not all waves have when KB < 4). A wait leaves the operations of the segments since in flight.
-  constexpr int kLater = 4 * CT + (KEEP ? NW * CT : 0);
+  // Memory operations complete in order, and a wait leaves those in flight that were issued after the copies it is for.
+  // What every wave issues after T's copies to the chunk's end: kept d's, the state's (if all waves have some), o's stores
+  constexpr int kLater = 4 * CT + (KEEP ? NW * CT * (KB == 4 ? 2 : 1) : 0);
   const auto chunk = [&](int n, char* ck, char* nk, float* gt, float* ng) __attribute__((always_inline)) {
     const int t0 = n * C, rows = min(C, a.T - t0), n1 = min(n + 1, a.NC - 1);  // (the last chunk's copies bring it once more)
     const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
@@ -636,11 +636,14 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
     for (int i = 0; i < CT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) vv[i][r] = value<E>(next[i][r]);
+    if constexpr (L::kDouble) {
+      stage<L::nP, 4>(lp, image(n) + I::kP, lane, w);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     load_v(n1);
     if constexpr (L::kDouble) {
       stage<1024, 1>(reinterpret_cast<char*>(ng), image(n1) + I::kGate, lane, 0);
       stage<L::nK, 4>(nk, image(n1) + I::kK, lane, w);
-      stage<L::nP, 4>(lp, image(n) + I::kP, lane, w);
     }
     const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
     const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row);
@@ -670,7 +673,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
       put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
       oa[i] *= a.scale * eg;
     }
-    sync<L::kDouble ? 4 * CT + 1 + L::cK + L::cP : -1>();  // y is there, and T
+    sync<L::kDouble ? kLater + L::cP + 4 * CT + 1 + L::cK : -1>();  // y is there, and T
     if constexpr (L::kDouble) stage<L::nK, 4>(lq, image(n1) + I::kQ, lane, w);
     f32x4 d[CT];
 #pragma unroll
@@ -697,8 +700,11 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
       split4(d[i], dl[i]);
       put_half<2 * CT>(xd, 2 * i + pw, lane, w & 1, dl[i]);
     }
-    sync<L::kDouble ? L::cK : -1>();  // d is there, and P
-    if constexpr (L::kDouble) stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+    sync<L::kDouble ? 4 * CT + 1 + 2 * L::cK : -1>();  // d is there, and P
+    if constexpr (L::kDouble) {
+      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (KEEP) {
 #pragma unroll
       for (int i = 0; i < CT; ++i) keep_half<NI>(a.dw, c, p.col(i), dl[i], a, p);
@@ -812,14 +818,18 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
   put_go();
   publish<KP, NI>(S, xs, a.dSw, static_cast<int64_t>(p.bh) * a.NC + last_n, a, p);
   sync<0>();
+  constexpr int kLater = NW * CT * (KB == 4 ? 2 : 1);  // after T's copies to the chunk's end: kept dy's, the state's
   const auto chunk = [&](int n, char* ck, char* nk, float* gt, float* ng) __attribute__((always_inline)) {
     const int t0 = n * C, rows = min(C, a.T - t0), n1 = max(n - 1, 0);  // (the last chunk's copies bring it once more)
     const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
+    if constexpr (L::kDouble) {
+      stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     load_go(n1);
     if constexpr (L::kDouble) {
       stage<1024, 1>(reinterpret_cast<char*>(ng), image(n1) + I::kGate, lane, 0);
       stage<L::nK, 4>(nk, image(n1) + I::kK, lane, w);
-      stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
     }
     const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
     const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row);
@@ -860,10 +870,11 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
       split4(dd[i], l);
       put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
     }
-    sync<L::kDouble ? 4 * CT + 1 + 2 * L::cK : -1>();  // dd is there, and T
-    if constexpr (L::kDouble)
+    sync<L::kDouble ? kLater + 4 * CT + 1 + 2 * L::cK : -1>();  // dd is there, and T
+    if constexpr (L::kDouble) {
       stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
-    else
+      __builtin_amdgcn_sched_barrier(0);
+    } else
       stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
     f32x4 dy[CT];
 #pragma unroll
@@ -894,8 +905,11 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
       split4(a.scale * eg * go[i], l);
       put_half<2 * CT>(xu, 2 * i + pw, lane, w & 1, l);
     }
-    sync<L::kDouble ? L::cP + 4 * CT : 0>();  // they are there, and q
-    if constexpr (L::kDouble) stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+    sync<L::kDouble ? 4 * CT + 1 + L::cK + L::cP + 4 * CT : 0>();  // they are there, and q
+    if constexpr (L::kDouble) {
+      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
       uint2 l[NW];
@@ -927,7 +941,7 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
     if constexpr (L::kDouble) {
       put_go();
       publish<KP, NI>(S, xs, n > 0 ? a.dSw : nullptr, c - 1, a, p);
-      sync<L::cT + NW * CT>();  // the state and do are there, and k, P and the vectors
+      sync<4 * CT + L::cT + kLater>();  // the state and do are there, and k, P and the vectors
     } else {
       sync<-1>();
       stage<L::nK, 4>(ck, image(n1) + I::kK, lane, w);
