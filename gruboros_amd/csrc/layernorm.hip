@@ -8,7 +8,7 @@
 //   dxn = r (g - mean(g) - h mean(g h)) + dres,  ddelta = keep(delta) dxn / (1 - p)
 //   dw  = sum over rows of dy h,  db = sum over rows of dy
 //
-// A row belongs to one wave up to 2048 columns (16 bytes of fp32 per lane and
+// A row belongs to one wave up to 1024 columns (16 bytes of fp32 per lane and
 // step), else to a workgroup of 256 threads, and stays in registers between its passes: the
 // variance is that of the centred values, not a difference of two sums. Any D:
 // the loads are 16 bytes wide at whatever alignment the rows have (the memory
@@ -24,6 +24,9 @@ namespace mg {
 namespace layernorm {
 
 constexpr int kThreads = 256;
+
+template <int N>
+struct int_c { static constexpr int value = N; };
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -78,19 +81,38 @@ __device__ __forceinline__ void store4(bf16_t* p, const f4& v, int left) {
   }
 }
 
+// The sum over a wave's lanes, in every lane: within rows of 16 lanes by cross-lane operands, then
+// from row to row, where the last lane has the whole
+__device__ __forceinline__ float wave_sum(float x) {
+  const auto add = [](float x, auto ctrl, auto rows) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  x = add(x, int_c<0xb1>{}, int_c<0xf>{});   // lane ^ 1
+  x = add(x, int_c<0x4e>{}, int_c<0xf>{});   // lane ^ 2
+  x = add(x, int_c<0x141>{}, int_c<0xf>{});  // mirrored in 8
+  x = add(x, int_c<0x140>{}, int_c<0xf>{});  // mirrored in 16
+  x = add(x, int_c<0x142>{}, int_c<0xa>{});  // row 0 into 1, 2 into 3
+  x = add(x, int_c<0x143>{}, int_c<0xc>{});  // the lower half into the upper
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
 // The sums of (a, b) over the threads of a row; every thread gets them
 template <int TPR>
 __device__ __forceinline__ void row_sum(float& a, float& b, float2* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o, 64), b += __shfl_xor(b, o, 64);
+  a = wave_sum(a), b = wave_sum(b);
   if constexpr (TPR > 64) {
-    const int wave = threadIdx.x / 64;
     __syncthreads();
-    if (threadIdx.x % 64 == 0) red[wave] = make_float2(a, b);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = make_float2(a, b);
     __syncthreads();
     a = (red[0].x + red[1].x) + (red[2].x + red[3].x);
     b = (red[0].y + red[1].y) + (red[2].y + red[3].y);
   }
+}
+
+// The first row of this wave (of this workgroup, where a row has more waves than one)
+template <int TPR>
+__device__ __forceinline__ int64_t first_row() {
+  return static_cast<int64_t>(blockIdx.x) * (kThreads / TPR) + (TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
 }
 
 __device__ __forceinline__ void drop4(f4& v, uint64_t e, bool even, const Drop& d, uint64_t key) {
@@ -115,30 +137,30 @@ struct Fwd {
   Drop drop;
 };
 
-template <typename Tx, typename Td, typename Ty, int TPR, int STEPS>
+template <typename Tx, typename Td, typename Ty, int TPR, int STEPS, int WHOLE>
 __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd a) {
   __shared__ float2 red[4];
   constexpr int kRows = kThreads / TPR;
   const int t = threadIdx.x % TPR;
   const float inv = 1.0f / static_cast<float>(a.D);
+  const auto left = [&](int i, int c) { return i < WHOLE ? 4 : a.D - c; };
   const bool even = a.D % 4 == 0, drop = a.delta && a.drop.threshold;
   const uint64_t key = drop ? a.drop.key() : 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR; row < a.N;
-       row += static_cast<int64_t>(gridDim.x) * kRows) {
+  for (int64_t row = first_row<TPR>(); row < a.N; row += static_cast<int64_t>(gridDim.x) * kRows) {
     const int64_t base = row * a.D;
     f4 v[STEPS];
     float s = 0.0f, ss = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int c = 4 * (t + TPR * i);
-      v[i] = load4(static_cast<const Tx*>(a.x) + base + c, a.D - c);
+      v[i] = load4(static_cast<const Tx*>(a.x) + base + c, left(i, c));
     }
     if (a.delta) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int c = 4 * (t + TPR * i);
-        f4 d = load4(static_cast<const Td*>(a.delta) + base + c, a.D - c);
-        if (drop && c < a.D) drop4(d, static_cast<uint64_t>(base + c), even, a.drop, key);
+        f4 d = load4(static_cast<const Td*>(a.delta) + base + c, left(i, c));
+        if (drop && left(i, c) > 0) drop4(d, static_cast<uint64_t>(base + c), even, a.drop, key);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i].v[j] += d.v[j];
       }
@@ -147,8 +169,8 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd a) {
     for (int i = 0; i < STEPS; ++i) {
       const int c = 4 * (t + TPR * i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s += c + j < a.D ? v[i].v[j] : 0.0f;
-      if (a.delta) store4(a.x_out + base + c, v[i], a.D - c);
+      for (int j = 0; j < 4; ++j) s += v[i].v[j];  // (0 past the row)
+      if (a.delta) store4(a.x_out + base + c, v[i], left(i, c));
     }
     row_sum<TPR>(s, none, red);
     const float mu = s * inv;
@@ -158,19 +180,19 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd a) {
       for (int j = 0; j < 4; ++j) {
         const float d = v[i].v[j] - mu;
         v[i].v[j] = d;
-        ss += 4 * (t + TPR * i) + j < a.D ? d * d : 0.0f;
+        ss += j < left(i, 4 * (t + TPR * i)) ? d * d : 0.0f;
       }
     row_sum<TPR>(ss, none, red);
     const float r = 1.0f / sqrtf(ss * inv + a.eps);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int c = 4 * (t + TPR * i);
-      const f4 w = load4(a.w + c, a.D - c);
+      const f4 w = load4(a.w + c, left(i, c));
       f4 b = io4<float>::fill(0.0f), o;
-      if (a.b) b = load4(a.b + c, a.D - c);
+      if (a.b) b = load4(a.b + c, left(i, c));
 #pragma unroll
       for (int j = 0; j < 4; ++j) o.v[j] = v[i].v[j] * r * w.v[j] + b.v[j];
-      store4(static_cast<Ty*>(a.y) + base + c, o, a.D - c);
+      store4(static_cast<Ty*>(a.y) + base + c, o, left(i, c));
     }
     if (t == 0 && a.mean) a.mean[row] = mu, a.rstd[row] = r;
   }
@@ -188,34 +210,36 @@ struct Bwd {
   Drop drop;
 };
 
-template <typename Tx, typename Tg, typename Td, int TPR, int STEPS>
-__global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd a) {
+template <typename Tx, typename Tg, typename Td, int TPR, int STEPS, int WHOLE>
+__global__ __launch_bounds__(kThreads, TPR == 64 || STEPS <= 2 ? 4 : STEPS <= 4 ? 2 : 1) void bwd_kernel(Bwd a) {
   __shared__ float2 red[4];
   __shared__ f4 s_sum[2][4][64];
   constexpr int kRows = kThreads / TPR;
   const int t = threadIdx.x % TPR;
   const float inv = 1.0f / static_cast<float>(a.D);
+  const auto left = [&](int i, int c) { return i < WHOLE ? 4 : a.D - c; };
   const bool even = a.D % 4 == 0, drop = a.ddelta && a.drop.threshold;
   const uint64_t key = drop ? a.drop.key() : 0;
   f4 dw[STEPS], db[STEPS];
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) dw[i] = db[i] = io4<float>::fill(0.0f);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR; row < a.N;
-       row += static_cast<int64_t>(gridDim.x) * kRows) {
+  for (int64_t row = first_row<TPR>(); row < a.N; row += static_cast<int64_t>(gridDim.x) * kRows) {
     const int64_t base = row * a.D;
     const float mu = a.mean[row], r = a.rstd[row];
-    f4 h[STEPS], g[STEPS];
+    f4 h[STEPS], g[STEPS], d[STEPS];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int c = 4 * (t + TPR * i);
-      h[i] = load4(static_cast<const Tx*>(a.xn) + base + c, a.D - c);
-      g[i] = load4(static_cast<const Tg*>(a.dy) + base + c, a.D - c);  // (0 past the row: adds nothing below)
+      h[i] = load4(static_cast<const Tx*>(a.xn) + base + c, left(i, c));
+      g[i] = load4(static_cast<const Tg*>(a.dy) + base + c, left(i, c));  // (0 past the row: adds nothing below)
+      d[i] = io4<float>::fill(0.0f);
+      if (a.dres) d[i] = load4(a.dres + base + c, left(i, c));
     }
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int c = 4 * (t + TPR * i);
-      const f4 w = load4(a.w + c, a.D - c);
+      const f4 w = load4(a.w + c, left(i, c));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         h[i].v[j] = (h[i].v[j] - mu) * r;
@@ -231,15 +255,13 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd a) {
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int c = 4 * (t + TPR * i);
-      if (c < a.D) {
-        f4 d = io4<float>::fill(0.0f);
-        if (a.dres) d = load4(a.dres + base + c, a.D - c);
+      if (left(i, c) > 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d.v[j] += r * (g[i].v[j] - s1 - h[i].v[j] * s2);
-        if (a.dx) store4(static_cast<Tx*>(a.dx) + base + c, d, a.D - c);
+        for (int j = 0; j < 4; ++j) d[i].v[j] += r * (g[i].v[j] - s1 - h[i].v[j] * s2);
+        if (a.dx) store4(static_cast<Tx*>(a.dx) + base + c, d[i], left(i, c));
         if (a.ddelta) {
-          if (drop) drop4(d, static_cast<uint64_t>(base + c), even, a.drop, key);
-          store4(static_cast<Td*>(a.ddelta) + base + c, d, a.D - c);
+          if (drop) drop4(d[i], static_cast<uint64_t>(base + c), even, a.drop, key);
+          store4(static_cast<Td*>(a.ddelta) + base + c, d[i], left(i, c));
         }
       }
     }
@@ -249,8 +271,8 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd a) {
   for (int i = 0; i < STEPS; ++i) {
     const int c = 4 * (t + TPR * i);
     if constexpr (TPR > 64) {
-      store4(part + c, dw[i], a.D - c);
-      store4(part + a.D + c, db[i], a.D - c);
+      store4(part + c, dw[i], left(i, c));
+      store4(part + a.D + c, db[i], left(i, c));
     } else {
       const int wave = threadIdx.x / 64;
       __syncthreads();
@@ -263,58 +285,62 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd a) {
         for (int q = 1; q < 4; ++q)
 #pragma unroll
           for (int j = 0; j < 4; ++j) x.v[j] += s_sum[wave][q][t].v[j];
-        store4(part + wave * a.D + c, x, a.D - c);
+        store4(part + wave * a.D + c, x, left(i, c));
       }
     }
   }
 }
 
-// [P][n] partial rows to n sums, 64 columns per workgroup, each wave a quarter of the rows
+// [P][n] partial rows to n sums: 16 columns per workgroup, four to a thread, 64 threads' rows of each
 __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ part, int P, int n, int D,
                                                         float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float s[4][64];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int c = blockIdx.x * 64 + lane;
-  float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
-  if (c < n) {
-    int p = wave;
-    for (; p + 12 < P; p += 16) {
-      a0 += part[static_cast<int64_t>(p) * n + c];
-      a1 += part[static_cast<int64_t>(p + 4) * n + c];
-      a2 += part[static_cast<int64_t>(p + 8) * n + c];
-      a3 += part[static_cast<int64_t>(p + 12) * n + c];
-    }
-    for (; p < P; p += 4) a0 += part[static_cast<int64_t>(p) * n + c];
+  __shared__ float s[64][17];
+  const int c = 16 * blockIdx.x + 4 * (threadIdx.x % 4), g = threadIdx.x / 4;
+  f4 x = io4<float>::fill(0.0f);
+#pragma unroll 4
+  for (int p = g; p < P; p += 64) {
+    const f4 y = load4(part + static_cast<int64_t>(p) * n + c, n - c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] += y.v[j];
   }
-  s[wave][lane] = (a0 + a1) + (a2 + a3);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[g][4 * (threadIdx.x % 4) + j] = x.v[j];
   __syncthreads();
-  if (wave == 0 && c < n) {
-    const float x = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
-    if (c < D) {
-      if (dw) dw[c] = x;
+  const int col = threadIdx.x / 16, q = threadIdx.x % 16, e = 16 * blockIdx.x + col;
+  float sum = (s[q][col] + s[q + 16][col]) + (s[q + 32][col] + s[q + 48][col]);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 16);
+  if (q == 0 && e < n) {
+    if (e < D) {
+      if (dw) dw[e] = sum;
     } else if (db) {
-      db[c - D] = x;
+      db[e - D] = sum;
     }
   }
 }
 
 constexpr int kMaxD = 16384;
 
-// Workgroups: two rows of waves per SIMD's worth of the device, so that the partial rows stay few
-inline int grid_for(int64_t N, int D) {
-  const int64_t per = D <= 2048 ? 4 : 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((N + per - 1) / per, 1024)));
-}
+constexpr int kWaveD = 1024;  // rows up to here belong to one wave
 
-#define MG_LN_SIZES(GO)                                                                             \
-  if (D <= 256) { GO(64, 1) } else if (D <= 512) { GO(64, 2) } else if (D <= 1024) { GO(64, 4) }     \
-  else if (D <= 2048) { GO(64, 8) } else if (D <= 4096) { GO(256, 4) } else if (D <= 8192) { GO(256, 8) } \
-  else { GO(256, 16) }
+// Workgroups. A backward's are as many as the device holds at once, so that the partial rows stay few
+inline int grid_for(int64_t N, int D, int64_t most) {
+  const int64_t per = D <= kWaveD ? 4 : 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((N + per - 1) / per, most)));
+}
+constexpr int kFwdGrid = 65536, kBwdGrid = 1024;
+
+// Threads per row, steps of four values per thread, and how many of the steps lie within the row for
+// every D that takes them
+#define MG_LN_SIZES(GO)                                                                                          \
+  if (D <= 256) { GO(64, 1, 0) } else if (D <= 512) { GO(64, 2, 1) } else if (D <= 768) { GO(64, 3, 2) }          \
+  else if (D <= 1024) { GO(64, 4, 3) } else if (D <= 2048) { GO(256, 2, 1) } else if (D <= 4096) { GO(256, 4, 2) } \
+  else if (D <= 8192) { GO(256, 8, 4) } else { GO(256, 16, 8) }
 
 template <typename Tx, typename Td, typename Ty>
 int launch_fwd(const Fwd& a, hipStream_t st) {
-  const int D = a.D, grid = grid_for(a.N, D);
-#define GO(T, S) hipLaunchKernelGGL((fwd_kernel<Tx, Td, Ty, T, S>), dim3(grid), dim3(kThreads), 0, st, a);
+  const int D = a.D, grid = grid_for(a.N, D, kFwdGrid);
+#define GO(T, S, F) hipLaunchKernelGGL((fwd_kernel<Tx, Td, Ty, T, S, F>), dim3(grid), dim3(kThreads), 0, st, a);
   MG_LN_SIZES(GO)
 #undef GO
   return check_launch("mg_layernorm_fwd");
@@ -322,12 +348,12 @@ int launch_fwd(const Fwd& a, hipStream_t st) {
 
 template <typename Tx, typename Tg, typename Td>
 int launch_bwd(const Bwd& a, float* dw, float* db, hipStream_t st) {
-  const int D = a.D, grid = grid_for(a.N, D);
-#define GO(T, S) hipLaunchKernelGGL((bwd_kernel<Tx, Tg, Td, T, S>), dim3(grid), dim3(kThreads), 0, st, a);
+  const int D = a.D, grid = grid_for(a.N, D, kBwdGrid);
+#define GO(T, S, F) hipLaunchKernelGGL((bwd_kernel<Tx, Tg, Td, T, S, F>), dim3(grid), dim3(kThreads), 0, st, a);
   MG_LN_SIZES(GO)
 #undef GO
   if (dw || db)
-    hipLaunchKernelGGL(sum_parts_kernel, dim3((2 * D + 63) / 64), dim3(256), 0, st, a.part, grid, 2 * D, D, dw, db);
+    hipLaunchKernelGGL(sum_parts_kernel, dim3((2 * D + 15) / 16), dim3(256), 0, st, a.part, grid, 2 * D, D, dw, db);
   return check_launch("mg_layernorm_bwd");
 }
 
@@ -382,7 +408,7 @@ extern "C" int mg_layernorm_fwd(int x_dtype, const void* x, int delta_dtype, con
 
 extern "C" size_t mg_layernorm_bwd_workspace_bytes(int64_t N, int D) {
   if (N < 1 || D < 1 || D > layernorm::kMaxD) return 0;
-  return static_cast<size_t>(layernorm::grid_for(N, D)) * 2 * D * sizeof(float);
+  return static_cast<size_t>(layernorm::grid_for(N, D, layernorm::kBwdGrid)) * 2 * D * sizeof(float);
 }
 
 extern "C" int mg_layernorm_bwd(int x_dtype, const void* xn, const float* w, const float* mean, const float* rstd, int dy_dtype,
