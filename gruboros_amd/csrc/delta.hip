@@ -142,6 +142,12 @@ __device__ __forceinline__ float ld(const float* p) { return *p; }
 __device__ __forceinline__ float ld(const bf16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ void st(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st(bf16_t* p, float x) { *p = f32_to_bf16(x); }
+// four values, 16 (fp32) or 8 bytes aligned
+__device__ __forceinline__ void st4(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
+__device__ __forceinline__ void st4(bf16_t* p, const f32x4& x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(static_cast<uint32_t>(f32_to_bf16(x[0])) | static_cast<uint32_t>(f32_to_bf16(x[1])) << 16,
+                                            static_cast<uint32_t>(f32_to_bf16(x[2])) | static_cast<uint32_t>(f32_to_bf16(x[3])) << 16);
+}
 
 // Column accesses of the passes over the chunks: a buffer over the chunk's rows of one head, the lane's
 // column and first row in its offset, a scalar offset per register. Rows and columns past the end are
@@ -963,116 +969,178 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
 }
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
 
+// 8 values at any alignment: where one row's start and its length are multiples of 8 elements the memory
+// pipe takes them in one piece (two of fp32)
+typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+template <typename E> struct raw8;
+template <> struct raw8<bf16_t> {
+  u16x8u v = {0, 0, 0, 0, 0, 0, 0, 0};
+  __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u16x8u*>(p); }
+  __device__ __forceinline__ void limbs(bf16x8 (&out)[1]) const { out[0] = __builtin_bit_cast(bf16x8, v); }
+};
+template <> struct raw8<float> {
+  f32x4u v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  __device__ __forceinline__ void load(const float* p) {
+    v[0] = reinterpret_cast<const f32x4u*>(p)[0], v[1] = reinterpret_cast<const f32x4u*>(p)[1];
+  }
+  __device__ __forceinline__ void limbs(bf16x8 (&out)[3]) const {
+    const float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+    split<3>(x, out);
+  }
+};
+
 template <int KP, int NI>
 struct GradTile {
   static constexpr int W = KP / 16;                                           // a wave for 16 columns of dq, dk
   static constexpr int NW = kKept<NI>;
-  static constexpr int kState = NW * 32 * KP * 2, kVec = NW * 32 * C * 2;     // bytes of 32 columns of a state, of d or dy
-  static constexpr int kS = 0, kE = kState, kD = 2 * kState, kY = kD + kVec;  // S, dS', d, dy, 32 columns at a time;
-  static constexpr int kK = 0, kQ = NI * C * KP * 2;                          // then in their place k, q
-  static constexpr int kF = 2 * kQ, kN = kF + NW * kPlane * 2;                // and F, N
-  static constexpr int kSums = kY + kVec > kN + NW * kPlane * 2 ? kY + kVec : kN + NW * kPlane * 2;
-  static constexpr int kBytes = kSums + (2 * W * 64 + 64 + W) * 4;            // floats: q.dq, k.Z [W][64], dy.v [64], [W]
+  static constexpr int kState = NW * 32 * KP * 2, kVec = NW * 32 * C * 2;     // bytes of 32 columns of a state, of d or dy,
+  static constexpr int kRows = NI * C * 32 * 2;                               // of do or v
+  static constexpr int kK = 0, kS = NI * C * KP * 2;                          // k; S, dS', d, dy, do, v, 32 columns at a time;
+  static constexpr int kE = kS + kState, kD = kE + kState, kY = kD + kVec, kO = kY + kVec, kV = kO + kRows;
+  static constexpr int kQ = kS, kF = kQ + NI * C * KP * 2, kN = kF + NW * kPlane * 2;  // then in their place q, F, N
+  static constexpr int kEnd = kV + kRows > kN + NW * kPlane * 2 ? kV + kRows : kN + NW * kPlane * 2;
+  static constexpr int kG = kEnd, kGate = kG + 512;                           // the chunk's G (doubles) and gates
+  static constexpr int kSums = kGate + 1024;                                  // floats: q.dq, k.Z [W][64], dy.v [64], [W]
+  static constexpr int kBytes = kSums + (2 * W * 64 + 64 + W) * 4;
 };
 
+// 16-byte unit u of row r of a matrix with four: a fragment's 16 rows spread over all banks
+__device__ __forceinline__ int at4(int r, int u) { return (r * 4 + (u ^ ((r >> 2) & 3))) * 16; }
+
+// bf16, 128 columns: two workgroups of 8 waves per CU, whose waits for the operands the other one fills
 template <int KP, int NI>
-__global__ __launch_bounds__(64 * (KP / 16)) void grad_kernel(Args a) {
+__global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) void grad_kernel(Args a) {
   using E = typename elem<NI>::type;
   using L = GradTile<KP, NI>;
   constexpr int NW = L::NW, U = KP / 8, W = L::W;
   __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x;
-  const int n = static_cast<int>(c % a.NC), bh = static_cast<int>(c / a.NC), h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
+  const int bh = blockIdx.x / a.NC, n = blockIdx.x - bh * a.NC, h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
   const int hk = h / grp, t0 = n * C, rows = min(C, a.T - t0);
   float* vec = reinterpret_cast<float*>(lds + L::kSums);
   const char* img = a.img + c * Tile<KP, NI>::kBytes;
-  const float* gt = reinterpret_cast<const float*>(img + Tile<KP, NI>::kGate);
-  const double* Gd = a.Gd + c * 64;
+  const float* gt = reinterpret_cast<const float*>(lds + L::kGate);
+  const double* Gd = reinterpret_cast<const double*>(lds + L::kG);
+
+  // do and v go through registers, one 32-column block ahead: 4 threads to a row, of both (W = 4) or of one each
+  const int lr = (tid >> 2) & 63, lu = tid & 3;
+  const bool second = W == 8 && wave >= 4;
+  const E* orow = reinterpret_cast<const E*>(a.dout) + b * a.do_sb + (t0 + lr) * a.do_st + h * a.do_sh + 8 * lu;
+  const E* vrow = reinterpret_cast<const E*>(a.v) + b * a.v_sb + (t0 + lr) * a.v_st + h * a.v_sh + 8 * lu;
+  raw8<E> ro[W == 4 ? 2 : 1];
+  const auto load_rows = [&](int vb) {
+    if (lr < rows && 32 * vb + 8 * lu < a.V) {
+      ro[0].load((second ? vrow : orow) + 32 * vb);
+      if constexpr (W == 4) ro[1].load(vrow + 32 * vb);
+    } else {
+      ro[0] = raw8<E>();
+      if constexpr (W == 4) ro[1] = raw8<E>();
+    }
+  };
+  const auto put_rows = [&](const raw8<E>& x, int base) {
+    bf16x8 l[NI];
+    x.limbs(l);
+#pragma unroll
+    for (int q = 0; q < NI; ++q) *reinterpret_cast<bf16x8*>(lds + base + q * C * 64 + at4(lr, lu)) = l[q];
+  };
+  const auto row_frags = [&](int base, int t, int ln, bf16x8 (&out)[NI]) {
+#pragma unroll
+    for (int q = 0; q < NI; ++q) out[q] = *reinterpret_cast<const bf16x8*>(lds + base + q * C * 64 + at4(16 * t + (ln & 15), ln >> 4));
+  };
+  load_rows(0);
+  stage<L::kS, W>(lds + L::kK, img, lane, wave);
+  if (wave == 0) {
+    reinterpret_cast<float4*>(lds + L::kGate)[lane] = reinterpret_cast<const float4*>(img + Tile<KP, NI>::kGate)[lane];
+    reinterpret_cast<double*>(lds + L::kG)[lane] = a.Gd[c * 64 + lane];
+  }
+  float gv = 0.0f;
+  if (wave == 0 && lane < rows) gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
 
   // Products over the value columns, 32 at a time, in this wave's 16 columns of K: W1 = dy S^T, W2 = do S^T,
   // W3 = d dS'^T, and a diagonal block of S dS'^T. Of the 64 x 64 products dy d^T and do d^T a wave takes 16 rows of
   // both (W = 4) or of one (W = 8: waves 0 to 3 the first, 4 to 7 the second); waves 0 to 3 also a diagonal block of dy v^T.
+  // All but the diagonals are held transposed: a lane has one token (of F and N one row) and four consecutive
+  // columns, so that gates are a value per lane, sums over K stay in registers and the outputs are stored four at a time.
   f32x4 w1[4], w2[4], w3[4], m1[4], m2[W == 4 ? 4 : 1], ss = {0, 0, 0, 0}, yv = ss;
 #pragma unroll
   for (int t = 0; t < 4; ++t) w1[t] = w2[t] = w3[t] = m1[t] = m2[W == 4 ? t : 0] = f32x4{0, 0, 0, 0};
-  const int mr = wave & 3;
-  const E* orow = reinterpret_cast<const E*>(a.dout) + b * a.do_sb + t0 * a.do_st + h * a.do_sh + 8 * g;
-  const E* vrow = reinterpret_cast<const E*>(a.v) + b * a.v_sb + (t0 + 16 * mr + m) * a.v_st + h * a.v_sh + 8 * g;
-  for (int vb = 0; vb < a.VP / 32; ++vb) {
-    const int64_t blk = c * (a.VP / 32) + vb;
-    if (vb) __syncthreads();
+  const int mr = wave & 3, blocks = a.VP / 32;
+#pragma unroll 1
+  for (int vb = 0; vb < blocks; ++vb) {
+    const int64_t blk = c * blocks + vb;
+    __syncthreads();
     stage<L::kState, W>(lds + L::kS, a.Sw + blk * NW * 32 * KP, lane, wave);
     stage<L::kState, W>(lds + L::kE, a.dSw + blk * NW * 32 * KP, lane, wave);
     stage<L::kVec, W>(lds + L::kD, a.dw + blk * NW * 32 * C, lane, wave);
     stage<L::kVec, W>(lds + L::kY, a.yw + blk * NW * 32 * C, lane, wave);
-    bf16x8 fo[4][NI], fv[NI];
-    const bool cols = 32 * vb + 8 * g < a.V;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) load8(orow + (16 * t + m) * a.do_st + 32 * vb, 16 * t + m < rows && cols, fo[t]);
-    if (wave < 4) {
-      float x[8];  // (v may lie at any alignment)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 16 * mr + m < rows && cols ? ld(vrow + 32 * vb + j) : 0.0f;
-      split<NI>(x, fv);
-    }
+    put_rows(ro[0], second ? L::kV : L::kO);
+    if constexpr (W == 4) put_rows(ro[1], L::kV);
     staged();
-    bf16x8 s[NW], ds[NW];
-    frags_t<U, false>(lds + L::kS, 32 * KP * 2, wave, 0, lane, s);
-    frags_t<U, false>(lds + L::kE, 32 * KP * 2, wave, 0, lane, ds);
+    if (vb + 1 < blocks) load_rows(vb + 1);
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (addresses made anew in each block: kept, they cost the registers of the products)
+    bf16x8 s[NW], ds[NW], yr[NW], vr[NI], orr[W == 4 ? NI : 1];
+    frags_t<U, false>(lds + L::kS, 32 * KP * 2, wave, 0, ln, s);
+    frags_t<U, false>(lds + L::kE, 32 * KP * 2, wave, 0, ln, ds);
     ss = mm<NW>(s, ds, ss);
-    bf16x8 yr[NW], orr[NI];
-    frags_t<8, false>(lds + L::kY, 32 * C * 2, mr, 0, lane, yr);
-    if (wave < 4) yv = mm<NW>(yr, fv, yv);
-    load8(orow + (16 * mr + m) * a.do_st + 32 * vb, 16 * mr + m < rows && cols, orr);
+    if (second) {  // (do as the first limbs)
+      bf16x8 x[NI];
+      row_frags(L::kO, mr, ln, x);
+#pragma unroll
+      for (int q = 0; q < NW; ++q) yr[q] = q < NI ? x[q < NI ? q : 0] : bf16x8{};
+    } else {
+      frags_t<8, false>(lds + L::kY, 32 * C * 2, mr, 0, ln, yr);
+    }
+    row_frags(L::kV, mr, ln, vr);
+    yv = mm<NW>(yr, vr, yv);  // (read where W = 4 or not `second`)
+    if constexpr (W == 4) row_frags(L::kO, mr, ln, orr);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      bf16x8 fy[NW], fd[NW];
-      frags_t<8, false>(lds + L::kY, 32 * C * 2, t, 0, lane, fy);
-      frags_t<8, false>(lds + L::kD, 32 * C * 2, t, 0, lane, fd);
-      w1[t] = mm<NW>(fy, s, w1[t]);
-      w2[t] = mm<NW>(fo[t], s, w2[t]);
-      w3[t] = mm<NW>(fd, ds, w3[t]);
-      if (t <= mr) {
-        if constexpr (W == 4) {
-          m1[t] = mm<NW>(yr, fd, m1[t]);
-          m2[t] = mm<NW>(orr, fd, m2[t]);
-        } else if (wave < 4) {
-          m1[t] = mm<NW>(yr, fd, m1[t]);
-        } else {
-          m1[t] = mm<NW>(orr, fd, m1[t]);
-        }
-      }
+      bf16x8 f[NW], fo[NI];
+      frags_t<8, false>(lds + L::kY, 32 * C * 2, t, 0, ln, f);
+      w1[t] = mm<NW>(s, f, w1[t]);
+      row_frags(L::kO, t, ln, fo);
+      w2[t] = mm<NW>(s, fo, w2[t]);
+      frags_t<8, false>(lds + L::kD, 32 * C * 2, t, 0, ln, f);
+      w3[t] = mm<NW>(ds, f, w3[t]);
+      m1[t] = mm<NW>(f, yr, m1[t]);  // (above the diagonal too: fewer branches are worth more than the products)
+      if constexpr (W == 4) m2[t] = mm<NW>(f, orr, m2[t]);
     }
   }
   __syncthreads();
-  stage<2 * L::kQ, W>(lds, img, lane, wave);  // k and q
+  stage<L::kS, W>(lds + L::kQ, img + L::kS, lane, wave);  // (k, then q, in the image)
   // F and N, in this wave's rows, to LDS
-  const auto put = [&](int plane, int row, int col, float x) {
-    const int pos = at<8>(row, col >> 3) + (col & 7) * 2;
+  const auto put = [&](int plane, int row, int col, const f32x4& x) {
+    uint2 l[NW];
+    split4<NW>(x, l);
 #pragma unroll
-    for (int l = 0; l < NW; ++l) {
-      const uint32_t u = __float_as_uint(x);
-      *reinterpret_cast<bf16_t*>(lds + plane + l * kPlane * 2 + pos) = NW == 2 && l == 1 ? f32_to_bf16(x) : static_cast<bf16_t>(u >> 16);
-      x -= __uint_as_float(u & 0xffff0000u);
-    }
+    for (int q = 0; q < NW; ++q) *reinterpret_cast<uint2*>(lds + plane + q * kPlane * 2 + at<8>(row, col >> 3) + (col & 7) * 2) = l[q];
   };
+  {
+    const int row = 16 * mr + m;
+    const double Gr = Gd[row];
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t) {
+      const int col = 16 * t + 4 * g;
+      f32x4 f, x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * mr + 4 * g + r, col = 16 * t + m;
-      const float dec = col <= row ? expf(static_cast<float>(Gd[row] - Gd[col])) : 0.0f;
-      if (W == 4 || wave < 4) put(L::kF, row, col, col < row ? dec * m1[t][r] : 0.0f);
-      if (W == 4 || wave >= 4) put(L::kN, row, col, col <= row ? a.scale * dec * (W == 4 ? m2[W == 4 ? t : 0][r] : m1[t][r]) : 0.0f);
+      for (int r = 0; r < 4; ++r) {
+        const float dec = expf(col + r <= row ? static_cast<float>(Gr - Gd[col + r]) : 0.0f);
+        f[r] = col + r < row ? dec * m1[t][r] : 0.0f;
+        x[r] = col + r <= row ? a.scale * dec * (W == 4 ? m2[W == 4 ? t : 0][r] : m1[t][r]) : 0.0f;
+      }
+      if (W == 4 || !second) put(L::kF, row, col, f);
+      if (W == 4 || second) put(L::kN, row, col, x);
     }
+  }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 4; ++t) {
+    const float e = gt[16 * t + m], tail = gt[64 + 16 * t + m];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * t + 4 * g + r;
-      w1[t][r] *= gt[i], w2[t][r] *= a.scale * gt[i], w3[t][r] *= gt[64 + i];
-    }
+    for (int r = 0; r < 4; ++r) w1[t][r] *= e, w2[t][r] *= a.scale * e, w3[t][r] *= tail;
+  }
   if (wave < 4) {  // the diagonals' lanes
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -1084,19 +1152,24 @@ __global__ __launch_bounds__(64 * (KP / 16)) void grad_kernel(Args a) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) dot += 4 * g + r == m ? ss[r] : 0.0f;
   dot *= gt[63];
-  const int d = 16 * wave + m;
+  const int d = 16 * wave + 4 * g;
   // k and q where this wave's accumulators are
   const auto at_acc = [&](int base, int row) {
-    float x = 0.0f;
+    f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-    for (int l = 0; l < NI; ++l)
-      x += bf16_to_f32(*reinterpret_cast<const bf16_t*>(lds + base + l * C * KP * 2 + at<U>(row, d >> 3) + (d & 7) * 2));
+    for (int l = 0; l < NI; ++l) {
+      const uint2 u = *reinterpret_cast<const uint2*>(lds + base + l * C * KP * 2 + at<U>(row, d >> 3) + (d & 7) * 2);
+      x[0] += __uint_as_float(u.x << 16), x[1] += __uint_as_float(u.x & 0xffff0000u);
+      x[2] += __uint_as_float(u.y << 16), x[3] += __uint_as_float(u.y & 0xffff0000u);
+    }
     return x;
   };
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 4; ++t) {
+    const f32x4 k = at_acc(L::kK, 16 * t + m);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) dot += at_acc(L::kK, 16 * t + 4 * g + r) * w3[t][r];
+    for (int r = 0; r < 4; ++r) dot += k[r] * w3[t][r];
+  }
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     bf16x8 kf[NI], qf[NI], bk[NW];
@@ -1119,41 +1192,43 @@ __global__ __launch_bounds__(64 * (KP / 16)) void grad_kernel(Args a) {
       if (p <= t / 2) {
 #pragma unroll
         for (int l = 0; l < NW; ++l) f[l] = frag_plain<8>(lds + L::kF + l * kPlane * 2, t, p, lane);
-        w1[t] = mm<NW>(f, kf, w1[t]);
+        w1[t] = mm<NW>(kf, f, w1[t]);
 #pragma unroll
         for (int l = 0; l < NW; ++l) f[l] = frag_plain<8>(lds + L::kN + l * kPlane * 2, t, p, lane);
-        w2[t] = mm<NW>(f, kf, w2[t]);
+        w2[t] = mm<NW>(kf, f, w2[t]);
       }
       if (p >= t / 2) {
         frags_t<8, false>(lds + L::kN, kPlane * 2, t, p, lane, f);
-        w3[t] = mm<NW>(f, qf, w3[t]);
+        w3[t] = mm<NW>(qf, f, w3[t]);
         frags_t<8, false>(lds + L::kF, kPlane * 2, t, p, lane, f);
-        w3[t] = mm<NW>(f, bk, w3[t]);
+        w3[t] = mm<NW>(bk, f, w3[t]);
       }
     }
   }
   // outputs, and the row sums q.dq and k.Z
   const int64_t tok0 = static_cast<int64_t>(b) * a.T + t0;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 4; ++t) {
+    const int row = 16 * t + m;
+    const float be = gt[128 + row];
+    const f32x4 dq = w2[t], z = w1[t], q = at_acc(L::kQ, row), k = at_acc(L::kK, row);
+    f32x4 dk;
+    float qd = 0.0f, kz = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * g + r;
-      const float dq = w2[t][r], z = w1[t][r], dk = w3[t][r] - gt[128 + row] * z;
-      float qd = at_acc(L::kQ, row) * dq, kz = at_acc(L::kK, row) * z;
-      if (row < rows && d < a.K) {
-        if (grp == 1) {
-          st(reinterpret_cast<E*>(a.dq) + ((tok0 + row) * a.Hk + hk) * a.K + d, dq);
-          st(reinterpret_cast<E*>(a.dk) + ((tok0 + row) * a.Hk + hk) * a.K + d, dk);
-        } else {
-          a.dqp[((tok0 + row) * a.H + h) * a.K + d] = dq;
-          a.dkp[((tok0 + row) * a.H + h) * a.K + d] = dk;
-        }
+    for (int r = 0; r < 4; ++r) dk[r] = w3[t][r] - be * z[r], qd += q[r] * dq[r], kz += k[r] * z[r];
+    if (row < rows && d < a.K) {
+      if (grp == 1) {
+        st4(reinterpret_cast<E*>(a.dq) + ((tok0 + row) * a.Hk + hk) * a.K + d, dq);
+        st4(reinterpret_cast<E*>(a.dk) + ((tok0 + row) * a.Hk + hk) * a.K + d, dk);
+      } else {
+        st4(a.dqp + ((tok0 + row) * a.H + h) * a.K + d, dq);
+        st4(a.dkp + ((tok0 + row) * a.H + h) * a.K + d, dk);
       }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) qd += __shfl_xor(qd, o, 64), kz += __shfl_xor(kz, o, 64);
-      if (m == 0) vec[wave * 64 + row] = qd, vec[(W + wave) * 64 + row] = kz;
     }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) qd += __shfl_xor(qd, o, 64), kz += __shfl_xor(kz, o, 64);
+    if (g == 0) vec[wave * 64 + row] = qd, vec[(W + wave) * 64 + row] = kz;
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
   if (lane == 0) vec[(2 * W + 1) * 64 + wave] = dot;
@@ -1171,7 +1246,6 @@ __global__ __launch_bounds__(64 * (KP / 16)) void grad_kernel(Args a) {
     }
     if (lane < rows) {
       const int64_t tok = (tok0 + lane) * a.H + h;
-      const float gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
       // a decay that is zero in fp32 passes nothing on
       st(reinterpret_cast<E*>(a.dg) + tok, gv < -104.0f ? 0.0f : static_cast<float>(s + all));
       st(reinterpret_cast<E*>(a.db) + tok, y - kz);
@@ -1459,7 +1533,7 @@ extern "C" int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows*
     return rc;
   for (const void* p : {dq, dk, dv, dg, dbeta})
     if (!p || !aligned(p, dtype == MG_F32 ? 4 : 2)) return fail(MG_ERR_ARG, "%s: a gradient is NULL or misaligned", fn);
-  if (dims->H > dims->Hk && (!aligned(dq, 16) || !aligned(dk, 16)))
+  if (!aligned(dq, 16) || !aligned(dk, 16))
     return fail(MG_ERR_ARG, "%s: dq and dk must be 16-byte aligned", fn);
   if (!aligned(dstate, 4) || !aligned(dh0, 4)) return fail(MG_ERR_ARG, "%s: state gradient misaligned", fn);
   const delta::Layout l = delta::layout(dtype, *dims, true);

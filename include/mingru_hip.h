@@ -673,7 +673,8 @@ int mg_decode_head_f16(int B, int D, int V, const float* x_in, const void* pendi
  *
  * mg_rows: element (b, t, h, d) of an operand at p + b sb + t st + h sh + d
  * (elements; d contiguous; g and beta have no d). q, k and dout: p and the
- * strides multiples of 16 bytes. o, dv: dense [B, T, H, V]; dq, dk: dense
+ * strides multiples of 16 bytes; dq and dk 16-byte aligned. o, dv: dense
+ * [B, T, H, V]; dq, dk: dense
  * [B, T, Hk, K]; dg, dbeta: dense [B, T, H].
  * K and V multiples of 8, K <= 128, V <= 256; T >= 1;
  * B H ceil(T / 64) < 2^31; 64 token strides below 2 GiB.
