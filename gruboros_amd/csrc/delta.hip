@@ -177,20 +177,26 @@ __device__ __forceinline__ void store_col(__amdgpu_buffer_rsrc_t r, uint32_t off
     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, off, row_off, 0);
 }
 
-// 8 consecutive values as limbs; nothing (zero) unless ok
-__device__ __forceinline__ void load8(const bf16_t* p, bool ok, bf16x8 (&out)[1]) {
-  const u32x4 z = {0, 0, 0, 0};
-  out[0] = __builtin_bit_cast(bf16x8, ok ? *reinterpret_cast<const u32x4*>(p) : z);
-}
-__device__ __forceinline__ void load8(const float* p, bool ok, bf16x8 (&out)[3]) {
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float4 v = ok ? reinterpret_cast<const float4*>(p)[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+// 8 values at any alignment: where one row's start and its length are multiples of 8 elements the memory
+// pipe takes them in one piece (two of fp32)
+typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+template <typename E> struct raw8;
+template <> struct raw8<bf16_t> {
+  u16x8u v = {0, 0, 0, 0, 0, 0, 0, 0};
+  __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u16x8u*>(p); }
+  __device__ __forceinline__ void limbs(bf16x8 (&out)[1]) const { out[0] = __builtin_bit_cast(bf16x8, v); }
+};
+template <> struct raw8<float> {
+  f32x4u v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  __device__ __forceinline__ void load(const float* p) {
+    v[0] = reinterpret_cast<const f32x4u*>(p)[0], v[1] = reinterpret_cast<const f32x4u*>(p)[1];
   }
-  split<3>(x, out);
-}
+  __device__ __forceinline__ void limbs(bf16x8 (&out)[3]) const {
+    const float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+    split<3>(x, out);
+  }
+};
 
 // ---------------------------------------------------------------- LDS operands
 //
@@ -260,6 +266,16 @@ __device__ __forceinline__ void staged() {
   __syncthreads();
 }
 
+// 4 values (one accumulator) as N limbs of half a fragment
+template <int N>
+__device__ __forceinline__ void split4(const f32x4& x, uint2 (&out)[N]) {
+  uint32_t a[N], b[N];
+  pair_limbs(x[0], x[1], a);
+  pair_limbs(x[2], x[3], b);
+#pragma unroll
+  for (int l = 0; l < N; ++l) out[l] = make_uint2(a[l], b[l]);
+}
+
 // ---------------------------------------------------------------- T, P and the decays of a chunk
 
 constexpr int LD = 68;  // floats per row of the 64 x 64 matrices in LDS
@@ -297,27 +313,57 @@ __device__ __forceinline__ void put_planes(const float* m, char* out, int tid) {
   }
 }
 
+// k and q are read once, all loads of a thread under way at a time, and go to the image and to LDS, which
+// A and T take over once k k^T and q k^T are in registers.
 template <int KP, int NI>
-__global__ __launch_bounds__(256) void chunk_kernel(Args a) {
+__global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
   using E = typename elem<NI>::type;
   using L = Tile<KP, NI>;
-  __shared__ float sA[C * LD], sP[C * LD], sT[C * LD];
+  constexpr int U = KP / 8, kRows = NI * C * KP * 2, kLds = 2 * kRows > 2 * C * LD * 4 ? 2 * kRows : 2 * C * LD * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ double sG[C];
   __shared__ float sB[C];
+  float *sA = reinterpret_cast<float*>(lds), *sT = sA + C * LD;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x;
-  const int n = static_cast<int>(c % a.NC), bh = static_cast<int>(c / a.NC), h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
+  const int bh = blockIdx.x / a.NC, n = blockIdx.x - bh * a.NC, h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
   const int hk = h / grp, t0 = n * C, rows = min(C, a.T - t0);
   const E* k = reinterpret_cast<const E*>(a.k) + b * a.k_sb + t0 * a.k_st + hk * a.k_sh;
   const E* q = reinterpret_cast<const E*>(a.q) + b * a.q_sb + t0 * a.q_st + hk * a.q_sh;
   char* img = a.img + c * L::kBytes;
-  if (wave == 0) {
-    float gv = 0.0f, bv = 0.0f;
-    if (lane < rows) {
-      gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
-      bv = ld(reinterpret_cast<const E*>(a.beta) + b * a.b_sb + (t0 + lane) * a.b_st + h * a.b_sh);
-      gv = gv < kMinLog ? kMinLog : gv;
+  float gv = 0.0f, bv = 0.0f;
+  if (wave == 0 && lane < rows) {
+    gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
+    bv = ld(reinterpret_cast<const E*>(a.beta) + b * a.b_sb + (t0 + lane) * a.b_st + h * a.b_sh);
+    gv = gv < kMinLog ? kMinLog : gv;
+  }
+  {
+    raw8<E> rk[C * U / 256], rq[C * U / 256];
+#pragma unroll
+    for (int i = 0; i < C * U / 256; ++i) {  // (what is outside reads the chunk's first values: no branches between the loads)
+      const int r = (tid + 256 * i) / U, u = tid % U;
+      const bool ok = r < rows && 8 * u < a.K;
+      rk[i].load(k + (ok ? r * a.k_st + 8 * u : 0));
+      rq[i].load(q + (ok ? r * a.q_st + 8 * u : 0));
     }
+#pragma unroll
+    for (int i = 0; i < C * U / 256; ++i) {
+      const int r = (tid + 256 * i) / U, u = tid % U;
+      if (!(r < rows && 8 * u < a.K)) rk[i] = rq[i] = raw8<E>();
+      bf16x8 lk[NI], lq[NI];
+      rk[i].limbs(lk);
+      rq[i].limbs(lq);
+#pragma unroll
+      for (int l = 0; l < NI; ++l) {
+        const int pos = l * C * KP * 2 + at<U>(r, u);
+        *reinterpret_cast<bf16x8*>(lds + pos) = lk[l];
+        *reinterpret_cast<bf16x8*>(lds + kRows + pos) = lq[l];
+        *reinterpret_cast<bf16x8*>(img + L::kK + pos) = lk[l];
+        *reinterpret_cast<bf16x8*>(img + L::kQ + pos) = lq[l];
+      }
+    }
+  }
+  if (wave == 0) {
     // the sums in 64 bits: what counts is their differences, also behind a token that forgets all
     double s = gv;
 #pragma unroll
@@ -335,41 +381,59 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
     gt[192 + lane] = 0.0f;
     a.Gd[c * 64 + lane] = s;
   }
-  // k k^T, rows 16 wave ...; q k^T, rows 16 (3 - wave) ...: five blocks of the lower triangles each
+  __syncthreads();
+  // k k^T, rows 16 wave ...; q k^T, rows 16 (3 - wave) ...: five blocks of the lower triangles each, transposed: a
+  // lane has one row and four consecutive columns
   const int wq = 3 - wave;
   f32x4 kk[4], qk[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) kk[i] = f32x4{0, 0, 0, 0}, qk[i] = f32x4{0, 0, 0, 0};
+  for (int i = 0; i < 4; ++i) kk[i] = qk[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int kb = 0; kb < KP / 32; ++kb) {
-    const int d = 32 * kb + 8 * g;
+    const auto rows_of = [&](int base, int t, bf16x8 (&out)[NI]) {
+#pragma unroll
+      for (int l = 0; l < NI; ++l) out[l] = frag_plain<U>(lds + base + l * C * KP * 2, t, kb, lane);
+    };
     bf16x8 ak[NI], aq[NI];
-    load8(k + (16 * wave + m) * a.k_st + d, 16 * wave + m < rows && d < a.K, ak);
-    load8(q + (16 * wq + m) * a.q_st + d, 16 * wq + m < rows && d < a.K, aq);
+    rows_of(0, wave, ak);
+    rows_of(kRows, wq, aq);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i <= wave || i <= wq) {
         bf16x8 bk[NI];
-        load8(k + (16 * i + m) * a.k_st + d, 16 * i + m < rows && d < a.K, bk);
-        if (i <= wave) kk[i] = mm<NI>(ak, bk, kk[i]);
-        if (i <= wq) qk[i] = mm<NI>(aq, bk, qk[i]);
+        rows_of(0, i, bk);
+        if (i <= wave) kk[i] = mm<NI>(bk, ak, kk[i]);
+        if (i <= wq) qk[i] = mm<NI>(bk, aq, qk[i]);
       }
     }
   }
   __syncthreads();
+  {
+    const int ra = 16 * wave + m, rp = 16 * wq + m;
+    const double ga = sG[ra], gp = sG[rp];
+    const float be = sB[ra];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
+      const int col = 16 * i + 4 * g;
+      f32x4 x = {0, 0, 0, 0}, p = x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int col = 16 * i + m;
-      if (i <= wave) {
-        const int row = 16 * wave + 4 * g + r;
-        sA[row * LD + col] = col < row ? sB[row] * expf(static_cast<float>(sG[row] - sG[col])) * kk[i][r] : 0.0f;
+      for (int r = 0; r < 4; ++r) {
+        const double gc = sG[col + r];
+        if (i <= wave) {
+          const float e = be * expf(col + r < ra ? static_cast<float>(ga - gc) : 0.0f) * kk[i][r];
+          x[r] = col + r < ra ? e : 0.0f;
+        }
+        if (i <= wq) {
+          const float e = a.scale * expf(col + r <= rp ? static_cast<float>(gp - gc) : 0.0f) * qk[i][r];
+          p[r] = col + r <= rp ? e : 0.0f;
+        }
       }
-      if (i <= wq) {
-        const int row = 16 * wq + 4 * g + r;
-        sP[row * LD + col] = col <= row ? a.scale * expf(static_cast<float>(sG[row] - sG[col])) * qk[i][r] : 0.0f;
-      }
+      if (i <= wave) *reinterpret_cast<f32x4*>(sA + ra * LD + col) = x;
+      uint2 l[L::NP];
+      split4<L::NP>(p, l);
+#pragma unroll
+      for (int j = 0; j < L::NP; ++j)
+        *reinterpret_cast<uint2*>(img + L::kP + j * kPlane * 2 + at<8>(rp, col >> 3) + (col & 7) * 2) = l[j];
     }
   }
   __syncthreads();
@@ -415,19 +479,6 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
   }
   __syncthreads();
   put_planes<3>(sT, img + L::kT, tid);
-  put_planes<L::NP>(sP, img + L::kP, tid);
-  for (int i = tid; i < C * L::U; i += 256) {
-    const int r = i / L::U, u = i % L::U;
-    const bool ok = r < rows && 8 * u < a.K;
-    bf16x8 lk[NI], lq[NI];
-    load8(k + r * a.k_st + 8 * u, ok, lk);
-    load8(q + r * a.q_st + 8 * u, ok, lq);
-#pragma unroll
-    for (int l = 0; l < NI; ++l) {
-      *reinterpret_cast<bf16x8*>(img + L::kK + l * C * KP * 2 + at<L::U>(r, u)) = lk[l];
-      *reinterpret_cast<bf16x8*>(img + L::kQ + l * C * KP * 2 + at<L::U>(r, u)) = lq[l];
-    }
-  }
 }
 
 // ---------------------------------------------------------------- the pass over the chunks
@@ -468,16 +519,6 @@ template <int U, bool PERM, int N>
 __device__ __forceinline__ void frags_t(const char* m, int plane, int t, int p, int lane, bf16x8 (&out)[N]) {
 #pragma unroll
   for (int l = 0; l < N; ++l) out[l] = frag_t<U, PERM>(m + l * plane, t, p, lane);
-}
-
-// 4 values (one accumulator) as N limbs of half a fragment
-template <int N>
-__device__ __forceinline__ void split4(const f32x4& x, uint2 (&out)[N]) {
-  uint32_t a[N], b[N];
-  pair_limbs(x[0], x[1], a);
-  pair_limbs(x[2], x[3], b);
-#pragma unroll
-  for (int l = 0; l < N; ++l) out[l] = make_uint2(a[l], b[l]);
 }
 
 // B operands in LDS, kFrag bytes per fragment and limb: fragment f of F, limb l at (l F + f) kFrag. The 16 bytes
@@ -968,27 +1009,6 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
   if (a.dh0 && w < KB) store_state(S, a.dh0, a, p);
 }
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
-
-// 8 values at any alignment: where one row's start and its length are multiples of 8 elements the memory
-// pipe takes them in one piece (two of fp32)
-typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-template <typename E> struct raw8;
-template <> struct raw8<bf16_t> {
-  u16x8u v = {0, 0, 0, 0, 0, 0, 0, 0};
-  __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u16x8u*>(p); }
-  __device__ __forceinline__ void limbs(bf16x8 (&out)[1]) const { out[0] = __builtin_bit_cast(bf16x8, v); }
-};
-template <> struct raw8<float> {
-  f32x4u v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-  __device__ __forceinline__ void load(const float* p) {
-    v[0] = reinterpret_cast<const f32x4u*>(p)[0], v[1] = reinterpret_cast<const f32x4u*>(p)[1];
-  }
-  __device__ __forceinline__ void limbs(bf16x8 (&out)[3]) const {
-    const float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
-    split<3>(x, out);
-  }
-};
 
 template <int KP, int NI>
 struct GradTile {
