@@ -54,6 +54,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+template <int N>
+struct int_c { static constexpr int value = N; };
+
 constexpr int C = 64;           // tokens per chunk
 constexpr int kPlane = C * C;   // elements of one limb of T or P
 constexpr float kMinLog = -200.0f;  // decays below e^-104 are zero in fp32: kept finite for the differences
@@ -235,17 +238,39 @@ __device__ __forceinline__ bf16x8 frag_t(const char* m, int t, int p, int lane) 
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// One chunk's operands as chunk_kernel leaves them in memory and the other kernels keep them in LDS:
-// limb planes of k and q [64][KP], of T and P [64][64], all with their units at at<>(), and the vectors
-// e^G, e^{G_C - G}, beta. An image is copied as it is, 1 KiB per wave instruction and straight into LDS:
-// no strides, masks or swizzles where the time counts, at the price of writing k and q once more.
+// One chunk's operands as chunk_kernel leaves them in memory: fragments of the matrix instructions, 1 KiB for a
+// limb of one (16 bytes per lane), each read by one wave of a pass straight into the registers that the instruction
+// takes them from. Rows of k and q [tile of 16 tokens, in row_of order][32 of K]; k^T and q^T [16 of K, in row_of
+// order][32 tokens]; of T and P the blocks of 16 rows and 32 columns that reach the diagonal, and of T^T and P^T;
+// each with its limbs. And the vectors e^G, e^{G_C - G}, beta. What only the backward reads comes last.
 template <int KP, int NI>
 struct Tile {
-  static constexpr int NP = NI == 3 ? 3 : 2;
-  static constexpr int U = KP / 8;
-  static constexpr int kK = 0, kQ = NI * C * KP * 2, kT = 2 * kQ, kP = kT + 3 * kPlane * 2, kGate = kP + NP * kPlane * 2;
-  static constexpr int kBytes = kGate + 1024;
+  static constexpr int NP = NI == 3 ? 3 : 2, KB = KP / 32, U = KP / 8;
+  static constexpr int F = 1024, kRows = 4 * KB * NI * F, nT = 6 * 3 * F, nP = 6 * NP * F;
+  static constexpr int kK = 0, kKT = kRows, kQ = 2 * kRows, kT = 3 * kRows, kP = kT + nT, kGate = kP + nP, kOnce = kGate + F;
+  static constexpr int kQT = kOnce, kTT = kQT + kRows, kPT = kTT + nT, kKept = kPT + nP;
+  // limb 0 of block (tile t, 32 of K or 32 tokens b)
+  static constexpr int rows(int t, int kb) { return (t * KB + kb) * NI * F; }
+  static constexpr int cols(int t, int p) { return (t * 2 + p) * NI * F; }
+  // the blocks (w, p) of T or P with p <= w / 2, and those of their transposes with p >= w / 2
+  static constexpr int low(int w, int p, int n) { return ((w < 2 ? w : 2 * w - 2) + p) * n * F; }
+  static constexpr int high(int w, int p, int n) { return (w < 2 ? 2 * w + p : w + 2) * n * F; }
+  // unit u of row r of k or q (limb 0) in `rows`' order
+  __device__ static int unit(int r, int u) {
+    return rows(2 * (r >> 5) + ((r >> 2) & 1), u >> 2) + (16 * (u & 3) + 4 * ((r >> 3) & 3) + (r & 3)) * 16;
+  }
 };
+
+template <int N>
+__device__ __forceinline__ void load_frag(const char* p, int lane, bf16x8 (&out)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) out[l] = *reinterpret_cast<const bf16x8*>(p + l * 1024 + lane * 16);
+}
+template <int N>
+__device__ __forceinline__ void store_frag(char* p, int lane, const bf16x8 (&x)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) *reinterpret_cast<bf16x8*>(p + l * 1024 + lane * 16) = x[l];
+}
 
 template <int BYTES, int WAVES>
 __device__ __forceinline__ void stage(char* lds, const void* src, int lane, int wave) {  // BYTES / 1024 / WAVES loads a wave, rounded up
@@ -264,6 +289,28 @@ __device__ __forceinline__ void stage(char* lds, const void* src, int lane, int 
 __device__ __forceinline__ void staged() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+}
+
+template <int U, int N>
+__device__ __forceinline__ void frags(const char* m, int plane, int t, int kb, int lane, bf16x8 (&out)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) out[l] = frag<U>(m + l * plane, t, kb, lane);
+}
+template <int U, bool PERM, int N>
+__device__ __forceinline__ void frags_t(const char* m, int plane, int t, int p, int lane, bf16x8 (&out)[N]) {
+#pragma unroll
+  for (int l = 0; l < N; ++l) out[l] = frag_t<U, PERM>(m + l * plane, t, p, lane);
+}
+// the same, columns in their own order, from k or q as they lie in a chunk's image
+template <typename L, int NI>
+__device__ __forceinline__ void frags_t_image(const char* x, int t, int p, int lane, bf16x8 (&out)[NI]) {
+  const int g = lane >> 4, j = (lane >> 2) & 3, q = lane & 3, r = 32 * p + 8 * g + j;
+#pragma unroll
+  for (int l = 0; l < NI; ++l) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + L::unit(r, 2 * t + (q >> 1)) + l * 1024 + 8 * (q & 1)));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + L::unit(r + 4, 2 * t + (q >> 1)) + l * 1024 + 8 * (q & 1)));
+    out[l] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
 }
 
 // 4 values (one accumulator) as N limbs of half a fragment
@@ -294,32 +341,38 @@ __device__ __forceinline__ f32x4 mm16(const float* a, f32x4 b, f32x4 c, int lane
   return c;
 }
 
-// A 64 x 64 lower triangle from LDS to N limb planes, 16 values per thread
+// The blocks of a 64 x 64 lower triangle in LDS, and with `both` those of its transpose, as limbs to the image: wave w's tiles w
 template <int N>
-__device__ __forceinline__ void put_planes(const float* m, char* out, int tid) {
-  const int r = tid >> 2, c0 = 16 * (tid & 3);
+__device__ __forceinline__ void put_blocks(const float* m, char* low, char* high, bool both, int lane, int w) {
+  using L = Tile<64, 1>;
+  const int r = row_of(w, lane & 15), g = lane >> 4;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int p = 0; p < 2; ++p) {
+    const int c0 = 32 * p + 8 * g;
     float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = c0 + 8 * u + i;
-      x[i] = c <= r ? m[r * LD + c] : 0.0f;
-    }
     bf16x8 l[N];
-    split<N>(x, l);
+    if (p <= w / 2) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<bf16x8*>(out + i * kPlane * 2 + at<8>(r, c0 / 8 + u)) = l[i];
+      for (int i = 0; i < 8; ++i) x[i] = c0 + i <= r ? m[r * LD + c0 + i] : 0.0f;
+      split<N>(x, l);
+      store_frag(low + L::low(w, p, N), lane, l);
+    }
+    if (both && p >= w / 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = r <= c0 + i ? m[(c0 + i) * LD + r] : 0.0f;
+      split<N>(x, l);
+      store_frag(high + L::high(w, p, N), lane, l);
+    }
   }
 }
 
 // k and q are read once, all loads of a thread under way at a time, and go to the image and to LDS, which
 // A and T take over once k k^T and q k^T are in registers.
 template <int KP, int NI>
-__global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
+__global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a, bool keep) {
   using E = typename elem<NI>::type;
   using L = Tile<KP, NI>;
-  constexpr int U = KP / 8, kRows = NI * C * KP * 2, kLds = 2 * kRows > 2 * C * LD * 4 ? 2 * kRows : 2 * C * LD * 4;
+  constexpr int U = KP / 8, KB = KP / 32, kRows = NI * C * KP * 2, kLds = 2 * kRows > 2 * C * LD * 4 ? 2 * kRows : 2 * C * LD * 4;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ double sG[C];
   __shared__ float sB[C];
@@ -330,7 +383,7 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
   const int hk = h / grp, t0 = n * C, rows = min(C, a.T - t0);
   const E* k = reinterpret_cast<const E*>(a.k) + b * a.k_sb + t0 * a.k_st + hk * a.k_sh;
   const E* q = reinterpret_cast<const E*>(a.q) + b * a.q_sb + t0 * a.q_st + hk * a.q_sh;
-  char* img = a.img + c * L::kBytes;
+  char* img = a.img + c * (keep ? L::kKept : L::kOnce);
   float gv = 0.0f, bv = 0.0f;
   if (wave == 0 && lane < rows) {
     gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
@@ -358,8 +411,6 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
         const int pos = l * C * KP * 2 + at<U>(r, u);
         *reinterpret_cast<bf16x8*>(lds + pos) = lk[l];
         *reinterpret_cast<bf16x8*>(lds + kRows + pos) = lq[l];
-        *reinterpret_cast<bf16x8*>(img + L::kK + pos) = lk[l];
-        *reinterpret_cast<bf16x8*>(img + L::kQ + pos) = lq[l];
       }
     }
   }
@@ -382,6 +433,30 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
     a.Gd[c * 64 + lane] = s;
   }
   __syncthreads();
+  {
+    const auto put = [&](int base, int from, int t) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        bf16x8 f[NI];
+        frags<U>(lds + from, C * KP * 2, t, kb, lane, f);
+        store_frag(img + base + L::rows(t, kb), lane, f);
+      }
+    };
+    const auto put_t = [&](int base, int from, int t) {
+#pragma unroll
+      for (int i = 0; i < KP / 64; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          bf16x8 f[NI];
+          frags_t<U, true>(lds + from, C * KP * 2, t + 4 * i, p, lane, f);
+          store_frag(img + base + L::cols(t + 4 * i, p), lane, f);
+        }
+    };
+    put(L::kK, 0, wave);
+    put(L::kQ, kRows, wave);
+    put_t(L::kKT, 0, wave);
+    if (keep) put_t(L::kQT, kRows, wave);
+  }
   // k k^T, rows 16 wave ...; q k^T, rows 16 (3 - wave) ...: five blocks of the lower triangles each, transposed: a
   // lane has one row and four consecutive columns
   const int wq = 3 - wave;
@@ -409,31 +484,21 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
   }
   __syncthreads();
   {
-    const int ra = 16 * wave + m, rp = 16 * wq + m;
-    const double ga = sG[ra], gp = sG[rp];
+    const int ra = 16 * wave + m;
+    const double ga = sG[ra];
     const float be = sB[ra];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int col = 16 * i + 4 * g;
-      f32x4 x = {0, 0, 0, 0}, p = x;
+      f32x4 x;
+      if (i <= wave) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const double gc = sG[col + r];
-        if (i <= wave) {
-          const float e = be * expf(col + r < ra ? static_cast<float>(ga - gc) : 0.0f) * kk[i][r];
+        for (int r = 0; r < 4; ++r) {
+          const float e = be * expf(col + r < ra ? static_cast<float>(ga - sG[col + r]) : 0.0f) * kk[i][r];
           x[r] = col + r < ra ? e : 0.0f;
         }
-        if (i <= wq) {
-          const float e = a.scale * expf(col + r <= rp ? static_cast<float>(gp - gc) : 0.0f) * qk[i][r];
-          p[r] = col + r <= rp ? e : 0.0f;
-        }
+        *reinterpret_cast<f32x4*>(sA + ra * LD + col) = x;
       }
-      if (i <= wave) *reinterpret_cast<f32x4*>(sA + ra * LD + col) = x;
-      uint2 l[L::NP];
-      split4<L::NP>(p, l);
-#pragma unroll
-      for (int j = 0; j < L::NP; ++j)
-        *reinterpret_cast<uint2*>(img + L::kP + j * kPlane * 2 + at<8>(rp, col >> 3) + (col & 7) * 2) = l[j];
     }
   }
   __syncthreads();
@@ -478,7 +543,24 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a) {
     put(i, j, x);
   }
   __syncthreads();
-  put_planes<3>(sT, img + L::kT, tid);
+  {  // P in A's place
+    const int rp = 16 * wq + m;
+    const double gp = sG[rp];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = 16 * i + 4 * g;
+      f32x4 x;
+      if (i <= wq) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[r] = a.scale * expf(col + r <= rp ? static_cast<float>(gp - sG[col + r]) : 0.0f) * qk[i][r];
+        *reinterpret_cast<f32x4*>(sA + rp * LD + col) = x;
+      }
+    }
+  }
+  put_blocks<3>(sT, img + L::kT, img + L::kTT, keep, lane, wave);
+  __syncthreads();
+  put_blocks<L::NP>(sA, img + L::kP, img + L::kPT, keep, lane, wave);
 }
 
 // ---------------------------------------------------------------- the pass over the chunks
@@ -510,21 +592,8 @@ __device__ __forceinline__ void place(int id, int BH, int tiles, int& bh, int& t
   }
 }
 
-template <int U, int N>
-__device__ __forceinline__ void frags(const char* m, int plane, int t, int kb, int lane, bf16x8 (&out)[N]) {
-#pragma unroll
-  for (int l = 0; l < N; ++l) out[l] = frag<U>(m + l * plane, t, kb, lane);
-}
-template <int U, bool PERM, int N>
-__device__ __forceinline__ void frags_t(const char* m, int plane, int t, int p, int lane, bf16x8 (&out)[N]) {
-#pragma unroll
-  for (int l = 0; l < N; ++l) out[l] = frag_t<U, PERM>(m + l * plane, t, p, lane);
-}
-
-// B operands in LDS, kFrag bytes per fragment and limb: fragment f of F, limb l at (l F + f) kFrag. The 16 bytes
-// past 1 KiB keep two halves' writes from being one instruction at distances that the compiler can merge: a merged
-// write is no longer known to miss the copies under way, and waits for all of them.
-constexpr int kFrag = 1040;
+// B operands in LDS, kFrag bytes per fragment and limb: fragment f of F, limb l at (l F + f) kFrag
+constexpr int kFrag = 1024;
 template <int F, int N>
 __device__ __forceinline__ void put_half(char* x, int f, int lane, int half, const uint2 (&v)[N]) {
 #pragma unroll
@@ -541,28 +610,12 @@ __device__ __forceinline__ void get(const char* x, int f, int lane, bf16x8 (&v)[
   for (int l = 0; l < N; ++l) v[l] = *reinterpret_cast<const bf16x8*>(x + (l * F + f) * kFrag + lane * 16);
 }
 
-// All waves' LDS accesses so far are done, and all but this wave's last N memory operations
-template <int N>
-__device__ __forceinline__ void sync() {
-  if constexpr (N < 0)
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  else
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
+// All waves' LDS accesses so far are done; loads to registers stay under way
+__device__ __forceinline__ void sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// LDS of a pass, in arrays of their own: the compiler then knows that reading one need not wait for the
-// copies under way to the others. NX: fragments and limbs of the exchange besides the state's.
-template <int KP, int NI, int CT, int NX>
-struct Team {
-  using T_ = Tile<KP, NI>;
-  static constexpr int KB = KP / 32, NP = T_::NP;
-  static constexpr int nK = NI * C * KP * 2, nT = 3 * kPlane * 2, nP = NP * kPlane * 2, nS = CT * KB * 3 * kFrag, nX = CT * NX * kFrag;
-  // k and the vectors twice (they are read to the end of a chunk, and at once in the next), where that fits
-  static constexpr bool kDouble = 3 * nK + nT + nP + 2048 + nS + nX <= 160 * 1024;
-  static constexpr int nK1 = kDouble ? nK : 16, nX1 = kDouble ? nX : 16, nG1 = kDouble ? 256 : 4;  // (else not used)
-  static constexpr int cK = nK / 4096, cT = nT / 4096, cP = nP / 4096;        // copies a wave
-  static_assert(kDouble || 2 * nK + nT + nP + 1024 + 64 + nS <= 160 * 1024, "the pass fits in LDS");
-};
+// All loads so far are there, as far as the compiler's own waits go too: what it counts in a loop are then the
+// loop's operations alone (0x0f70: vmcnt 0, the other counters as they are)
+__device__ __forceinline__ void settled() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // What a wave of a pass works on
 template <int CT>
@@ -606,7 +659,7 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[CT][2], float* s, c
 template <int KP, int NI, int CT, typename P>
 __device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, bf16_t* kept, int64_t c, const Args& a, const P& p) {
   constexpr int NW = kKept<NI>, U = KP / 8;
-  if (p.w < KP / 32) {
+  if (KP == 128 || p.w < KP / 32) {  // (four waves)
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
       const float x[8] = {S[i][0][0], S[i][0][1], S[i][0][2], S[i][0][3], S[i][1][0], S[i][1][1], S[i][1][2], S[i][1][3]};
@@ -630,31 +683,27 @@ __device__ __forceinline__ void keep_half(bf16_t* kept, int64_t c, int col, cons
   for (int q = 0; q < NW; ++q) *reinterpret_cast<uint2*>(img + q * 32 * C * 2) = l[q];
 }
 
-// Fragments of the exchange besides the state's: y, e^{G_C - G} d, d; and dd, -e^G beta dy, scale e^G do, do
-template <int NI> constexpr int kStateX = 2 * 3 + 2 * 3 + 2 * (NI == 3 ? 3 : 2);
-template <int NI> constexpr int kGradX = 3 * 2 * 3 + 2 * NI;
-
 template <int KP, int NI, bool KEEP, int CT>
 __global__ __launch_bounds__(256) void state_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
-  using L = Team<KP, NI, CT, kStateX<NI>>;
-  constexpr int KB = KP / 32, NP = L::NP, U = KP / 8, NW = kKept<NI>;
-  __shared__ __attribute__((aligned(16))) char lk0[L::nK], lk1[L::nK1], lq[L::nK], lt[L::nT], lp[L::nP], ls[L::nS], lx[L::nX1];
-  __shared__ __attribute__((aligned(16))) float lg0[256], lg1[L::nG1];
+  constexpr int KB = I::KB, NP = I::NP;
+  __shared__ __attribute__((aligned(16))) char xs[CT * KB * 3 * kFrag], xy[CT * 6 * kFrag], xe[CT * 6 * kFrag], xd[CT * 2 * NP * kFrag];
   const Place<CT> p(a);
   const int lane = p.lane, g = p.g, w = p.w, pw = w / 2;
-  // (without room of its own the exchange lies over q, which is read before it)
-  char *xs = ls, *xy = L::kDouble ? lx : lq, *xe = xy + CT * 6 * kFrag, *xd = xe + CT * 6 * kFrag;
   const int64_t o_st = static_cast<int64_t>(a.H) * a.V;
   const E* v = reinterpret_cast<const E*>(a.v) + p.b * a.v_sb + p.h * a.v_sh;
   E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
   const uint32_t vs = static_cast<uint32_t>(a.v_st * sizeof(E)), os = static_cast<uint32_t>(o_st * sizeof(E));
   const int row = row_of(w, 4 * g);  // the lane's first of four tokens
-  const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * I::kBytes;
-  const auto image = [&](int n) { return img + static_cast<int64_t>(n) * I::kBytes; };
+  constexpr int64_t kImage = KEEP ? I::kKept : I::kOnce;
+  const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * kImage;
 
-  uint32_t next[CT][4];  // v of a chunk, loaded one chunk ahead
+  // What a chunk takes from memory, each loaded anew for the next chunk once its last reader is through
+  uint32_t next[CT][4];
+  bf16x8 fk[KB][NI], fq[KB][NI], ft[2][3], fp[2][NP], kt[2][2][NI];
+  f32x4 eg, tail, be;
+  float last;
   const auto load_v = [&](int n) {
     const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
 #pragma unroll
@@ -662,155 +711,148 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(vr, p.col(i) < a.V ? row * vs + p.col(i) * sizeof(E) : kOutOfRange, r * vs);
   };
-  f32x4 S[CT][2];
-  load_state(S, a.h0, a, p);
-  load_v(0);
-  stage<L::nK, 4>(lk0, image(0) + I::kK, lane, w);
-  stage<L::nK, 4>(lq, image(0) + I::kQ, lane, w);
-  stage<L::nT, 4>(lt, image(0) + I::kT, lane, w);
-  stage<1024, 1>(reinterpret_cast<char*>(lg0), image(0) + I::kGate, lane, 0);
-  if constexpr (!L::kDouble) stage<L::nP, 4>(lp, image(0) + I::kP, lane, w);
-  publish<KP, NI>(S, xs, KEEP ? a.Sw : nullptr, static_cast<int64_t>(p.bh) * a.NC, a, p);
-  sync<0>();
-  // Memory operations complete in order, and a wait leaves those in flight that were issued after the copies it is for.
-  // What every wave issues after T's copies to the chunk's end: kept d's, the state's (if all waves have some), o's stores
-  constexpr int kLater = 4 * CT + (KEEP ? NW * CT * (KB == 4 ? 2 : 1) : 0);
-  const auto chunk = [&](int n, char* ck, char* nk, float* gt, float* ng) __attribute__((always_inline)) {
-    const int t0 = n * C, rows = min(C, a.T - t0), n1 = min(n + 1, a.NC - 1);  // (the last chunk's copies bring it once more)
-    const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
-    f32x4 vv[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) vv[i][r] = value<E>(next[i][r]);
-    if constexpr (L::kDouble) {
-      stage<L::nP, 4>(lp, image(n) + I::kP, lane, w);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    load_v(n1);
-    if constexpr (L::kDouble) {
-      stage<1024, 1>(reinterpret_cast<char*>(ng), image(n1) + I::kGate, lane, 0);
-      stage<L::nK, 4>(nk, image(n1) + I::kK, lane, w);
-    }
-    const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
-    const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row);
-    const float last = gt[63];
-    // y and the state's part of o: this wave's 16 tokens
-    f32x4 ks[CT], oa[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) ks[i] = oa[i] = f32x4{0, 0, 0, 0};
+  const auto load_rows = [&](int n) {
+    const char* x = img + n * kImage;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      bf16x8 fk[NI], fq[NI];
-      frags<U>(ck, C * KP * 2, w, kb, lane, fk);
-      frags<U>(lq, C * KP * 2, w, kb, lane, fq);
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        bf16x8 sb[3];
-        get<CT * KB>(xs, i * KB + kb, lane, sb);
-        ks[i] = mm<3>(fk, sb, ks[i]);
-        oa[i] = mm<NP>(fq, sb, oa[i]);  // (only o, which is rounded to the inputs' type, sees this product)
-      }
-    }
-    if constexpr (!L::kDouble) sync<-1>();  // (the exchange lies over q)
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      uint2 l[3];
-      split4(be * (vv[i] - eg * ks[i]), l);
-      put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
-      oa[i] *= a.scale * eg;
-    }
-    sync<L::kDouble ? kLater + L::cP + 4 * CT + 1 + L::cK : -1>();  // y is there, and T
-    if constexpr (L::kDouble) stage<L::nK, 4>(lq, image(n1) + I::kQ, lane, w);
-    f32x4 d[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) d[i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q <= pw) {
-        bf16x8 ft[3];
-        frags<8>(lt, kPlane * 2, w, q, lane, ft);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          bf16x8 yb[3];
-          get<2 * CT>(xy, 2 * i + q, lane, yb);
-          d[i] = mm<3>(ft, yb, d[i]);
-        }
-      }
-    }
-    uint2 dl[CT][NP];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      uint2 l[3];
-      split4(tail * d[i], l);
-      put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
-      split4(d[i], dl[i]);
-      put_half<2 * CT>(xd, 2 * i + pw, lane, w & 1, dl[i]);
-    }
-    sync<L::kDouble ? 4 * CT + 1 + 2 * L::cK : -1>();  // d is there, and P
-    if constexpr (L::kDouble) {
-      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (KEEP) {
-#pragma unroll
-      for (int i = 0; i < CT; ++i) keep_half<NI>(a.dw, c, p.col(i), dl[i], a, p);
-    }
-    if (w < KB) {
-#pragma unroll
-      for (int i = 0; i < CT; ++i) S[i][0] *= last, S[i][1] *= last;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        bf16x8 f0[NI], f1[NI];
-        frags_t<U, true>(ck, C * KP * 2, 2 * w, q, lane, f0);
-        frags_t<U, true>(ck, C * KP * 2, 2 * w + 1, q, lane, f1);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          bf16x8 eb[3];
-          get<2 * CT>(xe, 2 * i + q, lane, eb);
-          S[i][0] = mm<3>(f0, eb, S[i][0]);
-          S[i][1] = mm<3>(f1, eb, S[i][1]);
-        }
-      }
-    }
-    publish<KP, NI>(S, xs, KEEP && n + 1 < a.NC ? a.Sw : nullptr, c + 1, a, p);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q <= pw) {
-        bf16x8 fp[NP];
-        frags<8>(lp, kPlane * 2, w, q, lane, fp);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          bf16x8 db[NP];
-          get<2 * CT>(xd, 2 * i + q, lane, db);
-          oa[i] = mm<NP>(fp, db, oa[i]);
-        }
-      }
-    }
-    const __amdgpu_buffer_rsrc_t orr = rows_buffer(o + t0 * o_st, o_st, rows, a.V);
-#pragma unroll
-    for (int i = 0; i < CT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, oa[i][r]);
-    if constexpr (L::kDouble) {
-      sync<L::cT + kLater>();  // the state is there, and k, q and the vectors
-    } else {
-      sync<-1>();
-      stage<1024, 1>(reinterpret_cast<char*>(gt), image(n1) + I::kGate, lane, 0);
-      stage<L::nK, 4>(ck, image(n1) + I::kK, lane, w);
-      stage<L::nK, 4>(lq, image(n1) + I::kQ, lane, w);
-      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
-      stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
-      sync<0>();
+      load_frag(x + I::kK + I::rows(w, kb), lane, fk[kb]);
+      load_frag(x + I::kQ + I::rows(w, kb), lane, fq[kb]);
     }
   };
-  for (int n = 0;;) {
-    chunk(n, lk0, L::kDouble ? lk1 : lk0, lg0, L::kDouble ? lg1 : lg0);
-    if (++n >= a.NC) break;
-    chunk(n, L::kDouble ? lk1 : lk0, lk0, L::kDouble ? lg1 : lg0, lg0);
-    if (++n >= a.NC) break;
-  }
+  const auto load_gates = [&](int n) {
+    const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
+    eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
+    be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63];
+  };
+  const auto load_t = [&](auto half, int n) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (q <= half.value) load_frag(img + n * kImage + I::kT + I::low(w, q, 3), lane, ft[q]);
+  };
+  const auto load_p = [&](auto half, int n) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (q <= half.value) load_frag(img + n * kImage + I::kP + I::low(w, q, NP), lane, fp[q]);
+  };
+  const auto load_cols = [&](int n) {
+    if (KB == 4 || w < KB) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) load_frag(img + n * kImage + I::kKT + I::cols(2 * w + t, q), lane, kt[t][q]);
+    }
+  };
+  f32x4 S[CT][2];
+  load_state(S, a.h0, a, p);
+  // (a loop for each half of the waves: how many blocks of T and P a wave has is then known, and so is how many
+  // operations later than its loads a wait may leave under way)
+  const auto run = [&](auto half) __attribute__((always_inline)) {
+    load_rows(0), load_gates(0), load_v(0), load_t(half, 0), load_cols(0), load_p(half, 0);
+    publish<KP, NI>(S, xs, KEEP ? a.Sw : nullptr, static_cast<int64_t>(p.bh) * a.NC, a, p);
+    settled();
+    sync();
+#pragma unroll 1
+    for (int n = 0; n < a.NC; ++n) {
+      const int t0 = n * C, rows = min(C, a.T - t0), n1 = min(n + 1, a.NC - 1);  // (the last chunk loads itself once more)
+      const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
+      // y and the state's part of o: this wave's 16 tokens
+      f32x4 ks[CT], oa[CT];
+#pragma unroll
+      for (int i = 0; i < CT; ++i) ks[i] = oa[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 sb[3];
+          get<CT * KB>(xs, i * KB + kb, lane, sb);
+          ks[i] = mm<3>(fk[kb], sb, ks[i]);
+          oa[i] = mm<NP>(fq[kb], sb, oa[i]);  // (only o, which is rounded to the inputs' type, sees this product)
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        f32x4 vv;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vv[r] = value<E>(next[i][r]);
+        uint2 l[3];
+        split4(be * (vv - eg * ks[i]), l);
+        put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
+        oa[i] *= a.scale * eg;
+      }
+      const f32x4 tl = tail;
+      const float decay = last;
+      load_rows(n1), load_gates(n1), load_v(n1);
+      sync();  // y is there
+      f32x4 d[CT];
+#pragma unroll
+      for (int i = 0; i < CT; ++i) d[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (q <= half.value) {
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            bf16x8 yb[3];
+            get<2 * CT>(xy, 2 * i + q, lane, yb);
+            d[i] = mm<3>(ft[q], yb, d[i]);
+          }
+        }
+      }
+      uint2 dl[CT][NP];
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        uint2 l[3];
+        split4(tl * d[i], l);
+        put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
+        split4(d[i], dl[i]);
+        put_half<2 * CT>(xd, 2 * i + pw, lane, w & 1, dl[i]);
+      }
+      load_t(half, n1);
+      sync();  // d is there
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) keep_half<NI>(a.dw, c, p.col(i), dl[i], a, p);
+      }
+      if (KB == 4 || w < KB) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) S[i][0] *= decay, S[i][1] *= decay;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            bf16x8 eb[3];
+            get<2 * CT>(xe, 2 * i + q, lane, eb);
+            S[i][0] = mm<3>(kt[0][q], eb, S[i][0]);
+            S[i][1] = mm<3>(kt[1][q], eb, S[i][1]);
+          }
+        }
+      }
+      load_cols(n1);
+      publish<KP, NI>(S, xs, KEEP && n + 1 < a.NC ? a.Sw : nullptr, c + 1, a, p);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (q <= half.value) {
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            bf16x8 db[NP];
+            get<2 * CT>(xd, 2 * i + q, lane, db);
+            oa[i] = mm<NP>(fp[q], db, oa[i]);
+          }
+        }
+      }
+      load_p(half, n1);
+      const __amdgpu_buffer_rsrc_t orr = rows_buffer(o + t0 * o_st, o_st, rows, a.V);
+#pragma unroll
+      for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, oa[i][r]);
+      sync();  // the state is there
+    }
+  };
+  if (pw == 0)
+    run(int_c<0>{});
+  else
+    run(int_c<1>{});
   if (a.state && w < KB) store_state(S, a.state, a, p);
 }
 
@@ -818,25 +860,23 @@ template <int KP, int NI, int CT>
 __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
-  using L = Team<KP, NI, CT, kGradX<NI>>;
-  constexpr int KB = KP / 32, NP = L::NP, U = KP / 8, NW = kKept<NI>;
-  __shared__ __attribute__((aligned(16))) char lk0[L::nK], lk1[L::nK1], lq[L::nK], lt[L::nT], lp[L::nP], ls[L::nS], lx[L::nX1];
-  __shared__ __attribute__((aligned(16))) float lg0[256], lg1[L::nG1];
+  constexpr int KB = I::KB, NP = I::NP, NW = kKept<NI>;
+  __shared__ __attribute__((aligned(16))) char xs[CT * KB * 3 * kFrag], xy[CT * 6 * kFrag], xe[CT * 6 * kFrag], xu[CT * 6 * kFrag], xo[CT * 2 * NI * kFrag];
   const Place<CT> p(a);
   const int lane = p.lane, g = p.g, w = p.w, pw = w / 2;
-  // without room of its own the exchange lies over P, which is read before it, and do's over q, which comes after it
-  char *xs = ls, *xy = L::kDouble ? lx : lp, *xe = xy + CT * 6 * kFrag, *xu = xe + CT * 6 * kFrag;
-  char* xo = L::kDouble ? xu + CT * 6 * kFrag : lq;
   const int64_t v_st = static_cast<int64_t>(a.H) * a.V;
   const E* dout = reinterpret_cast<const E*>(a.dout) + p.b * a.do_sb + p.h * a.do_sh;
   E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
   const uint32_t is = static_cast<uint32_t>(a.do_st * sizeof(E)), os = static_cast<uint32_t>(v_st * sizeof(E));
   const int row = row_of(w, 4 * g);
-  const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * I::kBytes;
-  const auto image = [&](int n) { return img + static_cast<int64_t>(n) * I::kBytes; };
+  constexpr int64_t kImage = I::kKept;
+  const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * kImage;
 
-  uint32_t next[CT][4];  // do of a chunk, loaded one chunk ahead
+  uint32_t next[CT][4];  // do of a chunk
   f32x4 go[CT];
+  bf16x8 fk[KB][NI], ft[2][3], fp[2][NP], kt[2][2][NI], qt[2][2][NI];
+  f32x4 eg, tail, be;
+  float last;
   const auto load_go = [&](int n) {
     const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
 #pragma unroll
@@ -854,160 +894,154 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
       put_half<2 * CT>(xo, 2 * i + pw, lane, w & 1, l);
     }
   };
+  const auto load_rows = [&](int n) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) load_frag(img + n * kImage + I::kK + I::rows(w, kb), lane, fk[kb]);
+  };
+  const auto load_gates = [&](int n) {
+    const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
+    eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
+    be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63];
+  };
+  const auto load_t = [&](auto half, int n) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (q >= half.value) load_frag(img + n * kImage + I::kTT + I::high(w, q, 3), lane, ft[q]);
+  };
+  const auto load_p = [&](auto half, int n) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (q >= half.value) load_frag(img + n * kImage + I::kPT + I::high(w, q, NP), lane, fp[q]);
+  };
+  const auto load_cols = [&](int n) {
+    if (KB == 4 || w < KB) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          load_frag(img + n * kImage + I::kKT + I::cols(2 * w + t, q), lane, kt[t][q]);
+          load_frag(img + n * kImage + I::kQT + I::cols(2 * w + t, q), lane, qt[t][q]);
+        }
+    }
+  };
   f32x4 S[CT][2];  // the gradient of the state
   load_state(S, a.dstate, a, p);
   const int last_n = a.NC - 1;
-  load_go(last_n);
-  stage<L::nK, 4>(lk0, image(last_n) + I::kK, lane, w);
-  stage<1024, 1>(reinterpret_cast<char*>(lg0), image(last_n) + I::kGate, lane, 0);
-  stage<L::nT, 4>(lt, image(last_n) + I::kT, lane, w);
-  stage<L::nP, 4>(lp, image(last_n) + I::kP, lane, w);
-  put_go();
-  publish<KP, NI>(S, xs, a.dSw, static_cast<int64_t>(p.bh) * a.NC + last_n, a, p);
-  sync<0>();
-  constexpr int kLater = NW * CT * (KB == 4 ? 2 : 1);  // after T's copies to the chunk's end: kept dy's, the state's
-  const auto chunk = [&](int n, char* ck, char* nk, float* gt, float* ng) __attribute__((always_inline)) {
-    const int t0 = n * C, rows = min(C, a.T - t0), n1 = max(n - 1, 0);  // (the last chunk's copies bring it once more)
-    const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
-    if constexpr (L::kDouble) {
-      stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    load_go(n1);
-    if constexpr (L::kDouble) {
-      stage<1024, 1>(reinterpret_cast<char*>(ng), image(n1) + I::kGate, lane, 0);
-      stage<L::nK, 4>(nk, image(n1) + I::kK, lane, w);
-    }
-    const f32x4 eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
-    const f32x4 be = *reinterpret_cast<const f32x4*>(gt + 128 + row);
-    const float last = gt[63];
-    f32x4 dd[CT];
+  // (a loop for each half of the waves: how many blocks of T and P a wave has is then known, and so is how many
+  // operations later than its loads a wait may leave under way)
+  const auto run = [&](auto half) __attribute__((always_inline)) {
+    load_go(last_n), load_rows(last_n), load_gates(last_n), load_p(half, last_n), load_t(half, last_n), load_cols(last_n);
+    put_go();
+    load_go(max(last_n - 1, 0));
+    publish<KP, NI>(S, xs, a.dSw, static_cast<int64_t>(p.bh) * a.NC + last_n, a, p);
+    settled();
+    sync();
+#pragma unroll 1
+    for (int n = last_n; n >= 0; --n) {
+      const int t0 = n * C, rows = min(C, a.T - t0), n1 = max(n - 1, 0);  // (the last chunk loads itself once more)
+      const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
+      f32x4 dd[CT];
 #pragma unroll
-    for (int i = 0; i < CT; ++i) dd[i] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < CT; ++i) dd[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      bf16x8 f[NI];
-      frags<U>(ck, C * KP * 2, w, kb, lane, f);
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        bf16x8 sb[3];
-        get<CT * KB>(xs, i * KB + kb, lane, sb);
-        dd[i] = mm<3>(f, sb, dd[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < CT; ++i) dd[i] *= tail;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q >= pw) {
-        bf16x8 f[NP];
-        frags_t<8, true>(lp, kPlane * 2, w, q, lane, f);
+      for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
-          bf16x8 ob[NI];
-          get<2 * CT>(xo, 2 * i + q, lane, ob);
-          dd[i] = mm<3>(f, ob, dd[i]);
+          bf16x8 sb[3];
+          get<CT * KB>(xs, i * KB + kb, lane, sb);
+          dd[i] = mm<3>(fk[kb], sb, dd[i]);
         }
       }
-    }
-    if constexpr (!L::kDouble) sync<-1>();
+      load_rows(n1);
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      uint2 l[3];
-      split4(dd[i], l);
-      put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
-    }
-    sync<L::kDouble ? kLater + 4 * CT + 1 + 2 * L::cK : -1>();  // dd is there, and T
-    if constexpr (L::kDouble) {
-      stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
-      __builtin_amdgcn_sched_barrier(0);
-    } else
-      stage<L::nK, 4>(lq, image(n) + I::kQ, lane, w);
-    f32x4 dy[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) dy[i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q >= pw) {
-        bf16x8 f[3];
-        frags_t<8, true>(lt, kPlane * 2, w, q, lane, f);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          bf16x8 b[3];
-          get<2 * CT>(xy, 2 * i + q, lane, b);
-          dy[i] = mm<3>(f, b, dy[i]);
-        }
-      }
-    }
-    const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const f32x4 x = be * dy[i];
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, x[r]);
-      uint2 l[3];
-      split4(-eg * x, l);
-      put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
-      split4(a.scale * eg * go[i], l);
-      put_half<2 * CT>(xu, 2 * i + pw, lane, w & 1, l);
-    }
-    sync<L::kDouble ? 4 * CT + 1 + L::cK + L::cP + 4 * CT : 0>();  // they are there, and q
-    if constexpr (L::kDouble) {
-      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      uint2 l[NW];
-      split4(dy[i], l);
-      keep_half<NI>(a.yw, c, p.col(i), l, a, p);
-    }
-    if (w < KB) {
-#pragma unroll
-      for (int i = 0; i < CT; ++i) S[i][0] *= last, S[i][1] *= last;
+      for (int i = 0; i < CT; ++i) dd[i] *= tail;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        bf16x8 k0[NI], k1[NI], q0[NI], q1[NI];
-        frags_t<U, true>(ck, C * KP * 2, 2 * w, q, lane, k0);
-        frags_t<U, true>(ck, C * KP * 2, 2 * w + 1, q, lane, k1);
-        frags_t<U, true>(lq, C * KP * 2, 2 * w, q, lane, q0);
-        frags_t<U, true>(lq, C * KP * 2, 2 * w + 1, q, lane, q1);
+        if (q >= half.value) {
 #pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          bf16x8 b[3];
-          get<2 * CT>(xe, 2 * i + q, lane, b);
-          S[i][0] = mm<3>(k0, b, S[i][0]);
-          S[i][1] = mm<3>(k1, b, S[i][1]);
-          get<2 * CT>(xu, 2 * i + q, lane, b);
-          S[i][0] = mm<3>(q0, b, S[i][0]);
-          S[i][1] = mm<3>(q1, b, S[i][1]);
+          for (int i = 0; i < CT; ++i) {
+            bf16x8 ob[NI];
+            get<2 * CT>(xo, 2 * i + q, lane, ob);
+            dd[i] = mm<3>(fp[q], ob, dd[i]);
+          }
         }
       }
-    }
-    if constexpr (L::kDouble) {
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        uint2 l[3];
+        split4(dd[i], l);
+        put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
+      }
+      load_p(half, n1);
+      sync();  // dd is there
+      f32x4 dy[CT];
+#pragma unroll
+      for (int i = 0; i < CT; ++i) dy[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (q >= half.value) {
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            bf16x8 b[3];
+            get<2 * CT>(xy, 2 * i + q, lane, b);
+            dy[i] = mm<3>(ft[q], b, dy[i]);
+          }
+        }
+      }
+      load_t(half, n1);
+      const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        const f32x4 x = be * dy[i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, x[r]);
+        uint2 l[3];
+        split4(-eg * x, l);
+        put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
+        split4(a.scale * eg * go[i], l);
+        put_half<2 * CT>(xu, 2 * i + pw, lane, w & 1, l);
+      }
+      const float decay = last;
+      load_gates(n1);
+      sync();  // they are there
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        uint2 l[NW];
+        split4(dy[i], l);
+        keep_half<NI>(a.yw, c, p.col(i), l, a, p);
+      }
+      if (KB == 4 || w < KB) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) S[i][0] *= decay, S[i][1] *= decay;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            bf16x8 b[3];
+            get<2 * CT>(xe, 2 * i + q, lane, b);
+            S[i][0] = mm<3>(kt[0][q], b, S[i][0]);
+            S[i][1] = mm<3>(kt[1][q], b, S[i][1]);
+            get<2 * CT>(xu, 2 * i + q, lane, b);
+            S[i][0] = mm<3>(qt[0][q], b, S[i][0]);
+            S[i][1] = mm<3>(qt[1][q], b, S[i][1]);
+          }
+        }
+      }
+      load_cols(n1);
       put_go();
+      load_go(max(n - 2, 0));
       publish<KP, NI>(S, xs, n > 0 ? a.dSw : nullptr, c - 1, a, p);
-      sync<4 * CT + L::cT + kLater>();  // the state and do are there, and k, P and the vectors
-    } else {
-      sync<-1>();
-      stage<L::nK, 4>(ck, image(n1) + I::kK, lane, w);
-      stage<1024, 1>(reinterpret_cast<char*>(gt), image(n1) + I::kGate, lane, 0);
-      stage<L::nT, 4>(lt, image(n1) + I::kT, lane, w);
-      stage<L::nP, 4>(lp, image(n1) + I::kP, lane, w);
-      put_go();
-      publish<KP, NI>(S, xs, n > 0 ? a.dSw : nullptr, c - 1, a, p);
-      sync<0>();
+      sync();  // the state and do are there
     }
   };
-  for (int n = last_n;;) {
-    chunk(n, lk0, L::kDouble ? lk1 : lk0, lg0, L::kDouble ? lg1 : lg0);
-    if (--n < 0) break;
-    chunk(n, L::kDouble ? lk1 : lk0, lk0, L::kDouble ? lg1 : lg0, lg0);
-    if (--n < 0) break;
-  }
+  if (pw == 0)
+    run(int_c<0>{});
+  else
+    run(int_c<1>{});
   if (a.dh0 && w < KB) store_state(S, a.dh0, a, p);
 }
+
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
 
 template <int KP, int NI>
@@ -1033,6 +1067,7 @@ template <int KP, int NI>
 __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) void grad_kernel(Args a) {
   using E = typename elem<NI>::type;
   using L = GradTile<KP, NI>;
+  using I = Tile<KP, NI>;
   constexpr int NW = L::NW, U = KP / 8, W = L::W;
   __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
@@ -1040,7 +1075,7 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
   const int bh = blockIdx.x / a.NC, n = blockIdx.x - bh * a.NC, h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
   const int hk = h / grp, t0 = n * C, rows = min(C, a.T - t0);
   float* vec = reinterpret_cast<float*>(lds + L::kSums);
-  const char* img = a.img + c * Tile<KP, NI>::kBytes;
+  const char* img = a.img + c * I::kKept;
   const float* gt = reinterpret_cast<const float*>(lds + L::kGate);
   const double* Gd = reinterpret_cast<const double*>(lds + L::kG);
 
@@ -1070,9 +1105,9 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     for (int q = 0; q < NI; ++q) out[q] = *reinterpret_cast<const bf16x8*>(lds + base + q * C * 64 + at4(16 * t + (ln & 15), ln >> 4));
   };
   load_rows(0);
-  stage<L::kS, W>(lds + L::kK, img, lane, wave);
+  stage<I::kRows, W>(lds + L::kK, img + I::kK, lane, wave);
   if (wave == 0) {
-    reinterpret_cast<float4*>(lds + L::kGate)[lane] = reinterpret_cast<const float4*>(img + Tile<KP, NI>::kGate)[lane];
+    reinterpret_cast<float4*>(lds + L::kGate)[lane] = reinterpret_cast<const float4*>(img + I::kGate)[lane];
     reinterpret_cast<double*>(lds + L::kG)[lane] = a.Gd[c * 64 + lane];
   }
   float gv = 0.0f;
@@ -1130,7 +1165,7 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     }
   }
   __syncthreads();
-  stage<L::kS, W>(lds + L::kQ, img + L::kS, lane, wave);  // (k, then q, in the image)
+  stage<I::kRows, W>(lds + L::kQ, img + I::kQ, lane, wave);
   // F and N, in this wave's rows, to LDS
   const auto put = [&](int plane, int row, int col, const f32x4& x) {
     uint2 l[NW];
@@ -1178,7 +1213,7 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     f32x4 x = {0, 0, 0, 0};
 #pragma unroll
     for (int l = 0; l < NI; ++l) {
-      const uint2 u = *reinterpret_cast<const uint2*>(lds + base + l * C * KP * 2 + at<U>(row, d >> 3) + (d & 7) * 2);
+      const uint2 u = *reinterpret_cast<const uint2*>(lds + base + l * 1024 + I::unit(row, d >> 3) + (d & 7) * 2);
       x[0] += __uint_as_float(u.x << 16), x[1] += __uint_as_float(u.x & 0xffff0000u);
       x[2] += __uint_as_float(u.y << 16), x[3] += __uint_as_float(u.y & 0xffff0000u);
     }
@@ -1193,8 +1228,8 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     bf16x8 kf[NI], qf[NI], bk[NW];
-    frags_t<U, false>(lds + L::kK, C * KP * 2, wave, p, lane, kf);
-    frags_t<U, false>(lds + L::kQ, C * KP * 2, wave, p, lane, qf);
+    frags_t_image<I>(lds + L::kK, wave, p, lane, kf);
+    frags_t_image<I>(lds + L::kQ, wave, p, lane, qf);
     {
       float x[8];
 #pragma unroll
@@ -1373,15 +1408,17 @@ struct Layout {  // byte offsets of the forward's buffer
 inline int vpad(int V) { return (V + 31) / 32 * 32; }
 inline int64_t chunks(const mg_delta_dims& s) { return (static_cast<int64_t>(s.T) + C - 1) / C; }
 
+template <int KP, int NI>
+inline size_t image_bytes(bool keep) { return keep ? Tile<KP, NI>::kKept : Tile<KP, NI>::kOnce; }
 inline Layout layout(int dtype, const mg_delta_dims& s, bool keep_) {
   const size_t n = static_cast<size_t>(chunks(s)), bh = static_cast<size_t>(s.B) * s.H, c = bh * n;
-  const size_t vp = vpad(s.V), image = dtype == MG_F32 ? (s.K <= 64 ? Tile<64, 3>::kBytes : Tile<128, 3>::kBytes)
-                                                       : (s.K <= 64 ? Tile<64, 1>::kBytes : Tile<128, 1>::kBytes);
+  const size_t vp = vpad(s.V), nw = dtype == MG_F32 ? 3 : 2;
+  const size_t image = dtype == MG_F32 ? (s.K <= 64 ? image_bytes<64, 3>(keep_) : image_bytes<128, 3>(keep_))
+                                       : (s.K <= 64 ? image_bytes<64, 1>(keep_) : image_bytes<128, 1>(keep_));
   Layout l;
   l.img = 0;
   l.G = c * image;
   l.S = l.G + c * 512;
-  const size_t nw = dtype == MG_F32 ? 3 : 2;
   l.d = l.S + (keep_ ? c * vp * nw * (s.K <= 64 ? 64 : 128) * 2 : 0);
   l.end = l.d + (keep_ ? c * vp * nw * C * 2 : 0);
   return l;
@@ -1447,7 +1484,7 @@ inline void fill(Args& a, const mg_delta_dims& s, float scale, const mg_rows* q,
 template <int KP, int NI>
 int launch_fwd(const Args& a, bool keep_, hipStream_t st_) {
   const int64_t bh = static_cast<int64_t>(a.B) * a.H;
-  hipLaunchKernelGGL((chunk_kernel<KP, NI>), dim3(bh * a.NC), dim3(256), 0, st_, a);
+  hipLaunchKernelGGL((chunk_kernel<KP, NI>), dim3(bh * a.NC), dim3(256), 0, st_, a, keep_);
   const int ct = columns_for(bh, a.VP, NI);
   const dim3 grid(bh * (a.VP / 16 / ct));
   if constexpr (NI == 1) {
