@@ -72,14 +72,14 @@ struct Args {
   // chunk data, index c = (b H + h) NC + n
   char* img;             // [c][Tile::kBytes]: the chunk's operands as they lie in LDS
   double* Gd;            // [c][64]
-  bf16_t* Sw;            // kept for the backward: each chunk's entry state, [c][VP / 32][NW][32][KP]
-  bf16_t* dw;            // d, [c][VP / 32][NW][32][64]
+  char* Sw;            // kept for the backward: each chunk's entry state, [c][VP / 32][Kept::kState]
+  char* dw;            // d, [c][VP / 32][Kept::kVec]
   // backward
   const char* dout;      // [B, T, H, V]
   int64_t do_sb, do_st, do_sh;
   const float* dstate;   // or null
-  bf16_t* dSw;           // the gradients of the exit states, as Sw
-  bf16_t* yw;            // dy, as dw
+  char* dSw;           // the gradients of the exit states, as Sw
+  char* yw;            // dy, as dw
   char *dq, *dk, *dv, *dg, *db;
   float* dh0;
   float *dqp, *dkp;      // shared heads: [B, T, H, K] before their sum
@@ -178,6 +178,19 @@ __device__ __forceinline__ void store_col(__amdgpu_buffer_rsrc_t r, uint32_t off
     __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x), r, off, row_off, 0);
   else
     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, off, row_off, 0);
+}
+
+// four columns of a row
+template <typename E>
+__device__ __forceinline__ void store_cols(__amdgpu_buffer_rsrc_t r, uint32_t off, const f32x4& x) {
+  if constexpr (sizeof(E) == 2) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 v = {static_cast<uint32_t>(f32_to_bf16(x[0])) | static_cast<uint32_t>(f32_to_bf16(x[1])) << 16,
+                     static_cast<uint32_t>(f32_to_bf16(x[2])) | static_cast<uint32_t>(f32_to_bf16(x[3])) << 16};
+    __builtin_amdgcn_raw_buffer_store_b64(v, r, off, 0, 0);
+  } else {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, off, 0, 0);
+  }
 }
 
 // 8 values at any alignment: where one row's start and its length are multiples of 8 elements the memory
@@ -655,10 +668,37 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[CT][2], float* s, c
       }
 }
 
-// This wave's rows of the state to the other waves and, where kept, to memory: [columns][rows] images
+// What is kept of 32 value columns for the gradients, in the order of the accumulators, so that a wave writes whole
+// lines: S and dS' [16 columns][32 of K][limb], unit g (8 of K) of column m at 16 g + m; d and dy [16 columns]
+// [32 tokens][limb][wave's half], four tokens of column m at 16 g + m. Odd units and halves have m ^ 4: grad_kernel
+// reads across the columns, and these land on other banks then.
+template <int KP, int NI>
+struct Kept {
+  static constexpr int NW = kKept<NI>, kState = 2 * (KP / 32) * NW * 1024, kVec = 2 * 2 * NW * 1024;  // bytes of 32 columns
+  __device__ static int state(int col, int u) {  // limb 0 of unit u
+    return ((col >> 4) * (KP / 32) + (u >> 2)) * NW * 1024 + (16 * (u & 3) + ((col & 15) ^ (4 * (u & 1)))) * 16;
+  }
+  __device__ static int vec(int col, int t) {  // limb 0 of tokens t ... t + 3 (t a multiple of 4)
+    const int h = (t >> 2) & 1;
+    return ((col >> 4) * 2 + (t >> 5)) * NW * 1024 + h * 512 + (16 * ((t >> 3) & 3) + ((col & 15) ^ (4 * h))) * 8;
+  }
+};
+// Operand through the transposing read as frag_t: columns 16 t ... (of K, tokens) of the matrix, its 32 rows (value columns)
+template <typename P, int N>
+__device__ __forceinline__ void kept_frags(const char* x, P pos, int lane, bf16x8 (&out)[N]) {
+  const int g = lane >> 4, j = (lane >> 2) & 3, q = lane & 3, a0 = pos(8 * g + j, q), a1 = pos(8 * g + j + 4, q);
+#pragma unroll
+  for (int l = 0; l < N; ++l) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + a0 + l * 1024));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + a1 + l * 1024));
+    out[l] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// This wave's rows of the state to the other waves and, where kept, to memory
 template <int KP, int NI, int CT, typename P>
-__device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, bf16_t* kept, int64_t c, const Args& a, const P& p) {
-  constexpr int NW = kKept<NI>, U = KP / 8;
+__device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, char* kept, int64_t c, const Args& a, const P& p) {
+  using L = Kept<KP, NI>;
   if (KP == 128 || p.w < KP / 32) {  // (four waves)
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
@@ -667,20 +707,20 @@ __device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, bf16_
       split<3>(x, l);
       put_full<CT * (KP / 32)>(xs, i * (KP / 32) + p.w, p.lane, l);
       if (kept) {
-        char* img = reinterpret_cast<char*>(kept + (c * (a.VP / 32) + p.col(i) / 32) * NW * 32 * KP) + at<U>(p.col(i) % 32, 4 * p.w + p.g);
+        char* out = kept + (c * (a.VP / 32) + p.col(i) / 32) * L::kState + L::state(p.col(i) % 32, 4 * p.w + p.g);
 #pragma unroll
-        for (int q = 0; q < NW; ++q) *reinterpret_cast<bf16x8*>(img + q * 32 * KP * 2) = l[q];
+        for (int q = 0; q < L::NW; ++q) *reinterpret_cast<bf16x8*>(out + q * 1024) = l[q];
       }
     }
   }
 }
-// Half a fragment of d or dy to its image
-template <int NI, typename P>
-__device__ __forceinline__ void keep_half(bf16_t* kept, int64_t c, int col, const uint2 (&l)[kKept<NI>], const Args& a, const P& p) {
-  constexpr int NW = kKept<NI>;
-  char* img = reinterpret_cast<char*>(kept + (c * (a.VP / 32) + col / 32) * NW * 32 * C) + at<8>(col % 32, 4 * (p.w / 2) + p.g) + 8 * (p.w & 1);
+// Half a fragment of d or dy
+template <int KP, int NI, typename P>
+__device__ __forceinline__ void keep_half(char* kept, int64_t c, int col, const uint2 (&l)[kKept<NI>], const Args& a, const P& p) {
+  using L = Kept<KP, NI>;
+  char* out = kept + (c * (a.VP / 32) + col / 32) * L::kVec + L::vec(col % 32, row_of(p.w, 4 * p.g));
 #pragma unroll
-  for (int q = 0; q < NW; ++q) *reinterpret_cast<uint2*>(img + q * 32 * C * 2) = l[q];
+  for (int q = 0; q < L::NW; ++q) *reinterpret_cast<uint2*>(out + q * 1024) = l[q];
 }
 
 template <int KP, int NI, bool KEEP, int CT>
@@ -703,7 +743,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
   uint32_t next[CT][4];
   bf16x8 fk[KB][NI], fq[KB][NI], ft[2][3], fp[2][NP], kt[2][2][NI];
   f32x4 eg, tail, be;
-  float last;
+  float last, eo;
   const auto load_v = [&](int n) {
     const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
 #pragma unroll
@@ -722,7 +762,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
   const auto load_gates = [&](int n) {
     const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
     eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
-    be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63];
+    be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63], eo = gt[row_of(w, p.m)];
   };
   const auto load_t = [&](auto half, int n) {
 #pragma unroll
@@ -766,7 +806,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
           bf16x8 sb[3];
           get<CT * KB>(xs, i * KB + kb, lane, sb);
           ks[i] = mm<3>(fk[kb], sb, ks[i]);
-          oa[i] = mm<NP>(fq[kb], sb, oa[i]);  // (only o, which is rounded to the inputs' type, sees this product)
+          oa[i] = mm<NP>(sb, fq[kb], oa[i]);  // (transposed: a lane has a token and four columns; only o, which is rounded to the inputs' type, sees this product)
         }
       }
 #pragma unroll
@@ -777,7 +817,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
         uint2 l[3];
         split4(be * (vv - eg * ks[i]), l);
         put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
-        oa[i] *= a.scale * eg;
+        oa[i] *= a.scale * eo;
       }
       const f32x4 tl = tail;
       const float decay = last;
@@ -810,7 +850,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
       sync();  // d is there
       if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < CT; ++i) keep_half<NI>(a.dw, c, p.col(i), dl[i], a, p);
+        for (int i = 0; i < CT; ++i) keep_half<KP, NI>(a.dw, c, p.col(i), dl[i], a, p);
       }
       if (KB == 4 || w < KB) {
 #pragma unroll
@@ -835,17 +875,17 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
           for (int i = 0; i < CT; ++i) {
             bf16x8 db[NP];
             get<2 * CT>(xd, 2 * i + q, lane, db);
-            oa[i] = mm<NP>(fp[q], db, oa[i]);
+            oa[i] = mm<NP>(db, fp[q], oa[i]);
           }
         }
       }
       load_p(half, n1);
       const __amdgpu_buffer_rsrc_t orr = rows_buffer(o + t0 * o_st, o_st, rows, a.V);
 #pragma unroll
-      for (int i = 0; i < CT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, oa[i][r]);
+      for (int i = 0; i < CT; ++i) {
+        const int col = (p.tile * CT + i) * 16 + 4 * g;
+        store_cols<E>(orr, col < a.V ? row_of(w, p.m) * os + col * sizeof(E) : kOutOfRange, oa[i]);
+      }
       sync();  // the state is there
     }
   };
@@ -1009,7 +1049,7 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
       for (int i = 0; i < CT; ++i) {
         uint2 l[NW];
         split4(dy[i], l);
-        keep_half<NI>(a.yw, c, p.col(i), l, a, p);
+        keep_half<KP, NI>(a.yw, c, p.col(i), l, a, p);
       }
       if (KB == 4 || w < KB) {
 #pragma unroll
@@ -1048,7 +1088,7 @@ template <int KP, int NI>
 struct GradTile {
   static constexpr int W = KP / 16;                                           // a wave for 16 columns of dq, dk
   static constexpr int NW = kKept<NI>;
-  static constexpr int kState = NW * 32 * KP * 2, kVec = NW * 32 * C * 2;     // bytes of 32 columns of a state, of d or dy,
+  static constexpr int kState = Kept<KP, NI>::kState, kVec = Kept<KP, NI>::kVec;  // bytes of 32 columns of a state, of d or dy,
   static constexpr int kRows = NI * C * 32 * 2;                               // of do or v
   static constexpr int kK = 0, kS = NI * C * KP * 2;                          // k; S, dS', d, dy, do, v, 32 columns at a time;
   static constexpr int kE = kS + kState, kD = kE + kState, kY = kD + kVec, kO = kY + kVec, kV = kO + kRows;
@@ -1126,19 +1166,20 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
   for (int vb = 0; vb < blocks; ++vb) {
     const int64_t blk = c * blocks + vb;
     __syncthreads();
-    stage<L::kState, W>(lds + L::kS, a.Sw + blk * NW * 32 * KP, lane, wave);
-    stage<L::kState, W>(lds + L::kE, a.dSw + blk * NW * 32 * KP, lane, wave);
-    stage<L::kVec, W>(lds + L::kD, a.dw + blk * NW * 32 * C, lane, wave);
-    stage<L::kVec, W>(lds + L::kY, a.yw + blk * NW * 32 * C, lane, wave);
+    stage<L::kState, W>(lds + L::kS, a.Sw + blk * L::kState, lane, wave);
+    stage<L::kState, W>(lds + L::kE, a.dSw + blk * L::kState, lane, wave);
+    stage<L::kVec, W>(lds + L::kD, a.dw + blk * L::kVec, lane, wave);
+    stage<L::kVec, W>(lds + L::kY, a.yw + blk * L::kVec, lane, wave);
     put_rows(ro[0], second ? L::kV : L::kO);
     if constexpr (W == 4) put_rows(ro[1], L::kV);
     staged();
     if (vb + 1 < blocks) load_rows(vb + 1);
     int ln = lane;
     asm volatile("" : "+v"(ln));  // (addresses made anew in each block: kept, they cost the registers of the products)
+    const auto state_at = [&](int r, int q) { return Kept<KP, NI>::state(r, 2 * wave + (q >> 1)) + 8 * (q & 1); };
     bf16x8 s[NW], ds[NW], yr[NW], vr[NI], orr[W == 4 ? NI : 1];
-    frags_t<U, false>(lds + L::kS, 32 * KP * 2, wave, 0, ln, s);
-    frags_t<U, false>(lds + L::kE, 32 * KP * 2, wave, 0, ln, ds);
+    kept_frags(lds + L::kS, state_at, ln, s);
+    kept_frags(lds + L::kE, state_at, ln, ds);
     ss = mm<NW>(s, ds, ss);
     if (second) {  // (do as the first limbs)
       bf16x8 x[NI];
@@ -1146,19 +1187,20 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
 #pragma unroll
       for (int q = 0; q < NW; ++q) yr[q] = q < NI ? x[q < NI ? q : 0] : bf16x8{};
     } else {
-      frags_t<8, false>(lds + L::kY, 32 * C * 2, mr, 0, ln, yr);
+      kept_frags(lds + L::kY, [&](int r, int q) { return Kept<KP, NI>::vec(r, 16 * mr + 4 * q); }, ln, yr);
     }
     row_frags(L::kV, mr, ln, vr);
     yv = mm<NW>(yr, vr, yv);  // (read where W = 4 or not `second`)
     if constexpr (W == 4) row_frags(L::kO, mr, ln, orr);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
+      const auto tokens_at = [&](int r, int q) { return Kept<KP, NI>::vec(r, 16 * t + 4 * q); };
       bf16x8 f[NW], fo[NI];
-      frags_t<8, false>(lds + L::kY, 32 * C * 2, t, 0, ln, f);
+      kept_frags(lds + L::kY, tokens_at, ln, f);
       w1[t] = mm<NW>(s, f, w1[t]);
       row_frags(L::kO, t, ln, fo);
       w2[t] = mm<NW>(s, fo, w2[t]);
-      frags_t<8, false>(lds + L::kD, 32 * C * 2, t, 0, ln, f);
+      kept_frags(lds + L::kD, tokens_at, ln, f);
       w3[t] = mm<NW>(ds, f, w3[t]);
       m1[t] = mm<NW>(f, yr, m1[t]);  // (above the diagonal too: fewer branches are worth more than the products)
       if constexpr (W == 4) m2[t] = mm<NW>(f, orr, m2[t]);
@@ -1478,7 +1520,7 @@ inline void fill(Args& a, const mg_delta_dims& s, float scale, const mg_rows* q,
   a.g = static_cast<const char*>(g->p), a.g_sb = g->sb, a.g_st = g->st, a.g_sh = g->sh;
   a.beta = static_cast<const char*>(beta->p), a.b_sb = beta->sb, a.b_st = beta->st, a.b_sh = beta->sh;
   a.img = ws + l.img, a.Gd = reinterpret_cast<double*>(ws + l.G);
-  a.Sw = reinterpret_cast<bf16_t*>(ws + l.S), a.dw = reinterpret_cast<bf16_t*>(ws + l.d);
+  a.Sw = ws + l.S, a.dw = ws + l.d;
 }
 
 template <int KP, int NI>
@@ -1563,7 +1605,7 @@ extern "C" int mg_delta_fwd(int dtype, const mg_delta_dims* dims, const mg_rows*
       (rc = delta::check_rows(fn, "v", dtype, v, false)) || (rc = delta::check_rows(fn, "g", dtype, g, false)) ||
       (rc = delta::check_rows(fn, "beta", dtype, beta, false)))
     return rc;
-  if (!o || !aligned(o, dtype == MG_F32 ? 4 : 2)) return fail(MG_ERR_ARG, "%s: o is NULL or misaligned", fn);
+  if (!o || !aligned(o, 16)) return fail(MG_ERR_ARG, "%s: o must be 16-byte aligned", fn);
   if (!aligned(h0, 4) || !aligned(state, 4)) return fail(MG_ERR_ARG, "%s: state misaligned", fn);
   const delta::Layout l = delta::layout(dtype, *dims, keep != 0);
   if (!workspace || workspace_bytes < l.end || !aligned(workspace, 256))
@@ -1604,7 +1646,7 @@ extern "C" int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows*
   char* ws = static_cast<char*>(workspace);
   a.dout = static_cast<const char*>(dout->p), a.do_sb = dout->sb, a.do_st = dout->st, a.do_sh = dout->sh;
   a.dstate = dstate, a.dh0 = dh0;
-  a.dSw = reinterpret_cast<bf16_t*>(ws + w.dS), a.yw = reinterpret_cast<bf16_t*>(ws + w.y);
+  a.dSw = ws + w.dS, a.yw = ws + w.y;
   a.dqp = reinterpret_cast<float*>(ws + w.dqp), a.dkp = reinterpret_cast<float*>(ws + w.dkp);
   a.dq = static_cast<char*>(dq), a.dk = static_cast<char*>(dk), a.dv = static_cast<char*>(dv);
   a.dg = static_cast<char*>(dg), a.db = static_cast<char*>(dbeta);
