@@ -138,6 +138,17 @@ __device__ __forceinline__ f32x4 mm(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB]
 
 // ---------------------------------------------------------------- elements
 
+// the same into two sums in turn: half as long a chain of products that wait for one another
+template <int ORD, int NA, int NB>
+__device__ __forceinline__ void mm2(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 (&c)[2]) {
+  int n = 0;
+#pragma unroll
+  for (int s = ORD - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (s - i >= 0 && s - i < NB) c[n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c[n & 1], 0, 0, 0), ++n;
+}
+
 template <int NI> struct elem { using type = bf16_t; };
 template <> struct elem<3> { using type = float; };
 
@@ -724,7 +735,7 @@ __device__ __forceinline__ void keep_half(char* kept, int64_t c, int col, const 
 }
 
 template <int KP, int NI, bool KEEP, int CT>
-__global__ __launch_bounds__(256) void state_kernel(Args a) {
+__global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
   constexpr int KB = I::KB, NP = I::NP;
@@ -823,9 +834,9 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
       const float decay = last;
       load_rows(n1), load_gates(n1), load_v(n1);
       sync();  // y is there
-      f32x4 d[CT];
+      f32x4 d2[CT][2], d[CT];
 #pragma unroll
-      for (int i = 0; i < CT; ++i) d[i] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < CT; ++i) d2[i][0] = d2[i][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (q <= half.value) {
@@ -833,7 +844,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
           for (int i = 0; i < CT; ++i) {
             bf16x8 yb[3];
             get<2 * CT>(xy, 2 * i + q, lane, yb);
-            d[i] = mm<3>(ft[q], yb, d[i]);
+            mm2<3>(ft[q], yb, d2[i]);
           }
         }
       }
@@ -841,6 +852,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
         uint2 l[3];
+        d[i] = d2[i][0] + d2[i][1];
         split4(tl * d[i], l);
         put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
         split4(d[i], dl[i]);
@@ -897,7 +909,7 @@ __global__ __launch_bounds__(256) void state_kernel(Args a) {
 }
 
 template <int KP, int NI, int CT>
-__global__ __launch_bounds__(256) void dstate_kernel(Args a) {
+__global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void dstate_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
   constexpr int KB = I::KB, NP = I::NP, NW = kKept<NI>;
@@ -1014,9 +1026,9 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
       }
       load_p(half, n1);
       sync();  // dd is there
-      f32x4 dy[CT];
+      f32x4 d2[CT][2], dy[CT];
 #pragma unroll
-      for (int i = 0; i < CT; ++i) dy[i] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < CT; ++i) d2[i][0] = d2[i][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (q >= half.value) {
@@ -1024,7 +1036,7 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
           for (int i = 0; i < CT; ++i) {
             bf16x8 b[3];
             get<2 * CT>(xy, 2 * i + q, lane, b);
-            dy[i] = mm<3>(ft[q], b, dy[i]);
+            mm2<3>(ft[q], b, d2[i]);
           }
         }
       }
@@ -1032,6 +1044,7 @@ __global__ __launch_bounds__(256) void dstate_kernel(Args a) {
       const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
+        dy[i] = d2[i][0] + d2[i][1];
         const f32x4 x = be * dy[i];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
