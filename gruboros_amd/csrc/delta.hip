@@ -1383,18 +1383,35 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(const float* dqp, const 
 //
 // One workgroup per (batch, head, 32 value columns): thread (r, c) holds rows r, r + 32, ... and columns
 // 4 c ... 4 c + 3 of the state, read and written once. k S and q S are taken together from the old
-// state: o = scale (e^g q S + (q.k) d), d = beta (v - e^g k S).
-template <typename E, int KR>
+// state: o = scale (e^g q S + (q.k) d), d = beta (v - e^g k S). ONCE: past the caches, see launch_step.
+template <bool ONCE>
+__device__ __forceinline__ f4 load_state4(const float* p) {
+  f4 r;
+  const f32x4 v = ONCE ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)) : *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.v[j] = v[j];
+  return r;
+}
+template <bool ONCE>
+__device__ __forceinline__ void store_state4(float* p, const f4& x) {
+  const f32x4 v = {x.v[0], x.v[1], x.v[2], x.v[3]};
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p));
+  else
+    *reinterpret_cast<f32x4*>(p) = v;
+}
+template <typename E, int KR, bool ONCE>
 __global__ __launch_bounds__(256) void step_kernel(const E* __restrict__ q, const E* __restrict__ k, const E* __restrict__ v,
                                                    const E* __restrict__ gg, const E* __restrict__ beta, float* __restrict__ state,
                                                    E* __restrict__ o, int H, int Hk, int K, int V, float scale) {
   __shared__ float red[4][8][8];
   __shared__ float dots[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = tid >> 3, cc = tid & 7;
-  const int64_t bh = blockIdx.x;
+  const int tiles = (V + 31) / 32;  // (neighbours in memory at the same time)
+  const int64_t bh = blockIdx.x / tiles;
   const int h = static_cast<int>(bh % H), hk = h / (H / Hk);
   const int64_t bk = bh / H * Hk + hk;
-  const int col = blockIdx.y * 32 + 4 * cc;
+  const int col = static_cast<int>(blockIdx.x % tiles) * 32 + 4 * cc;
   const bool in = col < V;
   float* s = state + bh * K * V + col;
   f4 x[KR];
@@ -1402,7 +1419,7 @@ __global__ __launch_bounds__(256) void step_kernel(const E* __restrict__ q, cons
 #pragma unroll
   for (int i = 0; i < KR; ++i) {
     const int d = r + 32 * i;
-    x[i] = in && d < K ? io4<float>::load(s + static_cast<int64_t>(d) * V) : io4<float>::fill(0.0f);
+    x[i] = in && d < K ? load_state4<ONCE>(s + static_cast<int64_t>(d) * V) : io4<float>::fill(0.0f);
     kr[i] = d < K ? ld(k + bk * K + d) : 0.0f;
     qr[i] = d < K ? ld(q + bk * K + d) : 0.0f;
   }
@@ -1445,7 +1462,7 @@ __global__ __launch_bounds__(256) void step_kernel(const E* __restrict__ q, cons
       if (row < K) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i].v[j] = decay * x[i].v[j] + kr[i] * d[j];
-        io4<float>::store(s + static_cast<int64_t>(row) * V, x[i]);
+        store_state4<ONCE>(s + static_cast<int64_t>(row) * V, x[i]);
       }
     }
   }
@@ -1577,19 +1594,34 @@ int launch_bwd(const Args& a, hipStream_t st_) {
   return check_launch("mg_delta_bwd");
 }
 
+template <typename E, bool ONCE>
+void launch_step(const mg_delta_dims& s, const E* q, const E* k, const E* v, const E* g, const E* beta, float scale, float* state, E* o,
+                 hipStream_t st_) {
+  const dim3 grid(static_cast<int64_t>(s.B) * s.H * ((s.V + 31) / 32));
+#define GO(KR) hipLaunchKernelGGL((step_kernel<E, KR, ONCE>), grid, dim3(256), 0, st_, q, k, v, g, beta, state, o, s.H, s.Hk, s.K, s.V, scale)
+  if (s.K <= 32)
+    GO(1);
+  else if (s.K <= 64)
+    GO(2);
+  else
+    GO(4);
+#undef GO
+}
+
+// A call's states from 64 MiB on are taken to be out of the 256 MiB cache by the next token: a model steps
+// several layers' in between. Then it is no use to send them through it (128 MiB, states of six layers in turn:
+// 57 us through the caches, 52 past them; one layer's over and over: 44 and 50).
 template <typename E>
 int launch_step(const mg_delta_dims& s, const void* q, const void* k, const void* v, const void* g, const void* beta, float scale,
                 float* state, void* o, hipStream_t st_) {
-  const dim3 grid(s.B * s.H, (s.V + 31) / 32);
-  const E *qq = static_cast<const E*>(q), *kk = static_cast<const E*>(k), *vv = static_cast<const E*>(v),
-          *gg = static_cast<const E*>(g), *bb = static_cast<const E*>(beta);
-  E* oo = static_cast<E*>(o);
-  if (s.K <= 32)
-    hipLaunchKernelGGL((step_kernel<E, 1>), grid, dim3(256), 0, st_, qq, kk, vv, gg, bb, state, oo, s.H, s.Hk, s.K, s.V, scale);
-  else if (s.K <= 64)
-    hipLaunchKernelGGL((step_kernel<E, 2>), grid, dim3(256), 0, st_, qq, kk, vv, gg, bb, state, oo, s.H, s.Hk, s.K, s.V, scale);
+  const auto go = [&](auto once) {
+    launch_step<E, decltype(once)::value != 0>(s, static_cast<const E*>(q), static_cast<const E*>(k), static_cast<const E*>(v),
+                                               static_cast<const E*>(g), static_cast<const E*>(beta), scale, state, static_cast<E*>(o), st_);
+  };
+  if (static_cast<int64_t>(s.B) * s.H * s.K * s.V * 4 >= int64_t(64) << 20)
+    go(int_c<1>{});
   else
-    hipLaunchKernelGGL((step_kernel<E, 4>), grid, dim3(256), 0, st_, qq, kk, vv, gg, bb, state, oo, s.H, s.Hk, s.K, s.V, scale);
+    go(int_c<0>{});
   return check_launch("mg_delta_step");
 }
 
