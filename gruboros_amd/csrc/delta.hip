@@ -1121,7 +1121,7 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
   using E = typename elem<NI>::type;
   using L = GradTile<KP, NI>;
   using I = Tile<KP, NI>;
-  constexpr int NW = L::NW, U = KP / 8, W = L::W;
+  constexpr int NW = L::NW, W = L::W;
   __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x;

@@ -8,12 +8,16 @@
 // more than the GPU time of every block up to about 2000 rows and half of a
 // training step's; from here a launch costs 2 to 3 us. The maths stays in the
 // kernels and autograd stays in Python (blocks.py, linear.py, norm.py,
-// scan.py): these functions are the bodies of its Functions.
+// scan.py): these functions are the bodies of its Functions. Layer norm and
+// dropout have their autograd Functions here too: of one kernel each way, they
+// are called by themselves, and Python's part of that was a third of the time.
 //
 // Every function takes the handle of the current HIP stream and launches on
 // it; outputs and workspaces come from torch's caching allocator, so nothing
 // outlives a call here. The GIL is released while a call runs.
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -904,6 +908,98 @@ Tensor dropout(const Tensor& x, const Opt& residual, int out_type, double p, uin
   return y;
 }
 
+namespace ag = torch::autograd;
+
+// Gradients that come from a kernel have no gradient of their own: asked for one, the graph says so
+ag::variable_list once(ag::variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  ag::variable_list given;
+  for (const Tensor& g : grads)
+    if (g.defined()) given.push_back(g.detach().requires_grad_());
+  given = ag::DelayedError("trying to differentiate twice a function that has one derivative only", given.size())
+              .apply(std::move(given));
+  size_t i = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = given[i++];
+  return grads;
+}
+Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
+Tensor plain(const Opt& t) { return t ? *t : Tensor(); }
+
+// The backward launches on the forward's stream, which autograd has made the current one by then.
+struct LayerNormFn : ag::Function<LayerNormFn> {
+  static ag::variable_list forward(ag::AutogradContext* ctx, const Tensor& x, const Opt& delta, const Tensor& w, const Opt& b, bool bf16,
+                                   double eps, double p, int64_t seed, const Opt& seed_t, int64_t offset, int64_t stream) {
+    auto [xn, y, mean, rstd] =
+        layernorm_fwd(x, delta, w, b, bf16, eps, p, static_cast<uint64_t>(seed), seed_t, static_cast<uint64_t>(offset), stream);
+    ctx->save_for_backward({xn ? *xn : x, w, mean, rstd, plain(seed_t)});
+    ctx->set_materialize_grads(false);
+    auto& d = ctx->saved_data;
+    d["p"] = p, d["seed"] = seed, d["offset"] = offset, d["stream"] = stream;
+    d["delta"] = static_cast<int64_t>(delta ? code(*delta) : -1);
+    d["bias"] = b.has_value();
+    if (!xn) return {y};
+    return {y, *xn};
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    ag::variable_list out(11);
+    grads.resize(2);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    auto& d = ctx->saved_data;
+    const int delta = static_cast<int>(d["delta"].toInt());
+    const bool bias = d["bias"].toBool();
+    // (the edges of the tensors that were given: x, delta, w, b)
+    const size_t w = delta >= 0 ? 2 : 1;
+    const bool want_dd = delta >= 0 && ctx->needs_input_grad(1), want_db = bias && ctx->needs_input_grad(w + 1);
+    auto [dx, dd, dw, db] =
+        layernorm_bwd(saved[0], saved[1], saved[2], saved[3], opt(grads[0]), opt(grads[1]), ctx->needs_input_grad(0), want_dd ? delta : -1,
+                      want_db, d["p"].toDouble(), static_cast<uint64_t>(d["seed"].toInt()), opt(saved[4]),
+                      static_cast<uint64_t>(d["offset"].toInt()), d["stream"].toInt());
+    out[0] = plain(dx), out[1] = plain(dd), out[3] = plain(db);
+    if (ctx->needs_input_grad(w)) out[2] = dw;
+    return once(out);
+  }
+};
+
+// (x + dropout(delta) or none, its norm), with gradients
+std::tuple<Opt, Tensor> layer_norm(const Tensor& x, const Opt& delta, const Tensor& w, const Opt& b, bool bf16, double eps, double p,
+                                   uint64_t seed, const Opt& seed_t, uint64_t offset, int64_t stream) {
+  const auto out = LayerNormFn::apply(x, delta, w, b, bf16, eps, p, static_cast<int64_t>(seed), seed_t, static_cast<int64_t>(offset), stream);
+  return {out.size() > 1 ? Opt(out[1]) : std::nullopt, out[0]};
+}
+
+struct DropoutFn : ag::Function<DropoutFn> {
+  static Tensor forward(ag::AutogradContext* ctx, const Tensor& x, const Opt& residual, double p, int64_t seed, const Opt& seed_t,
+                        int64_t offset, int64_t stream) {
+    ctx->save_for_backward({plain(seed_t)});  // (a seed tensor advanced before the backward is an error there)
+    auto& d = ctx->saved_data;
+    d["p"] = p, d["seed"] = seed, d["offset"] = offset, d["stream"] = stream, d["type"] = static_cast<int64_t>(code(x));
+    d["residual"] = residual.has_value();
+    return dropout(x, residual, residual ? code(*residual) : code(x), p, static_cast<uint64_t>(seed), seed_t,
+                   static_cast<uint64_t>(offset), stream);
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    ag::variable_list out(7);
+    auto& d = ctx->saved_data;
+    const auto saved = ctx->get_saved_variables();
+    if (ctx->needs_input_grad(0)) {
+      Tensor dy = grads[0].contiguous();
+      if (reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone();
+      out[0] = dropout(dy, std::nullopt, static_cast<int>(d["type"].toInt()), d["p"].toDouble(), static_cast<uint64_t>(d["seed"].toInt()),
+                       opt(saved[0]), static_cast<uint64_t>(d["offset"].toInt()), d["stream"].toInt());
+    }
+    out = once(out);
+    if (d["residual"].toBool() && ctx->needs_input_grad(1)) out[1] = grads[0];
+    return out;
+  }
+};
+
+// x dropped out, plus a residual, with gradients
+Tensor dropout_add(const Tensor& x, const Opt& residual, double p, uint64_t seed, const Opt& seed_t, uint64_t offset, int64_t stream) {
+  return DropoutFn::apply(x, residual, p, static_cast<int64_t>(seed), seed_t, static_cast<int64_t>(offset), stream);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -933,9 +1029,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("head_backward", &head_backward, nogil());
   m.def("infer_layer", &infer_layer, nogil());
   m.def("column_sum", &column_sum, nogil());
-  m.def("layernorm_fwd", &layernorm_fwd, nogil());
-  m.def("layernorm_bwd", &layernorm_bwd, nogil());
-  m.def("dropout", &dropout, nogil());
+  m.def("layer_norm", &layer_norm, nogil());
+  m.def("dropout_add", &dropout_add, nogil());
   m.def("delta_fwd", &delta_fwd, nogil());
   m.def("delta_bwd", &delta_bwd, nogil());
   m.def("delta_step", &delta_step, nogil());

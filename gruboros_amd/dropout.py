@@ -4,7 +4,6 @@ makes the same choice again. Unlike nn.Dropout (reference mingru/minLM.py:72) it
 generator state: a step that is run again, on whatever stream, drops the same values.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._lib import dtype_code, native, require_cuda, stream_of
 
@@ -34,26 +33,6 @@ def _dense(t):
     return t.clone() if t.data_ptr() % 16 else t
 
 
-class DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, seed_t, offset):
-        y = native().dropout(x, residual, dtype_code(x.dtype if residual is None else residual.dtype), p, seed, seed_t, offset,
-                             stream_of(x))
-        ctx.save_for_backward(seed_t)  # (a seed tensor advanced before the backward is an error there)
-        ctx.args = p, seed, offset, x.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        p, seed, offset, dtype = ctx.args
-        (seed_t,) = ctx.saved_tensors
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = native().dropout(_dense(dy), None, dtype_code(dtype), p, seed, seed_t, offset, stream_of(dy))
-        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None, None
-
-
 def dropout(x, p, seed, offset=0, residual=None):
     """x with each value dropped (0) with probability p and the others divided by 1 - p; with
     `residual` (x's shape; float32, or x's dtype) the sum of it and that, in its dtype.
@@ -71,4 +50,4 @@ def dropout(x, p, seed, offset=0, residual=None):
         raise ValueError(f"residual {residual.dtype} {tuple(residual.shape)} must match x {tuple(x.shape)}, in float32 or {x.dtype}")
     if x.numel() == 0:
         return x.clone() if residual is None else residual.clone()
-    return DropoutFn.apply(_dense(x), None if residual is None else _dense(residual), p, seed, seed_t, offset)
+    return native().dropout_add(_dense(x), None if residual is None else _dense(residual), p, seed, seed_t, offset, stream_of(x))

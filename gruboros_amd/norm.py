@@ -15,7 +15,6 @@ Weights of any floating dtype are accepted (a model cast with
 them as fp32.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._lib import MG_BF16, dtype_code, native, require_cuda, stream_of
 from .dropout import check_drop
@@ -140,32 +139,6 @@ def add_rms_norm(x, delta, w, out_dtype=None, with_lo=False):
     return AddRMSNormFn.apply(x.contiguous(), delta.contiguous(), w, out_dtype, _lo_ok(out_dtype, with_lo))
 
 
-class LayerNormFn(torch.autograd.Function):
-    """(xn, y) with xn = x + dropout(delta), or (None, y) without a delta; see add_layer_norm."""
-
-    @staticmethod
-    def forward(ctx, x, delta, w, b, out_dtype, eps, drop):
-        p, seed, seed_t, offset = drop
-        xn, y, mean, rstd = native().layernorm_fwd(x, delta, w, b, dtype_code(out_dtype) == MG_BF16, eps, p, seed, seed_t, offset,
-                                                   stream_of(x))
-        ctx.save_for_backward(x if xn is None else xn, w, mean, rstd, seed_t)
-        ctx.args = p, seed, offset, -1 if delta is None else dtype_code(delta.dtype)
-        ctx.set_materialize_grads(False)
-        return xn, y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dx_out, dy):
-        if dx_out is None and dy is None:
-            return (None,) * 7
-        xn, w, mean, rstd, seed_t = ctx.saved_tensors
-        p, seed, offset, delta_type = ctx.args
-        need = ctx.needs_input_grad
-        dx, dd, dw, db = native().layernorm_bwd(xn, w, mean, rstd, dy, dx_out, need[0], delta_type if need[1] else -1, need[3],
-                                                p, seed, seed_t, offset, stream_of(xn))
-        return dx, dd, (dw if need[2] else None), db, None, None, None
-
-
 def _check_layer_norm(x, w, b, delta, out_dtype):
     require_cuda(x, w, b, delta)
     D = x.shape[-1] if x.dim() else 0
@@ -196,7 +169,7 @@ def layer_norm(x, w, b=None, out_dtype=None, eps=1e-5):
     w, b = _check_layer_norm(x, w, b, None, out_dtype)
     if x.numel() == 0:
         return torch.empty_like(x, dtype=out_dtype)
-    return LayerNormFn.apply(x.contiguous(), None, w, b, out_dtype, eps, (0.0, 0, None, 0))[1]
+    return native().layer_norm(x.contiguous(), None, w, b, out_dtype == torch.bfloat16, eps, 0.0, 0, None, 0, stream_of(x))[1]
 
 
 def add_layer_norm(x, delta, w, b=None, out_dtype=None, eps=1e-5, dropout_p=0.0, seed=None, offset=0):
@@ -209,4 +182,4 @@ def add_layer_norm(x, delta, w, b=None, out_dtype=None, eps=1e-5, dropout_p=0.0,
     drop = check_drop(dropout_p, 0 if seed is None and dropout_p == 0 else seed, offset, x.device)
     if x.numel() == 0:
         return x + delta.float(), torch.empty_like(x, dtype=out_dtype)
-    return LayerNormFn.apply(x.contiguous(), delta.contiguous(), w, b, out_dtype, eps, drop)
+    return native().layer_norm(x.contiguous(), delta.contiguous(), w, b, out_dtype == torch.bfloat16, eps, *drop, stream_of(x))
