@@ -1534,6 +1534,13 @@ inline int check_rows(const char* fn, const char* name, int dtype, const mg_rows
   return MG_OK;
 }
 
+// o and dv are dense: their rows' offsets in a chunk are held in 31 bits, as the operands' are
+inline int check_out(const char* fn, int dtype, const mg_delta_dims* s) {
+  if (static_cast<int64_t>(s->H) * s->V * (dtype == MG_F32 ? 4 : 2) * C >= (int64_t(1) << 31))
+    return fail(MG_ERR_ARG, "%s: 64 tokens' o must be below 2 GiB", fn);
+  return MG_OK;
+}
+
 // Value columns per workgroup of the passes over the chunks, in tiles of 16: two where that still leaves
 // a workgroup for every CU (the chunk's operands are then read for twice the columns), else one. fp32 has LDS for one.
 inline int columns_for(int64_t bh, int vp, int dtype_limbs) {
@@ -1645,7 +1652,7 @@ extern "C" int mg_delta_fwd(int dtype, const mg_delta_dims* dims, const mg_rows*
                             int keep, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "mg_delta_fwd";
   int rc;
-  if ((rc = delta::check_dims(fn, dtype, dims))) return rc;
+  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_out(fn, dtype, dims))) return rc;
   if ((rc = delta::check_rows(fn, "q", dtype, q, true)) || (rc = delta::check_rows(fn, "k", dtype, k, true)) ||
       (rc = delta::check_rows(fn, "v", dtype, v, false)) || (rc = delta::check_rows(fn, "g", dtype, g, false)) ||
       (rc = delta::check_rows(fn, "beta", dtype, beta, false)))
@@ -1670,7 +1677,7 @@ extern "C" int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows*
                             float* dh0, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "mg_delta_bwd";
   int rc;
-  if ((rc = delta::check_dims(fn, dtype, dims))) return rc;
+  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_out(fn, dtype, dims))) return rc;
   if ((rc = delta::check_rows(fn, "q", dtype, q, true)) || (rc = delta::check_rows(fn, "k", dtype, k, true)) ||
       (rc = delta::check_rows(fn, "v", dtype, v, false)) || (rc = delta::check_rows(fn, "g", dtype, g, false)) ||
       (rc = delta::check_rows(fn, "beta", dtype, beta, false)) || (rc = delta::check_rows(fn, "dout", dtype, dout, true)))

@@ -673,11 +673,12 @@ int mg_decode_head_f16(int B, int D, int V, const float* x_in, const void* pendi
  *
  * mg_rows: element (b, t, h, d) of an operand at p + b sb + t st + h sh + d
  * (elements; d contiguous; g and beta have no d). q, k and dout: p and the
- * strides multiples of 16 bytes; dq and dk 16-byte aligned. o, dv: dense
- * [B, T, H, V]; dq, dk: dense
- * [B, T, Hk, K]; dg, dbeta: dense [B, T, H].
+ * strides multiples of 16 bytes. o, dv: dense [B, T, H, V]; dq, dk: dense
+ * [B, T, Hk, K]; o, dq and dk 16-byte aligned; dg, dbeta: dense [B, T, H].
  * K and V multiples of 8, K <= 128, V <= 256; T >= 1;
- * B H ceil(T / 64) < 2^31; 64 token strides below 2 GiB.
+ * B H ceil(T / 64) < 2^31; 64 token strides (o's too) below 2 GiB.
+ * A value that is not finite spoils the 64 tokens of its chunk, earlier ones
+ * included: padding behind a sequence must be finite (g = -inf apart).
  *
  * mg_delta_fwd runs over chunks of 64 tokens. state (nullable) receives the
  * last state; it must not overlap h0. keep != 0 keeps in `workspace` what
