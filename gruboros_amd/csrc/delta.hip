@@ -645,8 +645,10 @@ __device__ __forceinline__ void settled() { __builtin_amdgcn_s_waitcnt(0x0f70); 
 template <int CT>
 struct Place {
   int lane, w, m, g, bh, h, b, tile;
+  bool chain;  // one of the waves 0 to 3
   __device__ __forceinline__ explicit Place(const Args& a) {
-    lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63, w = wave & 3, m = lane & 15, g = lane >> 4, chain = wave < 4;
     place(blockIdx.x, a.B * a.H, a.VP / 16 / CT, bh, tile);
     h = bh % a.H, b = bh / a.H;
   }
@@ -706,10 +708,9 @@ __device__ __forceinline__ void kept_frags(const char* x, P pos, int lane, bf16x
   }
 }
 
-// This wave's rows of the state to the other waves and, where kept, to memory
-template <int KP, int NI, int CT, typename P>
-__device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, char* kept, int64_t c, const Args& a, const P& p) {
-  using L = Kept<KP, NI>;
+// This wave's rows of the state to the other waves
+template <int KP, int CT, typename P>
+__device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, const P& p) {
   if (KP == 128 || p.w < KP / 32) {  // (four waves)
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
@@ -717,15 +718,43 @@ __device__ __forceinline__ void publish(const f32x4 (&S)[CT][2], char* xs, char*
       bf16x8 l[3];
       split<3>(x, l);
       put_full<CT * (KP / 32)>(xs, i * (KP / 32) + p.w, p.lane, l);
-      if (kept) {
-        char* out = kept + (c * (a.VP / 32) + p.col(i) / 32) * L::kState + L::state(p.col(i) % 32, 4 * p.w + p.g);
-#pragma unroll
-        for (int q = 0; q < L::NW; ++q) *reinterpret_cast<bf16x8*>(out + q * 1024) = l[q];
-      }
     }
   }
 }
-// Half a fragment of d or dy
+// What lies in LDS of the state, and of d, to memory: a fragment's limbs, or halves of one, by one wave each
+template <int KP, int NI, int CT, typename P>
+__device__ __forceinline__ void keep_state(char* kept, int64_t c, const char* xs, const Args& a, const P& p) {
+  using L = Kept<KP, NI>;
+  constexpr int KB = KP / 32, N = CT * KB;
+#pragma unroll
+  for (int j = 0; j < (N + 3) / 4; ++j) {
+    const int f = 4 * j + p.w;
+    if (N % 4 == 0 || f < N) {
+      const int col = (p.tile * CT + f / KB) * 16 + p.m;
+      char* out = kept + (c * (a.VP / 32) + col / 32) * L::kState + L::state(col % 32, 4 * (f % KB) + p.g);
+#pragma unroll
+      for (int q = 0; q < L::NW; ++q)
+        *reinterpret_cast<bf16x8*>(out + q * 1024) = *reinterpret_cast<const bf16x8*>(xs + (q * N + f) * kFrag + p.lane * 16);
+    }
+  }
+}
+template <int KP, int NI, int CT, typename P>
+__device__ __forceinline__ void keep_vec(char* kept, int64_t c, const char* xd, const Args& a, const P& p) {
+  using L = Kept<KP, NI>;
+  constexpr int N = 2 * CT * L::NW;
+#pragma unroll
+  for (int j = 0; j < (N + 3) / 4; ++j) {
+    const int x = 4 * j + p.w, f = x % (2 * CT), q = x / (2 * CT);
+    if (N % 4 == 0 || x < N) {
+      const int col = (p.tile * CT + f / 2) * 16 + p.m;
+      char* out = kept + (c * (a.VP / 32) + col / 32) * L::kVec + q * 1024;
+      const uint4 v = *reinterpret_cast<const uint4*>(xd + x * kFrag + p.lane * 16);
+      *reinterpret_cast<uint2*>(out + L::vec(col % 32, 32 * (f % 2) + 8 * p.g)) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2*>(out + L::vec(col % 32, 32 * (f % 2) + 8 * p.g + 4)) = make_uint2(v.z, v.w);
+    }
+  }
+}
+// Half a fragment of dy
 template <int KP, int NI, typename P>
 __device__ __forceinline__ void keep_half(char* kept, int64_t c, int col, const uint2 (&l)[kKept<NI>], const Args& a, const P& p) {
   using L = Kept<KP, NI>;
@@ -735,81 +764,68 @@ __device__ __forceinline__ void keep_half(char* kept, int64_t c, int col, const 
 }
 
 template <int KP, int NI, bool KEEP, int CT>
-__global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kernel(Args a) {
+__global__ __launch_bounds__(512) void state_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
   constexpr int KB = I::KB, NP = I::NP;
   __shared__ __attribute__((aligned(16))) char xs[CT * KB * 3 * kFrag], xy[CT * 6 * kFrag], xe[CT * 6 * kFrag], xd[CT * 2 * NP * kFrag];
   const Place<CT> p(a);
   const int lane = p.lane, g = p.g, w = p.w, pw = w / 2;
-  const int64_t o_st = static_cast<int64_t>(a.H) * a.V;
-  const E* v = reinterpret_cast<const E*>(a.v) + p.b * a.v_sb + p.h * a.v_sh;
-  E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
-  const uint32_t vs = static_cast<uint32_t>(a.v_st * sizeof(E)), os = static_cast<uint32_t>(o_st * sizeof(E));
-  const int row = row_of(w, 4 * g);  // the lane's first of four tokens
   constexpr int64_t kImage = KEEP ? I::kKept : I::kOnce;
   const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * kImage;
 
-  // What a chunk takes from memory, each loaded anew for the next chunk once its last reader is through
-  uint32_t next[CT][4];
-  bf16x8 fk[KB][NI], fq[KB][NI], ft[2][3], fp[2][NP], kt[2][2][NI];
-  f32x4 eg, tail, be;
-  float last, eo;
-  const auto load_v = [&](int n) {
-    const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
+  // What a chunk takes from memory is loaded anew for the next one once its last reader is through. (A loop for each
+  // half of the waves: how many blocks of T and P a wave has is then known, and so is how many operations later than
+  // its loads a wait may leave under way.)
+  const auto chain = [&](auto half) __attribute__((always_inline)) {
+    const E* v = reinterpret_cast<const E*>(a.v) + p.b * a.v_sb + p.h * a.v_sh;
+    const uint32_t vs = static_cast<uint32_t>(a.v_st * sizeof(E));
+    const int row = row_of(w, 4 * g);  // the lane's first of four tokens
+    uint32_t next[CT][4];
+    bf16x8 fk[KB][NI], ft[2][3], kt[2][2][NI];
+    f32x4 eg, tail, be;
+    float last;
+    const auto load_v = [&](int n) {
+      const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
+      for (int i = 0; i < CT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(vr, p.col(i) < a.V ? row * vs + p.col(i) * sizeof(E) : kOutOfRange, r * vs);
-  };
-  const auto load_rows = [&](int n) {
-    const char* x = img + n * kImage;
+        for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(vr, p.col(i) < a.V ? row * vs + p.col(i) * sizeof(E) : kOutOfRange, r * vs);
+    };
+    const auto load_rows = [&](int n) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      load_frag(x + I::kK + I::rows(w, kb), lane, fk[kb]);
-      load_frag(x + I::kQ + I::rows(w, kb), lane, fq[kb]);
-    }
-  };
-  const auto load_gates = [&](int n) {
-    const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
-    eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
-    be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63], eo = gt[row_of(w, p.m)];
-  };
-  const auto load_t = [&](auto half, int n) {
+      for (int kb = 0; kb < KB; ++kb) load_frag(img + n * kImage + I::kK + I::rows(w, kb), lane, fk[kb]);
+    };
+    const auto load_gates = [&](int n) {
+      const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
+      eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
+      be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63];
+    };
+    const auto load_t = [&](int n) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (q <= half.value) load_frag(img + n * kImage + I::kT + I::low(w, q, 3), lane, ft[q]);
-  };
-  const auto load_p = [&](auto half, int n) {
+      for (int q = 0; q < 2; ++q)
+        if (q <= half.value) load_frag(img + n * kImage + I::kT + I::low(w, q, 3), lane, ft[q]);
+    };
+    const auto load_cols = [&](int n) {
+      if (KB == 4 || w < KB) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (q <= half.value) load_frag(img + n * kImage + I::kP + I::low(w, q, NP), lane, fp[q]);
-  };
-  const auto load_cols = [&](int n) {
-    if (KB == 4 || w < KB) {
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) load_frag(img + n * kImage + I::kKT + I::cols(2 * w + t, q), lane, kt[t][q]);
-    }
-  };
-  f32x4 S[CT][2];
-  load_state(S, a.h0, a, p);
-  // (a loop for each half of the waves: how many blocks of T and P a wave has is then known, and so is how many
-  // operations later than its loads a wait may leave under way)
-  const auto run = [&](auto half) __attribute__((always_inline)) {
-    load_rows(0), load_gates(0), load_v(0), load_t(half, 0), load_cols(0), load_p(half, 0);
-    publish<KP, NI>(S, xs, KEEP ? a.Sw : nullptr, static_cast<int64_t>(p.bh) * a.NC, a, p);
+          for (int q = 0; q < 2; ++q) load_frag(img + n * kImage + I::kKT + I::cols(2 * w + t, q), lane, kt[t][q]);
+      }
+    };
+    f32x4 S[CT][2];
+    load_state(S, a.h0, a, p);
+    load_rows(0), load_gates(0), load_v(0), load_t(0), load_cols(0);
+    publish<KP>(S, xs, p);
     settled();
     sync();
 #pragma unroll 1
     for (int n = 0; n < a.NC; ++n) {
-      const int t0 = n * C, rows = min(C, a.T - t0), n1 = min(n + 1, a.NC - 1);  // (the last chunk loads itself once more)
-      const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
-      // y and the state's part of o: this wave's 16 tokens
-      f32x4 ks[CT], oa[CT];
+      const int n1 = min(n + 1, a.NC - 1);  // (the last chunk loads itself once more)
+      f32x4 ks[CT];  // y: this wave's 16 tokens
 #pragma unroll
-      for (int i = 0; i < CT; ++i) ks[i] = oa[i] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < CT; ++i) ks[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -817,7 +833,6 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kerne
           bf16x8 sb[3];
           get<CT * KB>(xs, i * KB + kb, lane, sb);
           ks[i] = mm<3>(fk[kb], sb, ks[i]);
-          oa[i] = mm<NP>(sb, fq[kb], oa[i]);  // (transposed: a lane has a token and four columns; only o, which is rounded to the inputs' type, sees this product)
         }
       }
 #pragma unroll
@@ -828,7 +843,6 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kerne
         uint2 l[3];
         split4(be * (vv - eg * ks[i]), l);
         put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
-        oa[i] *= a.scale * eo;
       }
       const f32x4 tl = tail;
       const float decay = last;
@@ -848,22 +862,17 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kerne
           }
         }
       }
-      uint2 dl[CT][NP];
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
-        uint2 l[3];
+        uint2 l[3], dl[NP];
         d[i] = d2[i][0] + d2[i][1];
         split4(tl * d[i], l);
         put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
-        split4(d[i], dl[i]);
-        put_half<2 * CT>(xd, 2 * i + pw, lane, w & 1, dl[i]);
+        split4(d[i], dl);
+        put_half<2 * CT>(xd, 2 * i + pw, lane, w & 1, dl);
       }
-      load_t(half, n1);
+      load_t(n1);
       sync();  // d is there
-      if constexpr (KEEP) {
-#pragma unroll
-        for (int i = 0; i < CT; ++i) keep_half<KP, NI>(a.dw, c, p.col(i), dl[i], a, p);
-      }
       if (KB == 4 || w < KB) {
 #pragma unroll
         for (int i = 0; i < CT; ++i) S[i][0] *= decay, S[i][1] *= decay;
@@ -879,7 +888,55 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kerne
         }
       }
       load_cols(n1);
-      publish<KP, NI>(S, xs, KEEP && n + 1 < a.NC ? a.Sw : nullptr, c + 1, a, p);
+      publish<KP>(S, xs, p);
+      sync();  // the state is there
+    }
+    if (a.state && w < KB) store_state(S, a.state, a, p);
+  };
+
+  // o, transposed (a lane has a token and four columns), and what is kept
+  const auto beside = [&](auto half) __attribute__((always_inline)) {
+    const int64_t o_st = static_cast<int64_t>(a.H) * a.V;
+    E* o = reinterpret_cast<E*>(a.o) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
+    const uint32_t os = static_cast<uint32_t>(o_st * sizeof(E));
+    const int row = row_of(w, p.m);
+    bf16x8 fq[KB][NI], fp[2][NP];
+    float eg;
+    const auto load_rows = [&](int n) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) load_frag(img + n * kImage + I::kQ + I::rows(w, kb), lane, fq[kb]);
+      eg = reinterpret_cast<const float*>(img + n * kImage + I::kGate)[row];
+    };
+    const auto load_p = [&](int n) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (q <= half.value) load_frag(img + n * kImage + I::kP + I::low(w, q, NP), lane, fp[q]);
+    };
+    load_rows(0), load_p(0);
+    settled();
+    sync();
+#pragma unroll 1
+    for (int n = 0; n < a.NC; ++n) {
+      const int t0 = n * C, rows = min(C, a.T - t0), n1 = min(n + 1, a.NC - 1);
+      const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
+      f32x4 oa[CT];
+#pragma unroll
+      for (int i = 0; i < CT; ++i) oa[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          bf16x8 sb[3];
+          get<CT * KB>(xs, i * KB + kb, lane, sb);
+          oa[i] = mm<NP>(sb, fq[kb], oa[i]);  // (only o, which is rounded to the inputs' type, sees this product)
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CT; ++i) oa[i] *= a.scale * eg;
+      if constexpr (KEEP) keep_state<KP, NI, CT>(a.Sw, c, xs, a, p);
+      load_rows(n1);
+      sync();
+      sync();  // d is there
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (q <= half.value) {
@@ -891,110 +948,90 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void state_kerne
           }
         }
       }
-      load_p(half, n1);
+      load_p(n1);
       const __amdgpu_buffer_rsrc_t orr = rows_buffer(o + t0 * o_st, o_st, rows, a.V);
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
         const int col = (p.tile * CT + i) * 16 + 4 * g;
-        store_cols<E>(orr, col < a.V ? row_of(w, p.m) * os + col * sizeof(E) : kOutOfRange, oa[i]);
+        store_cols<E>(orr, col < a.V ? row * os + col * sizeof(E) : kOutOfRange, oa[i]);
       }
+      if constexpr (KEEP) keep_vec<KP, NI, CT>(a.dw, c, xd, a, p);
       sync();  // the state is there
     }
   };
-  if (pw == 0)
-    run(int_c<0>{});
-  else
-    run(int_c<1>{});
-  if (a.state && w < KB) store_state(S, a.state, a, p);
+  if (p.chain) {
+    if (pw == 0)
+      chain(int_c<0>{});
+    else
+      chain(int_c<1>{});
+  } else {
+    if (pw == 0)
+      beside(int_c<0>{});
+    else
+      beside(int_c<1>{});
+  }
 }
 
 template <int KP, int NI, int CT>
-__global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void dstate_kernel(Args a) {
+__global__ __launch_bounds__(512) void dstate_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
   constexpr int KB = I::KB, NP = I::NP, NW = kKept<NI>;
-  __shared__ __attribute__((aligned(16))) char xs[CT * KB * 3 * kFrag], xy[CT * 6 * kFrag], xe[CT * 6 * kFrag], xu[CT * 6 * kFrag], xo[CT * 2 * NI * kFrag];
+  __shared__ __attribute__((aligned(16))) char xs[CT * KB * 3 * kFrag], xy[CT * 6 * kFrag], xe[CT * 6 * kFrag];
+  __shared__ __attribute__((aligned(16))) char xu[CT * 6 * kFrag], xo[CT * 2 * NI * kFrag];
+  __shared__ f32x4 xp[4][CT][64], xq[4][CT][2][64];  // P^T do and Q^T (scale e^G do) in the accumulators' order
   const Place<CT> p(a);
   const int lane = p.lane, g = p.g, w = p.w, pw = w / 2;
-  const int64_t v_st = static_cast<int64_t>(a.H) * a.V;
-  const E* dout = reinterpret_cast<const E*>(a.dout) + p.b * a.do_sb + p.h * a.do_sh;
-  E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
-  const uint32_t is = static_cast<uint32_t>(a.do_st * sizeof(E)), os = static_cast<uint32_t>(v_st * sizeof(E));
-  const int row = row_of(w, 4 * g);
   constexpr int64_t kImage = I::kKept;
   const char* img = a.img + static_cast<int64_t>(p.bh) * a.NC * kImage;
+  const int row = row_of(w, 4 * g), last_n = a.NC - 1;
 
-  uint32_t next[CT][4];  // do of a chunk
-  f32x4 go[CT];
-  bf16x8 fk[KB][NI], ft[2][3], fp[2][NP], kt[2][2][NI], qt[2][2][NI];
-  f32x4 eg, tail, be;
-  float last;
-  const auto load_go = [&](int n) {
-    const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
+  const auto chain = [&](auto half) __attribute__((always_inline)) {
+    const int64_t v_st = static_cast<int64_t>(a.H) * a.V;
+    E* dv = reinterpret_cast<E*>(a.dv) + (static_cast<int64_t>(p.b) * a.T * a.H + p.h) * a.V;
+    const uint32_t os = static_cast<uint32_t>(v_st * sizeof(E));
+    bf16x8 fk[KB][NI], ft[2][3], kt[2][2][NI];
+    f32x4 eg, tail, be;
+    float last;
+    const auto load_rows = [&](int n) {
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
+      for (int kb = 0; kb < KB; ++kb) load_frag(img + n * kImage + I::kK + I::rows(w, kb), lane, fk[kb]);
+    };
+    const auto load_gates = [&](int n) {
+      const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
+      eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
+      be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63];
+    };
+    const auto load_t = [&](int n) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(ir, p.col(i) < a.V ? row * is + p.col(i) * sizeof(E) : kOutOfRange, r * is);
-  };
-  const auto put_go = [&]() {
+      for (int q = 0; q < 2; ++q)
+        if (q >= half.value) load_frag(img + n * kImage + I::kTT + I::high(w, q, 3), lane, ft[q]);
+    };
+    const auto load_cols = [&](int n) {
+      if (KB == 4 || w < KB) {
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) go[i][r] = value<E>(next[i][r]);
-      uint2 l[NI];
-      split4(go[i], l);
-      put_half<2 * CT>(xo, 2 * i + pw, lane, w & 1, l);
-    }
-  };
-  const auto load_rows = [&](int n) {
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) load_frag(img + n * kImage + I::kK + I::rows(w, kb), lane, fk[kb]);
-  };
-  const auto load_gates = [&](int n) {
-    const float* gt = reinterpret_cast<const float*>(img + n * kImage + I::kGate);
-    eg = *reinterpret_cast<const f32x4*>(gt + row), tail = *reinterpret_cast<const f32x4*>(gt + 64 + row);
-    be = *reinterpret_cast<const f32x4*>(gt + 128 + row), last = gt[63];
-  };
-  const auto load_t = [&](auto half, int n) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (q >= half.value) load_frag(img + n * kImage + I::kTT + I::high(w, q, 3), lane, ft[q]);
-  };
-  const auto load_p = [&](auto half, int n) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (q >= half.value) load_frag(img + n * kImage + I::kPT + I::high(w, q, NP), lane, fp[q]);
-  };
-  const auto load_cols = [&](int n) {
-    if (KB == 4 || w < KB) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          load_frag(img + n * kImage + I::kKT + I::cols(2 * w + t, q), lane, kt[t][q]);
-          load_frag(img + n * kImage + I::kQT + I::cols(2 * w + t, q), lane, qt[t][q]);
-        }
-    }
-  };
-  f32x4 S[CT][2];  // the gradient of the state
-  load_state(S, a.dstate, a, p);
-  const int last_n = a.NC - 1;
-  // (a loop for each half of the waves: how many blocks of T and P a wave has is then known, and so is how many
-  // operations later than its loads a wait may leave under way)
-  const auto run = [&](auto half) __attribute__((always_inline)) {
-    load_go(last_n), load_rows(last_n), load_gates(last_n), load_p(half, last_n), load_t(half, last_n), load_cols(last_n);
-    put_go();
-    load_go(max(last_n - 1, 0));
-    publish<KP, NI>(S, xs, a.dSw, static_cast<int64_t>(p.bh) * a.NC + last_n, a, p);
+          for (int q = 0; q < 2; ++q) load_frag(img + n * kImage + I::kKT + I::cols(2 * w + t, q), lane, kt[t][q]);
+      }
+    };
+    f32x4 S[CT][2];  // the gradient of the state
+    load_state(S, a.dstate, a, p);
+    load_rows(last_n), load_gates(last_n), load_t(last_n), load_cols(last_n);
+    publish<KP>(S, xs, p);
     settled();
+    sync();
     sync();
 #pragma unroll 1
     for (int n = last_n; n >= 0; --n) {
       const int t0 = n * C, rows = min(C, a.T - t0), n1 = max(n - 1, 0);  // (the last chunk loads itself once more)
       const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
-      f32x4 dd[CT];
+      f32x4 dd[CT], add[CT][2];
 #pragma unroll
-      for (int i = 0; i < CT; ++i) dd[i] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < CT; ++i) {
+        dd[i] = f32x4{0, 0, 0, 0};
+        add[i][0] = xq[w][i][0][lane], add[i][1] = xq[w][i][1][lane];
+      }
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -1006,25 +1043,11 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void dstate_kern
       }
       load_rows(n1);
 #pragma unroll
-      for (int i = 0; i < CT; ++i) dd[i] *= tail;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if (q >= half.value) {
-#pragma unroll
-          for (int i = 0; i < CT; ++i) {
-            bf16x8 ob[NI];
-            get<2 * CT>(xo, 2 * i + q, lane, ob);
-            dd[i] = mm<3>(fp[q], ob, dd[i]);
-          }
-        }
-      }
-#pragma unroll
       for (int i = 0; i < CT; ++i) {
         uint2 l[3];
-        split4(dd[i], l);
+        split4(tail * dd[i] + xp[w][i][lane], l);
         put_half<2 * CT>(xy, 2 * i + pw, lane, w & 1, l);
       }
-      load_p(half, n1);
       sync();  // dd is there
       f32x4 d2[CT][2], dy[CT];
 #pragma unroll
@@ -1040,33 +1063,25 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void dstate_kern
           }
         }
       }
-      load_t(half, n1);
+      load_t(n1);
       const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
         dy[i] = d2[i][0] + d2[i][1];
         const f32x4 x = be * dy[i];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, x[r]);
         uint2 l[3];
         split4(-eg * x, l);
         put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
-        split4(a.scale * eg * go[i], l);
-        put_half<2 * CT>(xu, 2 * i + pw, lane, w & 1, l);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, x[r]);
       }
       const float decay = last;
       load_gates(n1);
-      sync();  // they are there
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        uint2 l[NW];
-        split4(dy[i], l);
-        keep_half<KP, NI>(a.yw, c, p.col(i), l, a, p);
-      }
+      sync();  // e^G beta dy is there
       if (KB == 4 || w < KB) {
 #pragma unroll
-        for (int i = 0; i < CT; ++i) S[i][0] *= decay, S[i][1] *= decay;
+        for (int i = 0; i < CT; ++i) S[i][0] = decay * S[i][0] + add[i][0], S[i][1] = decay * S[i][1] + add[i][1];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -1075,24 +1090,117 @@ __global__ __launch_bounds__(256, NI == 3 && KP == 128 ? 1 : 2) void dstate_kern
             get<2 * CT>(xe, 2 * i + q, lane, b);
             S[i][0] = mm<3>(kt[0][q], b, S[i][0]);
             S[i][1] = mm<3>(kt[1][q], b, S[i][1]);
-            get<2 * CT>(xu, 2 * i + q, lane, b);
-            S[i][0] = mm<3>(qt[0][q], b, S[i][0]);
-            S[i][1] = mm<3>(qt[1][q], b, S[i][1]);
           }
         }
       }
       load_cols(n1);
+      publish<KP>(S, xs, p);
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        uint2 l[NW];
+        split4(dy[i], l);
+        keep_half<KP, NI>(a.yw, c, p.col(i), l, a, p);
+      }
+      sync();  // the state is there
+    }
+    if (a.dh0 && w < KB) store_state(S, a.dh0, a, p);
+  };
+
+  // What depends on do alone, a chunk ahead of the chain, and what is kept of the state's gradient
+  const auto beside = [&](auto half) __attribute__((always_inline)) {
+    const E* dout = reinterpret_cast<const E*>(a.dout) + p.b * a.do_sb + p.h * a.do_sh;
+    const uint32_t is = static_cast<uint32_t>(a.do_st * sizeof(E));
+    uint32_t next[CT][4];
+    bf16x8 fp[2][NP], qt[2][2][NI];
+    f32x4 eg;
+    const auto load_go = [&](int n) {
+      const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
+#pragma unroll
+      for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(ir, p.col(i) < a.V ? row * is + p.col(i) * sizeof(E) : kOutOfRange, r * is);
+      eg = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(img + n * kImage + I::kGate) + row);
+    };
+    const auto put_go = [&]() {
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        f32x4 go;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) go[r] = value<E>(next[i][r]);
+        uint2 l[NI], u[3];
+        split4(go, l);
+        put_half<2 * CT>(xo, 2 * i + pw, lane, w & 1, l);
+        split4(a.scale * eg * go, u);
+        put_half<2 * CT>(xu, 2 * i + pw, lane, w & 1, u);
+      }
+    };
+    const auto load_pq = [&](int n) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (q >= half.value) load_frag(img + n * kImage + I::kPT + I::high(w, q, NP), lane, fp[q]);
+      if (KB == 4 || w < KB) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) load_frag(img + n * kImage + I::kQT + I::cols(2 * w + t, q), lane, qt[t][q]);
+      }
+    };
+    const auto products = [&]() {
+      f32x4 x[CT], y[CT][2];
+#pragma unroll
+      for (int i = 0; i < CT; ++i) x[i] = y[i][0] = y[i][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          if (q >= half.value) {
+            bf16x8 b[NI];
+            get<2 * CT>(xo, 2 * i + q, lane, b);
+            x[i] = mm<3>(fp[q], b, x[i]);
+          }
+          if (KB == 4 || w < KB) {
+            bf16x8 b[3];
+            get<2 * CT>(xu, 2 * i + q, lane, b);
+            y[i][0] = mm<3>(qt[0][q], b, y[i][0]);
+            y[i][1] = mm<3>(qt[1][q], b, y[i][1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CT; ++i) xp[w][i][lane] = x[i], xq[w][i][0][lane] = y[i][0], xq[w][i][1][lane] = y[i][1];
+    };
+    load_go(last_n), load_pq(last_n);
+    put_go();
+    load_go(max(last_n - 1, 0));
+    sync();
+    products();
+    load_pq(max(last_n - 1, 0));
+    settled();
+    sync();
+#pragma unroll 1
+    for (int n = last_n; n >= 0; --n) {
+      const int64_t c = static_cast<int64_t>(p.bh) * a.NC + n;
       put_go();
       load_go(max(n - 2, 0));
-      publish<KP, NI>(S, xs, n > 0 ? a.dSw : nullptr, c - 1, a, p);
-      sync();  // the state and do are there
+      keep_state<KP, NI, CT>(a.dSw, c, xs, a, p);
+      sync();  // do is there, and the last products have been read
+      products();
+      load_pq(max(n - 2, 0));
+      sync();
+      sync();  // the state is there
     }
   };
-  if (pw == 0)
-    run(int_c<0>{});
-  else
-    run(int_c<1>{});
-  if (a.dh0 && w < KB) store_state(S, a.dh0, a, p);
+  if (p.chain) {
+    if (pw == 0)
+      chain(int_c<0>{});
+    else
+      chain(int_c<1>{});
+  } else {
+    if (pw == 0)
+      beside(int_c<0>{});
+    else
+      beside(int_c<1>{});
+  }
 }
 
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
@@ -1569,16 +1677,16 @@ int launch_fwd(const Args& a, bool keep_, hipStream_t st_) {
   if constexpr (NI == 1) {
     if (ct == 2) {
       if (keep_)
-        hipLaunchKernelGGL((state_kernel<KP, NI, true, 2>), grid, dim3(256), 0, st_, a);
+        hipLaunchKernelGGL((state_kernel<KP, NI, true, 2>), grid, dim3(512), 0, st_, a);
       else
-        hipLaunchKernelGGL((state_kernel<KP, NI, false, 2>), grid, dim3(256), 0, st_, a);
+        hipLaunchKernelGGL((state_kernel<KP, NI, false, 2>), grid, dim3(512), 0, st_, a);
       return check_launch("mg_delta_fwd");
     }
   }
   if (keep_)
-    hipLaunchKernelGGL((state_kernel<KP, NI, true, 1>), grid, dim3(256), 0, st_, a);
+    hipLaunchKernelGGL((state_kernel<KP, NI, true, 1>), grid, dim3(512), 0, st_, a);
   else
-    hipLaunchKernelGGL((state_kernel<KP, NI, false, 1>), grid, dim3(256), 0, st_, a);
+    hipLaunchKernelGGL((state_kernel<KP, NI, false, 1>), grid, dim3(512), 0, st_, a);
   return check_launch("mg_delta_fwd");
 }
 
@@ -1589,9 +1697,9 @@ int launch_bwd(const Args& a, hipStream_t st_) {
   const int ct = columns_for(bh, a.VP, NI);
   const dim3 grid(bh * (a.VP / 16 / ct));
   if constexpr (NI == 1) {
-    if (ct == 2) hipLaunchKernelGGL((dstate_kernel<KP, NI, 2>), grid, dim3(256), 0, st_, a);
+    if (ct == 2) hipLaunchKernelGGL((dstate_kernel<KP, NI, 2>), grid, dim3(512), 0, st_, a);
   }
-  if (ct == 1) hipLaunchKernelGGL((dstate_kernel<KP, NI, 1>), grid, dim3(256), 0, st_, a);
+  if (ct == 1) hipLaunchKernelGGL((dstate_kernel<KP, NI, 1>), grid, dim3(512), 0, st_, a);
   hipLaunchKernelGGL((grad_kernel<KP, NI>), dim3(bh * a.NC), dim3(64 * GradTile<KP, NI>::W), 0, st_, a);
   if (a.H > a.Hk) {
     const int64_t n = static_cast<int64_t>(a.B) * a.T * a.Hk * a.K;
