@@ -24,16 +24,14 @@
 // sees v_i / c_i, c_i q_i and (at the end) c_C; the gradient of log c_i follows
 // from theirs.
 //
-// Three kinds of kernel:
-//   chunk_kernel  one workgroup per (chunk, head), all in parallel: T, P and the decays;
-//   state_kernel, dstate_kernel  the pass over the chunks in order. A wave owns
-//     16 value columns of S for good, in the accumulators of its matrix
-//     instructions: every product of the chain (K S, T y, P d, K^T d) contracts
-//     the rows and keeps the columns, and the accumulator layout (lane = column,
-//     registers = rows) is the B operand's layout up to the order of the rows,
-//     which the A operands read from LDS make up for. So the chain never leaves
-//     the wave's registers, and waves only share the chunk's A operands in LDS;
-//   grad_kernel   one workgroup per (chunk, head): what contracts the value columns.
+// The kernels:
+//   chunk_kernel  one workgroup per (chunk, head), all in parallel: T, P, the decays, and the
+//     chunk's operands in the order in which the passes load them;
+//   state_kernel, dstate_kernel  the pass over the chunks in order, forward and backward, which alone
+//     holds the state (or its gradient); the products that contract the tokens or K;
+//   grad_kernel   one workgroup per (chunk, head): what contracts the value columns;
+//   step_kernel   single tokens.
+// Times below are for K = V = 128 in bf16: B8 T2047 H8, forward and backward, and B2 T16381 H16, forward.
 //
 // Matrix operands are bf16. An fp32 value enters as limbs, x = h + m + l with 8
 // bits each (exact), and the limb products down to 2^-16 of the leading one are
@@ -390,8 +388,11 @@ __device__ __forceinline__ void put_blocks(const float* m, char* low, char* high
   }
 }
 
-// k and q are read once, all loads of a thread under way at a time, and go to the image and to LDS, which
-// A and T take over once k k^T and q k^T are in registers.
+// k and q are read once, all loads of a thread under way at a time, and go to LDS and from there, as fragments, to the
+// image; A and T take over the LDS once k k^T and q k^T are in registers, P A's once T is done: 36 KB, four workgroups
+// to a CU. Bound by memory, by what the image takes: 66 us for 330 MB (125 KB a chunk with what the backward
+// reads), 182 us for 930 MB (79 KB a chunk): 5.0 and 5.1 TB/s. (Reading k and q where they were needed, one
+// load after the other: 84 us for a smaller image, at 2.6 TB/s.)
 template <int KP, int NI>
 __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a, bool keep) {
   using E = typename elem<NI>::type;
@@ -589,17 +590,22 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a, boo
 
 // ---------------------------------------------------------------- the pass over the chunks
 //
-// A workgroup of four waves owns 16 CT value columns of one head's state and takes the chunks in order.
-// The state never leaves its accumulators: wave w holds rows 32 w ... 32 w + 31 of S and, in each chunk,
-// makes rows 16 w' ... (16 of the 64 tokens) of y, d and o. What the other waves need as a B operand,
-// S for K S and Q S, y for T y, d for K^T d and P d, goes through LDS as limbs, already in the operand's
-// register order (an accumulator's lane is the operand's lane: a fragment is 16 bytes per lane, written and
-// read without conflicts). Three barriers a chunk; its operands arrive by asynchronous copies that
-// are issued as soon as the part of LDS is free that they go to, up to a chunk ahead.
+// A workgroup of eight waves owns 16 CT value columns of one head's state and takes the chunks in order. Four of
+// them are the chain: the state never leaves their accumulators. Wave w holds rows 32 w ... 32 w + 31 of S and, in
+// each chunk, makes 16 of the 64 tokens' y and d (dd and dy in the backward). What other waves need as a B
+// operand, S for K S, y for T y, d for K^T d, goes through LDS as limbs, already in the operand's register order (an
+// accumulator's lane is the operand's lane: a fragment is 16 bytes per lane, written and read without conflicts).
+// The A operands are different for every wave, so they pass no LDS: each wave loads its own fragments from the
+// chunk's image into registers, a chunk ahead. Three barriers a chunk. The other four waves do what the chain does
+// not wait for, between the same barriers: o = scale e^G Q S + P d and what is kept; in the backward P^T do and
+// Q^T (scale e^G do), a chunk ahead.
 //
-// Against a wave of its own for each 16 columns (no exchange, no barriers, 4 to 8 times fewer
-// waves): the chain of one chunk, not the work, bounds the pass, and one wave took 4.1 us a chunk
-// for it (B2 T16381 H16 K128 V128, 1053 us).
+// Bound by the chain: 482 us for 256 chunks are 1.9 us a chunk, of which 1.3 pass with no loads at all (dependent
+// products, limbs, three exchanges) and the rest are loads that come late when all CUs draw on the L2s (each of a head's
+// workgroups loads all of its image). B8 T2047 H8: state 131, its gradient 130 us, 3.3 TB/s for the 430 MB each that
+// cross memory. Tried before, B2 T16381 H16: a wave of its own for each 16 columns with no exchange, 1053 us; the
+// operands through LDS by asynchronous copies, 553; no separate waves for o, 504. Asking for the image two chunks
+// ahead so that the loads find it in L2 changed nothing.
 
 // Workgroups of one (batch, head) differ by the value columns and read the same chunk operands: ids
 // that are equal modulo the 8 XCDs, so that they share an L2.
@@ -1223,7 +1229,10 @@ struct GradTile {
 // 16-byte unit u of row r of a matrix with four: a fragment's 16 rows spread over all banks
 __device__ __forceinline__ int at4(int r, int u) { return (r * 4 + (u ^ ((r >> 2) & 3))) * 16; }
 
-// bf16, 128 columns: two workgroups of 8 waves per CU, whose waits for the operands the other one fills
+// A wave has 16 columns of K. The kept operands come through LDS, 32 value columns at a time; two workgroups to a CU (bf16:
+// 128 registers, 78 KB), one of which works while the other waits for its operands. Bound by memory: 145 us for 590 MB,
+// 4.1 TB/s. (One workgroup to a CU, do read by every wave that needed it, and a lane per column, whose sums
+// over K crossed lanes and whose stores were of two bytes: 278 us.)
 template <int KP, int NI>
 __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) void grad_kernel(Args a) {
   using E = typename elem<NI>::type;
@@ -1490,7 +1499,7 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(const float* dqp, const 
 // ---------------------------------------------------------------- single tokens
 //
 // One workgroup per (batch, head, 32 value columns): thread (r, c) holds rows r, r + 32, ... and columns
-// 4 c ... 4 c + 3 of the state, read and written once. k S and q S are taken together from the old
+// 4 c ... 4 c + 3 of the state, read and written once: bound by memory, B128 H16 52 us for 270 MB, 5.2 TB/s. k S and q S are taken together from the old
 // state: o = scale (e^g q S + (q.k) d), d = beta (v - e^g k S). ONCE: past the caches, see launch_step.
 template <bool ONCE>
 __device__ __forceinline__ f4 load_state4(const float* p) {
@@ -1649,8 +1658,9 @@ inline int check_out(const char* fn, int dtype, const mg_delta_dims* s) {
   return MG_OK;
 }
 
-// Value columns per workgroup of the passes over the chunks, in tiles of 16: two where that still leaves
-// a workgroup for every CU (the chunk's operands are then read for twice the columns), else one. fp32 has LDS for one.
+// Value columns per workgroup of the passes over the chunks, in tiles of 16: two where that still leaves a workgroup
+// for every CU, so that a chunk's operands are loaded for twice the columns (B8 T2047 H8: 131 and 130 us against
+// 170 and 170 with one), else one, for more workgroups. fp32 loads three limbs for one and is kept at one.
 inline int columns_for(int64_t bh, int vp, int dtype_limbs) {
   return dtype_limbs == 1 && bh * (vp / 32) >= kCUs ? 2 : 1;
 }

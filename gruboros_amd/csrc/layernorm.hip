@@ -8,13 +8,18 @@
 //   dxn = r (g - mean(g) - h mean(g h)) + dres,  ddelta = keep(delta) dxn / (1 - p)
 //   dw  = sum over rows of dy h,  db = sum over rows of dy
 //
-// A row belongs to one wave up to 1024 columns (16 bytes of fp32 per lane and
-// step), else to a workgroup of 256 threads, and stays in registers between its passes: the
-// variance is that of the centred values, not a difference of two sums. Any D:
-// the loads are 16 bytes wide at whatever alignment the rows have (the memory
-// pipe takes them), and the last vector of a row is done element by element.
-// The weight's gradients: lanes sum over their rows, a workgroup's lanes in
-// LDS, its sum goes to a partial row, and a second kernel adds the partial rows in order.
+// A row belongs to one wave up to 1024 columns (16 bytes of fp32 per lane and step), else to a workgroup of 256
+// threads, and stays in registers between its passes: the variance is that of the centred values, not a difference of
+// two sums. How many steps a row of D has is known at compile time, and all but the last ones are whole, so that they
+// carry no masks (with a mask per element a row's masks alone overflowed the scalar registers: 134 us for the forward
+// below, against 76). Any D: the loads are 16 bytes wide at whatever alignment the rows have (the memory pipe takes
+// them), and the last vector of a row is done element by element.
+// The weight's gradients: lanes sum over their rows, a workgroup's lanes in LDS, its sum goes to a partial row, and a
+// second kernel adds the partial rows in order. The backward's grid is what the device holds at once, 1024 workgroups
+// (768: 3% slower at D 1024, as fast at D 2048).
+//
+// Bound by memory. fp32 stream, bf16 branch, N 16376 D 1024: forward 42 us (4.7 TB/s), backward 45 us (5.9), partial
+// rows 5 us; N 16380 D 2048 with dropout: 76 us (5.3), 104 us (5.2).
 
 #include <algorithm>
 

@@ -87,8 +87,12 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, scale=None, return_st
 
     Returns o [B, T, H, V] in the inputs' dtype, or (o, last state float32 [B, H, K, V]) with
     return_state. Gradients reach all six tensors (not twice: no double backward). Where gradients
-    are recorded, each 64 tokens of a head keep their state, updates and small matrices for the
-    backward: about 4 K V + 256 V + 41000 bytes (65000 in float32)."""
+    are recorded, each 64 tokens of a head keep their state, updates and operands for the backward:
+    4 K V + 256 V + 128500 bytes for K > 64, 95700 in place of the last for K <= 64 (float32:
+    6 K V + 384 V + 271900 or 173600), with K rounded up to 64 or 128 and V to a multiple of 32.
+
+    A value that is not finite spoils the 64 tokens of its chunk, earlier ones included: padding
+    behind a sequence must be finite."""
     _check(q, k, v, g, beta, initial_state, "initial_state", 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if q.shape[0] == 0 or q.shape[1] == 0:  # no token: nothing is written
