@@ -264,13 +264,14 @@ __device__ __forceinline__ bf16x8 frag_t(const char* m, int t, int p, int lane) 
 // limb of one (16 bytes per lane), each read by one wave of a pass straight into the registers that the instruction
 // takes them from. Rows of k and q [tile of 16 tokens, in row_of order][32 of K]; k^T and q^T [16 of K, in row_of
 // order][32 tokens]; of T and P the blocks of 16 rows and 32 columns that reach the diagonal, and of T^T and P^T;
-// each with its limbs. And the vectors e^G, e^{G_C - G}, beta. What only the backward reads comes last.
+// each with its limbs (of P two for bf16, whose o is rounded to it; of P^T
+// three, as the state's gradient is fp32). And the vectors e^G, e^{G_C - G}, beta. What only the backward reads comes last.
 template <int KP, int NI>
 struct Tile {
   static constexpr int NP = NI == 3 ? 3 : 2, KB = KP / 32, U = KP / 8;
   static constexpr int F = 1024, kRows = 4 * KB * NI * F, nT = 6 * 3 * F, nP = 6 * NP * F;
   static constexpr int kK = 0, kKT = kRows, kQ = 2 * kRows, kT = 3 * kRows, kP = kT + nT, kGate = kP + nP, kOnce = kGate + F;
-  static constexpr int kQT = kOnce, kTT = kQT + kRows, kPT = kTT + nT, kKept = kPT + nP;
+  static constexpr int kQT = kOnce, kTT = kQT + kRows, kPT = kTT + nT, kKept = kPT + nT;
   // limb 0 of block (tile t, 32 of K or 32 tokens b)
   static constexpr int rows(int t, int kb) { return (t * KB + kb) * NI * F; }
   static constexpr int cols(int t, int p) { return (t * 2 + p) * NI * F; }
@@ -363,7 +364,8 @@ __device__ __forceinline__ f32x4 mm16(const float* a, f32x4 b, f32x4 c, int lane
   return c;
 }
 
-// The blocks of a 64 x 64 lower triangle in LDS, and with `both` those of its transpose, as limbs to the image: wave w's tiles w
+// The blocks of a 64 x 64 lower triangle in LDS as N limbs, and with `both` those of its transpose as three, to the
+// image: wave w's tiles w
 template <int N>
 __device__ __forceinline__ void put_blocks(const float* m, char* low, char* high, bool both, int lane, int w) {
   using L = Tile<64, 1>;
@@ -372,7 +374,7 @@ __device__ __forceinline__ void put_blocks(const float* m, char* low, char* high
   for (int p = 0; p < 2; ++p) {
     const int c0 = 32 * p + 8 * g;
     float x[8];
-    bf16x8 l[N];
+    bf16x8 l[N], h[3];
     if (p <= w / 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = c0 + i <= r ? m[r * LD + c0 + i] : 0.0f;
@@ -382,15 +384,15 @@ __device__ __forceinline__ void put_blocks(const float* m, char* low, char* high
     if (both && p >= w / 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = r <= c0 + i ? m[(c0 + i) * LD + r] : 0.0f;
-      split<N>(x, l);
-      store_frag(high + L::high(w, p, N), lane, l);
+      split<3>(x, h);
+      store_frag(high + L::high(w, p, 3), lane, h);
     }
   }
 }
 
 // k and q are read once, all loads of a thread under way at a time, and go to LDS and from there, as fragments, to the
 // image; A and T take over the LDS once k k^T and q k^T are in registers, P A's once T is done: 36 KB, four workgroups
-// to a CU. Bound by memory, by what the image takes: 66 us for 330 MB (125 KB a chunk with what the backward
+// to a CU. Bound by memory, by what the image takes: 68 us for 340 MB (131 KB a chunk with what the backward
 // reads), 182 us for 930 MB (79 KB a chunk): 5.0 and 5.1 TB/s. (Reading k and q where they were needed, one
 // load after the other: 84 us for a smaller image, at 2.6 TB/s.)
 template <int KP, int NI>
@@ -982,7 +984,7 @@ template <int KP, int NI, int CT>
 __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
   using E = typename elem<NI>::type;
   using I = Tile<KP, NI>;
-  constexpr int KB = I::KB, NP = I::NP, NW = kKept<NI>;
+  constexpr int KB = I::KB, NW = kKept<NI>;
   __shared__ __attribute__((aligned(16))) char xs[CT * KB * 3 * kFrag], xy[CT * 6 * kFrag], xe[CT * 6 * kFrag];
   __shared__ __attribute__((aligned(16))) char xu[CT * 6 * kFrag], xo[CT * 2 * NI * kFrag];
   __shared__ f32x4 xp[4][CT][64], xq[4][CT][2][64];  // P^T do and Q^T (scale e^G do) in the accumulators' order
@@ -1117,7 +1119,7 @@ __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
     const E* dout = reinterpret_cast<const E*>(a.dout) + p.b * a.do_sb + p.h * a.do_sh;
     const uint32_t is = static_cast<uint32_t>(a.do_st * sizeof(E));
     uint32_t next[CT][4];
-    bf16x8 fp[2][NP], qt[2][2][NI];
+    bf16x8 fp[2][3], qt[2][2][NI];
     f32x4 eg;
     const auto load_go = [&](int n) {
       const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
@@ -1143,7 +1145,7 @@ __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
     const auto load_pq = [&](int n) {
 #pragma unroll
       for (int q = 0; q < 2; ++q)
-        if (q >= half.value) load_frag(img + n * kImage + I::kPT + I::high(w, q, NP), lane, fp[q]);
+        if (q >= half.value) load_frag(img + n * kImage + I::kPT + I::high(w, q, 3), lane, fp[q]);
       if (KB == 4 || w < KB) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)

@@ -88,7 +88,7 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, scale=None, return_st
     Returns o [B, T, H, V] in the inputs' dtype, or (o, last state float32 [B, H, K, V]) with
     return_state. Gradients reach all six tensors (not twice: no double backward). Where gradients
     are recorded, each 64 tokens of a head keep their state, updates and operands for the backward:
-    4 K V + 256 V + 128500 bytes for K > 64, 95700 in place of the last for K <= 64 (float32:
+    4 K V + 256 V + 134700 bytes for K > 64, 101900 in place of the last for K <= 64 (float32:
     6 K V + 384 V + 271900 or 173600), with K rounded up to 64 or 128 and V to a multiple of 32.
 
     A value that is not finite spoils the 64 tokens of its chunk, earlier ones included: padding
