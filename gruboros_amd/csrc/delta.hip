@@ -1224,8 +1224,8 @@ struct GradTile {
   static constexpr int kQ = kS, kF = kQ + NI * C * KP * 2, kN = kF + NW * kPlane * 2;  // then in their place q, F, N
   static constexpr int kEnd = kV + kRows > kN + NW * kPlane * 2 ? kV + kRows : kN + NW * kPlane * 2;
   static constexpr int kG = kEnd, kGate = kG + 512;                           // the chunk's G (doubles) and gates
-  static constexpr int kSums = kGate + 1024;                                  // floats: q.dq, k.Z [W][64], dy.v [64], [W]
-  static constexpr int kBytes = kSums + (2 * W * 64 + 64 + W) * 4;
+  static constexpr int kSums = kGate + 1024;                                  // floats: q.dq, k.Z [W][64], dy.v [64], [W], [W]
+  static constexpr int kBytes = kSums + (2 * W * 64 + 64 + 2 * W) * 4;
 };
 
 // 16-byte unit u of row r of a matrix with four: a fragment's 16 rows spread over all banks
@@ -1294,6 +1294,7 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
 #pragma unroll
   for (int t = 0; t < 4; ++t) w1[t] = w2[t] = w3[t] = m1[t] = m2[W == 4 ? t : 0] = f32x4{0, 0, 0, 0};
   const int mr = wave & 3, blocks = a.VP / 32;
+  bool state = n > 0;  // whether the chunk begins with one that is not zero
 #pragma unroll 1
   for (int vb = 0; vb < blocks; ++vb) {
     const int64_t blk = c * blocks + vb;
@@ -1312,6 +1313,10 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     bf16x8 s[NW], ds[NW], yr[NW], vr[NI], orr[W == 4 ? NI : 1];
     kept_frags(lds + L::kS, state_at, ln, s);
     kept_frags(lds + L::kE, state_at, ln, ds);
+    if (n == 0) {
+      const u32x4 x = __builtin_bit_cast(u32x4, s[0]);
+      state = state || __any((x[0] | x[1] | x[2] | x[3]) & 0x7fff7fffu);
+    }
     ss = mm<NW>(s, ds, ss);
     if (second) {  // (do as the first limbs)
       bf16x8 x[NI];
@@ -1460,12 +1465,12 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-  if (lane == 0) vec[(2 * W + 1) * 64 + wave] = dot;
+  if (lane == 0) vec[(2 * W + 1) * 64 + wave] = dot, vec[(2 * W + 1) * 64 + W + wave] = state ? 1.0f : 0.0f;
   __syncthreads();
   if (wave == 0) {
-    float qd = 0.0f, kz = 0.0f, all = 0.0f;
+    float qd = 0.0f, kz = 0.0f, all = 0.0f, begun = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) qd += vec[w * 64 + lane], kz += vec[(W + w) * 64 + lane], all += vec[(2 * W + 1) * 64 + w];
+    for (int w = 0; w < W; ++w) qd += vec[w * 64 + lane], kz += vec[(W + w) * 64 + lane], all += vec[(2 * W + 1) * 64 + w], begun += vec[(2 * W + 1) * 64 + W + w];
     const float y = vec[2 * W * 64 + lane], be = gt[128 + lane];
     double s = static_cast<double>(qd) - static_cast<double>(be) * y;
 #pragma unroll
@@ -1475,8 +1480,9 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     }
     if (lane < rows) {
       const int64_t tok = (tok0 + lane) * a.H + h;
-      // a decay that is zero in fp32 passes nothing on
-      st(reinterpret_cast<E*>(a.dg) + tok, gv < -104.0f ? 0.0f : static_cast<float>(s + all));
+      // a decay that is zero in fp32 passes nothing on, and no state has none: exactly, not as a difference of sums
+      const bool none = gv < -104.0f || (lane == 0 && begun == 0.0f);
+      st(reinterpret_cast<E*>(a.dg) + tok, none ? 0.0f : static_cast<float>(s + all));
       st(reinterpret_cast<E*>(a.db) + tok, y - kz);
     }
   }

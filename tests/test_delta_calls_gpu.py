@@ -339,3 +339,19 @@ def test_one_derivative_only():
         gated_delta_step(*(t[:, 0] for t in xs), state)
     with pytest.raises(RuntimeError):
         y.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 70])
+def test_the_first_decay_without_a_state(T, dtype):
+    """Nothing is there to decay at the first token: its g has no gradient at all, exactly."""
+    from gruboros_amd.delta import gated_delta_rule
+
+    xs, do = _inputs(2, T, 1, 2, 72, 40, dtype)
+    dev = [t.to(DEV).requires_grad_(True) for t in xs]
+    for h0 in (None, torch.zeros(2, 2, 72, 40, device=DEV)):
+        dg = torch.autograd.grad(gated_delta_rule(*dev, initial_state=h0), dev, do.to(DEV))[3]
+        assert bool((dg[:, 0] == 0).all()) and (T == 1 or bool((dg[:, 1:] != 0).any()))
+    h0[1] = 1.0  # one sequence has a state
+    dg = torch.autograd.grad(gated_delta_rule(*dev, initial_state=h0), dev, do.to(DEV))[3]
+    assert bool((dg[0, 0] == 0).all()) and bool((dg[1, 0] != 0).all())
