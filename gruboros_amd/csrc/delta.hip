@@ -602,9 +602,9 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a, boo
 // not wait for, between the same barriers: o = scale e^G Q S + P d and what is kept; in the backward P^T do and
 // Q^T (scale e^G do), a chunk ahead.
 //
-// Bound by the chain: 482 us for 256 chunks are 1.9 us a chunk, of which 1.3 pass with no loads at all (dependent
+// Bound by the chain: 490 us for 256 chunks are 1.9 us a chunk, of which 1.3 pass with no loads at all (dependent
 // products, limbs, three exchanges) and the rest are loads that come late when all CUs draw on the L2s (each of a head's
-// workgroups loads all of its image). B8 T2047 H8: state 131, its gradient 130 us, 3.3 TB/s for the 430 MB each that
+// workgroups loads all of its image). B8 T2047 H8: state 134, its gradient 134 us, 3.2 TB/s for the 430 MB each that
 // cross memory. Tried before, B2 T16381 H16: a wave of its own for each 16 columns with no exchange, 1053 us; the
 // operands through LDS by asynchronous copies, 553; no separate waves for o, 504. Asking for the image two chunks
 // ahead so that the loads find it in L2 changed nothing.
@@ -1232,8 +1232,8 @@ struct GradTile {
 __device__ __forceinline__ int at4(int r, int u) { return (r * 4 + (u ^ ((r >> 2) & 3))) * 16; }
 
 // A wave has 16 columns of K. The kept operands come through LDS, 32 value columns at a time; two workgroups to a CU (bf16:
-// 128 registers, 78 KB), one of which works while the other waits for its operands. Bound by memory: 145 us for 590 MB,
-// 4.1 TB/s. (One workgroup to a CU, do read by every wave that needed it, and a lane per column, whose sums
+// 128 registers, 78 KB), one of which works while the other waits for its operands. Bound by memory: 149 us for 600 MB,
+// 4.0 TB/s. (One workgroup to a CU, do read by every wave that needed it, and a lane per column, whose sums
 // over K crossed lanes and whose stores were of two bytes: 278 us.)
 template <int KP, int NI>
 __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) void grad_kernel(Args a) {

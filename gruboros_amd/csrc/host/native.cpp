@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <optional>
 #include <sstream>
 #include <stdexcept>
@@ -833,6 +834,35 @@ Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   return o;
 }
 
+// The same for operands as generation has them: dense, aligned, nothing to record. None for any others (which
+// gruboros_amd.delta then brings into this form, or refuses): all that is asked of them is asked here, in one call.
+Opt delta_step_plain(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& state,
+                     std::optional<double> scale, int64_t stream) {
+  const auto type = q.scalar_type();
+  if ((type != at::kFloat && type != at::kBFloat16) || state.scalar_type() != at::kFloat || q.dim() != 3 || v.dim() != 3 ||
+      state.dim() != 4 || !k.sizes().equals(q.sizes()) || !beta.sizes().equals(g.sizes()) || g.dim() != 2)
+    return std::nullopt;
+  for (const Tensor* t : {&q, &k, &v, &g, &beta, &state})
+    if ((t != &state && t->scalar_type() != type) || !t->is_cuda() || t->device() != q.device() || !t->is_contiguous() ||
+        (t->requires_grad() && at::GradMode::is_enabled()))
+      return std::nullopt;
+  const int64_t B = v.size(0), H = v.size(1), V = v.size(2), Hk = q.size(1), K = q.size(2);
+  if (B < 1 || q.size(0) != B || g.size(0) != B || g.size(1) != H || Hk < 1 || H < 1 || H % Hk || K % 8 || K < 8 || K > 128 || V % 8 ||
+      V < 8 || V > 256 || state.size(0) != B || state.size(1) != H || state.size(2) != K || state.size(3) != V || B > INT32_MAX ||
+      H > INT32_MAX)
+    return std::nullopt;
+  for (const Tensor* t : {&v, &state})
+    if (reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16) return std::nullopt;
+  c10::DeviceGuard guard(q.device());
+  const mg_delta_dims d = {static_cast<int>(B), 1, static_cast<int>(Hk), static_cast<int>(H), static_cast<int>(K), static_cast<int>(V)};
+  Tensor o = make(v.sizes(), type, v);
+  check(mg_delta_step(code(q), &d, ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), scale ? *scale : 1.0 / std::sqrt(static_cast<double>(K)),
+                      fp(state), ptr(o), st(stream)),
+        "mg_delta_step");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return o;
+}
+
 // ------------------------------------------------------------------ layer norm, dropout
 
 // seed: a device int64 scalar read by the kernels, or the number itself
@@ -1034,4 +1064,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("delta_fwd", &delta_fwd, nogil());
   m.def("delta_bwd", &delta_bwd, nogil());
   m.def("delta_step", &delta_step, nogil());
+  m.def("delta_step_plain", &delta_step_plain, nogil());
 }

@@ -116,6 +116,8 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None):
     [B, H] as in gated_delta_rule, state float32 [B, H, K, V], contiguous, which is updated in
     place. Returns o [B, H, V]. No gradients are recorded: operands that require them are refused
     where they would be."""
+    if q.is_cuda and (o := native().delta_step_plain(q, k, v, g, beta, state, scale, stream_of(q))) is not None:
+        return o
     _check(q, k, v, g, beta, state, "state", 1)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
         raise ValueError("gated_delta_step records no gradients: call it under torch.no_grad(), or use gated_delta_rule")
