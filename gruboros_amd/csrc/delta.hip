@@ -86,7 +86,6 @@ struct Args {
 // ---------------------------------------------------------------- limbs
 
 __device__ __forceinline__ uint32_t hi16x2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-__device__ __forceinline__ uint32_t lo16x2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 
 // 8 fp32 values as N limbs. N = 3: by cutting the mantissa (8 + 8 + 8 bits, exact). N = 2: both rounded to
 // nearest, off by 2^-18 at most.
