@@ -160,32 +160,36 @@ __device__ __forceinline__ void st4(bf16_t* p, const f32x4& x) {
                                             static_cast<uint32_t>(f32_to_bf16(x[2])) | static_cast<uint32_t>(f32_to_bf16(x[3])) << 16);
 }
 
-// Column accesses of the passes over the chunks: a buffer over the chunk's rows of one head, the lane's
-// column and first row in its offset, a scalar offset per register. Rows and columns past the end are
-// out of the buffer's range: they read as zero and are not written.
+// Column accesses of the passes over the chunks. A lane has a column and, one register each, the rows `row` to
+// row + 3: a buffer over the chunk's rows of one head from row r on for register r, and the lane's column and first
+// row in its offset. Rows and columns past the end are out of that buffer's range (which is empty if the chunk ends
+// before r): they read as zero and are not written. (A scalar offset for r would be left out of the range check; a
+// check of every row by its lane took 40 registers more.) Rows that are closer than their length, a broadcast's, may
+// read a row that is there in place of one that is not: finite, and multiplied by the zeros of T, P and q beyond the end.
 constexpr uint32_t kOutOfRange = 0x80000000u;
 template <typename E>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const E* p, int64_t st_, int rows, int cols) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(p), static_cast<short>(0),
-                                           static_cast<int>(((rows - 1) * st_ + cols) * sizeof(E)), 0x00020000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const E* p, int64_t st_, int rows, int cols, int r = 0) {
+  const int64_t records = rows > r ? (rows - 1 - r) * st_ + cols : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(p) + (rows > r ? r * st_ : 0), static_cast<short>(0),
+                                           static_cast<int>(records * sizeof(E)), 0x00020000);
 }
 template <typename E>
-__device__ __forceinline__ uint32_t load_col(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t row_off) {  // raw
+__device__ __forceinline__ uint32_t load_col(__amdgpu_buffer_rsrc_t r, uint32_t off) {  // raw
   if constexpr (sizeof(E) == 2)
-    return __builtin_amdgcn_raw_buffer_load_b16(r, off, row_off, 0);
+    return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
   else
-    return __builtin_amdgcn_raw_buffer_load_b32(r, off, row_off, 0);
+    return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
 }
 template <typename E>
 __device__ __forceinline__ float value(uint32_t raw) {
   return __uint_as_float(sizeof(E) == 2 ? raw << 16 : raw);
 }
 template <typename E>
-__device__ __forceinline__ void store_col(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t row_off, float x) {
+__device__ __forceinline__ void store_col(__amdgpu_buffer_rsrc_t r, uint32_t off, float x) {
   if constexpr (sizeof(E) == 2)
-    __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x), r, off, row_off, 0);
+    __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x), r, off, 0, 0);
   else
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, off, row_off, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, off, 0, 0);
 }
 
 // four columns of a row
@@ -793,11 +797,12 @@ __global__ __launch_bounds__(512) void state_kernel(Args a) {
     f32x4 eg, tail, be;
     float last;
     const auto load_v = [&](int n) {
-      const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V);
 #pragma unroll
-      for (int i = 0; i < CT; ++i)
+      for (int r = 0; r < 4; ++r) {
+        const __amdgpu_buffer_rsrc_t vr = rows_buffer(v + static_cast<int64_t>(n) * C * a.v_st, a.v_st, min(C, a.T - n * C), a.V, r);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(vr, p.col(i) < a.V ? row * vs + p.col(i) * sizeof(E) : kOutOfRange, r * vs);
+        for (int i = 0; i < CT; ++i) next[i][r] = load_col<E>(vr, p.col(i) < a.V ? row * vs + p.col(i) * sizeof(E) : kOutOfRange);
+      }
     };
     const auto load_rows = [&](int n) {
 #pragma unroll
@@ -1071,7 +1076,6 @@ __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
         }
       }
       load_t(n1);
-      const __amdgpu_buffer_rsrc_t orr = rows_buffer(dv + t0 * v_st, v_st, rows, a.V);
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
         dy[i] = d2[i][0] + d2[i][1];
@@ -1081,7 +1085,7 @@ __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
         put_half<2 * CT>(xe, 2 * i + pw, lane, w & 1, l);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          store_col<E>(orr, p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, r * os, x[r]);
+          store_col<E>(rows_buffer(dv + t0 * v_st, v_st, rows, a.V, r), p.col(i) < a.V ? row * os + p.col(i) * sizeof(E) : kOutOfRange, x[r]);
       }
       const float decay = last;
       load_gates(n1);
@@ -1121,11 +1125,12 @@ __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
     bf16x8 fp[2][3], qt[2][2][NI];
     f32x4 eg;
     const auto load_go = [&](int n) {
-      const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V);
 #pragma unroll
-      for (int i = 0; i < CT; ++i)
+      for (int r = 0; r < 4; ++r) {
+        const __amdgpu_buffer_rsrc_t ir = rows_buffer(dout + static_cast<int64_t>(n) * C * a.do_st, a.do_st, min(C, a.T - n * C), a.V, r);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) next[i][r] = load_col<E>(ir, p.col(i) < a.V ? row * is + p.col(i) * sizeof(E) : kOutOfRange, r * is);
+        for (int i = 0; i < CT; ++i) next[i][r] = load_col<E>(ir, p.col(i) < a.V ? row * is + p.col(i) * sizeof(E) : kOutOfRange);
+      }
       eg = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(img + n * kImage + I::kGate) + row);
     };
     const auto put_go = [&]() {
