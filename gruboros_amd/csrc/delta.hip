@@ -19,10 +19,12 @@
 //   dq = scale e^G (do S^T) + N K,
 //   dk = e^{G_C - G} (d dS'^T) + N^T Q - F^T (beta K) - beta Z,
 //   dbeta = dy.v - k.Z,
-//   dg_t = <S', dS'> + sum_{i >= t in the chunk} (q_i.dq_i - v_i.dv_i).
-// The last line: with c_i = e^{G_i}, the rule for S_i / c_i has no decay and
-// sees v_i / c_i, c_i q_i and (at the end) c_C; the gradient of log c_i follows
-// from theirs.
+//   dg_t = e^{G_C} <S, dS'> + sum_{i >= t > j} M_ij
+//        + sum_{i >= t} (q_i.(scale e^G do S^T)_i - beta_i k_i.(e^G dy S^T)_i) + sum_{j < t} k_j.(e^{G_C - G} d dS'^T)_j,
+//   M_ij = N_ij q_i.k_j - beta_i F_ij k_i.k_j (j < i).
+// The last lines: every factor e^{G_i - G_j} that a result contains is multiplied with its gradient, and g_t is in those
+// with i >= t > j. Only these are summed, all of them as small as e^{g_t}: what a token that forgets passes on is no
+// difference of larger sums.
 //
 // The kernels:
 //   chunk_kernel  one workgroup per (chunk, head), all in parallel: T, P, the decays, and the
@@ -1215,6 +1217,48 @@ __global__ __launch_bounds__(512) void dstate_kernel(Args a) {
   }
 }
 
+// ---------------------------------------------------------------- sums over lanes
+
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float x) {  // another lane's value, 0 where there is none or the row of 16 is not in ROWS
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xf, false));
+}
+// x: a in even rows of 16 lanes and the even rows' b in odd ones; y: the odd rows' a in even rows and b in odd ones
+__device__ __forceinline__ void swap16(float a, float b, float& x, float& y) {
+  const auto v = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  x = __uint_as_float(v[0]), y = __uint_as_float(v[1]);
+}
+__device__ __forceinline__ void swap32(float a, float b, float& x, float& y) {  // the same with halves of 32
+  const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  x = __uint_as_float(v[0]), y = __uint_as_float(v[1]);
+}
+// The sums of four values over the four lanes m, m + 16, ...: of value g in row g
+__device__ __forceinline__ float sum_groups(const float (&v)[4]) {
+  float a, b, c, d;
+  swap32(v[0], v[2], a, b);
+  swap32(v[1], v[3], c, d);
+  swap16(a + b, c + d, a, b);
+  return a + b;
+}
+// The sums over the lanes up to each, and from each on (g: its row)
+__device__ __forceinline__ float sum_up_to(float x) {
+  x += dpp<0x111>(x);
+  x += dpp<0x112>(x);
+  x += dpp<0x114>(x);
+  x += dpp<0x118>(x);
+  x += dpp<0x142, 0xa>(x);  // row 0 into 1, 2 into 3
+  return x + dpp<0x143, 0xc>(x);
+}
+__device__ __forceinline__ float sum_from(float x, int g) {
+  x += dpp<0x101>(x);
+  x += dpp<0x102>(x);
+  x += dpp<0x104>(x);
+  x += dpp<0x108>(x);
+  const auto row = [&](int r) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 16 * r)); };
+  const float r1 = row(1), r2 = row(2), r3 = row(3);
+  return x + ((g < 1 ? r1 : 0.0f) + (g < 2 ? r2 : 0.0f) + (g < 3 ? r3 : 0.0f));
+}
+
 // ---------------------------------------------------------------- dq, dk, dg, dbeta of a chunk
 
 template <int KP, int NI>
@@ -1228,8 +1272,8 @@ struct GradTile {
   static constexpr int kQ = kS, kF = kQ + NI * C * KP * 2, kN = kF + NW * kPlane * 2;  // then in their place q, F, N
   static constexpr int kEnd = kV + kRows > kN + NW * kPlane * 2 ? kV + kRows : kN + NW * kPlane * 2;
   static constexpr int kG = kEnd, kGate = kG + 512;                           // the chunk's G (doubles) and gates
-  static constexpr int kSums = kGate + 1024;                                  // floats: q.dq, k.Z [W][64], dy.v [64], [W], [W]
-  static constexpr int kBytes = kSums + (2 * W * 64 + 64 + 2 * W) * 4;
+  static constexpr int kSums = kGate + 1024;                                  // floats: dg, k.Z [W][64], dy.v [64]
+  static constexpr int kBytes = kSums + (2 * W * 64 + 64) * 4;
 };
 
 // 16-byte unit u of row r of a matrix with four: a fragment's 16 rows spread over all banks
@@ -1246,7 +1290,8 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
   using I = Tile<KP, NI>;
   constexpr int NW = L::NW, W = L::W;
   __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x;
   const int bh = blockIdx.x / a.NC, n = blockIdx.x - bh * a.NC, h = bh % a.H, b = bh / a.H, grp = a.H / a.Hk;
   const int hk = h / grp, t0 = n * C, rows = min(C, a.T - t0);
@@ -1286,8 +1331,6 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     reinterpret_cast<float4*>(lds + L::kGate)[lane] = reinterpret_cast<const float4*>(img + I::kGate)[lane];
     reinterpret_cast<double*>(lds + L::kG)[lane] = a.Gd[c * 64 + lane];
   }
-  float gv = 0.0f;
-  if (wave == 0 && lane < rows) gv = ld(reinterpret_cast<const E*>(a.g) + b * a.g_sb + (t0 + lane) * a.g_st + h * a.g_sh);
 
   // Products over the value columns, 32 at a time, in this wave's 16 columns of K: W1 = dy S^T, W2 = do S^T,
   // W3 = d dS'^T, and a diagonal block of S dS'^T. Of the 64 x 64 products dy d^T and do d^T a wave takes 16 rows of
@@ -1298,7 +1341,6 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
 #pragma unroll
   for (int t = 0; t < 4; ++t) w1[t] = w2[t] = w3[t] = m1[t] = m2[W == 4 ? t : 0] = f32x4{0, 0, 0, 0};
   const int mr = wave & 3, blocks = a.VP / 32;
-  bool state = n > 0;  // whether the chunk begins with one that is not zero
 #pragma unroll 1
   for (int vb = 0; vb < blocks; ++vb) {
     const int64_t blk = c * blocks + vb;
@@ -1317,10 +1359,6 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     bf16x8 s[NW], ds[NW], yr[NW], vr[NI], orr[W == 4 ? NI : 1];
     kept_frags(lds + L::kS, state_at, ln, s);
     kept_frags(lds + L::kE, state_at, ln, ds);
-    if (n == 0) {
-      const u32x4 x = __builtin_bit_cast(u32x4, s[0]);
-      state = state || __any((x[0] | x[1] | x[2] | x[3]) & 0x7fff7fffu);
-    }
     ss = mm<NW>(s, ds, ss);
     if (second) {  // (do as the first limbs)
       bf16x8 x[NI];
@@ -1347,9 +1385,11 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
       if constexpr (W == 4) m2[t] = mm<NW>(f, orr, m2[t]);
     }
   }
+  asm volatile("" : "+v"(lane));  // (as in the blocks: the places below are not held through them)
+  m = lane & 15, g = lane >> 4;
   __syncthreads();
   stage<I::kRows, W>(lds + L::kQ, img + I::kQ, lane, wave);
-  // F and N, in this wave's rows, to LDS
+  // F and N, in this wave's rows, to LDS, and what of them M takes
   const auto put = [&](int plane, int row, int col, const f32x4& x) {
     uint2 l[NW];
     split4<NW>(x, l);
@@ -1359,6 +1399,7 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
   {
     const int row = 16 * mr + m;
     const double Gr = Gd[row];
+    const float be = gt[128 + row];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int col = 16 * t + 4 * g;
@@ -1371,6 +1412,10 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
       }
       if (W == 4 || !second) put(L::kF, row, col, f);
       if (W == 4 || second) put(L::kN, row, col, x);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = col + r < row ? x[r] : 0.0f;
+      m1[t] = W == 8 && second ? x : -be * f;
+      if constexpr (W == 4) m2[t] = x;
     }
   }
 #pragma unroll
@@ -1385,11 +1430,6 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
       if (4 * g + r == m) vec[2 * W * 64 + 16 * mr + m] = yv[r];
   }
   staged();
-  // <S', dS'> = e^{G_C} <S, dS'> + sum_j k_j.(e^{G_C - G_j} (d dS'^T)_j): its first part from the diagonals
-  float dot = 0.0f;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) dot += 4 * g + r == m ? ss[r] : 0.0f;
-  dot *= gt[63];
   const int d = 16 * wave + 4 * g;
   // k and q where this wave's accumulators are
   const auto at_acc = [&](int base, int row) {
@@ -1402,11 +1442,87 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
     }
     return x;
   };
+  {
+    // This wave's part of dg. M in its 16 rows: tiles left of the diagonal one are summed over the rows first, then
+    // over the columns up to each; in the diagonal tile a row adds its columns up to each that lies before it.
+    const auto rows_of = [&](int base, int t, int kb, bf16x8 (&out)[NI]) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const f32x4 k = at_acc(L::kK, 16 * t + m);
+      for (int l = 0; l < NI; ++l) out[l] = *reinterpret_cast<const bf16x8*>(lds + base + l * 1024 + I::unit(16 * t + m, 4 * kb + g));
+    };
+    float c[16], before = 0.0f;  // columns 16 t + 4 g + r at 4 t + r
 #pragma unroll
-    for (int r = 0; r < 4; ++r) dot += k[r] * w3[t][r];
+    for (int t = 0; t < 4; ++t) {
+      f32x4 x = {0, 0, 0, 0}, y = x;
+      if (t <= mr) {
+#pragma unroll
+        for (int kb = 0; kb < KP / 32; ++kb) {
+          bf16x8 col[NI], row[NI];
+          rows_of(L::kK, t, kb, col);
+          rows_of(second ? L::kQ : L::kK, mr, kb, row);
+          x = mm<NI>(col, row, x);
+          if constexpr (W == 4) {
+            rows_of(L::kQ, mr, kb, row);
+            y = mm<NI>(col, row, y);
+          }
+        }
+        x *= m1[t];
+        if constexpr (W == 4) x += m2[t] * y;
+        if (t == mr) {
+          x[1] += x[0], x[2] += x[1], x[3] += x[2];
+          float r0, r1, r2, r3, all, other;
+          swap16(x[3], x[3], r0, r1);
+          swap32(r0, r0, r0, r2);
+          swap32(r1, r1, r1, r3);
+          swap16(before, before, all, other);
+          all += other;
+          swap32(all, all, all, other);
+          all += other + ((g > 0 ? r0 : 0.0f) + (g > 1 ? r1 : 0.0f) + (g > 2 ? r2 : 0.0f));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = 4 * g + r < m ? all + x[r] : 0.0f;
+        } else {
+          before += (x[0] + x[1]) + (x[2] + x[3]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c[4 * t + r] = x[r];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // the sum over the rows m, half of the values to each half of the lanes at a time: value m is left
+    const auto halve = [&](auto o, auto ctrl) {
+#pragma unroll
+      for (int i = 0; i < decltype(o)::value; ++i) {
+        const bool hi = m & decltype(o)::value;
+        const float mine = hi ? c[i + decltype(o)::value] : c[i], other = hi ? c[i] : c[i + decltype(o)::value];
+        c[i] = mine + dpp<decltype(ctrl)::value>(other);
+      }
+    };
+    halve(int_c<8>{}, int_c<0x140>{});  // lanes mirrored in 16
+    halve(int_c<4>{}, int_c<0x141>{});  // mirrored in 8
+    halve(int_c<2>{}, int_c<0x4e>{});   // lane ^ 2
+    halve(int_c<1>{}, int_c<0xb1>{});   // lane ^ 1
+    vec[wave * 64 + 16 * (m >> 2) + 4 * g + (m & 3)] = c[0];
+    __builtin_amdgcn_wave_barrier();
+    // what goes through the chunk's first and last state, in this wave's 16 columns of K: a lane's token is `lane`
+    float in[4], out[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      asm volatile("" ::: "memory");  // (one tile's operands in registers at a time, and none kept for what follows)
+      const f32x4 k = at_acc(L::kK, 16 * t + m), q = at_acc(L::kQ, 16 * t + m);
+      const float be = gt[128 + 16 * t + m];
+      in[t] = out[t] = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) in[t] += q[r] * w2[t][r] - be * (k[r] * w1[t][r]), out[t] += k[r] * w3[t][r];
+    }
+    float from = sum_groups(in), before_it = sum_groups(out);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // (<S, dS'> is in every sum once: each lane's part is before a token or not)
+      const float dot = 4 * g + r == m ? gt[63] * ss[r] : 0.0f;
+      from += dot, before_it += dot;
+    }
+    const float col = vec[wave * 64 + lane], cols = sum_up_to(lane < 16 * mr ? col : 0.0f);
+    before_it = __shfl_up(sum_up_to(before_it) + (lane < 16 * mr ? cols : col), 1, 64);
+    vec[wave * 64 + lane] = sum_from(from, g) + (lane > 0 ? before_it : 0.0f);
+    asm volatile("" ::: "memory");
   }
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
@@ -1443,17 +1559,18 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
       }
     }
   }
-  // outputs, and the row sums q.dq and k.Z
+  // outputs, and the row sums k.Z
   const int64_t tok0 = static_cast<int64_t>(b) * a.T + t0;
+  float kz[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const int row = 16 * t + m;
     const float be = gt[128 + row];
-    const f32x4 dq = w2[t], z = w1[t], q = at_acc(L::kQ, row), k = at_acc(L::kK, row);
+    const f32x4 dq = w2[t], z = w1[t], k = at_acc(L::kK, row);
     f32x4 dk;
-    float qd = 0.0f, kz = 0.0f;
+    kz[t] = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) dk[r] = w3[t][r] - be * z[r], qd += q[r] * dq[r], kz += k[r] * z[r];
+    for (int r = 0; r < 4; ++r) dk[r] = w3[t][r] - be * z[r], kz[t] += k[r] * z[r];
     if (row < rows && d < a.K) {
       if (grp == 1) {
         st4(reinterpret_cast<E*>(a.dq) + ((tok0 + row) * a.Hk + hk) * a.K + d, dq);
@@ -1463,32 +1580,16 @@ __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) vo
         st4(a.dkp + ((tok0 + row) * a.H + h) * a.K + d, dk);
       }
     }
-#pragma unroll
-    for (int o = 16; o < 64; o <<= 1) qd += __shfl_xor(qd, o, 64), kz += __shfl_xor(kz, o, 64);
-    if (g == 0) vec[wave * 64 + row] = qd, vec[(W + wave) * 64 + row] = kz;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-  if (lane == 0) vec[(2 * W + 1) * 64 + wave] = dot, vec[(2 * W + 1) * 64 + W + wave] = state ? 1.0f : 0.0f;
+  vec[(W + wave) * 64 + lane] = sum_groups(kz);
   __syncthreads();
-  if (wave == 0) {
-    float qd = 0.0f, kz = 0.0f, all = 0.0f, begun = 0.0f;
+  if (wave == 0 && lane < rows) {
+    float kz = 0.0f, dg = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) qd += vec[w * 64 + lane], kz += vec[(W + w) * 64 + lane], all += vec[(2 * W + 1) * 64 + w], begun += vec[(2 * W + 1) * 64 + W + w];
-    const float y = vec[2 * W * 64 + lane], be = gt[128 + lane];
-    double s = static_cast<double>(qd) - static_cast<double>(be) * y;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double x = __shfl_down(s, o, 64);
-      if (lane + o < 64) s += x;
-    }
-    if (lane < rows) {
-      const int64_t tok = (tok0 + lane) * a.H + h;
-      // a decay that is zero in fp32 passes nothing on, and no state has none: exactly, not as a difference of sums
-      const bool none = gv < -104.0f || (lane == 0 && begun == 0.0f);
-      st(reinterpret_cast<E*>(a.dg) + tok, none ? 0.0f : static_cast<float>(s + all));
-      st(reinterpret_cast<E*>(a.db) + tok, y - kz);
-    }
+    for (int w = 0; w < W; ++w) dg += vec[w * 64 + lane], kz += vec[(W + w) * 64 + lane];
+    const int64_t tok = (tok0 + lane) * a.H + h;
+    st(reinterpret_cast<E*>(a.dg) + tok, dg);
+    st(reinterpret_cast<E*>(a.db) + tok, vec[2 * W * 64 + lane] - kz);
   }
 }
 

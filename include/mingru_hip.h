@@ -669,7 +669,9 @@ int mg_decode_head_f16(int B, int D, int V, const float* x_in, const void* pendi
  * H value heads share Hk query/key heads (H a multiple of Hk; head h reads
  * q, k of head h / (H / Hk), whose gradient is the sum over its value heads).
  * g is the logarithm of the decay; below -200 it counts as -200 (e^g is 0 in
- * fp32 from -104 on, where dg is 0): -inf forgets the state.
+ * fp32 from -104 on): -inf forgets the state. dg_t is summed from what crosses
+ * token t alone, terms as small as e^{g_t}: it keeps its relative accuracy
+ * where the decay is strong.
  *
  * mg_rows: element (b, t, h, d) of an operand at p + b sb + t st + h sh + d
  * (elements; d contiguous; g and beta have no d). q, k and dout: p and the
