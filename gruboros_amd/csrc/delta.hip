@@ -35,11 +35,13 @@
 //   step_kernel   single tokens.
 // Times below are for K = V = 128 in bf16: B8 T2047 H8, forward and backward, and B2 T16381 H16, forward.
 //
-// Matrix operands are bf16. An fp32 value enters as limbs, x = h + m + l with 8
-// bits each (exact), and the limb products down to 2^-16 of the leading one are
-// summed in fp32: states, T, y and d are never rounded to bf16. bf16 inputs are
-// one limb, so a product with one costs three instructions at most; fp32 inputs
-// are three, and a product six.
+// Matrix operands are bf16. An fp32 value enters as limbs, x = h + m + l (exact,
+// |m| <= 2^-9 |x|, |l| <= 2^-18 |x|), and the limb products down to 2^-18 of the
+// leading one are summed in fp32 (what is left out: 2^-26). States, T, y and d are
+// never rounded to bf16 in the passes; o and the gradients that bf16 inputs take
+// in their own type are made from two limbs (2^-18). bf16 inputs are one limb, so
+// a product with one costs three instructions at most; fp32 inputs are three, and
+// a product six.
 
 #include <algorithm>
 
@@ -89,20 +91,18 @@ struct Args {
 
 __device__ __forceinline__ uint32_t hi16x2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// 8 fp32 values as N limbs. N = 3: by cutting the mantissa (8 + 8 + 8 bits, exact). N = 2: both rounded to
-// nearest, off by 2^-18 at most.
-__device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[3]) {
-  w[0] = hi16x2(__float_as_uint(a), __float_as_uint(b));
-  a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-  b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-  w[1] = hi16x2(__float_as_uint(a), __float_as_uint(b));
-  a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-  b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-  w[2] = hi16x2(__float_as_uint(a), __float_as_uint(b));
-}
+// Two fp32 values as limbs, each the rest rounded to nearest: off by 2^-9 after one, 2^-18 after two, and nothing is
+// left after three. (Where three are made and two are used, as of a state, these are rounded too: cut limbs would be
+// off by up to 2^-15, always towards zero.)
 __device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[2]) {
   w[0] = pack_bf16x2(a, b);
   w[1] = pack_bf16x2(a - __uint_as_float(w[0] << 16), b - __uint_as_float(w[0] & 0xffff0000u));
+}
+__device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[3]) {
+  w[0] = pack_bf16x2(a, b);
+  a -= __uint_as_float(w[0] << 16), b -= __uint_as_float(w[0] & 0xffff0000u);
+  w[1] = pack_bf16x2(a, b);
+  w[2] = hi16x2(__float_as_uint(a - __uint_as_float(w[1] << 16)), __float_as_uint(b - __uint_as_float(w[1] & 0xffff0000u)));
 }
 __device__ __forceinline__ void pair_limbs(float a, float b, uint32_t (&w)[1]) { w[0] = hi16x2(__float_as_uint(a), __float_as_uint(b)); }
 template <int N>
@@ -119,7 +119,7 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[N]) {
   for (int l = 0; l < N; ++l) out[l] = __builtin_bit_cast(bf16x8, w[l]);
 }
 
-// Limbs of what is kept for the backward's products: two of a state or update of bf16 inputs (2^-16,
+// Limbs of what is kept for the backward's products: two of a state or update of bf16 inputs (2^-18,
 // far below the rounding of the gradients they end in), all three of fp32 inputs.
 template <int NI>
 constexpr int kKept = NI == 3 ? 3 : 2;
