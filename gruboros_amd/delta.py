@@ -11,6 +11,7 @@ gradients; ``gated_delta_step`` one token of generation on a state that it updat
 Both take float32 or bfloat16 and keep the state in fp32.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import dtype_code, native, require_cuda, stream_of
@@ -52,7 +53,8 @@ class GatedDeltaRule(torch.autograd.Function):
 
 
 def _check(q, k, v, g, beta, state, name, lead):
-    """Shapes, types and devices; lead: the dimensions before the heads."""
+    """Shapes, types and devices; lead: the dimensions before the heads. Tangents, which the kernels do
+    not carry, are refused: an operand that has one need not require gradients."""
     require_cuda(q, k, v, g, beta, state)
     dtype_code(q.dtype)
     if q.dim() != lead + 2 or k.shape != q.shape:
@@ -75,6 +77,9 @@ def _check(q, k, v, g, beta, state, name, lead):
             raise ValueError(f"operands on {q.device} and {t.device}")
     if state is not None and (state.shape != (v.shape[0], H, K, V) or state.dtype != torch.float32):
         raise ValueError(f"{name} must be float32 [{v.shape[0]}, {H}, {K}, {V}], got {state.dtype} {tuple(state.shape)}")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (q, k, v, g, beta, state)):
+        raise NotImplementedError("the gated delta rule has no forward-mode derivative")
 
 
 def gated_delta_rule(q, k, v, g, beta, initial_state=None, scale=None, return_state=False):
@@ -86,9 +91,9 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, scale=None, return_st
     [B, H, K, V] or None (zeros). scale: K ** -0.5 by default. g = -inf forgets the state.
 
     Returns o [B, T, H, V] in the inputs' dtype, or (o, last state float32 [B, H, K, V]) with
-    return_state. Gradients reach all six tensors (not twice: no double backward). Where gradients
-    are recorded, each 64 tokens of a head keep their state, updates and operands for the backward:
-    4 K V + 256 V + 134700 bytes for K > 64, 101900 in place of the last for K <= 64 (float32:
+    return_state. Gradients reach all six tensors, once and in reverse mode (no double backward, and
+    dual tensors are refused). Where gradients are recorded, each 64 tokens of a head keep their
+    state, updates and operands for the backward: 4 K V + 256 V + 134700 bytes for K > 64, 101900 in place of the last for K <= 64 (float32:
     6 K V + 384 V + 271900 or 173600), with K rounded up to 64 or 128 and V to a multiple of 32.
 
     A value that is not finite spoils the 64 tokens of its chunk, earlier ones included: padding
@@ -116,8 +121,10 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None):
     [B, H] as in gated_delta_rule, state float32 [B, H, K, V], contiguous, which is updated in
     place. Returns o [B, H, V]. No gradients are recorded: operands that require them are refused
     where they would be."""
-    if q.is_cuda and (o := native().delta_step_plain(q, k, v, g, beta, state, scale, stream_of(q))) is not None:
-        return o
+    if q.is_cuda and forward_ad._current_level < 0:  # (one call for the operands that generation has)
+        o = native().delta_step_plain(q, k, v, g, beta, state, scale, stream_of(q))
+        if o is not None:
+            return o
     _check(q, k, v, g, beta, state, "state", 1)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
         raise ValueError("gated_delta_step records no gradients: call it under torch.no_grad(), or use gated_delta_rule")
