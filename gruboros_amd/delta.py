@@ -14,7 +14,7 @@ import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
-from ._lib import dtype_code, native, require_cuda, stream_of
+from ._lib import dtype_code, native, no_values, require_cuda, stream_of
 
 
 def _operand(t, heads_dim=True):
@@ -93,19 +93,21 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, scale=None, return_st
     Returns o [B, T, H, V] in the inputs' dtype, or (o, last state float32 [B, H, K, V]) with
     return_state. Gradients reach all six tensors, once and in reverse mode (no double backward, and
     dual tensors are refused). Where gradients are recorded, each 64 tokens of a head keep their
-    state, updates and operands for the backward: 4 K V + 256 V + 134700 bytes for K > 64, 101900 in place of the last for K <= 64 (float32:
-    6 K V + 384 V + 271900 or 173600), with K rounded up to 64 or 128 and V to a multiple of 32.
+    state, updates and operands for the backward: 4 K V + 256 V + 134700 bytes for K > 64, 101900 in
+    place of the last for K <= 64 (float32: 6 K V + 384 V + 271900 or 173600), with K rounded up to
+    64 or 128 and V to a multiple of 32.
 
     A value that is not finite spoils the 64 tokens of its chunk, earlier ones included: padding
     behind a sequence must be finite."""
     _check(q, k, v, g, beta, initial_state, "initial_state", 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if q.shape[0] == 0 or q.shape[1] == 0:  # no token: nothing is written
-        o = v.new_zeros(v.shape)
+        o = no_values(v.new_zeros(v.shape), q, k, v, g, beta, initial_state)
         if not return_state:
             return o
         size = (v.shape[0], v.shape[2], q.shape[3], v.shape[3])
-        return o, (torch.zeros(size, device=v.device) if initial_state is None else initial_state.clone())
+        state = torch.zeros(size, device=v.device) if initial_state is None else initial_state.clone()
+        return o, (state if q.shape[0] else no_values(state, q, k, v, g, beta))
     q, k, v = _operand(q), _operand(k), _operand(v)
     g, beta = _operand(g, False), _operand(beta, False)
     h0 = None if initial_state is None else initial_state.contiguous()

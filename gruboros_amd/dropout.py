@@ -5,7 +5,7 @@ generator state: a step that is run again, on whatever stream, drops the same va
 """
 import torch
 
-from ._lib import dtype_code, native, require_cuda, stream_of
+from ._lib import dtype_code, native, no_values, require_cuda, stream_of
 
 
 def check_drop(p, seed, offset, device):
@@ -49,5 +49,5 @@ def dropout(x, p, seed, offset=0, residual=None):
                                  or residual.device != x.device):
         raise ValueError(f"residual {residual.dtype} {tuple(residual.shape)} must match x {tuple(x.shape)}, in float32 or {x.dtype}")
     if x.numel() == 0:
-        return x.clone() if residual is None else residual.clone()
+        return x.clone() if residual is None else no_values(residual.clone(), x)
     return native().dropout_add(_dense(x), None if residual is None else _dense(residual), p, seed, seed_t, offset, stream_of(x))

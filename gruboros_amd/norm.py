@@ -16,7 +16,7 @@ them as fp32.
 """
 import torch
 
-from ._lib import MG_BF16, dtype_code, native, require_cuda, stream_of
+from ._lib import MG_BF16, dtype_code, native, no_values, require_cuda, stream_of
 from .dropout import check_drop
 
 FP32_EPS = float(torch.finfo(torch.float32).eps)
@@ -168,7 +168,7 @@ def layer_norm(x, w, b=None, out_dtype=None, eps=1e-5):
     out_dtype = out_dtype or x.dtype
     w, b = _check_layer_norm(x, w, b, None, out_dtype)
     if x.numel() == 0:
-        return torch.empty_like(x, dtype=out_dtype)
+        return no_values(torch.empty_like(x, dtype=out_dtype), x, w, b)
     return native().layer_norm(x.contiguous(), None, w, b, out_dtype == torch.bfloat16, eps, 0.0, 0, None, 0, stream_of(x))[1]
 
 
@@ -181,5 +181,5 @@ def add_layer_norm(x, delta, w, b=None, out_dtype=None, eps=1e-5, dropout_p=0.0,
     w, b = _check_layer_norm(x, w, b, delta, out_dtype)
     drop = check_drop(dropout_p, 0 if seed is None and dropout_p == 0 else seed, offset, x.device)
     if x.numel() == 0:
-        return x + delta.float(), torch.empty_like(x, dtype=out_dtype)
+        return x + delta.float(), no_values(torch.empty_like(x, dtype=out_dtype), x, delta, w, b)
     return native().layer_norm(x.contiguous(), delta.contiguous(), w, b, out_dtype == torch.bfloat16, eps, *drop, stream_of(x))
