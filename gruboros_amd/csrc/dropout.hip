@@ -17,12 +17,15 @@ constexpr int kThreads = 256;
 template <typename Tin, typename Tout>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(const Tin* __restrict__ x, const Tout* __restrict__ residual,
                                                            Tout* __restrict__ y, int64_t n, Drop d) {
-  const uint64_t key = d.key();
+  const bool drop = d.threshold;  // (none are dropped else: nothing is drawn)
+  const uint64_t key = drop ? d.key() : 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; 8 * i < n; i += step) {
-    uint32_t w[2][4];
-    philox(2 * i, d.offset, key, w[0]);
-    philox(2 * i + 1, d.offset, key, w[1]);
+    uint32_t w[2][4] = {};
+    if (drop) {
+      philox(2 * i, d.offset, key, w[0]);
+      philox(2 * i + 1, d.offset, key, w[1]);
+    }
     if (8 * i + 8 <= n) {
       fv<8> v = iov<Tin, 8>::load(x + 8 * i);
       fv<8> r = residual ? iov<Tout, 8>::load(residual + 8 * i) : iov<Tout, 8>::fill(0.0f);
