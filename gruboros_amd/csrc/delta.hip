@@ -1747,8 +1747,17 @@ inline int check_dims(const char* fn, int dtype, const mg_delta_dims* s) {
     return fail(MG_ERR_ARG, "%s: needs B, T, H, Hk >= 1 and H a multiple of Hk", fn);
   if (s->K < 8 || s->K % 8 || s->K > 128 || s->V < 8 || s->V % 8 || s->V > 256)
     return fail(MG_ERR_ARG, "%s: K=%d and V=%d must be multiples of 8, K <= 128, V <= 256", fn, s->K, s->V);
-  if (static_cast<int64_t>(s->B) * s->H * chunks(*s) >= (int64_t(1) << 31))
-    return fail(MG_ERR_ARG, "%s: B * H * ceil(T / 64) must be below 2^31", fn);
+  return MG_OK;
+}
+
+// A launch has less than 2^32 threads: a workgroup of up to 512 for every chunk, of 512 for every 16 value columns
+// of a head (a pass over the chunks), or of 256 for every 32 (a step).
+inline int check_launches(const char* fn, const mg_delta_dims* s, bool step) {
+  const int64_t bh = static_cast<int64_t>(s->B) * s->H, tiles = (s->V + 31) / 32;
+  const auto below = [&](int bits, int64_t each) { return bh <= ((int64_t(1) << bits) - 1) / each; };
+  if (step) return below(24, tiles) ? MG_OK : fail(MG_ERR_ARG, "%s: B * H * ceil(V / 32) must be below 2^24", fn);
+  if (!below(23, chunks(*s)) || !below(22, tiles))
+    return fail(MG_ERR_ARG, "%s: B * H * ceil(T / 64) must be below 2^23, B * H * ceil(V / 32) below 2^22", fn);
   return MG_OK;
 }
 
@@ -1869,12 +1878,14 @@ int launch_step(const mg_delta_dims& s, const void* q, const void* k, const void
 using namespace mg;
 
 extern "C" size_t mg_delta_fwd_workspace_bytes(int dtype, const mg_delta_dims* dims, int keep) {
-  if (delta::check_dims("mg_delta_fwd_workspace_bytes", dtype, dims)) return 0;
+  const char* fn = "mg_delta_fwd_workspace_bytes";
+  if (delta::check_dims(fn, dtype, dims) || delta::check_launches(fn, dims, false)) return 0;
   return delta::layout(dtype, *dims, keep != 0).end;
 }
 
 extern "C" size_t mg_delta_bwd_workspace_bytes(int dtype, const mg_delta_dims* dims) {
-  if (delta::check_dims("mg_delta_bwd_workspace_bytes", dtype, dims)) return 0;
+  const char* fn = "mg_delta_bwd_workspace_bytes";
+  if (delta::check_dims(fn, dtype, dims) || delta::check_launches(fn, dims, false)) return 0;
   return delta::bwd_layout(dtype, *dims).end;
 }
 
@@ -1883,7 +1894,9 @@ extern "C" int mg_delta_fwd(int dtype, const mg_delta_dims* dims, const mg_rows*
                             int keep, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "mg_delta_fwd";
   int rc;
-  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_out(fn, dtype, dims))) return rc;
+  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_launches(fn, dims, false)) ||
+      (rc = delta::check_out(fn, dtype, dims)))
+    return rc;
   if ((rc = delta::check_rows(fn, "q", dtype, q, true)) || (rc = delta::check_rows(fn, "k", dtype, k, true)) ||
       (rc = delta::check_rows(fn, "v", dtype, v, false)) || (rc = delta::check_rows(fn, "g", dtype, g, false)) ||
       (rc = delta::check_rows(fn, "beta", dtype, beta, false)))
@@ -1908,7 +1921,9 @@ extern "C" int mg_delta_bwd(int dtype, const mg_delta_dims* dims, const mg_rows*
                             float* dh0, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "mg_delta_bwd";
   int rc;
-  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_out(fn, dtype, dims))) return rc;
+  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_launches(fn, dims, false)) ||
+      (rc = delta::check_out(fn, dtype, dims)))
+    return rc;
   if ((rc = delta::check_rows(fn, "q", dtype, q, true)) || (rc = delta::check_rows(fn, "k", dtype, k, true)) ||
       (rc = delta::check_rows(fn, "v", dtype, v, false)) || (rc = delta::check_rows(fn, "g", dtype, g, false)) ||
       (rc = delta::check_rows(fn, "beta", dtype, beta, false)) || (rc = delta::check_rows(fn, "dout", dtype, dout, true)))
@@ -1942,7 +1957,7 @@ extern "C" int mg_delta_step(int dtype, const mg_delta_dims* dims, const void* q
                              const void* beta, float scale, float* state, void* o, void* stream) {
   const char* fn = "mg_delta_step";
   int rc;
-  if ((rc = delta::check_dims(fn, dtype, dims))) return rc;
+  if ((rc = delta::check_dims(fn, dtype, dims)) || (rc = delta::check_launches(fn, dims, true))) return rc;
   if (dims->T != 1) return fail(MG_ERR_ARG, "%s: T must be 1", fn);
   const size_t e = dtype == MG_F32 ? 4 : 2;
   if (!q || !k || !g || !beta || !aligned(q, e) || !aligned(k, e) || !aligned(g, e) || !aligned(beta, e))

@@ -678,7 +678,8 @@ int mg_decode_head_f16(int B, int D, int V, const float* x_in, const void* pendi
  * strides multiples of 16 bytes. o, dv: dense [B, T, H, V]; dq, dk: dense
  * [B, T, Hk, K]; o, dq and dk 16-byte aligned; dg, dbeta: dense [B, T, H].
  * K and V multiples of 8, K <= 128, V <= 256; T >= 1;
- * B H ceil(T / 64) < 2^31; 64 token strides (o's too) below 2 GiB.
+ * B H ceil(T / 64) < 2^23 and B H ceil(V / 32) < 2^22 (2^24 for a step);
+ * 64 token strides (o's too) below 2 GiB.
  * A value that is not finite spoils the 64 tokens of its chunk, earlier ones
  * included: padding behind a sequence must be finite (g = -inf apart).
  *
