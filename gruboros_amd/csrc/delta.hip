@@ -1780,11 +1780,13 @@ inline int check_out(const char* fn, int dtype, const mg_delta_dims* s) {
   return MG_OK;
 }
 
-// Value columns per workgroup of the passes over the chunks, in tiles of 16: two where that still leaves a workgroup
-// for every CU, so that a chunk's operands are loaded for twice the columns (B8 T2047 H8: 131 and 130 us against
-// 170 and 170 with one), else one, for more workgroups. fp32 loads three limbs for one and is kept at one.
+// Value columns per workgroup of the passes over the chunks, in tiles of 16: one as long as every tile has a CU of its
+// own, for more of them, else two, so that a chunk's operands are loaded for twice the columns. T 2048, K = V = 128,
+// forward (the backward alike), one against two: 256 tiles 107 and 125 us, 264 133 and 125, 320 159 and 140, 512 245
+// and 201, 2048 878 and 716; T 16384, 264 tiles, 1192 and 1098; K = V = 64, 256 tiles 109 and 122, 264 136 and 131.
+// fp32 loads three limbs for one and is kept at one.
 inline int columns_for(int64_t bh, int vp, int dtype_limbs) {
-  return dtype_limbs == 1 && bh * (vp / 32) >= kCUs ? 2 : 1;
+  return dtype_limbs == 1 && bh * (vp / 16) > kCUs ? 2 : 1;
 }
 
 inline void fill(Args& a, const mg_delta_dims& s, float scale, const mg_rows* q, const mg_rows* k, const mg_rows* v,
@@ -1856,8 +1858,9 @@ void launch_step(const mg_delta_dims& s, const E* q, const E* k, const E* v, con
 }
 
 // A call's states from 64 MiB on are taken to be out of the 256 MiB cache by the next token: a model steps
-// several layers' in between. Then it is no use to send them through it (128 MiB, states of six layers in turn:
-// 57 us through the caches, 52 past them; one layer's over and over: 44 and 50).
+// several layers' in between. Then it is no use to send them through it. Through the caches and past them, one layer
+// over and over, and 16 in turn: 32 MiB 10.1 and 12.7 us, 15.3 and 12.5; 64 MiB 22.6 and 22.5, 30.6 and 25.1; 128 MiB
+// 43 and 48, 54 and 50; 256 MiB 87 and 96, 107 and 97.
 template <typename E>
 int launch_step(const mg_delta_dims& s, const void* q, const void* k, const void* v, const void* g, const void* beta, float scale,
                 float* state, void* o, hipStream_t st_) {
