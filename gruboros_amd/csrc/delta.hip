@@ -397,8 +397,8 @@ __device__ __forceinline__ void put_blocks(const float* m, char* low, char* high
 
 // k and q are read once, all loads of a thread under way at a time, and go to LDS and from there, as fragments, to the
 // image; A and T take over the LDS once k k^T and q k^T are in registers, P A's once T is done: 36 KB, four workgroups
-// to a CU. Bound by memory, by what the image takes: 68 us for 340 MB (131 KB a chunk with what the backward
-// reads), 182 us for 930 MB (79 KB a chunk): 5.0 and 5.1 TB/s. (Reading k and q where they were needed, one
+// to a CU. Bound by memory, by what the image takes: 69 us for 340 MB (131 KB a chunk with what the backward
+// reads), 184 us for 930 MB (79 KB a chunk): 5.0 and 5.1 TB/s. (Reading k and q where they were needed, one
 // load after the other: 84 us for a smaller image, at 2.6 TB/s.)
 template <int KP, int NI>
 __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a, bool keep) {
@@ -607,9 +607,9 @@ __global__ __launch_bounds__(256, NI == 1 ? 4 : 1) void chunk_kernel(Args a, boo
 // not wait for, between the same barriers: o = scale e^G Q S + P d and what is kept; in the backward P^T do and
 // Q^T (scale e^G do), a chunk ahead.
 //
-// Bound by the chain: 490 us for 256 chunks are 1.9 us a chunk, of which 1.3 pass with no loads at all (dependent
+// Bound by the chain: 521 us for 256 chunks are 2.0 us a chunk, of which 1.3 pass with no loads at all (dependent
 // products, limbs, three exchanges) and the rest are loads that come late when all CUs draw on the L2s (each of a head's
-// workgroups loads all of its image). B8 T2047 H8: state 134, its gradient 134 us, 3.2 TB/s for the 430 MB each that
+// workgroups loads all of its image). B8 T2047 H8: state 135, its gradient 144 us, 3.1 TB/s for the 430 MB each that
 // cross memory. Tried before, B2 T16381 H16: a wave of its own for each 16 columns with no exchange, 1053 us; the
 // operands through LDS by asynchronous copies, 553; no separate waves for o, 504. Asking for the image two chunks
 // ahead so that the loads find it in L2 changed nothing.
@@ -1280,8 +1280,8 @@ struct GradTile {
 __device__ __forceinline__ int at4(int r, int u) { return (r * 4 + (u ^ ((r >> 2) & 3))) * 16; }
 
 // A wave has 16 columns of K. The kept operands come through LDS, 32 value columns at a time; two workgroups to a CU (bf16:
-// 128 registers, 78 KB), one of which works while the other waits for its operands. Bound by memory: 149 us for 600 MB,
-// 4.0 TB/s. (One workgroup to a CU, do read by every wave that needed it, and a lane per column, whose sums
+// 128 registers, 78 KB), one of which works while the other waits for its operands. Bound by memory: 161 us for 600 MB,
+// 3.7 TB/s, 7 of them for the terms of dg (with the sums over lanes through LDS, 17). (One workgroup to a CU, do read by every wave that needed it, and a lane per column, whose sums
 // over K crossed lanes and whose stores were of two bytes: 278 us.)
 template <int KP, int NI>
 __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) void grad_kernel(Args a) {
@@ -1612,8 +1612,8 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(const float* dqp, const 
 // ---------------------------------------------------------------- single tokens
 //
 // One workgroup per (batch, head, 32 value columns): thread (r, c) holds rows r, r + 32, ... and columns
-// 4 c ... 4 c + 3 of the state, read and written once: bound by memory, B128 H16 52 us for 270 MB, 5.2 TB/s. k S and q S are taken together from the old
-// state: o = scale (e^g q S + (q.k) d), d = beta (v - e^g k S). ONCE: past the caches, see launch_step.
+// 4 c ... 4 c + 3 of the state, read and written once: bound by memory, B128 H16 49 us for 270 MB, 5.5 TB/s. k S and
+// q S are taken together from the old state: o = scale (e^g q S + (q.k) d), d = beta (v - e^g k S). ONCE: past the caches, see launch_step.
 template <bool ONCE>
 __device__ __forceinline__ f4 load_state4(const float* p) {
   f4 r;
