@@ -98,6 +98,9 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, scale=None, return_st
     64 or 128 and V to a multiple of 32. Without, a call takes 81408 or 56832 bytes (float32: 185856 or
     112128) for as long as it runs.
 
+    The 64 tokens of a chunk are solved as a triangular system, whose condition grows with beta |k|^2
+    where keys are alike: all keys the same, float32 is off by 1e-6 at 1, by 2e-4 at 2.
+
     A value that is not finite spoils the 64 tokens of its chunk, earlier ones included: padding
     behind a sequence must be finite."""
     _check(q, k, v, g, beta, initial_state, "initial_state", 2)

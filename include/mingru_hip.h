@@ -680,6 +680,7 @@ int mg_decode_head_f16(int B, int D, int V, const float* x_in, const void* pendi
  * K and V multiples of 8, K <= 128, V <= 256; T >= 1;
  * B H ceil(T / 64) < 2^23 and B H ceil(V / 32) < 2^22 (2^24 for a step);
  * 64 token strides (o's too) below 2 GiB.
+ * States are finite below 2^128 - 2^119 (the largest bf16 and half a step).
  * A value that is not finite spoils the 64 tokens of its chunk, earlier ones
  * included: padding behind a sequence must be finite (g = -inf apart).
  *

@@ -4,7 +4,8 @@ at most and to either side. Cut limbs would be off by half of 2^-15 on average, 
 A chunk that writes nothing (beta = 0, g = 0) gives o = scale q S and dq = scale do S^T of its entry
 state alone. Along the exact result the error is its bias: of N values rounded to bf16 the rounding,
 to either side and of 2^-8 / sqrt(3) at most, leaves 2^-8 / sqrt(N) (normal values: sum x^4 = 3 N,
-sum x^2 = N), 1.9e-6 for N = 2^22. The limit 2^-17 = 7.6e-6 is four times that; limbs cut at 2^-15 lie
+sum x^2 = N), 1.9e-6 for N = 2^22, and the slope of the values' density within a binade
+2^-18 = 3.8e-6 at most. The limit 2^-17 = 7.6e-6 is more than both; limbs cut at 2^-15 lie
 0.69 2^-16 = 1.05e-5 off (the mean of the cut part over mantissas from 1 to 2)."""
 import pytest
 import torch
