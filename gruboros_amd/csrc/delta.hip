@@ -167,7 +167,8 @@ __device__ __forceinline__ void st4(bf16_t* p, const f32x4& x) {
 // row in its offset. Rows and columns past the end are out of that buffer's range (which is empty if the chunk ends
 // before r): they read as zero and are not written. (A scalar offset for r would be left out of the range check; a
 // check of every row by its lane took 40 registers more.) Rows that are closer than their length, a broadcast's, may
-// read a row that is there in place of one that is not: finite, and multiplied by the zeros of T, P and q beyond the end.
+// read a row that is there in place of one that is not: beta, P and q are zero there, and what they multiply is an
+// operand's own value.
 constexpr uint32_t kOutOfRange = 0x80000000u;
 template <typename E>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const E* p, int64_t st_, int rows, int cols, int r = 0) {
@@ -1281,8 +1282,9 @@ __device__ __forceinline__ int at4(int r, int u) { return (r * 4 + (u ^ ((r >> 2
 
 // A wave has 16 columns of K. The kept operands come through LDS, 32 value columns at a time; two workgroups to a CU (bf16:
 // 128 registers, 78 KB), one of which works while the other waits for its operands. Bound by memory: 161 us for 600 MB,
-// 3.7 TB/s, 7 of them for the terms of dg (with the sums over lanes through LDS, 17). (One workgroup to a CU, do read by every wave that needed it, and a lane per column, whose sums
-// over K crossed lanes and whose stores were of two bytes: 278 us.)
+// 3.7 TB/s, 7 of them for the terms of dg (with the sums over lanes through LDS, 17). (One workgroup to a CU, do read
+// by every wave that needed it, and a lane per column, whose sums over K crossed lanes and whose stores were of two
+// bytes: 278 us.)
 template <int KP, int NI>
 __global__ __launch_bounds__(64 * (KP / 16), NI == 3 ? 1 : KP == 128 ? 4 : 3) void grad_kernel(Args a) {
   using E = typename elem<NI>::type;
