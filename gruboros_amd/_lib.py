@@ -113,6 +113,14 @@ SIGNATURES = {
                                   ctypes.c_double, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp, _c_size, _vp]),
     "mg_dropout": (_c_int, [_c_int, _vp, _c_int, _vp, _vp, _c_i64, ctypes.c_double, ctypes.c_uint64, _vp,
                             ctypes.c_uint64, _vp]),
+    "mg_recurrence_keep_elems": (_c_i64, [_c_int] * 3),
+    "mg_recurrence_fwd_workspace_bytes": (_c_size, [_c_int] * 3),
+    "mg_recurrence_bwd_workspace_bytes": (_c_size, [_c_int] * 3),
+    "mg_recurrence_fwd": (_c_int, [_c_int] + [_vp] * 3 + [_fp, ctypes.c_float, _fp, _vp, _vp, _fp, _fp] + [_c_int] * 3
+                          + [_vp, _c_size, _vp]),
+    "mg_recurrence_bwd": (_c_int, [_c_int] + [_vp] * 3 + [_fp, ctypes.c_float, _fp, _vp, _fp, _vp, _fp, _vp, _vp, _vp, _fp, _fp]
+                          + [_c_int] * 3 + [_vp, _c_size, _vp]),
+    "mg_recurrence_step": (_c_int, [_c_int] + [_vp, _c_i64] * 3 + [_fp, ctypes.c_float, _fp, _vp, _c_int, _c_int, _vp]),
     "mg_gemm_wgrad_pair_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
 }
 

@@ -1030,6 +1030,130 @@ Tensor dropout_add(const Tensor& x, const Opt& residual, double p, uint64_t seed
   return DropoutFn::apply(x, residual, p, static_cast<int64_t>(seed), seed_t, static_cast<int64_t>(offset), stream);
 }
 
+// ------------------------------------------------------------------ gated linear recurrence
+
+// a [B, T, D] operand as the kernels read it: unit inner stride, steps at 32-bit distances
+Tensor steps(const Tensor& t) {
+  const bool unit = t.size(2) == 1 || t.stride(2) == 1, near = t.size(1) == 1 || t.stride(1) < (int64_t(1) << 28);
+  return unit && near ? t : t.contiguous();
+}
+mg_seq seq(const Tensor& t) {
+  const auto s = [&](int i) { return t.size(i) == 1 ? int64_t(0) : t.stride(i); };
+  return {ptr(t), s(0), s(1)};
+}
+struct RecurrenceDims {
+  int B, T, D;
+};
+RecurrenceDims recurrence_dims(const Tensor& x, const Tensor& gi, const Tensor& gr, const Tensor& decay, const Opt& h0, const Opt& reset) {
+  need_cuda(x);
+  if (x.dim() != 3) fail("x: expected [B, T, D]");
+  alike(x, {&gi, &gr});
+  shape(gi, x.sizes(), "input_gate");
+  shape(gr, x.sizes(), "decay_gate");
+  for (int64_t n : x.sizes())
+    if (n < 1 || n > INT32_MAX) fail("x: a dimension is empty or too large");
+  const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
+  const auto here = [&](const Tensor& t, const char* name) {
+    if (!t.is_contiguous() || t.device() != x.device()) fail(std::string(name) + ": expected a contiguous tensor on " + x.device().str());
+  };
+  shape(decay, {D}, "decay");
+  here(decay, "decay");
+  if (h0) shape(*h0, {B, D}, "initial state"), here(*h0, "initial state");
+  if (reset) {
+    shape(*reset, {B, T}, "reset"), here(*reset, "reset");
+    if (reset->scalar_type() != at::kByte && reset->scalar_type() != at::kBool) fail("reset: expected bool or uint8");
+  }
+  return {static_cast<int>(B), static_cast<int>(T), static_cast<int>(D)};
+}
+
+struct RecurrenceFn : ag::Function<RecurrenceFn> {
+  static ag::variable_list forward(ag::AutogradContext* ctx, const Tensor& x_, const Tensor& gi_, const Tensor& gr_, const Tensor& decay,
+                                   const Opt& h0, const Opt& reset, double c, bool want_state, bool record, int64_t stream) {
+    const auto [B, T, D] = recurrence_dims(x_, gi_, gr_, decay, h0, reset);
+    c10::DeviceGuard guard(x_.device());
+    const Tensor x = steps(x_), gi = steps(gi_), gr = steps(gr_);
+    const mg_seq sx = seq(x), si = seq(gi), sr = seq(gr);
+    Tensor h = make(x.sizes(), x.scalar_type(), x), keep;
+    Opt last;
+    if (want_state) last = make({B, D}, at::kFloat, x);
+    if (record) keep = make({std::max<int64_t>(mg_recurrence_keep_elems(B, T, D), 1)}, at::kFloat, x);
+    const size_t wsb = mg_recurrence_fwd_workspace_bytes(B, T, D);
+    Tensor ws;
+    if (wsb) ws = bytes(wsb, x);
+    check(mg_recurrence_fwd(code(x), &sx, &si, &sr, fp(decay), c, fp(h0), static_cast<const uint8_t*>(ptr(reset)), ptr(h), fp(last),
+                            record ? fp(keep) : nullptr, B, T, D, wsb ? ptr(ws) : nullptr, wsb, st(stream)),
+          "mg_recurrence_fwd");
+    ctx->set_materialize_grads(false);
+    if (record) ctx->save_for_backward({x, gi, gr, decay, plain(h0), plain(reset), keep});
+    auto& d = ctx->saved_data;
+    d["c"] = c, d["stream"] = stream, d["h0"] = h0.has_value();
+    if (!last) return {h};
+    return {h, *last};
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    ag::variable_list out(10);
+    grads.resize(2);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &gi = saved[1], &gr = saved[2], &decay = saved[3], &keep = saved[6];
+    const Opt h0 = opt(saved[4]), reset = opt(saved[5]);
+    auto& d = ctx->saved_data;
+    const auto [B, T, D] = recurrence_dims(x, gi, gr, decay, h0, reset);
+    c10::DeviceGuard guard(x.device());
+    const Tensor dh = grads[0].defined() ? steps(grads[0].to(x.scalar_type())) : at::zeros_like(x, at::MemoryFormat::Contiguous);
+    shape(dh, x.sizes(), "dh");
+    Opt dlast;
+    if (grads[1].defined()) dlast = grads[1].to(at::kFloat).contiguous();
+    const mg_seq sx = seq(x), si = seq(gi), sr = seq(gr), sd = seq(dh);
+    Tensor dx = make(x.sizes(), x.scalar_type(), x), di = make(x.sizes(), x.scalar_type(), x), dr = make(x.sizes(), x.scalar_type(), x);
+    Opt dd, dh0;
+    if (ctx->needs_input_grad(3)) dd = make({D}, at::kFloat, x);
+    if (h0 && ctx->needs_input_grad(4)) dh0 = make({B, D}, at::kFloat, x);
+    const size_t wsb = mg_recurrence_bwd_workspace_bytes(B, T, D);
+    Tensor ws = bytes(wsb, x);
+    check(mg_recurrence_bwd(code(x), &sx, &si, &sr, fp(decay), d["c"].toDouble(), fp(h0), static_cast<const uint8_t*>(ptr(reset)), fp(keep),
+                            &sd, fp(dlast), ptr(dx), ptr(di), ptr(dr), fp(dd), fp(dh0), B, T, D, ptr(ws), wsb, st(d["stream"].toInt())),
+          "mg_recurrence_bwd");
+    if (ctx->needs_input_grad(0)) out[0] = dx;
+    if (ctx->needs_input_grad(1)) out[1] = di;
+    if (ctx->needs_input_grad(2)) out[2] = dr;
+    out[3] = plain(dd), out[4] = plain(dh0);
+    return once(out);
+  }
+};
+
+// (h, last state or none), with gradients
+std::tuple<Tensor, Opt> recurrence(const Tensor& x, const Tensor& gi, const Tensor& gr, const Tensor& decay, const Opt& h0,
+                                   const Opt& reset, double c, bool want_state, int64_t stream) {
+  bool record = false;
+  for (const Tensor* t : {&x, &gi, &gr, &decay}) record |= t->requires_grad();
+  record = (record || (h0 && h0->requires_grad())) && at::GradMode::is_enabled();
+  const auto out = RecurrenceFn::apply(x, gi, gr, decay, h0, reset, c, want_state, record, stream);
+  return {out[0], out.size() > 1 ? Opt(out[1]) : std::nullopt};
+}
+
+// One token: x and the gates [B, D] with unit inner strides, state [B, D] in place; the last state's row of h. None for
+// operands in another form, which gruboros_amd.recurrence brings into this one or refuses.
+Opt recurrence_step(const Tensor& x, const Tensor& gi, const Tensor& gr, const Tensor& decay, const Tensor& state, double c, int64_t stream) {
+  const auto type = x.scalar_type();
+  if ((type != at::kFloat && type != at::kBFloat16) || x.dim() != 2 || x.numel() == 0 || state.scalar_type() != at::kFloat ||
+      decay.scalar_type() != at::kFloat || decay.dim() != 1 || !state.is_contiguous() || !decay.is_contiguous() ||
+      !state.sizes().equals(x.sizes()) || decay.size(0) != x.size(1) || x.size(0) > INT32_MAX || x.size(1) > INT32_MAX)
+    return std::nullopt;
+  for (const Tensor* t : {&x, &gi, &gr, &decay, &state})
+    if (!t->is_cuda() || t->device() != x.device() || (t->requires_grad() && at::GradMode::is_enabled())) return std::nullopt;
+  for (const Tensor* t : {&x, &gi, &gr})
+    if (t->scalar_type() != type || !t->sizes().equals(x.sizes()) || (t->size(1) > 1 && t->stride(1) != 1)) return std::nullopt;
+  c10::DeviceGuard guard(x.device());
+  const auto ld = [](const Tensor& t) { return t.size(0) == 1 ? int64_t(0) : t.stride(0); };
+  Tensor h = make(x.sizes(), type, x);
+  check(mg_recurrence_step(code(x), ptr(x), ld(x), ptr(gi), ld(gi), ptr(gr), ld(gr), fp(decay), c, fp(state), ptr(h), x.size(0),
+                           x.size(1), st(stream)),
+        "mg_recurrence_step");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return h;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -1065,4 +1189,6 @@ PYBIND11_MODULE(_native, m) {
   m.def("delta_bwd", &delta_bwd, nogil());
   m.def("delta_step", &delta_step, nogil());
   m.def("delta_step_plain", &delta_step_plain, nogil());
+  m.def("recurrence", &recurrence, nogil());
+  m.def("recurrence_step", &recurrence_step, nogil());
 }

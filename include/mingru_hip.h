@@ -746,6 +746,48 @@ int mg_layernorm_bwd(int x_dtype, const void* xn, const float* w, const float* m
 int mg_dropout(int x_dtype, const void* x, int y_dtype, const void* residual, void* y, int64_t n, double p,
                uint64_t seed, const int64_t* seed_p, uint64_t offset, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Gated linear recurrence, per batch row and channel, beside the minGRU scan:
+ *   r = sigmoid(decay_gate), i = sigmoid(input_gate),
+ *   a = exp(-c softplus(decay) r)   (0 where reset is nonzero),
+ *   h_t = a h_{t-1} + sqrt(1 - a^2) i x_t,   h_{-1} = h0 (0 when NULL).
+ * No counterpart in the reference.
+ *
+ * dtype (MG_F32 or MG_BF16) is that of x, the gates, h and their gradients;
+ * states, decay [D] and ddecay are fp32, states dense [B, D]. mg_seq: element
+ * (b, t, d) of an operand at p + b sb + t st + d (elements, of any alignment;
+ * strides >= 0, st < 2^28). Outputs are dense [B, T, D]. reset (nullable):
+ * bytes [B, T], nonzero where a sequence starts: nothing before such a step
+ * reaches it or what follows, values that are not finite included, and no
+ * gradient crosses it (with reset given). c >= 0.
+ * mg_recurrence_fwd: h_last (nullable) receives the last state; keep
+ * (nullable, mg_recurrence_keep_elems floats) what mg_recurrence_bwd reads.
+ * mg_recurrence_bwd: dh_last (nullable) is the gradient of the last state;
+ * ddecay and dh0 are nullable; bf16 gradients are rounded to nearest, and
+ * ddecay is summed in a fixed order. Where the decay gate is shut (r = 0 in
+ * fp32) its gradient is 0.
+ * Workspaces: 16-byte aligned, any contents, one call's each. B D < 2^31,
+ * B ceil(D / 64) ceil(T / 64) < 2^24.
+ * mg_recurrence_step: one token, row b of an operand at p + b ld, state
+ * [B, D] in place, h dense [B, D]. */
+typedef struct {
+  const void* p;
+  int64_t sb, st;
+} mg_seq;
+int64_t mg_recurrence_keep_elems(int B, int T, int D);
+size_t mg_recurrence_fwd_workspace_bytes(int B, int T, int D);
+size_t mg_recurrence_bwd_workspace_bytes(int B, int T, int D);
+int mg_recurrence_fwd(int dtype, const mg_seq* x, const mg_seq* input_gate, const mg_seq* decay_gate, const float* decay,
+                      float c, const float* h0, const uint8_t* reset, void* h, float* h_last, float* keep, int B, int T,
+                      int D, void* workspace, size_t workspace_bytes, void* stream);
+int mg_recurrence_bwd(int dtype, const mg_seq* x, const mg_seq* input_gate, const mg_seq* decay_gate, const float* decay,
+                      float c, const float* h0, const uint8_t* reset, const float* keep, const mg_seq* dh,
+                      const float* dh_last, void* dx, void* dinput_gate, void* ddecay_gate, float* ddecay, float* dh0,
+                      int B, int T, int D, void* workspace, size_t workspace_bytes, void* stream);
+int mg_recurrence_step(int dtype, const void* x, int64_t x_ld, const void* input_gate, int64_t input_gate_ld,
+                       const void* decay_gate, int64_t decay_gate_ld, const float* decay, float c, float* state, void* h,
+                       int B, int D, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
