@@ -1030,6 +1030,84 @@ Tensor dropout_add(const Tensor& x, const Opt& residual, double p, uint64_t seed
   return DropoutFn::apply(x, residual, p, static_cast<int64_t>(seed), seed_t, static_cast<int64_t>(offset), stream);
 }
 
+// ------------------------------------------------------------------ the norms around a block
+
+// (x + scale act(gate) norm(branch), its norm); act as in mg_block_norm_fwd
+struct BlockNormFn : ag::Function<BlockNormFn> {
+  static ag::variable_list forward(ag::AutogradContext* ctx, const Tensor& x_, const Tensor& f_, const Tensor& wf, const Tensor& w,
+                                   const Opt& g_, const Opt& scale, int64_t act, bool bf16, double eps, bool record, int64_t stream) {
+    need_cuda(x_);
+    c10::DeviceGuard guard(x_.device());
+    const Tensor x = x_.contiguous(), f = f_.contiguous();
+    Opt g;
+    if (g_) {
+      g = g_->contiguous();
+      alike(f, {&*g});
+      shape(*g, x.sizes(), "gate");
+    }
+    shape(f, x.sizes(), "branch");
+    dense(f, x, "branch");
+    if ((act != 0) != g.has_value()) fail("a gate and its activation come together");
+    const int64_t D = x.size(-1), N = x.numel() / std::max<int64_t>(D, 1);
+    if (D > INT32_MAX) fail("rows are too long");
+    for (const Tensor* t : {&wf, &w}) if (t->device() != x.device()) fail("operands on different devices");
+    if (scale && scale->device() != x.device()) fail("operands on different devices");
+    Tensor xn = make(x.sizes(), at::kFloat, x), y = make(x.sizes(), bf16 ? at::kBFloat16 : at::kFloat, x), rf, rx;
+    if (record) rf = make({N}, at::kFloat, x), rx = make({N}, at::kFloat, x);
+    check(mg_block_norm_fwd(fp(x), code(f), ptr(f), ptr(g), act, vec(wf, D, "weight"), scale ? vec(*scale, D, "scale") : nullptr,
+                            vec(w, D, "weight"), fp(xn), code(y), ptr(y), record ? fp(rf) : nullptr, record ? fp(rx) : nullptr, N, D, eps,
+                            st(stream)),
+          "mg_block_norm_fwd");
+    ctx->set_materialize_grads(false);
+    if (record) ctx->save_for_backward({xn, f, plain(g), wf, w, plain(scale), rf, rx});
+    auto& d = ctx->saved_data;
+    d["act"] = act, d["stream"] = stream, d["bf16"] = bf16;
+    return {xn, y};
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    ag::variable_list out(11);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &xn = saved[0], &f = saved[1], &wf = saved[3], &w = saved[4], &rf = saved[6], &rx = saved[7];
+    const Opt g = opt(saved[2]), scale = opt(saved[5]);
+    auto& d = ctx->saved_data;
+    c10::DeviceGuard guard(xn.device());
+    const int64_t D = xn.size(-1), N = xn.numel() / std::max<int64_t>(D, 1);
+    const auto type = d["bf16"].toBool() ? at::kBFloat16 : at::kFloat;
+    const Tensor dy = grads[1].defined() ? grads[1].to(type).contiguous() : at::zeros(xn.sizes(), xn.options().dtype(type));
+    Opt dres, dx, df, dg, dwf, dscale, dw;
+    if (grads[0].defined()) dres = grads[0].to(at::kFloat).contiguous();
+    dense(dy, xn, "dy");
+    if (dres) dense(*dres, xn, "dx");
+    // (the edges of the tensors that were given: x, branch, the weights, gate, scale)
+    const size_t at_scale = g ? 5 : 4;
+    if (ctx->needs_input_grad(0)) dx = make(xn.sizes(), at::kFloat, xn);
+    if (ctx->needs_input_grad(1)) df = make(f.sizes(), f.scalar_type(), f);
+    if (ctx->needs_input_grad(2)) dwf = make({D}, at::kFloat, xn);
+    if (ctx->needs_input_grad(3)) dw = make({D}, at::kFloat, xn);
+    if (g && ctx->needs_input_grad(4)) dg = make(f.sizes(), f.scalar_type(), f);
+    if (scale && ctx->needs_input_grad(at_scale)) dscale = make({D}, at::kFloat, xn);
+    const size_t wsb = dwf || dw || dscale ? mg_block_norm_bwd_workspace_bytes(N, D) : 0;
+    Tensor ws;
+    if (wsb) ws = bytes(wsb, xn);
+    check(mg_block_norm_bwd(fp(xn), code(f), ptr(f), ptr(g), d["act"].toInt(), fp(wf), fp(scale), fp(w), fp(rf), fp(rx), code(dy), ptr(dy),
+                            fp(dres), fp(dx), ptr(df), ptr(dg), fp(dwf), fp(dscale), fp(dw), N, D, wsb ? ptr(ws) : nullptr, wsb,
+                            st(d["stream"].toInt())),
+          "mg_block_norm_bwd");
+    out[0] = plain(dx), out[1] = plain(df), out[2] = plain(dwf), out[3] = plain(dw), out[4] = plain(dg), out[5] = plain(dscale);
+    return once(out);
+  }
+};
+
+std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const Tensor& f, const Tensor& wf, const Tensor& w, const Opt& g, const Opt& scale,
+                                      int64_t act, bool bf16, double eps, int64_t stream) {
+  bool record = false;
+  for (const Tensor* t : {&x, &f, &wf, &w}) record |= t->requires_grad();
+  for (const Opt* t : {&g, &scale}) record |= *t && (*t)->requires_grad();
+  const auto out = BlockNormFn::apply(x, f, wf, w, g, scale, act, bf16, eps, record && at::GradMode::is_enabled(), stream);
+  return {out[0], out[1]};
+}
+
 // ------------------------------------------------------------------ gated linear recurrence
 
 // a [B, T, D] operand as the kernels read it: unit inner stride, steps at 32-bit distances
@@ -1189,6 +1267,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("delta_bwd", &delta_bwd, nogil());
   m.def("delta_step", &delta_step, nogil());
   m.def("delta_step_plain", &delta_step_plain, nogil());
+  m.def("block_norm", &block_norm, nogil());
   m.def("recurrence", &recurrence, nogil());
   m.def("recurrence_step", &recurrence_step, nogil());
 }

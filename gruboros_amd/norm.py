@@ -9,7 +9,9 @@ a hi/lo pair [N, 2D] = [bf16(y) | bf16(y - bf16(y))] whose hi half is the
 usual output: the operand of the fp32-accurate products (gemm HILO).
 layer_norm and add_layer_norm are the same pair for the other usual norm
 (mg_layernorm_fwd / mg_layernorm_bwd; no counterpart in the reference), with
-the dropout of the joining branch in the same pass.
+the dropout of the joining branch in the same pass. add_gated_rms_norm
+(mg_block_norm_fwd / mg_block_norm_bwd; no counterpart either) is add_rms_norm
+for a block whose output is normed, gated and scaled before it joins.
 Weights of any floating dtype are accepted (a model cast with
 .to(torch.bfloat16), as reference generate.py:140-142 does); the kernels read
 them as fp32.
@@ -183,3 +185,55 @@ def add_layer_norm(x, delta, w, b=None, out_dtype=None, eps=1e-5, dropout_p=0.0,
     if x.numel() == 0:
         return x + delta.float(), no_values(torch.empty_like(x, dtype=out_dtype), x, delta, w, b)
     return native().layer_norm(x.contiguous(), delta.contiguous(), w, b, out_dtype == torch.bfloat16, eps, *drop, stream_of(x))
+
+
+_ACTIVATIONS = {"sigmoid": 1, "silu": 2}
+
+
+def add_gated_rms_norm(x, branch, w_branch, w, gate=None, activation="silu", scale=None, out_dtype=None, eps=FP32_EPS):
+    """Returns (xn, y): the norm after a block, its gate, its residual scale, the residual add and the
+    norm before the next block, in one pass:
+
+        xn = x + scale * activation(gate) * rms_norm(branch) * w_branch
+        y = rms_norm(xn) * w
+
+    over the last dim (1 to 16384 values), statistics in fp32. x: the fp32 residual stream. branch:
+    x's shape, float32 or bfloat16. gate: branch's dtype, broadcast to x's shape, before its
+    activation ("silu" or "sigmoid"), or None for none. w_branch, w and scale: vectors of any floating
+    dtype; scale may be None. y in out_dtype (default x's). Gradients reach all six tensors, once and
+    in reverse mode."""
+    require_cuda(x, branch, w_branch, w, gate, scale)
+    D = x.shape[-1] if x.dim() else 0
+    if not 1 <= D <= 16384:
+        raise ValueError(f"rows hold 1 to 16384 values, got {D}")
+    if x.dtype != torch.float32:
+        raise ValueError(f"the residual stream must be float32, got {x.dtype}")
+    out_dtype = out_dtype or x.dtype
+    dtype_code(out_dtype)
+    dtype_code(branch.dtype)
+    if branch.shape != x.shape:
+        raise ValueError(f"branch {tuple(branch.shape)} must match x {tuple(x.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    for t, name in ((w_branch, "w_branch"), (w, "w"), (scale, "scale")):
+        if t is not None and (not t.is_floating_point() or t.shape != (D,)):
+            raise ValueError(f"{name} must be a floating [{D}] vector, got {t.dtype} {tuple(t.shape)}")
+    if gate is not None and gate.dtype != branch.dtype:
+        raise ValueError(f"gate is {gate.dtype}, branch is {branch.dtype}: they must share a dtype")
+    for t in (branch, w_branch, w, gate, scale):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"operands on {x.device} and {t.device}")
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if gate is not None and gate.shape != x.shape:
+        if gate.dim() > x.dim() or any(n not in (1, m) for n, m in zip(reversed(gate.shape), reversed(x.shape))):
+            raise ValueError(f"gate {tuple(gate.shape)} must broadcast to x {tuple(x.shape)}")
+        gate = gate.expand(x.shape)
+    w_branch, w = w_branch.float().contiguous(), w.float().contiguous()
+    scale = None if scale is None else scale.float().contiguous()
+    if x.numel() == 0:
+        operands = (x, branch, w_branch, w, gate, scale)
+        return no_values(x.clone(), *operands), no_values(torch.empty_like(x, dtype=out_dtype), *operands)
+    act = 0 if gate is None else _ACTIVATIONS[activation]
+    return native().block_norm(x, branch, w_branch, w, gate, scale, act, out_dtype == torch.bfloat16, eps, stream_of(x))

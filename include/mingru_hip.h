@@ -788,6 +788,30 @@ int mg_recurrence_step(int dtype, const void* x, int64_t x_ld, const void* input
                        const void* decay_gate, int64_t decay_gate_ld, const float* decay, float c, float* state, void* h,
                        int B, int D, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The norms around a block with its gate and its residual scale, in the pass
+ * of the residual add (mg_add_rmsnorm's for a block whose output is normed
+ * too; no counterpart in the reference):
+ *   xn = x + scale act(g) f / sqrt(mean(f^2) + eps) w_branch
+ *   y  = xn / sqrt(mean(xn^2) + eps) w
+ * over rows of D (1 to 16384) elements, dense [N, D], of any alignment. x and
+ * xn are fp32; f and g (the gate before its activation) of f_dtype; y of
+ * y_dtype; w_branch, scale (nullable: 1) and w fp32 [D]. act: 0 none (g is
+ * not read), 1 sigmoid, 2 silu. rstd_branch and rstd [N] (nullable together)
+ * receive what the backward reads.
+ * mg_block_norm_bwd: dres (nullable) is the gradient of xn from its other use;
+ * dx (fp32), df, dg, dw_branch, dscale and dw are nullable, the last three
+ * fp32 [D], summed in a fixed order through the workspace (not needed without
+ * them). bf16 gradients are rounded to nearest. */
+int mg_block_norm_fwd(const float* x, int f_dtype, const void* f, const void* g, int act, const float* w_branch,
+                      const float* scale, const float* w, float* x_out, int y_dtype, void* y, float* rstd_branch,
+                      float* rstd, int64_t N, int D, float eps, void* stream);
+size_t mg_block_norm_bwd_workspace_bytes(int64_t N, int D);
+int mg_block_norm_bwd(const float* xn, int f_dtype, const void* f, const void* g, int act, const float* w_branch,
+                      const float* scale, const float* w, const float* rstd_branch, const float* rstd, int dy_dtype,
+                      const void* dy, const float* dres, float* dx, void* df, void* dg, float* dw_branch, float* dscale,
+                      float* dw, int64_t N, int D, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
