@@ -1,0 +1,513 @@
+// Scaled token embedding for any vocabulary and its gradient by sorted tokens, for gfx950 (embed.hip has the gradient
+// of byte-sized vocabularies).
+//   y[n, :] = scale table[ids[n], :]
+//   dw[v, :] = scale sum over n with ids[n] = v of dy[n, :]
+// An id outside the table has a row of NaN and no gradient; the padding id has no gradient.
+//
+// The gradient: the tokens are sorted by id, stably, so that the rows of one id are one run of the sorted order and
+// are summed in token order whatever the timing; every row of dw is then written once, those of no token with zeros.
+//   1. Radix sort of (id, token) in passes of up to 10 bits, least digit first. hist_kernel counts a chunk's digits,
+//      scatter_kernel turns the counts of all chunks into first places and moves its chunk's pairs there; a token's
+//      rank among the wave's lanes of its digit comes from one ballot per bit. Up to 4096 tokens one workgroup does
+//      all passes in one launch. Ids without a gradient sort behind the table as id V.
+//   2. pieces_kernel: every 32 places that are all one id become one row of partial sums, so that an id of many
+//      tokens is not one wave's work.
+//   3. rows_kernel: a wave per row of dw adds the id's places before its first piece, its pieces, and those after the
+//      last. The first place of an id is searched for within its last digit's places. Ids of more than 16 pieces are
+//      left to all four waves of the workgroup.
+// Sums are fp32, rounded once to the table's type.
+//
+// Bound by memory: dy is read once, dw written once.
+
+#include <algorithm>
+
+#include "mg_vec.h"
+
+namespace mg {
+namespace embed_sorted {
+
+constexpr int kDigit = 10, kBins = 1 << kDigit;  // at most
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kSmall = 4096;       // tokens that one workgroup sorts
+constexpr int kMaxChunks = 256;
+constexpr int kPiece = 32;
+constexpr int kManyPieces = 16;
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kVec = 8, kCols = 64 * kVec;  // columns of a lane and of a wave
+constexpr int kRows = 16;                   // rows of dw per workgroup
+constexpr int64_t kMaxN = 1 << 30, kMaxV = 1 << 28;
+
+struct Pairs {
+  uint32_t *key, *pos;
+};
+
+// Passes and their digits: `bits` in all, `digit` each
+struct Plan {
+  int bits, passes, digit, bins, chunks;
+  int64_t chunk;  // tokens of a chunk
+};
+
+struct Ids {
+  const void* p;
+  int wide;  // int64, not int32
+  int64_t N, padding;
+  uint32_t V;
+  __device__ __forceinline__ uint32_t key(int64_t n) const {
+    const int64_t v = wide ? static_cast<const int64_t*>(p)[n] : static_cast<const int32_t*>(p)[n];
+    return v < 0 || v >= V || v == padding ? V : static_cast<uint32_t>(v);
+  }
+};
+
+// ------------------------------------------------------------------ lookup
+
+typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+
+__device__ __forceinline__ void load8(const float* p, float (&v)[kVec]) {
+  const f32x4u a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+}
+__device__ __forceinline__ void load8(const bf16_t* p, float (&v)[kVec]) {
+  const u16x8u a = *reinterpret_cast<const u16x8u*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = bf16_to_f32(a[j]);
+}
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const bf16_t* p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+// eight values from p on, of which the first `left` exist
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, float (&v)[kVec]) {
+  if (left >= kVec) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v[j] = j < left ? load1(p + j) : 0.0f;
+  }
+}
+__device__ __forceinline__ void store8(float* p, int left, const float (&v)[kVec]) {
+  if (left >= kVec) {
+    const f32x4u a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+    reinterpret_cast<f32x4u*>(p)[0] = a;
+    reinterpret_cast<f32x4u*>(p)[1] = b;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if (j < left) p[j] = v[j];
+  }
+}
+__device__ __forceinline__ void store8(bf16_t* p, int left, const float (&v)[kVec]) {
+  if (left >= kVec) {
+    u16x8u a;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) a[j] = f32_to_bf16(v[j]);
+    *reinterpret_cast<u16x8u*>(p) = a;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if (j < left) p[j] = f32_to_bf16(v[j]);
+  }
+}
+
+// `per` threads (a power of two) to a row
+template <typename Tw, typename Ty>
+__global__ __launch_bounds__(kThreads) void lookup_kernel(Ids ids, const Tw* __restrict__ table, Ty* __restrict__ y, int D, float scale,
+                                                          int per) {
+  const int rows = kThreads / per, t = threadIdx.x & (per - 1);
+  for (int64_t n = static_cast<int64_t>(blockIdx.x) * rows + threadIdx.x / per; n < ids.N; n += static_cast<int64_t>(gridDim.x) * rows) {
+    const uint32_t v = ids.key(n);
+    const Tw* row = table + static_cast<int64_t>(v) * D;
+    for (int c = t * kVec; c < D; c += per * kVec) {
+      float x[kVec];
+      if (v < ids.V) {
+        load8(row + c, D - c, x);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[j] *= scale;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[j] = __builtin_nanf("");
+      }
+      store8(y + n * D + c, D - c, x);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sort
+
+// Lanes of the wave with this lane's digit d (live lanes only)
+__device__ __forceinline__ uint64_t peers_of(bool live, uint32_t d, int bits) {
+  uint64_t m = __ballot(live);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = d >> b & 1;
+    const uint64_t with = __ballot(live && one);
+    m &= one ? with : ~with;
+  }
+  return m;
+}
+
+// A pass's source: the ids themselves first, then the pairs of the pass before
+struct Source {
+  Ids ids;
+  const uint32_t *key, *pos;
+  __device__ __forceinline__ uint32_t key_of(int64_t n) const { return key ? key[n] : ids.key(n); }
+  __device__ __forceinline__ uint32_t pos_of(int64_t n) const { return key ? pos[n] : static_cast<uint32_t>(n); }
+};
+
+// counts[chunk][bin] of the digit at `shift`
+__global__ __launch_bounds__(kSortThreads) void hist_kernel(Source src, int64_t chunk, int shift, int bins, int* __restrict__ counts) {
+  __shared__ int s_cnt[kBins];
+  for (int i = threadIdx.x; i < bins; i += kSortThreads) s_cnt[i] = 0;
+  __syncthreads();
+  const int64_t n0 = blockIdx.x * chunk, n1 = std::min<int64_t>(src.ids.N, n0 + chunk);
+  for (int64_t n = n0 + threadIdx.x; n < n1; n += kSortThreads) atomicAdd(&s_cnt[src.key_of(n) >> shift & (bins - 1)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i < bins; i += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * bins + i] = s_cnt[i];
+}
+
+struct SortShared {
+  int cnt[kSortWaves][kBins];  // of each wave's share of the chunk, then where its tokens of a digit go
+  int wave[kSortWaves];
+};
+
+// One pass over a chunk by the whole workgroup. counts: those of all chunks, or null where this is the only one;
+// starts (nullable): receives the first place of every bin, and N behind them.
+__device__ void scatter(SortShared& s, const Source& src, int64_t n0, int64_t n1, int chunk_i, int chunks, const int* counts, int shift,
+                        int digit, const Pairs& out, int* starts) {
+  const int bins = 1 << digit, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortThreads) (&s.cnt[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t per = (n1 - n0 + kSortWaves - 1) / kSortWaves;
+  const int64_t w0 = std::min<int64_t>(n1, n0 + wave * per), w1 = std::min<int64_t>(n1, w0 + per);
+  for (int64_t n = w0 + lane; n < w1; n += 64) atomicAdd(&s.cnt[wave][src.key_of(n) >> shift & (bins - 1)], 1);
+  __syncthreads();
+  // a thread per bin: the waves' first places within the chunk's tokens of the bin; all tokens of the bin, and those
+  // of the chunks before
+  const int bin = threadIdx.x;
+  int own = 0, all = 0, before = 0;
+  if (bin < bins) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = s.cnt[w][bin];
+      s.cnt[w][bin] = own;
+      own += c;
+    }
+    if (counts) {
+#pragma unroll 8
+      for (int g = 0; g < chunks; ++g) {
+        const int c = counts[static_cast<int64_t>(g) * bins + bin];
+        all += c;
+        before += g < chunk_i ? c : 0;
+      }
+    } else {
+      all = own;
+    }
+  }
+  // exclusive sums over the bins: within the wave, then over the waves
+  int sum = all;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 63) s.wave[wave] = sum;
+  __syncthreads();
+  int first = sum - all;
+  for (int w = 0; w < wave; ++w) first += s.wave[w];
+  if (bin < bins) {
+    if (starts) {
+      starts[bin] = first;
+      if (bin == bins - 1) starts[bins] = first + all;
+    }
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) s.cnt[w][bin] += first + before;
+  }
+  __syncthreads();
+  // (a wave's accesses to its counters are in program order)
+  for (int64_t base = w0; base < w1; base += 64) {
+    const int64_t n = base + lane;
+    const bool live = n < w1;
+    const uint32_t key = live ? src.key_of(n) : 0, pos = live ? src.pos_of(n) : 0, d = key >> shift & (bins - 1);
+    const uint64_t m = peers_of(live, d, digit);
+    if (live) {
+      const int at = s.cnt[wave][d];
+      const int p = at + __popcll(m & ((1ull << lane) - 1ull));
+      out.key[p] = key;
+      out.pos[p] = pos;
+      if (63 - __clzll(m) == lane) s.cnt[wave][d] = at + __popcll(m);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kSortThreads) void scatter_kernel(Source src, int64_t chunk, const int* __restrict__ counts, int shift,
+                                                               int digit, Pairs out, int* __restrict__ starts) {
+  __shared__ SortShared s;
+  const int64_t n0 = blockIdx.x * chunk, n1 = std::min<int64_t>(src.ids.N, n0 + chunk);
+  scatter(s, src, n0, n1, blockIdx.x, gridDim.x, counts, shift, digit, out, blockIdx.x == 0 ? starts : nullptr);
+}
+
+// All passes for up to kSmall tokens; the last one ends in `to`
+__global__ __launch_bounds__(kSortThreads) void sort_small_kernel(Ids ids, int passes, int digit, Pairs other, Pairs to, int* __restrict__ starts) {
+  __shared__ SortShared s;
+  Source src = {ids, nullptr, nullptr};
+  for (int p = 0; p < passes; ++p) {
+    const Pairs& out = (passes - 1 - p) % 2 ? other : to;
+    scatter(s, src, 0, ids.N, 0, 1, nullptr, p * digit, digit, out, p == passes - 1 ? starts : nullptr);
+    __threadfence_block();
+    __syncthreads();
+    src.key = out.key, src.pos = out.pos;
+  }
+}
+
+// ------------------------------------------------------------------ sums
+
+// acc += rows pos[i], i = i0 .. i1 - 1, in order, of columns c .. c + 7
+template <typename T>
+__device__ __forceinline__ void add_rows(const T* __restrict__ dy, const uint32_t* __restrict__ pos, int64_t i0, int64_t i1, int D, int c,
+                                         int left, float (&acc)[kVec]) {
+  constexpr int kAhead = 8;
+  int64_t i = i0;
+  for (; i + kAhead <= i1; i += kAhead) {
+    float x[kAhead][kVec];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) load8(dy + static_cast<int64_t>(pos[i + u]) * D + c, left, x[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) acc[j] += x[u][j];
+  }
+  for (; i < i1; ++i) {
+    float x[kVec];
+    load8(dy + static_cast<int64_t>(pos[i]) * D + c, left, x);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) acc[j] += x[j];
+  }
+}
+__device__ __forceinline__ void add_parts(const float* __restrict__ part, int64_t p0, int64_t p1, int D, int c, int left, float (&acc)[kVec]) {
+#pragma unroll 8
+  for (int64_t p = p0; p < p1; ++p) {
+    float x[kVec];
+    load8(part + p * D + c, left, x);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) acc[j] += x[j];
+  }
+}
+
+// part[p, :] = the sum of places [32 p, 32 p + 32) where they are all one id of the table; a wave per piece and kCols columns
+template <typename T>
+__global__ __launch_bounds__(kThreads) void pieces_kernel(const T* __restrict__ dy, Pairs sorted, int64_t pieces, int D, uint32_t V,
+                                                          float* __restrict__ part) {
+  const int64_t p = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (p >= pieces) return;
+  const uint32_t key = sorted.key[p * kPiece];
+  if (key >= V || key != sorted.key[p * kPiece + kPiece - 1]) return;
+  for (int c = (threadIdx.x % 64) * kVec + blockIdx.y * kCols; c < D; c += gridDim.y * kCols) {
+    float acc[kVec] = {};
+    add_rows(dy, sorted.pos, p * kPiece, (p + 1) * kPiece, D, c, D - c, acc);
+    store8(part + p * D + c, D - c, acc);
+  }
+}
+
+template <typename T, typename Tw>
+__global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ starts, int shift,
+                                                        const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
+  __shared__ int s_at[kRows + 1];
+  __shared__ float s_sum[kWaves][kCols];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kRows;
+  if (threadIdx.x <= kRows) {  // the first place of each row's id
+    const uint32_t v = static_cast<uint32_t>(std::min<int64_t>(v0 + threadIdx.x, V));
+    int lo = starts[v >> shift], hi = starts[(v >> shift) + 1];
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (sorted.key[mid] < v)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    s_at[threadIdx.x] = lo;
+  }
+  __syncthreads();
+  for (int r = wave; r < kRows && v0 + r < V; r += kWaves) {
+    const int64_t i0 = __builtin_amdgcn_readfirstlane(s_at[r]), i1 = __builtin_amdgcn_readfirstlane(s_at[r + 1]), p0 = (i0 + kPiece - 1) / kPiece, p1 = i1 / kPiece;
+    if (p1 - p0 > kManyPieces) continue;
+    Tw* out = dw + (v0 + r) * D;
+    for (int c = lane * kVec; c < D; c += kCols) {
+      float acc[kVec] = {};
+      if (p0 < p1) {
+        add_rows(dy, sorted.pos, i0, p0 * kPiece, D, c, D - c, acc);
+        add_parts(part, p0, p1, D, c, D - c, acc);
+        add_rows(dy, sorted.pos, p1 * kPiece, i1, D, c, D - c, acc);
+      } else {
+        add_rows(dy, sorted.pos, i0, i1, D, c, D - c, acc);
+      }
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) acc[j] *= scale;
+      store8(out + c, D - c, acc);
+    }
+  }
+  for (int r = 0; r < kRows && v0 + r < V; ++r) {  // ids of many pieces: a quarter of them to each wave
+    const int64_t i0 = __builtin_amdgcn_readfirstlane(s_at[r]), i1 = __builtin_amdgcn_readfirstlane(s_at[r + 1]), p0 = (i0 + kPiece - 1) / kPiece, p1 = i1 / kPiece;
+    if (p1 - p0 <= kManyPieces) continue;
+    const int64_t quarter = (p1 - p0 + kWaves - 1) / kWaves, q0 = std::min(p1, p0 + wave * quarter), q1 = std::min(p1, q0 + quarter);
+    for (int c0 = 0; c0 < D; c0 += kCols) {
+      const int c = c0 + lane * kVec, left = D - c;
+      float acc[kVec] = {};
+      if (left > 0) {
+        if (wave == 0) add_rows(dy, sorted.pos, i0, p0 * kPiece, D, c, left, acc);
+        add_parts(part, q0, q1, D, c, left, acc);
+        if (wave == kWaves - 1) add_rows(dy, sorted.pos, p1 * kPiece, i1, D, c, left, acc);
+      }
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) s_sum[wave][j * 64 + lane] = acc[j];
+      __syncthreads();
+      if (wave == 0 && left > 0) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          float t = s_sum[0][j * 64 + lane];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) t += s_sum[w][j * 64 + lane];
+          acc[j] = t * scale;
+        }
+        store8(dw + (v0 + r) * D + c, left, acc);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+inline Plan plan_of(int64_t N, int64_t V) {
+  Plan p = {};
+  p.bits = 1;
+  while (V >> p.bits) ++p.bits;  // (ids to V, which is the one without a gradient)
+  p.passes = (p.bits + kDigit - 1) / kDigit;
+  p.digit = (p.bits + p.passes - 1) / p.passes;
+  p.bins = 1 << p.digit;
+  if (N <= kSmall) {
+    p.chunks = 1, p.chunk = N;
+  } else {
+    p.chunk = std::max<int64_t>(kSortThreads, (N + kMaxChunks - 1) / kMaxChunks);
+    p.chunks = static_cast<int>((N + p.chunk - 1) / p.chunk);
+  }
+  return p;
+}
+
+// Workspace: [pieces][D] partial sums, counts of each chunk, starts, two sets of pairs
+struct Layout {
+  size_t counts, starts, pairs, total;
+  int64_t pieces;
+};
+inline Layout layout_of(int64_t N, int D, const Plan& p) {
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  Layout l;
+  l.pieces = N / kPiece;
+  l.counts = up(static_cast<size_t>(l.pieces) * D * 4);
+  l.starts = l.counts + up(static_cast<size_t>(p.chunks) * p.bins * 4);
+  l.pairs = l.starts + up((static_cast<size_t>(p.bins) + 1) * 4);
+  l.total = l.pairs + 4 * up(static_cast<size_t>(N) * 4);
+  return l;
+}
+
+inline int check_ids(const char* fn, int id_bytes, const void* ids, int64_t N, int D, int64_t V) {
+  if (N < 1 || N >= kMaxN || D < 1 || V < 1 || V >= kMaxV)
+    return fail(MG_ERR_ARG, "%s: N=%lld, D=%d, V=%lld must be at least 1, N below 2^30, V below 2^28", fn, (long long)N, D, (long long)V);
+  if (id_bytes != 4 && id_bytes != 8) return fail(MG_ERR_DTYPE, "%s: ids of %d bytes", fn, id_bytes);
+  if (!ids || !aligned(ids, id_bytes)) return fail(MG_ERR_ARG, "%s: ids NULL or misaligned", fn);
+  return MG_OK;
+}
+inline int check_p(const char* fn, const char* name, const void* p, int dt) {
+  if (dt != MG_F32 && dt != MG_BF16) return fail(MG_ERR_DTYPE, "%s: %s dtype %d unsupported", fn, name, dt);
+  if (!p || !aligned(p, dt == MG_F32 ? 4 : 2)) return fail(MG_ERR_ARG, "%s: %s NULL or misaligned", fn, name);
+  return MG_OK;
+}
+
+template <typename Tw, typename Ty>
+void launch_lookup(const Ids& ids, const void* table, void* y, int D, float scale, hipStream_t st) {
+  int per = 1;
+  while (per < kThreads && per * kVec < D) per *= 2;
+  const int64_t wgs = (ids.N + kThreads / per - 1) / (kThreads / per);
+  hipLaunchKernelGGL((lookup_kernel<Tw, Ty>), dim3(std::min<int64_t>(wgs, 1 << 20)), dim3(kThreads), 0, st, ids, static_cast<const Tw*>(table),
+                     static_cast<Ty*>(y), D, scale, per);
+}
+
+template <typename T, typename Tw>
+void launch_sums(const void* dy, const Pairs& sorted, const int* starts, int shift, float* part, int64_t pieces, void* dw, int D, int64_t V,
+                 float scale, hipStream_t st) {
+  if (pieces)
+    hipLaunchKernelGGL((pieces_kernel<T>), dim3((pieces + kWaves - 1) / kWaves, std::min((D + kCols - 1) / kCols, 64)), dim3(kThreads), 0, st,
+                       static_cast<const T*>(dy), sorted, pieces, D, static_cast<uint32_t>(V), part);
+  hipLaunchKernelGGL((rows_kernel<T, Tw>), dim3((V + kRows - 1) / kRows), dim3(kThreads), 0, st, static_cast<const T*>(dy), sorted, starts,
+                     shift, part, static_cast<Tw*>(dw), D, static_cast<uint32_t>(V), scale);
+}
+
+}  // namespace embed_sorted
+}  // namespace mg
+
+using namespace mg;
+
+extern "C" int mg_embedding_fwd(int id_bytes, const void* ids, int64_t N, int table_dtype, const void* table, int64_t V, int D, float scale,
+                                int y_dtype, void* y, void* stream) {
+  using namespace embed_sorted;
+  const char* fn = "mg_embedding_fwd";
+  int rc;
+  if ((rc = check_ids(fn, id_bytes, ids, N, D, V)) || (rc = check_p(fn, "table", table, table_dtype)) || (rc = check_p(fn, "y", y, y_dtype)))
+    return rc;
+  const Ids in = {ids, id_bytes == 8, N, -1, static_cast<uint32_t>(V)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (table_dtype == MG_BF16)
+    y_dtype == MG_BF16 ? launch_lookup<bf16_t, bf16_t>(in, table, y, D, scale, st) : launch_lookup<bf16_t, float>(in, table, y, D, scale, st);
+  else
+    y_dtype == MG_BF16 ? launch_lookup<float, bf16_t>(in, table, y, D, scale, st) : launch_lookup<float, float>(in, table, y, D, scale, st);
+  return check_launch(fn);
+}
+
+extern "C" size_t mg_embedding_sorted_bwd_workspace_bytes(int64_t N, int D, int64_t V) {
+  using namespace embed_sorted;
+  if (N < 1 || N >= kMaxN || D < 1 || V < 1 || V >= kMaxV) return 0;
+  return layout_of(N, D, plan_of(N, V)).total;
+}
+
+extern "C" int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N, int dy_dtype, const void* dy, int D, int64_t V, float scale,
+                                       int64_t padding, int dw_dtype, void* dw, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace embed_sorted;
+  const char* fn = "mg_embedding_sorted_bwd";
+  int rc;
+  if ((rc = check_ids(fn, id_bytes, ids, N, D, V)) || (rc = check_p(fn, "dy", dy, dy_dtype)) || (rc = check_p(fn, "dw", dw, dw_dtype))) return rc;
+  const Plan p = plan_of(N, V);
+  const Layout l = layout_of(N, D, p);
+  if (!workspace || workspace_bytes < l.total || !aligned(workspace, 256))
+    return fail(MG_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu (or misaligned)", fn, workspace_bytes, l.total);
+  char* ws = static_cast<char*>(workspace);
+  float* part = reinterpret_cast<float*>(ws);
+  int* counts = reinterpret_cast<int*>(ws + l.counts);
+  int* starts = reinterpret_cast<int*>(ws + l.starts);
+  const size_t each = (l.total - l.pairs) / 4;
+  uint32_t* arr[4];
+  for (int i = 0; i < 4; ++i) arr[i] = reinterpret_cast<uint32_t*>(ws + l.pairs + i * each);
+  const Pairs set[2] = {{arr[0], arr[1]}, {arr[2], arr[3]}};
+  const Ids in = {ids, id_bytes == 8, N, padding, static_cast<uint32_t>(V)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const Pairs& sorted = set[0];
+  if (p.chunks == 1 && N <= kSmall) {
+    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(kSortThreads), 0, st, in, p.passes, p.digit, set[1], set[0], starts);
+  } else {
+    Source src = {in, nullptr, nullptr};
+    for (int i = 0; i < p.passes; ++i) {
+      const Pairs& out = set[(p.passes - 1 - i) % 2];
+      hipLaunchKernelGGL(hist_kernel, dim3(p.chunks), dim3(kSortThreads), 0, st, src, p.chunk, i * p.digit, p.bins, counts);
+      hipLaunchKernelGGL(scatter_kernel, dim3(p.chunks), dim3(kSortThreads), 0, st, src, p.chunk, counts, i * p.digit, p.digit, out,
+                         i == p.passes - 1 ? starts : nullptr);
+      src.key = out.key, src.pos = out.pos;
+    }
+  }
+  const int shift = (p.passes - 1) * p.digit;
+  if (dy_dtype == MG_BF16)
+    dw_dtype == MG_BF16 ? launch_sums<bf16_t, bf16_t>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st)
+                        : launch_sums<bf16_t, float>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st);
+  else
+    dw_dtype == MG_BF16 ? launch_sums<float, bf16_t>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st)
+                        : launch_sums<float, float>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st);
+  return check_launch(fn);
+}

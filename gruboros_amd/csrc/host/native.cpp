@@ -1108,6 +1108,52 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const Tensor& f, const Te
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ scaled embedding
+
+struct EmbeddingFn : ag::Function<EmbeddingFn> {
+  static Tensor forward(ag::AutogradContext* ctx, const Tensor& ids_, const Tensor& weight, double scale, bool bf16, int64_t padding,
+                        int64_t stream) {
+    need_cuda(weight);
+    c10::DeviceGuard guard(weight.device());
+    if (weight.dim() != 2 || weight.size(1) > INT32_MAX) fail("weight: expected [V, D]");
+    if (ids_.device() != weight.device()) fail("ids: expected a tensor on " + weight.device().str());
+    if (ids_.scalar_type() != at::kLong && ids_.scalar_type() != at::kInt) fail("ids: expected int64 or int32");
+    const Tensor ids = ids_.contiguous(), w = weight.contiguous();
+    const int64_t V = w.size(0), D = w.size(1);
+    auto size = ids.sizes().vec();
+    size.push_back(D);
+    Tensor y = make(size, bf16 ? at::kBFloat16 : at::kFloat, w);
+    check(mg_embedding_fwd(ids.element_size(), ptr(ids), ids.numel(), code(w), ptr(w), V, D, scale, code(y), ptr(y), st(stream)),
+          "mg_embedding_fwd");
+    ctx->save_for_backward({ids});
+    auto& d = ctx->saved_data;
+    d["scale"] = scale, d["padding"] = padding, d["stream"] = stream, d["V"] = V, d["D"] = D, d["table"] = weight.scalar_type();
+    d["type"] = y.scalar_type();
+    return y;
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    ag::variable_list out(6);
+    const Tensor ids = ctx->get_saved_variables()[0];
+    auto& d = ctx->saved_data;
+    const int64_t V = d["V"].toInt(), D = d["D"].toInt();
+    c10::DeviceGuard guard(ids.device());
+    const Tensor dy = grads[0].to(d["type"].toScalarType()).contiguous();
+    if (dy.numel() != ids.numel() * D) fail("dy: expected a row per id");
+    Tensor dw = make({V, D}, d["table"].toScalarType(), dy);
+    const size_t wsb = mg_embedding_sorted_bwd_workspace_bytes(ids.numel(), D, V);
+    Tensor ws = bytes(wsb, dy);
+    check(mg_embedding_sorted_bwd(ids.element_size(), ptr(ids), ids.numel(), code(dy), ptr(dy), D, V, d["scale"].toDouble(),
+                                  d["padding"].toInt(), code(dw), ptr(dw), ptr(ws), wsb, st(d["stream"].toInt())),
+          "mg_embedding_sorted_bwd");
+    out[1] = dw;
+    return once(out);
+  }
+};
+
+Tensor scaled_embedding(const Tensor& ids, const Tensor& weight, double scale, bool bf16, int64_t padding, int64_t stream) {
+  return EmbeddingFn::apply(ids, weight, scale, bf16, padding, stream);
+}
+
 // ------------------------------------------------------------------ gated linear recurrence
 
 // a [B, T, D] operand as the kernels read it: unit inner stride, steps at 32-bit distances
@@ -1268,6 +1314,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("delta_step", &delta_step, nogil());
   m.def("delta_step_plain", &delta_step_plain, nogil());
   m.def("block_norm", &block_norm, nogil());
+  m.def("scaled_embedding", &scaled_embedding, nogil());
   m.def("recurrence", &recurrence, nogil());
   m.def("recurrence_step", &recurrence_step, nogil());
 }

@@ -8,11 +8,15 @@ anything to the host. torch's embedding backward copies a segment count to the
 host, which holds the host at the end of every backward pass while the GPU
 drains; the optimizer's host work then ran with the GPU idle (0.12-0.2 ms per
 cfg3 step, beside the 0.12 ms of the backward's own kernels).
+
+scaled_embedding (mg_embedding_fwd / mg_embedding_sorted_bwd) is the same for
+any vocabulary and table type, with a scale: lookup, scale and cast in one
+pass, and a gradient by tokens sorted on the GPU.
 """
 import torch
 import torch.nn.functional as F
 
-from ._lib import check, lib, ptr, stream_of
+from ._lib import check, dtype_code, lib, native, no_values, ptr, require_cuda, stream_of
 
 MAX_VOCAB = 512  # mg_embedding_bwd's table limit
 
@@ -54,3 +58,35 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
             and ids.numel() < (1 << 31)):
         return EmbeddingFn.apply(ids, weight)
     return F.embedding(ids, weight)
+
+
+def scaled_embedding(ids, weight, scale=1.0, out_dtype=None, padding_idx=None):
+    """scale * weight[ids] in out_dtype (default weight's), for tables of any size.
+
+    ids: int64 or int32 of any shape; weight [V, D], float32 or bfloat16, V < 2^28; fewer than 2^30
+    ids. The gradient reaches weight, in its dtype, once and in reverse mode: rows are summed in
+    fp32 in the order of the tokens and rounded once, so results repeat bit for bit. An id outside
+    the table (torch's lookup stops the process there) gives a row of NaN and no gradient. The row
+    of padding_idx, which counts from the end where it is negative, gets no gradient."""
+    require_cuda(ids, weight)
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
+    if weight.dim() != 2 or not 1 <= weight.shape[0] < 1 << 28:
+        raise ValueError(f"weight must be [V, D] with 1 <= V < 2^28, got {tuple(weight.shape)}")
+    if ids.numel() >= 1 << 30:
+        raise ValueError(f"{ids.numel()} ids: a call takes fewer than 2^30")
+    if ids.device != weight.device:
+        raise ValueError(f"operands on {ids.device} and {weight.device}")
+    dtype_code(weight.dtype)
+    out_dtype = out_dtype or weight.dtype
+    dtype_code(out_dtype)
+    V, D = weight.shape
+    scale = float(scale)
+    padding = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
+        padding = int(padding_idx) % V
+    if ids.numel() == 0 or D == 0:
+        return no_values(torch.empty(*ids.shape, D, dtype=out_dtype, device=weight.device), weight)
+    return native().scaled_embedding(ids, weight, scale, out_dtype == torch.bfloat16, padding, stream_of(weight))

@@ -812,6 +812,25 @@ int mg_block_norm_bwd(const float* xn, int f_dtype, const void* f, const void* g
                       const void* dy, const float* dres, float* dx, void* df, void* dg, float* dw_branch, float* dscale,
                       float* dw, int64_t N, int D, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Token embedding with a scale, for tables of any size and type (reference
+ * mingru/minLM.py:92,99 has no scale, and a vocabulary of bytes, whose gradient
+ * is mg_embedding_bwd):
+ *   y[n, :] = scale table[ids[n], :],   n < N
+ *   dw[v, :] = scale * sum over n with ids[n] == v of dy[n, :]
+ * ids: int32 or int64 (id_bytes 4 or 8); table and dw dense [V, D], y and dy
+ * dense [N, D], fp32 or bf16 each, of any alignment. An id outside [0, V)
+ * reads nothing: its row of y is NaN, and dy's adds to no row; nor does that
+ * of a token whose id is `padding` (a negative one: none). Every row of dw is
+ * written. Sums are fp32, in a fixed order: the same inputs give the same bits.
+ * N < 2^30, V < 2^28. The workspace is 256-byte aligned, any contents. */
+int mg_embedding_fwd(int id_bytes, const void* ids, int64_t N, int table_dtype, const void* table, int64_t V, int D,
+                     float scale, int y_dtype, void* y, void* stream);
+size_t mg_embedding_sorted_bwd_workspace_bytes(int64_t N, int D, int64_t V);
+int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N, int dy_dtype, const void* dy, int D, int64_t V,
+                            float scale, int64_t padding, int dw_dtype, void* dw, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
