@@ -113,6 +113,10 @@ SIGNATURES = {
                                   ctypes.c_double, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp, _c_size, _vp]),
     "mg_dropout": (_c_int, [_c_int, _vp, _c_int, _vp, _vp, _c_i64, ctypes.c_double, ctypes.c_uint64, _vp,
                             ctypes.c_uint64, _vp]),
+    "mg_distill_workspace_bytes": (_c_size, [_c_i64]),
+    "mg_distill": (_c_int, [_c_int, _vp, _c_i64, _c_i64, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, ctypes.c_float, ctypes.c_float,
+                            _fp, _vp, _vp, _c_size, _vp]),
+    "mg_scale_inplace": (_c_int, [_c_int, _vp, _c_i64, _fp, _vp]),
     "mg_embedding_fwd": (_c_int, [_c_int, _vp, _c_i64, _c_int, _vp, _c_i64, _c_int, ctypes.c_float, _c_int, _vp, _vp]),
     "mg_embedding_sorted_bwd_workspace_bytes": (_c_size, [_c_i64, _c_int, _c_i64]),
     "mg_embedding_sorted_bwd": (_c_int, [_c_int, _vp, _c_i64, _c_int, _vp, _c_int, _c_i64, ctypes.c_float, _c_i64, _c_int, _vp, _vp,

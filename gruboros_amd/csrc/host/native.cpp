@@ -1154,6 +1154,76 @@ Tensor scaled_embedding(const Tensor& ids, const Tensor& weight, double scale, b
   return EmbeddingFn::apply(ids, weight, scale, bf16, padding, stream);
 }
 
+// ------------------------------------------------------------------ distillation
+
+// The loss, with the logits' gradient made in the same pass. The backward multiplies that by the loss's gradient in
+// place (a factor of 1 costs nothing) and hands it over; asked a second time, it makes it again.
+struct DistillFn : ag::Function<DistillFn> {
+  static Tensor launch(const Tensor& logits, const Tensor& ids, const Tensor& top, const Opt& labels, double temperature, double alpha,
+                       const Opt& dlogits, int64_t stream) {
+    const int64_t V = logits.size(-1), B = logits.dim() == 3 ? logits.size(0) : 1, T = logits.size(-2), K = ids.size(-1);
+    if (V > INT32_MAX || K > INT32_MAX) fail("logits: rows are too long");
+    const mg_seq s = {ptr(logits), B > 1 ? logits.stride(0) : 0, T > 1 ? logits.stride(-2) : 0};
+    Tensor loss = make({}, at::kFloat, logits);
+    const size_t wsb = mg_distill_workspace_bytes(B * T);
+    Tensor ws = bytes(wsb, logits);
+    check(mg_distill(code(logits), &s, B, T, V, ids.element_size(), ptr(ids), code(top), ptr(top), K,
+                     static_cast<const int64_t*>(ptr(labels)), temperature, alpha, fp(loss), ptr(dlogits), ptr(ws), wsb, st(stream)),
+          "mg_distill");
+    return loss;
+  }
+  static Tensor forward(ag::AutogradContext* ctx, const Tensor& logits_, const Tensor& ids_, const Tensor& top_, const Opt& labels_,
+                        double temperature, double alpha, bool record, int64_t stream) {
+    need_cuda(logits_);
+    c10::DeviceGuard guard(logits_.device());
+    if (logits_.dim() != 2 && logits_.dim() != 3) fail("logits: expected [N, V] or [B, T, V]");
+    const Tensor logits = logits_.size(-1) == 1 || logits_.stride(-1) == 1 ? logits_ : logits_.contiguous();
+    const Tensor ids = ids_.contiguous(), top = top_.contiguous();
+    const int64_t N = logits.numel() / std::max<int64_t>(logits.size(-1), 1), K = ids.dim() ? ids.size(-1) : 0;
+    if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) fail("top_ids: expected int64 or int32");
+    if (K < 1 || ids.numel() != N * K || !top.sizes().equals(ids.sizes())) fail("top_ids and top_logits: expected K entries per row");
+    Opt labels;
+    if (labels_) {
+      labels = labels_->contiguous();
+      if (labels->scalar_type() != at::kLong || labels->numel() != N) fail("labels: expected an int64 per row");
+      if (labels->device() != logits.device()) fail("operands on different devices");
+    }
+    for (const Tensor* t : {&ids, &top})
+      if (t->device() != logits.device()) fail("operands on different devices");
+    Opt dl;
+    if (record) dl = make(logits.sizes(), logits.scalar_type(), logits);
+    Tensor loss = launch(logits, ids, top, labels, temperature, alpha, dl, stream);
+    if (record) {
+      ctx->save_for_backward({logits, ids, top, plain(labels)});
+      auto& d = ctx->saved_data;
+      d["dl"] = *dl, d["temperature"] = temperature, d["alpha"] = alpha, d["stream"] = stream;
+    }
+    return loss;
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    ag::variable_list out(8);
+    auto& d = ctx->saved_data;
+    Tensor dl;
+    const Tensor g = grads[0].to(at::kFloat);
+    c10::DeviceGuard guard(g.device());
+    if (d["dl"].isTensor()) {
+      dl = d["dl"].toTensor();
+      d["dl"] = c10::IValue();
+    } else {
+      const auto saved = ctx->get_saved_variables();
+      dl = make(saved[0].sizes(), saved[0].scalar_type(), saved[0]);
+      launch(saved[0], saved[1], saved[2], opt(saved[3]), d["temperature"].toDouble(), d["alpha"].toDouble(), dl, d["stream"].toInt());
+    }
+    check(mg_scale_inplace(code(dl), ptr(dl), dl.numel(), fp(g), st(d["stream"].toInt())), "mg_scale_inplace");
+    out[0] = dl;
+    return once(out);
+  }
+};
+
+Tensor distill(const Tensor& logits, const Tensor& ids, const Tensor& top, const Opt& labels, double temperature, double alpha, int64_t stream) {
+  return DistillFn::apply(logits, ids, top, labels, temperature, alpha, logits.requires_grad() && at::GradMode::is_enabled(), stream);
+}
+
 // ------------------------------------------------------------------ gated linear recurrence
 
 // a [B, T, D] operand as the kernels read it: unit inner stride, steps at 32-bit distances
@@ -1314,6 +1384,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("delta_step", &delta_step, nogil());
   m.def("delta_step_plain", &delta_step_plain, nogil());
   m.def("block_norm", &block_norm, nogil());
+  m.def("distill", &distill, nogil());
   m.def("scaled_embedding", &scaled_embedding, nogil());
   m.def("recurrence", &recurrence, nogil());
   m.def("recurrence_step", &recurrence_step, nogil());

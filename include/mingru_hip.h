@@ -831,6 +831,31 @@ int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N, int dy_dty
                             float scale, int64_t padding, int dw_dtype, void* dw, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Distillation from a teacher's top logits, with cross-entropy against labels
+ * beside it, and the gradient in the same pass (reference mingru/minLM.py:
+ * 146-149 has the cross-entropy alone; vocabularies of any size here). Per row
+ * of V logits z, K (1 to 512) teacher entries (id, t) and temperature:
+ *   p = softmax(t / temperature), KL = sum p (log p - log softmax(z / temperature)[id])
+ *   CE = -log softmax(z)[label]
+ *   loss = alpha temperature^2 mean(KL) + (1 - alpha) mean(CE)
+ * An entry with an id outside [0, V) or a t of -inf is none; KL's mean is over
+ * the rows with an entry, CE's over those with a label in [0, V); a part that
+ * no row is in is 0. A row in neither is not read and has a gradient of 0.
+ * labels NULL or alpha 1: no CE; alpha 0: no KL.
+ * logits: element (b, t, v) at p + b sb + t st + v, B T < 2^31 rows, fp32 or
+ * bf16, of any alignment. ids [B T, K] int32 or int64, top [B T, K] fp32 or
+ * bf16, labels [B T]. loss: one float. dlogits (nullable) [B T, V], dense, of
+ * logits' dtype, rounded to nearest; it must not overlap logits. Sums over
+ * rows are in double, in a fixed order. 1e-4 <= temperature <= 1e4.
+ * mg_scale_inplace: x *= *factor (read on the stream) over n values; a factor
+ * of 1 touches nothing. */
+size_t mg_distill_workspace_bytes(int64_t N);
+int mg_distill(int logits_dtype, const mg_seq* logits, int64_t B, int64_t T, int V, int id_bytes, const void* ids,
+               int top_dtype, const void* top, int K, const int64_t* labels, float temperature, float alpha,
+               float* loss, void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+int mg_scale_inplace(int dtype, void* x, int64_t n, const float* factor, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
