@@ -26,7 +26,7 @@ namespace mg {
 namespace distill {
 
 constexpr int kMaxTop = 512;
-constexpr int kCountWgs = 64, kRowWgs = 4096;
+constexpr int kCountRows = 64, kCountWgs = 256, kRowWgs = 4096;
 
 typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
 
@@ -35,54 +35,40 @@ template <typename T> struct Vec;
 template <> struct Vec<bf16_t> {
   static constexpr int kN = 8;
   uint32_t w[4];
-  __device__ __forceinline__ void load(const bf16_t* p, int left) {
-    if (left >= kN) {
-      const u16x8u x = *reinterpret_cast<const u16x8u*>(p);
-      const uint4 y = __builtin_bit_cast(uint4, x);
-      w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t lo = 2 * q < left ? p[2 * q] : 0xff80u, hi = 2 * q + 1 < left ? p[2 * q + 1] : 0xff80u;  // -inf past the row
-        w[q] = lo | hi << 16;
-      }
-    }
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    const uint4 y = __builtin_bit_cast(uint4, *reinterpret_cast<const u16x8u*>(p));
+    w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
   }
+  __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = 0xff80ff80u; }  // -inf
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16); }
-  __device__ __forceinline__ static void store(bf16_t* p, int left, const float (&v)[kN]) {
-    if (left >= kN) {
-      u16x8u x;
+  __device__ __forceinline__ static void store(bf16_t* p, const float (&v)[kN]) {
+    u16x8u x;
 #pragma unroll
-      for (int j = 0; j < kN; ++j) x[j] = f32_to_bf16(v[j]);
-      *reinterpret_cast<u16x8u*>(p) = x;
-    } else {
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (j < left) p[j] = f32_to_bf16(v[j]);
-    }
+    for (int j = 0; j < kN; ++j) x[j] = f32_to_bf16(v[j]);
+    *reinterpret_cast<u16x8u*>(p) = x;
   }
 };
 template <> struct Vec<float> {
   static constexpr int kN = 4;
   float w[4];
-  __device__ __forceinline__ void load(const float* p, int left) {
-    if (left >= kN) {
-      const f32x4u x = *reinterpret_cast<const f32x4u*>(p);
+  __device__ __forceinline__ void load(const float* p) {
+    const f32x4u x = *reinterpret_cast<const f32x4u*>(p);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = x[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = j < left ? p[j] : -INFINITY;
-    }
+    for (int j = 0; j < 4; ++j) w[j] = x[j];
   }
+  __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = -INFINITY; }
   __device__ __forceinline__ float get(int j) const { return w[j]; }
-  __device__ __forceinline__ static void store(float* p, int left, const float (&v)[kN]) {
-    f4 x;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x.v[j] = v[j];
-    store4(p, x, left);
+  __device__ __forceinline__ static void store(float* p, const float (&v)[kN]) {
+    const f32x4u x = {v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4u*>(p) = x;
   }
 };
+// What was computed from v so far is not kept for later: v is all that stays in registers
+template <typename T>
+__device__ __forceinline__ void forget(Vec<T>& v) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(v.w[q]));
+}
 __device__ __forceinline__ float value(const bf16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ float value(const float* p) { return *p; }
 __device__ __forceinline__ void put(bf16_t* p, float v) { *p = f32_to_bf16(v); }
@@ -112,24 +98,42 @@ struct Args {
   __device__ __forceinline__ bool counts_as(int64_t id, float t) const { return inside(id) && t != -INFINITY; }
 };
 
-__global__ __launch_bounds__(256) void count_kernel(Args a) {
-  __shared__ int s[2];
+// Rows that count, kCountRows at a time to a workgroup, a thread per row: its entries by eights, as few as it takes
+__global__ __launch_bounds__(kCountRows) void count_kernel(Args a) {
+  int n1 = 0, n2 = 0;
+  for (int64_t n = static_cast<int64_t>(blockIdx.x) * kCountRows + threadIdx.x; n < a.N; n += static_cast<int64_t>(gridDim.x) * kCountRows) {
+    bool any = !a.soft;
+    for (int k0 = 0; k0 < a.K && !any; k0 += 8) {
+      int64_t id[8];
+      float t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t i = n * a.K + std::min(k0 + j, a.K - 1);
+        id[j] = a.id(i), t[j] = a.teacher(i);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) any |= a.counts_as(id[j], t[j]);
+    }
+    n1 += any;
+    n2 += a.hard && a.inside(a.labels[n]);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n1 += __shfl_xor(n1, o, 64), n2 += __shfl_xor(n2, o, 64);
+  if (threadIdx.x == 0) a.counts[2 * blockIdx.x] = a.soft ? n1 : 0, a.counts[2 * blockIdx.x + 1] = n2;
+}
+
+// (n1, n2) by the first 256 threads of a workgroup; s is cleared, and everyone waits before and after
+__device__ __forceinline__ void all_counts(const Args& a, int (&s)[2]) {
+  const int64_t wgs = (a.N + kCountRows - 1) / kCountRows;
+  const int g = static_cast<int>(std::min<int64_t>(wgs, kCountWgs));
   if (threadIdx.x < 2) s[threadIdx.x] = 0;
   __syncthreads();
-  int n1 = 0, n2 = 0;
-  for (int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; n < a.N; n += static_cast<int64_t>(gridDim.x) * 256) {
-    if (a.soft)
-      for (int k = 0; k < a.K; ++k)
-        if (a.counts_as(a.id(n * a.K + k), a.teacher(n * a.K + k))) {
-          ++n1;
-          break;
-        }
-    if (a.hard && a.inside(a.labels[n])) ++n2;
+  if (threadIdx.x < g) {
+    const int2 c = reinterpret_cast<const int2*>(a.counts)[threadIdx.x];
+    atomicAdd(&s[0], c.x);
+    atomicAdd(&s[1], c.y);
   }
-  atomicAdd(&s[0], n1);
-  atomicAdd(&s[1], n2);
   __syncthreads();
-  if (threadIdx.x < 2) a.counts[2 * blockIdx.x + threadIdx.x] = s[threadIdx.x];
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -172,8 +176,10 @@ __device__ __forceinline__ void all_sum(float (&v)[M], float (&red)[M][NT / 64])
   }
 }
 
-// S vectors of a row to each of NT threads; S = 0: rows of any length, read twice
-template <typename T, int NT, int S>
+// S vectors of a row to each of NT threads, and one of the values behind the last whole vector to the first few;
+// S = 0: rows of any length, read twice. A row that counts for one part alone has a share of 0 of the other's
+// gradient.
+template <typename T, int NT, int S, bool kHard>
 __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
   using V16 = Vec<T>;
   constexpr int kN = V16::kN, kEntries = (kMaxTop + NT - 1) / NT;
@@ -182,14 +188,15 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
   __shared__ int s_count[2], s_id[kMaxTop];
   __shared__ float s_p[kMaxTop];
   const int tid = threadIdx.x;
-  if (tid < 64) {
-    const int g = a.N < kCountWgs * 256 ? static_cast<int>((a.N + 255) / 256) : kCountWgs;
-    int n1 = tid < g ? a.counts[2 * tid] : 0, n2 = tid < g ? a.counts[2 * tid + 1] : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n1 += __shfl_xor(n1, o, 64), n2 += __shfl_xor(n2, o, 64);
-    if (tid == 0) s_count[0] = n1, s_count[1] = n2;
-  }
-  __syncthreads();
+  const int whole = a.V / kN * kN, last = whole + tid;  // (last: this thread's value behind them, if it has one)
+  const uint32_t whole_bytes = static_cast<uint32_t>(whole) * sizeof(T);
+  // a thread's first byte of a row, computed anew wherever it is needed (kept from row to row, the places of all S
+  // vectors take two registers each)
+  const auto here = [](uint32_t t) {
+    asm volatile("" : "+v"(t));
+    return t * 16;
+  };
+  all_counts(a, s_count);
   const float w1 = s_count[0] ? a.alpha * a.temperature / static_cast<float>(s_count[0]) : 0.0f;
   const float w2 = s_count[1] ? (1.0f - a.alpha) / static_cast<float>(s_count[1]) : 0.0f;
   const float k1 = kLog2e / a.temperature, k2 = kLog2e;
@@ -197,12 +204,25 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
   for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
     const T* z = static_cast<const T*>(a.z) + n / a.T * a.sb + n % a.T * a.st;
     T* dz = a.dz ? static_cast<T*>(a.dz) + n * a.V : nullptr;
-    const int64_t label = a.hard ? a.labels[n] : -1;
-    const bool told = a.inside(label);
+    const int64_t label = kHard ? a.labels[n] : -1;
+    const bool told = kHard && a.inside(label);
+    V16 x[S ? S : 1];
+    if constexpr (S > 0) {
+      const uint32_t c0 = here(tid);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint32_t c = c0 + s * (NT * 16);
+        if (c < whole_bytes)
+          x[s].load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(z) + c));
+        else
+          x[s].none();
+      }
+    }
+    const float xl = last < a.V ? value(z + last) : -INFINITY;
     // the teacher's entries of this thread: at `id` the logit `at`, u = log2 of the unnormalised probability
     int id[kEntries];
     float u[kEntries], at[kEntries];
-    float most[3] = {-INFINITY, -INFINITY, 0.0f};  // of the row, of the teacher, whether an entry counts
+    float most[3] = {xl, -INFINITY, 0.0f};  // of the row, of the teacher, whether an entry counts
 #pragma unroll
     for (int i = 0; i < kEntries; ++i) {
       const int k = tid + i * NT;
@@ -217,53 +237,51 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
         }
       }
     }
-    V16 x[S ? S : 1];
-    if constexpr (S > 0) {
+    const float zl = told ? value(z + label) : 0.0f;
+    // f(vector, where it goes) over the row's whole vectors
+    const auto each = [&](auto&& f) {
+      if constexpr (S > 0) {
+        const uint32_t c0 = here(tid);
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int c = (tid + NT * s) * kN;
-        x[s].load(z + c, a.V - c);
+        for (int s = 0; s < S; ++s) {
+          const uint32_t c = c0 + s * (NT * 16);
+          forget(x[s]);
+          f(x[s], c < whole_bytes ? reinterpret_cast<T*>(reinterpret_cast<char*>(dz) + c) : nullptr);
+          __builtin_amdgcn_sched_barrier(0);  // (or the vectors' values are in registers all at once)
+        }
+      } else {
+        for (int c = tid * kN; c < whole; c += NT * kN) {
+          x[0].load(z + c);
+          f(x[0], dz + c);
+        }
       }
+    };
+    each([&](const V16& v, T*) {
 #pragma unroll
-      for (int s = 0; s < S; ++s)
-#pragma unroll
-        for (int j = 0; j < kN; ++j) most[0] = fmaxf(most[0], x[s].get(j));
-    } else {
-      for (int c = tid * kN; c < a.V; c += NT * kN) {
-        x[0].load(z + c, a.V - c);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) most[0] = fmaxf(most[0], x[0].get(j));
-      }
-    }
+      for (int j = 0; j < kN; ++j) most[0] = fmaxf(most[0], v.get(j));
+    });
     all_max<NT>(most, s_redm);
     const bool taught = most[2] != 0.0f;
     if (!taught && !told) {
-      if (dz)
-        for (int c = tid * kN; c < a.V; c += NT * kN) {
-          const float none[kN] = {};
-          V16::store(dz + c, a.V - c, none);
-        }
+      if (dz) {
+        const float none[kN] = {};
+        for (int c = tid * kN; c < whole; c += NT * kN) V16::store(dz + c, none);
+        if (last < a.V) put(dz + last, 0.0f);
+      }
       continue;
     }
     const float zm = most[0];
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of 2^((z - zm) k1), of 2^((z - zm) k2), of the teacher's 2^u, of 2^u (u - log2 of the student's)
-    const auto add = [&](const V16& v) {
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const float d = v.get(j) - zm;
-        if (taught) sum[0] += exp2_raw(d * k1);
-        if (told) sum[1] += exp2_raw(d * k2);
-      }
+    const auto add = [&](float zj) {
+      const float d = zj - zm;
+      sum[0] += exp2_raw(d * k1);
+      if constexpr (kHard) sum[1] += exp2_raw(d * k2);
     };
-    if constexpr (S > 0) {
+    each([&](const V16& v, T*) {
 #pragma unroll
-      for (int s = 0; s < S; ++s) add(x[s]);
-    } else {
-      for (int c = tid * kN; c < a.V; c += NT * kN) {
-        x[0].load(z + c, a.V - c);
-        add(x[0]);
-      }
-    }
+      for (int j = 0; j < kN; ++j) add(v.get(j));
+    });
+    add(xl);
     float p[kEntries];
 #pragma unroll
     for (int i = 0; i < kEntries; ++i) {
@@ -276,55 +294,45 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
       }
     }
     all_sum<NT>(sum, s_red);
-    const float zl = told ? value(z + label) : 0.0f;
     if (tid == 0) {
       if (taught) l1 += kLn2 * (sum[3] / sum[2] - log2f(sum[2]) + log2f(sum[0]));
       if (told) l2 += kLn2 * (log2f(sum[1]) - (zl - zm) * k2);
     }
     if (!dz) continue;
     const float c1 = taught ? w1 / sum[0] : 0.0f, c2 = told ? w2 / sum[1] : 0.0f;
+    const float wp = taught ? w1 / sum[2] : 0.0f;
+    const int entries = a.soft ? a.K : 0;
     const auto slope = [&](float zj) {
-      float d = 0.0f;
-      if (taught) d = c1 * exp2_raw((zj - zm) * k1);
-      if (told) d = __builtin_fmaf(c2, exp2_raw((zj - zm) * k2), d);
+      const float e = zj - zm;
+      float d = c1 * exp2_raw(e * k1);
+      if constexpr (kHard) d = __builtin_fmaf(c2, exp2_raw(e * k2), d);
       return d;
     };
-    const auto write = [&](const V16& v, int c) {
-      float d[kN];
+    each([&](const V16& v, T* to) {
+      if (to) {
+        float d[kN];
 #pragma unroll
-      for (int j = 0; j < kN; ++j) d[j] = slope(v.get(j));
-      V16::store(dz + c, a.V - c, d);
-    };
-    if constexpr (S > 0) {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int c = (tid + NT * s) * kN;
-        if (c < a.V) write(x[s], c);
+        for (int j = 0; j < kN; ++j) d[j] = slope(v.get(j));
+        V16::store(to, d);
       }
-    } else {
-      for (int c = tid * kN; c < a.V; c += NT * kN) {
-        x[0].load(z + c, a.V - c);
-        write(x[0], c);
-      }
-    }
+    });
+    if (last < a.V) put(dz + last, slope(xl));
     // the places of the entries and of the label, after the row
-    const float wp = taught ? w1 / sum[2] : 0.0f;
 #pragma unroll
     for (int i = 0; i < kEntries; ++i)
       if (tid + i * NT < kMaxTop) s_id[tid + i * NT] = id[i], s_p[tid + i * NT] = p[i] * wp;
     __syncthreads();
-    const int entries = a.soft ? a.K : 0;
 #pragma unroll
     for (int i = 0; i < kEntries; ++i) {
       if (id[i] < 0) continue;
-      float d = slope(at[i]) - (told && id[i] == label ? w2 : 0.0f), all = 0.0f;
+      float all = told && id[i] == label ? w2 : 0.0f;
       bool first = true;
       for (int k = 0; k < entries; ++k) {
         const bool same = s_id[k] == id[i];
         all += same ? s_p[k] : 0.0f;
         first &= !(same && k < tid + i * NT);
       }
-      if (first) put(dz + id[i], d - all);
+      if (first) put(dz + id[i], slope(at[i]) - all);
     }
     if (told && tid == NT - 1) {
       bool listed = false;
@@ -335,23 +343,18 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
   if (tid == 0) a.losses[2 * blockIdx.x] = l1, a.losses[2 * blockIdx.x + 1] = l2;
 }
 
-__global__ __launch_bounds__(256) void loss_kernel(Args a, int wgs, float* loss) {
-  __shared__ double s[256][2];
+__global__ __launch_bounds__(1024) void loss_kernel(Args a, int wgs, float* loss) {
+  __shared__ double s[1024][2];
   __shared__ int s_n[2];
   double l1 = 0.0, l2 = 0.0;
-  for (int i = threadIdx.x; i < wgs; i += 256) l1 += a.losses[2 * i], l2 += a.losses[2 * i + 1];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < wgs; i += 1024) l1 += a.losses[2 * i], l2 += a.losses[2 * i + 1];
   s[threadIdx.x][0] = l1, s[threadIdx.x][1] = l2;
-  if (threadIdx.x < 2) {
-    const int g = a.N < kCountWgs * 256 ? static_cast<int>((a.N + 255) / 256) : kCountWgs;
-    int n = 0;
-    for (int i = 0; i < g; ++i) n += a.counts[2 * i + threadIdx.x];
-    s_n[threadIdx.x] = n;
-  }
-  for (int o = 128; o > 0; o >>= 1) {
-    __syncthreads();
+  all_counts(a, s_n);
+  for (int o = 512; o > 0; o >>= 1) {
     if (threadIdx.x < o) s[threadIdx.x][0] += s[threadIdx.x + o][0], s[threadIdx.x][1] += s[threadIdx.x + o][1];
+    __syncthreads();
   }
-  __syncthreads();
   if (threadIdx.x == 0) {
     const double t = a.temperature, al = a.alpha;
     double l = 0.0;
@@ -367,24 +370,25 @@ __global__ __launch_bounds__(256) void scale_kernel(T* x, int64_t n, const float
   using V16 = Vec<T>;
   const float f = *g;
   if (f == 1.0f) return;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V16::kN; i < n; i += static_cast<int64_t>(gridDim.x) * 256 * V16::kN) {
-    const int left = static_cast<int>(std::min<int64_t>(n - i, V16::kN));
+  const int64_t whole = n / V16::kN * V16::kN, t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  for (int64_t i = t * V16::kN; i < whole; i += static_cast<int64_t>(gridDim.x) * 256 * V16::kN) {
     V16 v;
-    v.load(x + i, left);
+    v.load(x + i);
     float d[V16::kN];
 #pragma unroll
     for (int j = 0; j < V16::kN; ++j) d[j] = v.get(j) * f;
-    V16::store(x + i, left, d);
+    V16::store(x + i, d);
   }
+  if (whole + t < n) put(x + whole + t, value(x + whole + t) * f);
 }
 
 inline int row_wgs(int64_t N) { return static_cast<int>(std::min<int64_t>(N, kRowWgs)); }
 
-template <typename T>
+template <typename T, bool kHard>
 void launch_rows(const Args& a, hipStream_t st) {
   const int64_t vecs = (a.V + int64_t(Vec<T>::kN) - 1) / Vec<T>::kN;
   const dim3 grid(row_wgs(a.N));
-#define GO(NT, S) hipLaunchKernelGGL((rows_kernel<T, NT, S>), grid, dim3(NT), 0, st, a)
+#define GO(NT, S) hipLaunchKernelGGL((rows_kernel<T, NT, S, kHard>), grid, dim3(NT), 0, st, a)
   if (vecs <= 256) GO(256, 1);
   else if (vecs <= 512) GO(256, 2);
   else if (vecs <= 1024) GO(256, 4);
@@ -430,12 +434,12 @@ extern "C" int mg_distill(int logits_dtype, const mg_seq* logits, int64_t B, int
             labels && alpha < 1.0f, alpha, temperature, dlogits, static_cast<int*>(workspace),
             reinterpret_cast<double*>(static_cast<char*>(workspace) + kCountWgs * 2 * sizeof(int))};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(count_kernel, dim3(std::min<int64_t>((N + 255) / 256, kCountWgs)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(count_kernel, dim3(std::min<int64_t>((N + kCountRows - 1) / kCountRows, kCountWgs)), dim3(kCountRows), 0, st, a);
   if (logits_dtype == MG_BF16)
-    launch_rows<bf16_t>(a, st);
+    a.hard ? launch_rows<bf16_t, true>(a, st) : launch_rows<bf16_t, false>(a, st);
   else
-    launch_rows<float>(a, st);
-  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, st, a, row_wgs(N), loss);
+    a.hard ? launch_rows<float, true>(a, st) : launch_rows<float, false>(a, st);
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, a, row_wgs(N), loss);
   return check_launch(fn);
 }
 

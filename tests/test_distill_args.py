@@ -37,7 +37,7 @@ def test_arguments():
         assert _call(L, **kw) == DTYPE, kw
     for kw in (dict(ws=None), dict(ws=4100), dict(wsb=16)):
         assert _call(L, **kw) == WORKSPACE, kw
-    assert L.mg_distill_workspace_bytes(20) == 64 * 2 * 4 + 20 * 2 * 8 and L.mg_distill_workspace_bytes(0) == 0
+    assert L.mg_distill_workspace_bytes(20) == 256 * 2 * 4 + 20 * 2 * 8 and L.mg_distill_workspace_bytes(0) == 0
 
 
 def test_scale():
