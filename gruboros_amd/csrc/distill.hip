@@ -15,8 +15,7 @@
 // the type's lowest value.) The few places that an entry or the label changes are
 // written again after the row, by the threads that hold the entries. Losses are summed in double, in a fixed order.
 //
-// A small kernel counts n1 and n2 first (a thread per row, which seldom reads past a row's first entry); the last adds
-// the workgroups' losses.
+// A small kernel counts n1 and n2 first; the last adds the workgroups' losses.
 
 #include <algorithm>
 
@@ -26,48 +25,48 @@ namespace mg {
 namespace distill {
 
 constexpr int kMaxTop = 512;
-constexpr int kCountRows = 64, kCountWgs = 256, kRowWgs = 4096;
+constexpr int kCountRows = 32, kCountWgs = 256, kRowWgs = 3072;
 
+// The teacher's part alone; with the labels': an exponential for each, or, at the temperatures 1, 2 and 4, that of the
+// labels' as a power of the teacher's (e^z = (e^{z/T})^T).
+constexpr int kSoft = 0, kBoth = 1, kT1 = 2, kT2 = 3, kT4 = 4;
+
+constexpr bool ahead(int s) { return s >= 16; }
+
+// Waves per SIMD that a kernel leaves room for
+constexpr int waves_of(int nt, int s) { return s > 0 && s < 16 ? 6 : 4; }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
 
 // 16 bytes of a row as loaded
 template <typename T> struct Vec;
 template <> struct Vec<bf16_t> {
   static constexpr int kN = 8;
-  uint32_t w[4];
-  __device__ __forceinline__ void load(const bf16_t* p) {
-    const uint4 y = __builtin_bit_cast(uint4, *reinterpret_cast<const u16x8u*>(p));
-    w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
-  }
-  __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = 0xff80ff80u; }  // -inf
+  u32x4 w;
+  __device__ __forceinline__ void load(const bf16_t* p) { w = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8u*>(p)); }
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16); }
   __device__ __forceinline__ static void store(bf16_t* p, const float (&v)[kN]) {
     u16x8u x;
 #pragma unroll
     for (int j = 0; j < kN; ++j) x[j] = f32_to_bf16(v[j]);
-    *reinterpret_cast<u16x8u*>(p) = x;
+    __builtin_nontemporal_store(x, reinterpret_cast<u16x8u*>(p));
   }
 };
 template <> struct Vec<float> {
   static constexpr int kN = 4;
-  float w[4];
-  __device__ __forceinline__ void load(const float* p) {
-    const f32x4u x = *reinterpret_cast<const f32x4u*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = x[j];
-  }
-  __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = -INFINITY; }
-  __device__ __forceinline__ float get(int j) const { return w[j]; }
+  u32x4 w;
+  __device__ __forceinline__ void load(const float* p) { w = __builtin_bit_cast(u32x4, *reinterpret_cast<const f32x4u*>(p)); }
+  __device__ __forceinline__ float get(int j) const { return __uint_as_float(w[j]); }
   __device__ __forceinline__ static void store(float* p, const float (&v)[kN]) {
     const f32x4u x = {v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4u*>(p) = x;
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4u*>(p));
   }
 };
 // What was computed from v so far is not kept for later: v is all that stays in registers
 template <typename T>
 __device__ __forceinline__ void forget(Vec<T>& v) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(v.w[q]));
+  asm volatile("" : "+v"(v.w));
 }
 __device__ __forceinline__ float value(const bf16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ float value(const float* p) { return *p; }
@@ -98,72 +97,81 @@ struct Args {
   __device__ __forceinline__ bool counts_as(int64_t id, float t) const { return inside(id) && t != -INFINITY; }
 };
 
-// Rows that count, kCountRows at a time to a workgroup, a thread per row: its entries by eights, as few as it takes
-__global__ __launch_bounds__(kCountRows) void count_kernel(Args a) {
+// Rows that count, kCountRows at a time to a workgroup: eight threads to a row, each reads every eighth entry
+__global__ __launch_bounds__(8 * kCountRows) void count_kernel(Args a) {
+  __shared__ int s[2];
+  if (threadIdx.x < 2) s[threadIdx.x] = 0;
+  __syncthreads();
   int n1 = 0, n2 = 0;
-  for (int64_t n = static_cast<int64_t>(blockIdx.x) * kCountRows + threadIdx.x; n < a.N; n += static_cast<int64_t>(gridDim.x) * kCountRows) {
-    bool any = !a.soft;
-    for (int k0 = 0; k0 < a.K && !any; k0 += 8) {
-      int64_t id[8];
-      float t[8];
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * kCountRows; n0 < a.N; n0 += static_cast<int64_t>(gridDim.x) * kCountRows) {
+    const int64_t n = std::min<int64_t>(n0 + threadIdx.x / 8, a.N - 1);
+    const bool own = n == n0 + threadIdx.x / 8 && threadIdx.x % 8 == 0;
+    bool any = false;
+    if (a.soft)
+      for (int k0 = threadIdx.x % 8; k0 < a.K; k0 += 64) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t i = n * a.K + std::min(k0 + j, a.K - 1);
-        id[j] = a.id(i), t[j] = a.teacher(i);
+        for (int j = 0; j < 8; ++j) {
+          const int64_t i = n * a.K + std::min(k0 + 8 * j, a.K - 1);
+          any |= a.counts_as(a.id(i), a.teacher(i));
+        }
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) any |= a.counts_as(id[j], t[j]);
-    }
-    n1 += any;
-    n2 += a.hard && a.inside(a.labels[n]);
+    const bool row = (__ballot(any) >> (threadIdx.x % 64 / 8 * 8) & 0xff) != 0;
+    n1 += own && row;
+    n2 += own && a.hard && a.inside(a.labels[n]);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) n1 += __shfl_xor(n1, o, 64), n2 += __shfl_xor(n2, o, 64);
-  if (threadIdx.x == 0) a.counts[2 * blockIdx.x] = a.soft ? n1 : 0, a.counts[2 * blockIdx.x + 1] = n2;
+  if (n1) atomicAdd(&s[0], n1);
+  if (n2) atomicAdd(&s[1], n2);
+  __syncthreads();
+  if (threadIdx.x < 2) a.counts[2 * blockIdx.x + threadIdx.x] = s[threadIdx.x];
 }
 
-// (n1, n2) by the first 256 threads of a workgroup; s is cleared, and everyone waits before and after
+// (n1, n2), by a whole workgroup
 __device__ __forceinline__ void all_counts(const Args& a, int (&s)[2]) {
   const int64_t wgs = (a.N + kCountRows - 1) / kCountRows;
   const int g = static_cast<int>(std::min<int64_t>(wgs, kCountWgs));
   if (threadIdx.x < 2) s[threadIdx.x] = 0;
   __syncthreads();
-  if (threadIdx.x < g) {
-    const int2 c = reinterpret_cast<const int2*>(a.counts)[threadIdx.x];
-    atomicAdd(&s[0], c.x);
-    atomicAdd(&s[1], c.y);
-  }
+  int2 c = make_int2(0, 0);
+  for (int i = threadIdx.x; i < g; i += blockDim.x) c.x += a.counts[2 * i], c.y += a.counts[2 * i + 1];
+  atomicAdd(&s[0], c.x);
+  atomicAdd(&s[1], c.y);
   __syncthreads();
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+// The largest of a wave's lanes, in every lane (as wave_sum; a lane without a partner keeps its own)
+__device__ __forceinline__ float wave_max(float x) {
+  const auto most = [](float x, auto ctrl, auto rows) {
+    const int y = __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    return fmaxf(x, __int_as_float(y));
+  };
+  x = most(x, int_c<0xb1>{}, int_c<0xf>{});
+  x = most(x, int_c<0x4e>{}, int_c<0xf>{});
+  x = most(x, int_c<0x141>{}, int_c<0xf>{});
+  x = most(x, int_c<0x140>{}, int_c<0xf>{});
+  x = most(x, int_c<0x142>{}, int_c<0xa>{});
+  x = most(x, int_c<0x143>{}, int_c<0xc>{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// Over the NT threads of a workgroup; every thread gets them
-template <int NT, int M>
-__device__ __forceinline__ void all_max(float (&v)[M], float (&red)[M][NT / 64]) {
-#pragma unroll
-  for (int i = 0; i < M; ++i) v[i] = wave_max(v[i]);
+// Over the NT threads of a workgroup; every thread gets them. One wait each: a second use of the same `red` has to come
+// after another wait of the workgroup.
+// A value that is the same in all lanes, in a scalar register
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+
+template <int NT>
+__device__ __forceinline__ float all_max(float v, float (&red)[NT / 64]) {
+  v = wave_max(v);
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
   __syncthreads();
-  if (threadIdx.x % 64 == 0)
+  v = red[0];
 #pragma unroll
-    for (int i = 0; i < M; ++i) red[i][threadIdx.x / 64] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < M; ++i) {
-    v[i] = red[i][0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v[i] = fmaxf(v[i], red[i][w]);
-  }
+  for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
+  return uniform(v);
 }
 template <int NT, int M>
 __device__ __forceinline__ void all_sum(float (&v)[M], float (&red)[M][NT / 64]) {
 #pragma unroll
   for (int i = 0; i < M; ++i) v[i] = wave_sum(v[i]);
-  __syncthreads();
   if (threadIdx.x % 64 == 0)
 #pragma unroll
     for (int i = 0; i < M; ++i) red[i][threadIdx.x / 64] = v[i];
@@ -173,20 +181,31 @@ __device__ __forceinline__ void all_sum(float (&v)[M], float (&red)[M][NT / 64])
     v[i] = 0.0f;
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) v[i] += red[i][w];
+    v[i] = uniform(v[i]);
   }
 }
 
 // S vectors of a row to each of NT threads, and one of the values behind the last whole vector to the first few;
 // S = 0: rows of any length, read twice. A row that counts for one part alone has a share of 0 of the other's
 // gradient.
-template <typename T, int NT, int S, bool kHard>
-__global__ __launch_bounds__(NT) void rows_kernel(Args a) {
+// After a row's gradient (where a row has 16 vectors to a thread and few workgroups share a CU: while it is written,
+// each vector's registers in turn) the next row is loaded, and its entries before that, so that a row begins with all
+// of its loads under way; what is loaded early stays as it comes until it is needed, or the wait for it would come
+// early too. The last row's successor is itself (its first vectors, for all S). What the entries are made into waits
+// in LDS. Up to 64 entries are the first wave's business alone.
+template <typename T, int NT, int S, int kMode>
+__global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
+  constexpr bool kHard = kMode != kSoft, kAhead = ahead(S);
   using V16 = Vec<T>;
   constexpr int kN = V16::kN, kEntries = (kMaxTop + NT - 1) / NT;
   constexpr float kLn2 = 0.6931471805599453f;
-  __shared__ float s_red[4][NT / 64], s_redm[3][NT / 64];
-  __shared__ int s_count[2], s_id[kMaxTop];
-  __shared__ float s_p[kMaxTop];
+  __shared__ float s_max[NT / 64], s_teacher[NT / 64], s_sum[kHard ? 2 : 1][NT / 64], s_teach[2][NT / 64];
+  __shared__ int s_count[2], s_any[NT / 64], s_mine[NT / 64];
+  __shared__ double s_loss[2];
+  // of the entries: id (-1: none), unnormalised probability; of those that are the first of their id the place (else
+  // -1), the logit there and what the gradient there has beyond the student's
+  __shared__ int s_id[kMaxTop], s_place[kMaxTop];
+  __shared__ float s_p[kMaxTop], s_at[kMaxTop], s_put[kMaxTop];
   const int tid = threadIdx.x;
   const int whole = a.V / kN * kN, last = whole + tid;  // (last: this thread's value behind them, if it has one)
   const uint32_t whole_bytes = static_cast<uint32_t>(whole) * sizeof(T);
@@ -196,170 +215,271 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args a) {
     asm volatile("" : "+v"(t));
     return t * 16;
   };
+  const auto at_byte = [](auto* p, uint32_t c) {
+    using C = std::conditional_t<std::is_const_v<std::remove_pointer_t<decltype(p)>>, const char, char>;
+    return reinterpret_cast<decltype(p)>(reinterpret_cast<C*>(p) + c);
+  };
+  const auto row_of = [&](int64_t b, int64_t t) { return static_cast<const T*>(a.z) + b * a.sb + t * a.st; };
+  const int entries = a.soft ? a.K : 0;
+  const bool narrow = a.K <= 64;
   all_counts(a, s_count);
-  const float w1 = s_count[0] ? a.alpha * a.temperature / static_cast<float>(s_count[0]) : 0.0f;
-  const float w2 = s_count[1] ? (1.0f - a.alpha) / static_cast<float>(s_count[1]) : 0.0f;
-  const float k1 = kLog2e / a.temperature, k2 = kLog2e;
-  double l1 = 0.0, l2 = 0.0;
-  for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
-    const T* z = static_cast<const T*>(a.z) + n / a.T * a.sb + n % a.T * a.st;
-    T* dz = a.dz ? static_cast<T*>(a.dz) + n * a.V : nullptr;
-    const int64_t label = kHard ? a.labels[n] : -1;
-    const bool told = kHard && a.inside(label);
-    V16 x[S ? S : 1];
+  const float w1 = uniform(s_count[0] ? a.alpha * a.temperature / static_cast<float>(s_count[0]) : 0.0f);
+  const float w2 = uniform(s_count[1] ? (1.0f - a.alpha) / static_cast<float>(s_count[1]) : 0.0f);
+  const float k1 = uniform(kLog2e / a.temperature), k2 = kLog2e;
+  if (tid < 2) s_loss[tid] = 0.0;  // (the first thread's)
+
+  V16 x[S ? S : 1];
+  // this thread's entries, as loaded, then their ids; the logits there, at the label (-1: none) and behind the vectors
+  uint32_t raw_lo[kEntries], raw_hi[kEntries], raw_t[kEntries];
+  int id[kEntries], label = -1;
+  T at[kEntries], zl, xl;
+  int64_t raw_label = -1;
+  bool twice;  // an id of this wave's entries may be listed twice
+  const auto fetch_entries = [&](int64_t n) {
+    if (entries) {
+#pragma unroll
+      for (int i = 0; i < kEntries; ++i) {
+        const int64_t k = n * a.K + std::min(tid + i * NT, entries - 1);
+        if (a.wide) {
+          const uint2 v = static_cast<const uint2*>(a.ids)[k];
+          raw_lo[i] = v.x, raw_hi[i] = v.y;
+        } else {
+          raw_lo[i] = static_cast<const uint32_t*>(a.ids)[k];
+        }
+        raw_t[i] = a.top_bf16 ? static_cast<const uint16_t*>(a.top)[k] : static_cast<const uint32_t*>(a.top)[k];
+      }
+    }
+    if (kHard) raw_label = a.labels[n];
+  };
+  const auto teacher = [&](int i) { return __uint_as_float(a.top_bf16 ? raw_t[i] << 16 : raw_t[i]); };
+  const auto fetch_places = [&](const T* z) {
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      id[i] = -1;
+      if (tid + i * NT < entries) {
+        const int64_t v = a.wide ? static_cast<int64_t>(static_cast<uint64_t>(raw_hi[i]) << 32 | raw_lo[i]) : static_cast<int32_t>(raw_lo[i]);
+        if (a.counts_as(v, teacher(i))) id[i] = static_cast<int>(v);
+      }
+      at[i] = z[std::max(id[i], 0)];
+    }
+    if (kHard) {
+      label = a.inside(raw_label) ? static_cast<int>(raw_label) : -1;
+      zl = z[std::max(label, 0)];
+    }
+    xl = z[std::min(last, a.V - 1)];
+    twice = !narrow;
+    if (narrow && tid < 64) {  // (while the loads are under way; every entry that is none differs from all)
+      const int own = id[0] >= 0 ? id[0] : -1 - tid;
+      uint64_t same = 0;
+      for (int k = 0; k < entries; ++k) {
+        const uint64_t m = __ballot(own == __builtin_amdgcn_readlane(own, k));
+        same |= m & (m - 1);
+      }
+      twice = same != 0;
+    }
+  };
+  // a vector that the row does not have is its last one
+  const auto fetch = [&](V16& v, const T* z, uint32_t c) { v.load(at_byte(z, std::min(c, whole_bytes - 16))); };
+  int64_t row_b = blockIdx.x / a.T, row_t = blockIdx.x % a.T;
+  const int64_t next_b = gridDim.x / a.T, next_t = gridDim.x % a.T;
+  const T* z = row_of(row_b, row_t);
+  const auto fetch_row = [&](const T* z, uint32_t step) {
     if constexpr (S > 0) {
       const uint32_t c0 = here(tid);
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const uint32_t c = c0 + s * (NT * 16);
-        if (c < whole_bytes)
-          x[s].load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(z) + c));
-        else
-          x[s].none();
-      }
+      for (int s = 0; s < S; ++s) fetch(x[s], z, c0 + s * step);
     }
-    const float xl = last < a.V ? value(z + last) : -INFINITY;
-    // the teacher's entries of this thread: at `id` the logit `at`, u = log2 of the unnormalised probability
-    int id[kEntries];
-    float u[kEntries], at[kEntries];
-    float most[3] = {xl, -INFINITY, 0.0f};  // of the row, of the teacher, whether an entry counts
-#pragma unroll
-    for (int i = 0; i < kEntries; ++i) {
-      const int k = tid + i * NT;
-      id[i] = -1, u[i] = 0.0f, at[i] = 0.0f;
-      if (a.soft && k < a.K) {
-        const int64_t v = a.id(n * a.K + k);
-        const float t = a.teacher(n * a.K + k);
-        if (a.counts_as(v, t)) {
-          id[i] = static_cast<int>(v), u[i] = t * k1, most[2] = 1.0f;
-          most[1] = fmaxf(most[1], u[i]);
-          at[i] = value(z + v);
-        }
-      }
+  };
+  fetch_entries(blockIdx.x);
+  fetch_row(z, NT * 16);
+  fetch_places(z);
+  for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
+    T* dz = a.dz ? static_cast<T*>(a.dz) + n * a.V : nullptr;
+    const bool more_rows = n + gridDim.x < a.N, told = kHard && label >= 0;
+    const int64_t n_next = more_rows ? n + gridDim.x : n;
+    if (more_rows) {
+      row_b += next_b, row_t += next_t;
+      if (row_t >= a.T) row_t -= a.T, ++row_b;
     }
-    const float zl = told ? value(z + label) : 0.0f;
-    // f(vector, where it goes) over the row's whole vectors
-    const auto each = [&](auto&& f) {
+    const T* z_next = row_of(row_b, row_t);
+    const uint32_t step = more_rows ? NT * 16 : 0;
+    // f(vector, its first byte) over the row's whole vectors; `then`: after each of the S, with its number
+    const auto each = [&](auto&& f, auto&& then) {
       if constexpr (S > 0) {
         const uint32_t c0 = here(tid);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           const uint32_t c = c0 + s * (NT * 16);
           forget(x[s]);
-          f(x[s], c < whole_bytes ? reinterpret_cast<T*>(reinterpret_cast<char*>(dz) + c) : nullptr);
+          if (c < whole_bytes) f(x[s], c);
+          then(x[s], c0, s);
           __builtin_amdgcn_sched_barrier(0);  // (or the vectors' values are in registers all at once)
         }
       } else {
         for (int c = tid * kN; c < whole; c += NT * kN) {
           x[0].load(z + c);
-          f(x[0], dz + c);
+          f(x[0], static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)));
         }
       }
     };
-    each([&](const V16& v, T*) {
+    const auto nothing = [](V16&, uint32_t, int) {};
+
+    float zm = -INFINITY, tm = -INFINITY;
+    bool any = false;
 #pragma unroll
-      for (int j = 0; j < kN; ++j) most[0] = fmaxf(most[0], v.get(j));
-    });
-    all_max<NT>(most, s_redm);
-    const bool taught = most[2] != 0.0f;
-    if (!taught && !told) {
-      if (dz) {
-        const float none[kN] = {};
-        for (int c = tid * kN; c < whole; c += NT * kN) V16::store(dz + c, none);
-        if (last < a.V) put(dz + last, 0.0f);
-      }
-      continue;
+    for (int i = 0; i < kEntries; ++i) {
+      if (id[i] >= 0) tm = fmaxf(tm, teacher(i) * k1), any = true;
+      if (tid + i * NT < entries) s_id[tid + i * NT] = id[i];
     }
-    const float zm = most[0];
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of 2^((z - zm) k1), of 2^((z - zm) k2), of the teacher's 2^u, of 2^u (u - log2 of the student's)
-    const auto add = [&](float zj) {
+    each([&](const V16& v, uint32_t) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) zm = fmaxf(zm, v.get(j));
+    }, nothing);
+    const float behind = last < a.V ? value(&xl) : -INFINITY;
+    zm = fmaxf(zm, behind);
+    if (const int one = __any(any); tid % 64 == 0) s_any[tid / 64] = one;
+    zm = all_max<NT>(zm, s_max);
+    bool taught = false;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) taught |= s_any[w] != 0;
+    tm = narrow ? wave_max(tm) : all_max<NT>(tm, s_teacher);
+
+    // the teacher's distribution: the sums of 2^u and of 2^u (u - log2 of the student's)
+    float teach[2] = {};
+    bool mine = false;  // the label is one of this thread's entries
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      const int k = tid + i * NT;
+      if (k >= entries) continue;
+      float p = 0.0f;
+      if (id[i] >= 0) {
+        const float u = teacher(i) * k1 - tm, zk = value(&at[i]);
+        p = exp2_raw(u);
+        teach[0] += p;
+        if (p != 0.0f) teach[1] += p * (u - (zk - zm) * k1);
+        s_at[k] = zk;
+        mine |= told && id[i] == label;
+      }
+      s_p[k] = p;
+    }
+    if constexpr (kHard)
+      if (const int one = __any(mine); tid % 64 == 0) s_mine[tid / 64] = one;
+    if (narrow)
+      teach[0] = uniform(wave_sum(teach[0])), teach[1] = uniform(wave_sum(teach[1]));
+    else
+      all_sum<NT>(teach, s_teach);
+    const float wp = taught ? w1 / teach[0] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      const int k = tid + i * NT;
+      if (k >= entries) continue;
+      bool first = id[i] >= 0;
+      float all = s_p[k];
+      if (twice && first) {
+        all = 0.0f;
+#pragma unroll 8
+        for (int j = 0; j < entries; ++j) {
+          const bool same = s_id[j] == id[i];
+          first &= !(same && j < k);
+          all += same ? s_p[j] : 0.0f;
+        }
+      }
+      s_place[k] = first ? id[i] : -1;
+      s_put[k] = -wp * all - (told && id[i] == label ? w2 : 0.0f);
+    }
+
+    // 2^((z - zm) k1) and 2^((z - zm) k2) of a logit
+    const auto powers = [&](float zj, float& e1, float& e2) {
       const float d = zj - zm;
-      sum[0] += exp2_raw(d * k1);
-      if constexpr (kHard) sum[1] += exp2_raw(d * k2);
+      e1 = exp2_raw(d * k1);
+      if constexpr (kMode == kBoth) e2 = exp2_raw(d * k2);
+      if constexpr (kMode == kT1) e2 = e1;
+      if constexpr (kMode == kT2) e2 = e1 * e1;
+      if constexpr (kMode == kT4) e2 = (e1 * e1) * (e1 * e1);
     };
-    each([&](const V16& v, T*) {
+    float sum[kHard ? 2 : 1] = {};
+    const auto add = [&](float zj) {
+      float e1, e2;
+      powers(zj, e1, e2);
+      sum[0] += e1;
+      if constexpr (kHard) sum[1] += e2;
+    };
+    each([&](const V16& v, uint32_t) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) add(v.get(j));
-    });
-    add(xl);
-    float p[kEntries];
-#pragma unroll
-    for (int i = 0; i < kEntries; ++i) {
-      p[i] = 0.0f;
-      if (id[i] >= 0) {
-        u[i] -= most[1];
-        p[i] = exp2_raw(u[i]);
-        sum[2] += p[i];
-        if (p[i] != 0.0f) sum[3] += p[i] * (u[i] - (at[i] - zm) * k1);
-      }
-    }
-    all_sum<NT>(sum, s_red);
-    if (tid == 0) {
-      if (taught) l1 += kLn2 * (sum[3] / sum[2] - log2f(sum[2]) + log2f(sum[0]));
-      if (told) l2 += kLn2 * (log2f(sum[1]) - (zl - zm) * k2);
-    }
-    if (!dz) continue;
-    const float c1 = taught ? w1 / sum[0] : 0.0f, c2 = told ? w2 / sum[1] : 0.0f;
-    const float wp = taught ? w1 / sum[2] : 0.0f;
-    const int entries = a.soft ? a.K : 0;
+    }, nothing);
+    if (last < a.V) add(behind);
+    all_sum<NT>(sum, s_sum);
+    const float c1 = uniform(taught ? w1 / sum[0] : 0.0f), c2 = uniform(told ? w2 / sum[kHard ? 1 : 0] : 0.0f);
+    const bool counted = taught || told;
     const auto slope = [&](float zj) {
-      const float e = zj - zm;
-      float d = c1 * exp2_raw(e * k1);
-      if constexpr (kHard) d = __builtin_fmaf(c2, exp2_raw(e * k2), d);
-      return d;
+      float e1, e2;
+      powers(zj, e1, e2);
+      e1 *= c1;
+      if constexpr (kHard) e1 = __builtin_fmaf(c2, e2, e1);
+      return e1;
     };
-    each([&](const V16& v, T* to) {
-      if (to) {
-        float d[kN];
+    float label_put = 0.0f;
+    bool label_own = false;  // the label's place is this thread's to write: it is listed nowhere
+    if constexpr (kHard) {
+      const float zk = value(&zl);
+      bool listed = false;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) listed |= s_mine[w] != 0;
+      label_own = told && !listed && tid == NT - 1;
+      label_put = slope(zk) - w2;
+      if (tid == 0 && told) s_loss[1] += kLn2 * (__builtin_amdgcn_logf(sum[kHard ? 1 : 0]) - (zk - zm) * k2);
+    }
+    if (tid == 0 && taught) s_loss[0] += kLn2 * (teach[1] / teach[0] - __builtin_amdgcn_logf(teach[0]) + __builtin_amdgcn_logf(sum[0]));
+    if (dz && last < a.V) put(dz + last, counted ? slope(behind) : 0.0f);
+    const int label_place = label;
+    fetch_entries(n_next);
+    each([&](const V16& v, uint32_t c) {
+      if (!dz) return;
+      float d[kN] = {};  // (a row that does not count may hold anything: nothing is made of it)
+      if (counted) {
 #pragma unroll
         for (int j = 0; j < kN; ++j) d[j] = slope(v.get(j));
-        V16::store(to, d);
       }
+      V16::store(at_byte(dz, c), d);
+    }, [&](V16& v, uint32_t c0, int s) {
+      if constexpr (kAhead) fetch(v, z_next, c0 + s * step);
     });
-    if (last < a.V) put(dz + last, slope(xl));
-    // the places of the entries and of the label, after the row
+    if constexpr (!kAhead) fetch_row(z_next, step);
+    fetch_places(z_next);
+    __syncthreads();  // the row, and what lies behind its vectors, then its places
+    if (dz) {
 #pragma unroll
-    for (int i = 0; i < kEntries; ++i)
-      if (tid + i * NT < kMaxTop) s_id[tid + i * NT] = id[i], s_p[tid + i * NT] = p[i] * wp;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kEntries; ++i) {
-      if (id[i] < 0) continue;
-      float all = told && id[i] == label ? w2 : 0.0f;
-      bool first = true;
-      for (int k = 0; k < entries; ++k) {
-        const bool same = s_id[k] == id[i];
-        all += same ? s_p[k] : 0.0f;
-        first &= !(same && k < tid + i * NT);
+      for (int i = 0; i < kEntries; ++i) {
+        const int k = tid + i * NT;
+        if (k < entries && s_place[k] >= 0) put(dz + s_place[k], slope(s_at[k]) + s_put[k]);
       }
-      if (first) put(dz + id[i], slope(at[i]) - all);
+      if (label_own) put(dz + label_place, label_put);
     }
-    if (told && tid == NT - 1) {
-      bool listed = false;
-      for (int k = 0; k < entries; ++k) listed |= s_id[k] == label;
-      if (!listed) put(dz + label, slope(zl) - w2);
-    }
+    z = z_next;
   }
-  if (tid == 0) a.losses[2 * blockIdx.x] = l1, a.losses[2 * blockIdx.x + 1] = l2;
+  if (tid == 0) a.losses[2 * blockIdx.x] = s_loss[0], a.losses[2 * blockIdx.x + 1] = s_loss[1];
 }
 
-__global__ __launch_bounds__(1024) void loss_kernel(Args a, int wgs, float* loss) {
-  __shared__ double s[1024][2];
+__global__ __launch_bounds__(256) void loss_kernel(Args a, int wgs, float* loss) {
+  __shared__ double s[4][2];
   __shared__ int s_n[2];
   double l1 = 0.0, l2 = 0.0;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < wgs; i += 1024) l1 += a.losses[2 * i], l2 += a.losses[2 * i + 1];
-  s[threadIdx.x][0] = l1, s[threadIdx.x][1] = l2;
-  all_counts(a, s_n);
-  for (int o = 512; o > 0; o >>= 1) {
-    if (threadIdx.x < o) s[threadIdx.x][0] += s[threadIdx.x + o][0], s[threadIdx.x][1] += s[threadIdx.x + o][1];
-    __syncthreads();
+  for (int i = threadIdx.x; i < wgs; i += 256) {
+    const double2 l = reinterpret_cast<const double2*>(a.losses)[i];
+    l1 += l.x, l2 += l.y;
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l1 += __shfl_xor(l1, o, 64), l2 += __shfl_xor(l2, o, 64);
+  if (threadIdx.x % 64 == 0) s[threadIdx.x / 64][0] = l1, s[threadIdx.x / 64][1] = l2;
+  all_counts(a, s_n);  // (and waits)
   if (threadIdx.x == 0) {
     const double t = a.temperature, al = a.alpha;
+    l1 = (s[0][0] + s[1][0]) + (s[2][0] + s[3][0]), l2 = (s[0][1] + s[1][1]) + (s[2][1] + s[3][1]);
     double l = 0.0;
-    if (s_n[0]) l += al * t * t * s[0][0] / s_n[0];
-    if (s_n[1]) l += (1.0 - al) * s[0][1] / s_n[1];
+    if (s_n[0]) l += al * t * t * l1 / s_n[0];
+    if (s_n[1]) l += (1.0 - al) * l2 / s_n[1];
     *loss = static_cast<float>(l);
   }
 }
@@ -382,22 +502,40 @@ __global__ __launch_bounds__(256) void scale_kernel(T* x, int64_t n, const float
   if (whole + t < n) put(x + whole + t, value(x + whole + t) * f);
 }
 
-inline int row_wgs(int64_t N) { return static_cast<int>(std::min<int64_t>(N, kRowWgs)); }
+// As many workgroups as the device holds at once: 256 CUs of four SIMDs
+constexpr int wgs_of(int nt, int s) { return 256 * 4 * 64 * waves_of(nt, s) / nt; }
+inline int row_wgs(int64_t N, int most) { return static_cast<int>(std::min<int64_t>(N, most)); }
 
-template <typename T, bool kHard>
-void launch_rows(const Args& a, hipStream_t st) {
-  const int64_t vecs = (a.V + int64_t(Vec<T>::kN) - 1) / Vec<T>::kN;
-  const dim3 grid(row_wgs(a.N));
-#define GO(NT, S) hipLaunchKernelGGL((rows_kernel<T, NT, S, kHard>), grid, dim3(NT), 0, st, a)
-  if (vecs <= 256) GO(256, 1);
-  else if (vecs <= 512) GO(256, 2);
-  else if (vecs <= 1024) GO(256, 4);
-  else if (vecs <= 2048) GO(256, 8);
-  else if (vecs <= 4096) GO(512, 8);
-  else if (vecs <= 8192) GO(1024, 8);
-  else if (vecs <= 16384) GO(1024, 16);
-  else GO(1024, 0);
+// Few threads and many vectors to each: a row costs each of its waves about the same beyond its vectors (sums over the
+// workgroup, entries). Returns the workgroups
+template <typename T, int kMode>
+int launch_rows(const Args& a, hipStream_t st) {
+  const int64_t vecs = a.V / Vec<T>::kN;
+  int wgs;
+#define GO(NT, S)                                                                            \
+  {                                                                                          \
+    wgs = row_wgs(a.N, wgs_of(NT, S));                                                       \
+    hipLaunchKernelGGL((rows_kernel<T, NT, S, kMode>), dim3(wgs), dim3(NT), 0, st, a);       \
+  }
+  if (vecs == 0) GO(128, 0)
+  else if (vecs <= 512) GO(128, 4)
+  else if (vecs <= 1024) GO(128, 8)
+  else if (vecs <= 2048) GO(256, 8)
+  else if (vecs <= 4096) GO(512, 8)
+  else if (vecs <= 8192) GO(512, 16)
+  else if (vecs <= 16384) GO(1024, 16)
+  else GO(1024, 0)
 #undef GO
+  return wgs;
+}
+
+template <typename T>
+int launch_modes(const Args& a, hipStream_t st) {
+  if (!a.hard) return launch_rows<T, kSoft>(a, st);
+  if (a.temperature == 1.0f) return launch_rows<T, kT1>(a, st);
+  if (a.temperature == 2.0f) return launch_rows<T, kT2>(a, st);
+  if (a.temperature == 4.0f) return launch_rows<T, kT4>(a, st);
+  return launch_rows<T, kBoth>(a, st);
 }
 
 }  // namespace distill
@@ -406,7 +544,7 @@ void launch_rows(const Args& a, hipStream_t st) {
 using namespace mg;
 
 extern "C" size_t mg_distill_workspace_bytes(int64_t N) {
-  return N < 1 ? 0 : distill::kCountWgs * 2 * sizeof(int) + static_cast<size_t>(distill::row_wgs(N)) * 2 * sizeof(double);
+  return N < 1 ? 0 : distill::kCountWgs * 2 * sizeof(int) + static_cast<size_t>(distill::row_wgs(N, distill::kRowWgs)) * 2 * sizeof(double);
 }
 
 extern "C" int mg_distill(int logits_dtype, const mg_seq* logits, int64_t B, int64_t T, int V, int id_bytes, const void* ids, int top_dtype,
@@ -434,12 +572,9 @@ extern "C" int mg_distill(int logits_dtype, const mg_seq* logits, int64_t B, int
             labels && alpha < 1.0f, alpha, temperature, dlogits, static_cast<int*>(workspace),
             reinterpret_cast<double*>(static_cast<char*>(workspace) + kCountWgs * 2 * sizeof(int))};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(count_kernel, dim3(std::min<int64_t>((N + kCountRows - 1) / kCountRows, kCountWgs)), dim3(kCountRows), 0, st, a);
-  if (logits_dtype == MG_BF16)
-    a.hard ? launch_rows<bf16_t, true>(a, st) : launch_rows<bf16_t, false>(a, st);
-  else
-    a.hard ? launch_rows<float, true>(a, st) : launch_rows<float, false>(a, st);
-  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, a, row_wgs(N), loss);
+  hipLaunchKernelGGL(count_kernel, dim3(std::min<int64_t>((N + kCountRows - 1) / kCountRows, kCountWgs)), dim3(8 * kCountRows), 0, st, a);
+  const int wgs = logits_dtype == MG_BF16 ? launch_modes<bf16_t>(a, st) : launch_modes<float>(a, st);
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, st, a, wgs, loss);
   return check_launch(fn);
 }
 
