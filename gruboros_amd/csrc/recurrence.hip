@@ -36,7 +36,25 @@ constexpr int kThreads = kLanes * kRuns;
 constexpr int kKeep = 8;             // steps between the states kept
 constexpr int kFwdRows = 8, kBwdRows = 4;
 constexpr uint32_t kMaxPolls = 1u << 22;
-static_assert(kFwdRows == kKeep && 2 * kBwdRows == kKeep, "runs and kept states");
+// the last cache: operands beyond it are loaded past the caches (B2 T16381 D2048 forward 138 -> 130 us, backward 288 ->
+// 266; B8 T2047 D1024, which it holds, 43 -> 47, 68 -> 76)
+constexpr size_t kCacheBytes = size_t(256) << 20;
+static_assert(kKeep % kFwdRows == 0 && 2 * kBwdRows == kKeep, "runs and kept states");
+
+// Results are read by other kernels, and by then from the next cache: past this one
+template <typename T>
+__device__ __forceinline__ void store4_nt(T* p, const f4& v, int left) {
+  if (left < kVec) return store4(p, v, left);
+  if constexpr (sizeof(T) == 2) {
+    u16x4u x;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x[j] = f32_to_bf16(v.v[j]);
+    __builtin_nontemporal_store(x, reinterpret_cast<u16x4u*>(p));
+  } else {
+    const f32x4u x = {v.v[0], v.v[1], v.v[2], v.v[3]};
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4u*>(p));
+  }
+}
 
 struct Seq {
   const void* p;
@@ -54,9 +72,13 @@ struct Grid {
 template <typename T> struct Raw;
 template <> struct Raw<bf16_t> {
   uint2 r;
+  template <bool kOnce>
   __device__ __forceinline__ void load(const bf16_t* p) {
-    const u16x4u x = *reinterpret_cast<const u16x4u*>(p);
-    r = __builtin_bit_cast(uint2, x);
+    const u16x4u* v = reinterpret_cast<const u16x4u*>(p);
+    if constexpr (kOnce)
+      r = __builtin_bit_cast(uint2, __builtin_nontemporal_load(v));
+    else
+      r = __builtin_bit_cast(uint2, *v);
   }
   __device__ __forceinline__ void load(const bf16_t* p, int left) {
     uint32_t v[4] = {0, 0, 0, 0};
@@ -72,9 +94,13 @@ template <> struct Raw<bf16_t> {
 };
 template <> struct Raw<float> {
   float4 r;
+  template <bool kOnce>
   __device__ __forceinline__ void load(const float* p) {
-    const f32x4u x = *reinterpret_cast<const f32x4u*>(p);
-    r = make_float4(x[0], x[1], x[2], x[3]);
+    const f32x4u* v = reinterpret_cast<const f32x4u*>(p);
+    if constexpr (kOnce)
+      r = __builtin_bit_cast(float4, __builtin_nontemporal_load(v));
+    else
+      r = __builtin_bit_cast(float4, *v);
   }
   __device__ __forceinline__ void load(const float* p, int left) {
     const f4 x = load4(p, left);
@@ -83,16 +109,34 @@ template <> struct Raw<float> {
   __device__ __forceinline__ float get(int j) const { return j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w; }
 };
 
-// kRows rows of four channels; those past the sequence or the last channel are zero
-template <typename T, int kRows>
+// kRows rows of four channels; those past the sequence or the last channel are zero. kOnce: without a place in the
+// caches, for operands that are larger than those.
+template <bool kOnce, typename T, int kRows>
 __device__ __forceinline__ void load_rows(const T* p, int st, int rows, int left, Raw<T> (&v)[kRows]) {
   if (rows >= kRows && left >= kVec) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) v[i].load(p + i * st);
+    for (int i = 0; i < kRows; ++i) v[i].template load<kOnce>(p + i * st);
   } else {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) v[i].load(p + i * st, i < rows ? left : 0);
   }
+}
+
+// Bit i: a sequence starts at the i-th of kRows steps from p on, `rows` of which exist
+template <int kRows>
+__device__ __forceinline__ uint32_t starts(const uint8_t* p, int rows) {
+  typedef uint8_t u8s __attribute__((ext_vector_type(kRows), aligned(1)));
+  uint32_t bits = 0;
+  if (rows >= kRows) {
+    const u8s v = *reinterpret_cast<const u8s*>(p);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) bits |= v[i] ? 1u << i : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (i < rows && p[i]) bits |= 1u << i;
+  }
+  return bits;
 }
 
 // ------------------------------------------------------------------ a step's terms
@@ -172,31 +216,59 @@ __device__ __forceinline__ int take_tile(const Grid& g, uint32_t* tickets, uint3
 // What enters tile k of channel c: back (step -1) or on (+1) to the nearest tile whose result is known, then through
 // the maps of those between, in their order. A map becomes a result as this would compute it, so the carry does not
 // depend on which of the two was seen. `end` always gives a result.
+// Words are read four at a time: one at a time the walk over the tiles that run at once takes longer than their work.
 template <bool kReset>
 __device__ __forceinline__ float look_back(const uint64_t* words, int64_t BD, int k, int step, int end) {
+  constexpr int kAt = 4;
+  const auto read = [&](int first, int last, uint64_t (&x)[kAt]) {  // first, first + step, ..., none past `last`
+#pragma unroll
+    for (int q = 0; q < kAt; ++q) {
+      const int i = first + q * step;
+      x[q] = poll_word(words + (step < 0 ? std::max(i, last) : std::min(i, last)) * BD);
+    }
+  };
+  const auto value = [](uint64_t x) { return __uint_as_float(static_cast<uint32_t>(x >> 32)); };
   int j = k + step;
   uint32_t polls = 0;
-  float carry;
-  while (true) {
-    const uint64_t x = poll_word(words + j * BD);
-    const uint32_t tag = static_cast<uint32_t>(x);
-    if (tag == kTagIncl) {
-      carry = __uint_as_float(static_cast<uint32_t>(x >> 32));
-      break;
+  float carry = 0.0f;
+  for (bool found = false; !found;) {
+    uint64_t x[kAt];
+    read(j, end, x);
+    bool ready = true;
+#pragma unroll
+    for (int q = 0; q < kAt; ++q) {
+      if (!ready || found) continue;
+      const uint32_t tag = static_cast<uint32_t>(x[q]);
+      if (tag == kTagIncl) {
+        carry = value(x[q]);
+        found = true;
+      } else if (j != end && (tag & kTagAggBit)) {
+        j += step;
+        polls = 0;
+      } else {
+        ready = false;
+      }
     }
-    if (j != end && (tag & kTagAggBit)) {
-      j += step;
-      polls = 0;
-    } else {
+    if (!ready) {
       if (++polls > kMaxPolls) return __builtin_nanf("");
-      __builtin_amdgcn_s_sleep(2);
+      __builtin_amdgcn_s_sleep(1);
     }
   }
-  for (int i = j - step; i != k; i -= step) {
-    const uint64_t x = poll_word(words + i * BD);
-    const uint32_t tag = static_cast<uint32_t>(x);
-    const float v = __uint_as_float(static_cast<uint32_t>(x >> 32));
-    carry = tag == kTagIncl ? v : apply<kReset>(__uint_as_float(tag & ~kTagAggBit), carry, v);
+  for (int i = j - step; i != k;) {
+    uint64_t x[kAt];
+    // (back towards k: the words of tiles that were seen ready)
+#pragma unroll
+    for (int q = 0; q < kAt; ++q) {
+      const int n = i - q * step;
+      x[q] = poll_word(words + (step < 0 ? std::min(n, k - 1) : std::max(n, k + 1)) * BD);
+    }
+#pragma unroll
+    for (int q = 0; q < kAt; ++q) {
+      if (i == k) continue;
+      const uint32_t tag = static_cast<uint32_t>(x[q]);
+      carry = tag == kTagIncl ? value(x[q]) : apply<kReset>(__uint_as_float(tag & ~kTagAggBit), carry, value(x[q]));
+      i -= step;
+    }
   }
   return carry;
 }
@@ -215,7 +287,7 @@ struct Fwd {
   uint64_t* words;
 };
 
-template <typename T, bool kReset>
+template <typename T, bool kReset, bool kOnce>
 __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
   __shared__ uint32_t s_ticket;
   __shared__ Maps s_maps;
@@ -231,15 +303,11 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
   const auto at = [&](const Seq& q) { return static_cast<const T*>(q.p) + b * q.sb + static_cast<int64_t>(t0) * q.st + d; };
 
   Raw<T> x[kFwdRows], gi[kFwdRows], gr[kFwdRows];
-  load_rows(at(p.gr), p.gr.st, rows, left, gr);
-  load_rows(at(p.gi), p.gi.st, rows, left, gi);
-  load_rows(at(p.x), p.x.st, rows, left, x);
+  load_rows<kOnce>(at(p.gr), p.gr.st, rows, left, gr);
+  load_rows<kOnce>(at(p.gi), p.gi.st, rows, left, gi);
+  load_rows<kOnce>(at(p.x), p.x.st, rows, left, x);
   uint32_t fresh = 0;  // bit i: a sequence starts at step t0 + i
-  if constexpr (kReset) {
-#pragma unroll
-    for (int i = 0; i < kFwdRows; ++i)
-      if (i < rows && p.reset[static_cast<int64_t>(b) * g.T + t0 + i]) fresh |= 1u << i;
-  }
+  if constexpr (kReset) fresh = starts<kFwdRows>(p.reset + static_cast<int64_t>(b) * g.T + t0, rows);
   if (tid < kCh) s_rate[tid] = d0 + tid < g.D ? p.c * softplus(p.decay[d0 + tid]) : 0.0f;
   __syncthreads();
   const f4 rate = *reinterpret_cast<const f4*>(&s_rate[cl * kVec]);
@@ -289,10 +357,11 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
   for (int i = 0; i < kFwdRows; ++i) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) h.v[j] = apply<kReset>(a[i][j], h.v[j], v[i][j]);
-    if (i < rows) store4(out + static_cast<int64_t>(i) * g.D, h, left);
+    if (i < rows) store4_nt(out + static_cast<int64_t>(i) * g.D, h, left);
     if (i + 1 == rows && p.last) store4(p.last + row, h, left);
   }
-  if (p.keep && rows >= kKeep) store4(p.keep + (t0 / kKeep) * BD + row, h, left);
+  const int t1 = t0 + kFwdRows;
+  if (p.keep && rows >= kFwdRows && t1 % kKeep == 0) store4(p.keep + (t1 / kKeep - 1) * BD + row, h, left);
 }
 
 // ------------------------------------------------------------------ backward
@@ -309,8 +378,9 @@ struct Bwd {
   uint64_t* words;
 };
 
-template <typename T, bool kReset>
-__global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd p) {
+// (four waves per SIMD fit bf16 operands without spills: B2 T16381 D2048 268 -> 248 us)
+template <typename T, bool kReset, bool kOnce>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(Bwd p) {
   constexpr int kRows = kBwdRows;
   __shared__ uint32_t s_ticket;
   __shared__ Maps s_maps;
@@ -330,16 +400,12 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd p) {
   const auto at = [&](const Seq& q) { return static_cast<const T*>(q.p) + b * q.sb + static_cast<int64_t>(t0) * q.st + d; };
 
   Raw<T> x[kRows], gi[kRows], gr[kRows], dh[kRows];
-  load_rows(at(p.gr), p.gr.st, rows, left, gr);
-  load_rows(at(p.gi), p.gi.st, rows, left, gi);
-  load_rows(at(p.x), p.x.st, rows, left, x);
-  load_rows(at(p.dh), p.dh.st, rows, left, dh);
+  load_rows<kOnce>(at(p.gr), p.gr.st, rows, left, gr);
+  load_rows<kOnce>(at(p.gi), p.gi.st, rows, left, gi);
+  load_rows<kOnce>(at(p.x), p.x.st, rows, left, x);
+  load_rows<kOnce>(at(p.dh), p.dh.st, rows, left, dh);
   uint32_t fresh = 0;
-  if constexpr (kReset) {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (i < rows && p.reset[static_cast<int64_t>(b) * g.T + t0 + i]) fresh |= 1u << i;
-  }
+  if constexpr (kReset) fresh = starts<kRows>(p.reset + static_cast<int64_t>(b) * g.T + t0, rows);
   f4 h = io4<float>::fill(0.0f);  // the state that enters the run
   if (!(s & 1) && rows > 0 && left > 0) {
     if (t0 > 0)
@@ -437,9 +503,9 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Bwd p) {
       }
       if (i < rows) {
         const int64_t o = out + static_cast<int64_t>(i) * g.D;
-        store4(static_cast<T*>(p.dx) + o, ox, left);
-        store4(static_cast<T*>(p.dgi) + o, oi, left);
-        store4(static_cast<T*>(p.dgr) + o, og, left);
+        store4_nt(static_cast<T*>(p.dx) + o, ox, left);
+        store4_nt(static_cast<T*>(p.dgi) + o, oi, left);
+        store4_nt(static_cast<T*>(p.dgr) + o, og, left);
       }
     }
   }
@@ -598,17 +664,13 @@ extern "C" int mg_recurrence_fwd(int dtype, const mg_seq* x, const mg_seq* input
   hipStream_t st = static_cast<hipStream_t>(stream);
   clear(workspace, clear_bytes(p.g), st);
   const dim3 grid(static_cast<unsigned>(p.g.chains) * p.g.tiles), block(kThreads);
-  if (dtype == MG_BF16) {
-    if (reset)
-      hipLaunchKernelGGL((fwd_kernel<bf16_t, true>), grid, block, 0, st, p);
-    else
-      hipLaunchKernelGGL((fwd_kernel<bf16_t, false>), grid, block, 0, st, p);
-  } else {
-    if (reset)
-      hipLaunchKernelGGL((fwd_kernel<float, true>), grid, block, 0, st, p);
-    else
-      hipLaunchKernelGGL((fwd_kernel<float, false>), grid, block, 0, st, p);
-  }
+  const bool once = static_cast<size_t>(B) * T * D * e * 3 > kCacheBytes;
+  const auto go = [&](auto t, auto cut, auto single) {
+    hipLaunchKernelGGL((fwd_kernel<decltype(t), decltype(cut)::value, decltype(single)::value>), grid, block, 0, st, p);
+  };
+  const auto by_size = [&](auto t, auto cut) { once ? go(t, cut, std::true_type{}) : go(t, cut, std::false_type{}); };
+  const auto by_reset = [&](auto t) { reset ? by_size(t, std::true_type{}) : by_size(t, std::false_type{}); };
+  dtype == MG_BF16 ? by_reset(bf16_t{}) : by_reset(0.0f);
   return check_launch(fn);
 }
 
@@ -647,17 +709,13 @@ extern "C" int mg_recurrence_bwd(int dtype, const mg_seq* x, const mg_seq* input
   hipStream_t st = static_cast<hipStream_t>(stream);
   clear(workspace, cleared, st);
   const dim3 grid(static_cast<unsigned>(p.g.chains) * p.g.tiles), block(kThreads);
-  if (dtype == MG_BF16) {
-    if (reset)
-      hipLaunchKernelGGL((bwd_kernel<bf16_t, true>), grid, block, 0, st, p);
-    else
-      hipLaunchKernelGGL((bwd_kernel<bf16_t, false>), grid, block, 0, st, p);
-  } else {
-    if (reset)
-      hipLaunchKernelGGL((bwd_kernel<float, true>), grid, block, 0, st, p);
-    else
-      hipLaunchKernelGGL((bwd_kernel<float, false>), grid, block, 0, st, p);
-  }
+  const bool once = static_cast<size_t>(B) * T * D * e * 4 > kCacheBytes;
+  const auto go = [&](auto t, auto cut, auto single) {
+    hipLaunchKernelGGL((bwd_kernel<decltype(t), decltype(cut)::value, decltype(single)::value>), grid, block, 0, st, p);
+  };
+  const auto by_size = [&](auto t, auto cut) { once ? go(t, cut, std::true_type{}) : go(t, cut, std::false_type{}); };
+  const auto by_reset = [&](auto t) { reset ? by_size(t, std::true_type{}) : by_size(t, std::false_type{}); };
+  dtype == MG_BF16 ? by_reset(bf16_t{}) : by_reset(0.0f);
   if (ddecay) hipLaunchKernelGGL(ddecay_kernel, dim3((D + 15) / 16), dim3(256), 0, st, p.part, B * p.g.tiles, D, decay, ddecay);
   return check_launch(fn);
 }
