@@ -9,12 +9,12 @@
 //   1. Radix sort of (id, token) in passes of up to 10 bits, least digit first. hist_kernel counts a chunk's digits,
 //      scatter_kernel turns the counts of all chunks into first places and moves its chunk's pairs there; a token's
 //      rank among the wave's lanes of its digit comes from one ballot per bit. Up to 4096 tokens one workgroup does
-//      all passes in one launch. Ids without a gradient sort behind the table as id V.
+//      all passes in one launch. Ids without a gradient sort behind the table as id V. places_kernel then searches
+//      every id's first place within its last digit's places.
 //   2. pieces_kernel: every 32 places that are all one id become one row of partial sums, so that an id of many
-//      tokens is not one wave's work.
-//   3. rows_kernel: a wave per row of dw adds the id's places before its first piece, its pieces, and those after the
-//      last. The first place of an id is searched for within its last digit's places. Ids of more than 16 pieces are
-//      left to all four waves of the workgroup.
+//      tokens is not one wave's work; runs_kernel: an id of more than 16 pieces is a workgroup's.
+//   3. rows_kernel: a wave has four rows of dw, and where they have few tokens loads those all at once. Else it adds a
+//      row's places before its first piece, its pieces, and those after the last.
 // Sums are fp32, rounded once to the table's type.
 //
 // Bound by memory: dy is read once, dw written once.
@@ -31,11 +31,13 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSmall = 4096;       // tokens that one workgroup sorts
 constexpr int kMaxChunks = 256;
 constexpr int kPiece = 32;
-constexpr int kManyPieces = 16;
+constexpr int kManyPieces = 16;    // an id of more is runs_kernel's
+constexpr int kRunThreads = 512, kRunWaves = kRunThreads / 64;
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kVec = 8, kCols = 64 * kVec;  // columns of a lane and of a wave
-constexpr int kRows = 16;                   // rows of dw per workgroup
-constexpr int64_t kMaxN = 1 << 30, kMaxV = 1 << 28;
+constexpr int kRows = 4;                    // rows of dw per wave
+constexpr int kFew = 8;                     // tokens of a wave's rows that are loaded at once
+constexpr int64_t kMaxN = 1 << 27, kMaxV = 1 << 28;
 
 struct Pairs {
   uint32_t *key, *pos;
@@ -261,6 +263,32 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(Ids ids, int p
 
 // ------------------------------------------------------------------ sums
 
+// Eight values as loaded
+template <typename T> struct Pack;
+template <> struct Pack<bf16_t> {
+  u16x8u v;
+  __device__ __forceinline__ void load(const bf16_t* p, int left) {
+    if (left >= kVec) {
+      v = *reinterpret_cast<const u16x8u*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[j] = j < left ? p[j] : bf16_t(0);
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&acc)[kVec]) const {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) acc[j] += bf16_to_f32(v[j]);
+  }
+};
+template <> struct Pack<float> {
+  float v[kVec];
+  __device__ __forceinline__ void load(const float* p, int left) { load8(p, left, v); }
+  __device__ __forceinline__ void add_to(float (&acc)[kVec]) const {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) acc[j] += v[j];
+  }
+};
+
 // acc += rows pos[i], i = i0 .. i1 - 1, in order, of columns c .. c + 7
 template <typename T>
 __device__ __forceinline__ void add_rows(const T* __restrict__ dy, const uint32_t* __restrict__ pos, int64_t i0, int64_t i1, int D, int c,
@@ -268,19 +296,16 @@ __device__ __forceinline__ void add_rows(const T* __restrict__ dy, const uint32_
   constexpr int kAhead = 8;
   int64_t i = i0;
   for (; i + kAhead <= i1; i += kAhead) {
-    float x[kAhead][kVec];
+    Pack<T> x[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) load8(dy + static_cast<int64_t>(pos[i + u]) * D + c, left, x[u]);
+    for (int u = 0; u < kAhead; ++u) x[u].load(dy + static_cast<int64_t>(pos[i + u]) * D + c, left);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) acc[j] += x[u][j];
+    for (int u = 0; u < kAhead; ++u) x[u].add_to(acc);
   }
   for (; i < i1; ++i) {
-    float x[kVec];
-    load8(dy + static_cast<int64_t>(pos[i]) * D + c, left, x);
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) acc[j] += x[j];
+    Pack<T> x;
+    x.load(dy + static_cast<int64_t>(pos[i]) * D + c, left);
+    x.add_to(acc);
   }
 }
 __device__ __forceinline__ void add_parts(const float* __restrict__ part, int64_t p0, int64_t p1, int D, int c, int left, float (&acc)[kVec]) {
@@ -308,70 +333,115 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(const T* __restrict__ 
   }
 }
 
-template <typename T, typename Tw>
-__global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ starts, int shift,
-                                                        const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
-  __shared__ int s_at[kRows + 1];
-  __shared__ float s_sum[kWaves][kCols];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kRows;
-  if (threadIdx.x <= kRows) {  // the first place of each row's id
-    const uint32_t v = static_cast<uint32_t>(std::min<int64_t>(v0 + threadIdx.x, V));
-    int lo = starts[v >> shift], hi = starts[(v >> shift) + 1];
-    while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      if (sorted.key[mid] < v)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    s_at[threadIdx.x] = lo;
+// first[v]: the first place of id v, and of V
+__global__ __launch_bounds__(kThreads) void places_kernel(const uint32_t* __restrict__ key, const int* __restrict__ starts, int shift, uint32_t V,
+                                                          int* __restrict__ first) {
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (n > V) return;
+  const uint32_t v = static_cast<uint32_t>(n);
+  int lo = starts[v >> shift], hi = starts[(v >> shift) + 1];
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (key[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
   }
-  __syncthreads();
-  for (int r = wave; r < kRows && v0 + r < V; r += kWaves) {
-    const int64_t i0 = __builtin_amdgcn_readfirstlane(s_at[r]), i1 = __builtin_amdgcn_readfirstlane(s_at[r + 1]), p0 = (i0 + kPiece - 1) / kPiece, p1 = i1 / kPiece;
-    if (p1 - p0 > kManyPieces) continue;
-    Tw* out = dw + (v0 + r) * D;
-    for (int c = lane * kVec; c < D; c += kCols) {
-      float acc[kVec] = {};
-      if (p0 < p1) {
-        add_rows(dy, sorted.pos, i0, p0 * kPiece, D, c, D - c, acc);
-        add_parts(part, p0, p1, D, c, D - c, acc);
-        add_rows(dy, sorted.pos, p1 * kPiece, i1, D, c, D - c, acc);
-      } else {
-        add_rows(dy, sorted.pos, i0, i1, D, c, D - c, acc);
+  first[v] = lo;
+}
+
+// The pieces of the run [i0, i1): [p0, p1)
+struct Run {
+  int64_t i0, i1, p0, p1;
+  __device__ __forceinline__ Run(int64_t a, int64_t b) : i0(a), i1(b), p0((a + kPiece - 1) / kPiece), p1(b / kPiece) {}
+  __device__ __forceinline__ bool many() const { return p1 - p0 > kManyPieces; }
+};
+
+// Ids of many pieces, a workgroup per piece, of which only the first of such an id's does anything: each wave sums a
+// share of the pieces, the first wave the places before them too, the last those behind, and the shares are added in order
+template <typename T, typename Tw>
+__global__ __launch_bounds__(kRunThreads) void runs_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ first,
+                                                           const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
+  __shared__ float s_sum[kRunWaves][kCols];
+  const int64_t p = blockIdx.x;
+  const uint32_t key = sorted.key[p * kPiece];
+  if (key >= V) return;
+  const Run r(first[key], first[key + 1]);
+  if (r.p0 != p || !r.many()) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int64_t share = (r.p1 - r.p0 + kRunWaves - 1) / kRunWaves, q0 = std::min(r.p1, r.p0 + wave * share), q1 = std::min(r.p1, q0 + share);
+  for (int c0 = blockIdx.y * kCols; c0 < D; c0 += gridDim.y * kCols) {
+    const int c = c0 + lane * kVec, left = D - c;
+    float acc[kVec] = {};
+    if (left > 0) {
+      if (wave == 0) add_rows(dy, sorted.pos, r.i0, r.p0 * kPiece, D, c, left, acc);
+      add_parts(part, q0, q1, D, c, left, acc);
+      if (wave == kRunWaves - 1) add_rows(dy, sorted.pos, r.p1 * kPiece, r.i1, D, c, left, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) s_sum[wave][j * 64 + lane] = acc[j];
+    __syncthreads();
+    if (wave == 0 && left > 0) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        float t = s_sum[0][j * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kRunWaves; ++w) t += s_sum[w][j * 64 + lane];
+        acc[j] = t * scale;
       }
+      store8(dw + static_cast<int64_t>(key) * D + c, left, acc);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, typename Tw>
+__global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ first,
+                                                        const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
+  const int64_t v0 = (static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
+  if (v0 >= V) return;
+  int at[kRows + 1];
+#pragma unroll
+  for (int q = 0; q <= kRows; ++q) at[q] = first[std::min<int64_t>(v0 + q, V)];
+  const int n = at[kRows] - at[0];
+  for (int c = (threadIdx.x % 64) * kVec + blockIdx.y * kCols; c < D; c += gridDim.y * kCols) {
+    const int left = D - c;
+    Tw* out = dw + v0 * D + c;
+    const auto write = [&](int q, float (&acc)[kVec]) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) acc[j] *= scale;
-      store8(out + c, D - c, acc);
-    }
-  }
-  for (int r = 0; r < kRows && v0 + r < V; ++r) {  // ids of many pieces: a quarter of them to each wave
-    const int64_t i0 = __builtin_amdgcn_readfirstlane(s_at[r]), i1 = __builtin_amdgcn_readfirstlane(s_at[r + 1]), p0 = (i0 + kPiece - 1) / kPiece, p1 = i1 / kPiece;
-    if (p1 - p0 <= kManyPieces) continue;
-    const int64_t quarter = (p1 - p0 + kWaves - 1) / kWaves, q0 = std::min(p1, p0 + wave * quarter), q1 = std::min(p1, q0 + quarter);
-    for (int c0 = 0; c0 < D; c0 += kCols) {
-      const int c = c0 + lane * kVec, left = D - c;
-      float acc[kVec] = {};
-      if (left > 0) {
-        if (wave == 0) add_rows(dy, sorted.pos, i0, p0 * kPiece, D, c, left, acc);
-        add_parts(part, q0, q1, D, c, left, acc);
-        if (wave == kWaves - 1) add_rows(dy, sorted.pos, p1 * kPiece, i1, D, c, left, acc);
+      store8(out + static_cast<int64_t>(q) * D, left, acc);
+    };
+    if (n <= kFew) {
+      Pack<T> x[kFew];
+#pragma unroll
+      for (int u = 0; u < kFew; ++u)
+        if (u < n) x[u].load(dy + static_cast<int64_t>(sorted.pos[at[0] + u]) * D + c, left);
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) {
+        if (v0 + q >= V) break;
+        float acc[kVec] = {};
+#pragma unroll
+        for (int u = 0; u < kFew; ++u)
+          if (at[0] + u >= at[q] && at[0] + u < at[q + 1]) x[u].add_to(acc);
+        write(q, acc);
       }
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) s_sum[wave][j * 64 + lane] = acc[j];
-      __syncthreads();
-      if (wave == 0 && left > 0) {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          float t = s_sum[0][j * 64 + lane];
-#pragma unroll
-          for (int w = 1; w < kWaves; ++w) t += s_sum[w][j * 64 + lane];
-          acc[j] = t * scale;
+    } else {
+#pragma unroll 1
+      for (int q = 0; q < kRows; ++q) {
+        if (v0 + q >= V) break;
+        const Run r(first[v0 + q], first[v0 + q + 1]);
+        if (r.many()) continue;
+        float acc[kVec] = {};
+        if (r.p0 < r.p1) {
+          add_rows(dy, sorted.pos, r.i0, r.p0 * kPiece, D, c, left, acc);
+          add_parts(part, r.p0, r.p1, D, c, left, acc);
+          add_rows(dy, sorted.pos, r.p1 * kPiece, r.i1, D, c, left, acc);
+        } else {
+          add_rows(dy, sorted.pos, r.i0, r.i1, D, c, left, acc);
         }
-        store8(dw + (v0 + r) * D + c, left, acc);
+        write(q, acc);
       }
-      __syncthreads();
     }
   }
 }
@@ -394,25 +464,27 @@ inline Plan plan_of(int64_t N, int64_t V) {
   return p;
 }
 
-// Workspace: [pieces][D] partial sums, counts of each chunk, starts, two sets of pairs
+// Workspace: [pieces][D] partial sums, counts of each chunk, first places of the last digits and of the ids, two sets
+// of pairs
 struct Layout {
-  size_t counts, starts, pairs, total;
+  size_t counts, starts, first, pairs, total;
   int64_t pieces;
 };
-inline Layout layout_of(int64_t N, int D, const Plan& p) {
+inline Layout layout_of(int64_t N, int D, int64_t V, const Plan& p) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   Layout l;
   l.pieces = N / kPiece;
   l.counts = up(static_cast<size_t>(l.pieces) * D * 4);
   l.starts = l.counts + up(static_cast<size_t>(p.chunks) * p.bins * 4);
-  l.pairs = l.starts + up((static_cast<size_t>(p.bins) + 1) * 4);
+  l.first = l.starts + up((static_cast<size_t>(p.bins) + 1) * 4);
+  l.pairs = l.first + up((static_cast<size_t>(V) + 1) * 4);
   l.total = l.pairs + 4 * up(static_cast<size_t>(N) * 4);
   return l;
 }
 
 inline int check_ids(const char* fn, int id_bytes, const void* ids, int64_t N, int D, int64_t V) {
   if (N < 1 || N >= kMaxN || D < 1 || V < 1 || V >= kMaxV)
-    return fail(MG_ERR_ARG, "%s: N=%lld, D=%d, V=%lld must be at least 1, N below 2^30, V below 2^28", fn, (long long)N, D, (long long)V);
+    return fail(MG_ERR_ARG, "%s: N=%lld, D=%d, V=%lld must be at least 1, N below 2^27, V below 2^28", fn, (long long)N, D, (long long)V);
   if (id_bytes != 4 && id_bytes != 8) return fail(MG_ERR_DTYPE, "%s: ids of %d bytes", fn, id_bytes);
   if (!ids || !aligned(ids, id_bytes)) return fail(MG_ERR_ARG, "%s: ids NULL or misaligned", fn);
   return MG_OK;
@@ -433,13 +505,18 @@ void launch_lookup(const Ids& ids, const void* table, void* y, int D, float scal
 }
 
 template <typename T, typename Tw>
-void launch_sums(const void* dy, const Pairs& sorted, const int* starts, int shift, float* part, int64_t pieces, void* dw, int D, int64_t V,
-                 float scale, hipStream_t st) {
+void launch_sums(const void* dy, const Pairs& sorted, const int* first, float* part, int64_t pieces, void* dw, int D, int64_t V, float scale,
+                 hipStream_t st) {
+  const int cols = std::min((D + kCols - 1) / kCols, 64);
+  const uint32_t v = static_cast<uint32_t>(V);
+  const T* g = static_cast<const T*>(dy);
+  Tw* w = static_cast<Tw*>(dw);
   if (pieces)
-    hipLaunchKernelGGL((pieces_kernel<T>), dim3((pieces + kWaves - 1) / kWaves, std::min((D + kCols - 1) / kCols, 64)), dim3(kThreads), 0, st,
-                       static_cast<const T*>(dy), sorted, pieces, D, static_cast<uint32_t>(V), part);
-  hipLaunchKernelGGL((rows_kernel<T, Tw>), dim3((V + kRows - 1) / kRows), dim3(kThreads), 0, st, static_cast<const T*>(dy), sorted, starts,
-                     shift, part, static_cast<Tw*>(dw), D, static_cast<uint32_t>(V), scale);
+    hipLaunchKernelGGL((pieces_kernel<T>), dim3((pieces + kWaves - 1) / kWaves, cols), dim3(kThreads), 0, st, g, sorted, pieces, D, v, part);
+  if (pieces > kManyPieces)
+    hipLaunchKernelGGL((runs_kernel<T, Tw>), dim3(pieces - kManyPieces, cols), dim3(kRunThreads), 0, st, g, sorted, first, part, w, D, v, scale);
+  hipLaunchKernelGGL((rows_kernel<T, Tw>), dim3((V + kWaves * kRows - 1) / (kWaves * kRows), cols), dim3(kThreads), 0, st, g, sorted, first,
+                     part, w, D, v, scale);
 }
 
 }  // namespace embed_sorted
@@ -466,7 +543,7 @@ extern "C" int mg_embedding_fwd(int id_bytes, const void* ids, int64_t N, int ta
 extern "C" size_t mg_embedding_sorted_bwd_workspace_bytes(int64_t N, int D, int64_t V) {
   using namespace embed_sorted;
   if (N < 1 || N >= kMaxN || D < 1 || V < 1 || V >= kMaxV) return 0;
-  return layout_of(N, D, plan_of(N, V)).total;
+  return layout_of(N, D, V, plan_of(N, V)).total;
 }
 
 extern "C" int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N, int dy_dtype, const void* dy, int D, int64_t V, float scale,
@@ -476,7 +553,7 @@ extern "C" int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N,
   int rc;
   if ((rc = check_ids(fn, id_bytes, ids, N, D, V)) || (rc = check_p(fn, "dy", dy, dy_dtype)) || (rc = check_p(fn, "dw", dw, dw_dtype))) return rc;
   const Plan p = plan_of(N, V);
-  const Layout l = layout_of(N, D, p);
+  const Layout l = layout_of(N, D, V, p);
   if (!workspace || workspace_bytes < l.total || !aligned(workspace, 256))
     return fail(MG_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu (or misaligned)", fn, workspace_bytes, l.total);
   char* ws = static_cast<char*>(workspace);
@@ -502,12 +579,14 @@ extern "C" int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N,
       src.key = out.key, src.pos = out.pos;
     }
   }
-  const int shift = (p.passes - 1) * p.digit;
+  int* first = reinterpret_cast<int*>(ws + l.first);
+  hipLaunchKernelGGL(places_kernel, dim3((V + kThreads) / kThreads), dim3(kThreads), 0, st, sorted.key, starts, (p.passes - 1) * p.digit,
+                     static_cast<uint32_t>(V), first);
   if (dy_dtype == MG_BF16)
-    dw_dtype == MG_BF16 ? launch_sums<bf16_t, bf16_t>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st)
-                        : launch_sums<bf16_t, float>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st);
+    dw_dtype == MG_BF16 ? launch_sums<bf16_t, bf16_t>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st)
+                        : launch_sums<bf16_t, float>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st);
   else
-    dw_dtype == MG_BF16 ? launch_sums<float, bf16_t>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st)
-                        : launch_sums<float, float>(dy, sorted, starts, shift, part, l.pieces, dw, D, V, scale, st);
+    dw_dtype == MG_BF16 ? launch_sums<float, bf16_t>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st)
+                        : launch_sums<float, float>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st);
   return check_launch(fn);
 }

@@ -24,7 +24,7 @@ def _bwd(L, **kw):
 def test_both():
     L = _lib.lib()
     for call in (_fwd, _bwd):
-        for kw in (dict(N=0), dict(N=1 << 30), dict(V=0), dict(V=1 << 28), dict(D=0), dict(ids=None), dict(ids=4100)):
+        for kw in (dict(N=0), dict(N=1 << 27), dict(V=0), dict(V=1 << 28), dict(D=0), dict(ids=None), dict(ids=4100)):
             assert call(L, **kw) == ARG, kw
         assert call(L, idb=2) == DTYPE and call(L, wt=2) == DTYPE
     for kw in (dict(w=None), dict(w=4098), dict(y=None), dict(y=4097)):
