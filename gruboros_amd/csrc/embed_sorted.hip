@@ -36,7 +36,7 @@ constexpr int kRunThreads = 512, kRunWaves = kRunThreads / 64;
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kVec = 8, kCols = 64 * kVec;  // columns of a lane and of a wave
 constexpr int kRows = 4;                    // rows of dw per wave
-constexpr int kFew = 8;                     // tokens of a wave's rows that are loaded at once
+constexpr int kFew = 4;                     // tokens of a wave's rows that are loaded at once
 constexpr int64_t kMaxN = 1 << 27, kMaxV = 1 << 28;
 
 struct Pairs {
@@ -62,75 +62,83 @@ struct Ids {
 
 // ------------------------------------------------------------------ lookup
 
-typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
-
-__device__ __forceinline__ void load8(const float* p, float (&v)[kVec]) {
-  const f32x4u a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
+// N values (4 or 8) as loaded, of which the first `left` exist
+template <typename T, int N> struct Pack {
+  typedef T Raw __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  Raw v;
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if (left >= N) {
+      v = *reinterpret_cast<const Raw*>(p);
+    } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-}
-__device__ __forceinline__ void load8(const bf16_t* p, float (&v)[kVec]) {
-  const u16x8u a = *reinterpret_cast<const u16x8u*>(p);
+      for (int j = 0; j < N; ++j) v[j] = j < left ? p[j] : T(0);
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 2)
+      return bf16_to_f32(v[j]);
+    else
+      return v[j];
+  }
+  __device__ __forceinline__ void add_to(float (&acc)[N]) const {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = bf16_to_f32(a[j]);
-}
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const bf16_t* p) { return bf16_to_f32(*p); }
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(bf16_t* p, float v) { *p = f32_to_bf16(v); }
-// eight values from p on, of which the first `left` exist
+    for (int j = 0; j < N; ++j) acc[j] += get(j);
+  }
+  // kPast: past the nearest caches, as nothing here reads it again
+  template <bool kPast>
+  __device__ __forceinline__ static void store(T* p, int left, const float (&x)[N]) {
+    Raw r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (sizeof(T) == 2)
+        r[j] = f32_to_bf16(x[j]);
+      else
+        r[j] = x[j];
+    }
+    if (left >= N) {
+      if constexpr (kPast)
+        __builtin_nontemporal_store(r, reinterpret_cast<Raw*>(p));
+      else
+        *reinterpret_cast<Raw*>(p) = r;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < left) p[j] = r[j];
+    }
+  }
+};
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, float (&v)[kVec]) {
-  if (left >= kVec) {
-    load8(p, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) v[j] = j < left ? load1(p + j) : 0.0f;
-  }
-}
-__device__ __forceinline__ void store8(float* p, int left, const float (&v)[kVec]) {
-  if (left >= kVec) {
-    const f32x4u a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    reinterpret_cast<f32x4u*>(p)[0] = a;
-    reinterpret_cast<f32x4u*>(p)[1] = b;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (j < left) p[j] = v[j];
-  }
-}
-__device__ __forceinline__ void store8(bf16_t* p, int left, const float (&v)[kVec]) {
-  if (left >= kVec) {
-    u16x8u a;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) a[j] = f32_to_bf16(v[j]);
-    *reinterpret_cast<u16x8u*>(p) = a;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (j < left) p[j] = f32_to_bf16(v[j]);
-  }
+constexpr int wide_of() { return 16 / sizeof(T); }  // values of an output that a lane stores at once: a wave's stores have no gaps
+// Results larger than most of the last cache (256 MB) go past the caches where their rows fill cache lines: the
+// gradient of a V131071 D1024 bf16 table 157 -> 115 us, of its fp32 one 256 -> 195; one that stays there is read from
+// there next, and V32000 D1024 in fp32 takes 64 us, not 70. Lines that two rows share are better put together in the
+// caches (V50001 D777: 78, not 91).
+template <typename T>
+inline bool past_caches(const T* p, int64_t rows, int D) {
+  return aligned(p, 64) && D * sizeof(T) % 64 == 0 && static_cast<size_t>(rows) * D * sizeof(T) > size_t(192) << 20;
 }
 
 // `per` threads (a power of two) to a row
-template <typename Tw, typename Ty>
+template <typename Tw, typename Ty, bool kPast>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(Ids ids, const Tw* __restrict__ table, Ty* __restrict__ y, int D, float scale,
                                                           int per) {
+  constexpr int N = wide_of<Ty>();
   const int rows = kThreads / per, t = threadIdx.x & (per - 1);
   for (int64_t n = static_cast<int64_t>(blockIdx.x) * rows + threadIdx.x / per; n < ids.N; n += static_cast<int64_t>(gridDim.x) * rows) {
     const uint32_t v = ids.key(n);
     const Tw* row = table + static_cast<int64_t>(v) * D;
-    for (int c = t * kVec; c < D; c += per * kVec) {
-      float x[kVec];
+    for (int c = t * N; c < D; c += per * N) {
+      float x[N];
       if (v < ids.V) {
-        load8(row + c, D - c, x);
+        Pack<Tw, N> w;
+        w.load(row + c, D - c);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] *= scale;
+        for (int j = 0; j < N; ++j) x[j] = w.get(j) * scale;
       } else {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] = __builtin_nanf("");
+        for (int j = 0; j < N; ++j) x[j] = __builtin_nanf("");
       }
-      store8(y + n * D + c, D - c, x);
+      Pack<Ty, N>::template store<kPast>(y + n * D + c, D - c, x);
     }
   }
 }
@@ -156,7 +164,8 @@ struct Source {
   __device__ __forceinline__ uint32_t pos_of(int64_t n) const { return key ? pos[n] : static_cast<uint32_t>(n); }
 };
 
-// counts[chunk][bin] of the digit at `shift`
+// counts[chunk][bin] of the digit at `shift` (added up by scatter_kernel where it moves the pairs, with atomics, the
+// counts take 10 us of 65528 tokens, of which a few ids are many; this launch takes 3 to 5)
 __global__ __launch_bounds__(kSortThreads) void hist_kernel(Source src, int64_t chunk, int shift, int bins, int* __restrict__ counts) {
   __shared__ int s_cnt[kBins];
   for (int i = threadIdx.x; i < bins; i += kSortThreads) s_cnt[i] = 0;
@@ -263,58 +272,32 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(Ids ids, int p
 
 // ------------------------------------------------------------------ sums
 
-// Eight values as loaded
-template <typename T> struct Pack;
-template <> struct Pack<bf16_t> {
-  u16x8u v;
-  __device__ __forceinline__ void load(const bf16_t* p, int left) {
-    if (left >= kVec) {
-      v = *reinterpret_cast<const u16x8u*>(p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) v[j] = j < left ? p[j] : bf16_t(0);
-    }
-  }
-  __device__ __forceinline__ void add_to(float (&acc)[kVec]) const {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) acc[j] += bf16_to_f32(v[j]);
-  }
-};
-template <> struct Pack<float> {
-  float v[kVec];
-  __device__ __forceinline__ void load(const float* p, int left) { load8(p, left, v); }
-  __device__ __forceinline__ void add_to(float (&acc)[kVec]) const {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) acc[j] += v[j];
-  }
-};
-
-// acc += rows pos[i], i = i0 .. i1 - 1, in order, of columns c .. c + 7
-template <typename T>
+// acc += rows pos[i], i = i0 .. i1 - 1, in order, of N columns from c on
+template <int N, typename T>
 __device__ __forceinline__ void add_rows(const T* __restrict__ dy, const uint32_t* __restrict__ pos, int64_t i0, int64_t i1, int D, int c,
-                                         int left, float (&acc)[kVec]) {
+                                         int left, float (&acc)[N]) {
   constexpr int kAhead = 8;
   int64_t i = i0;
   for (; i + kAhead <= i1; i += kAhead) {
-    Pack<T> x[kAhead];
+    Pack<T, N> x[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) x[u].load(dy + static_cast<int64_t>(pos[i + u]) * D + c, left);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) x[u].add_to(acc);
   }
   for (; i < i1; ++i) {
-    Pack<T> x;
+    Pack<T, N> x;
     x.load(dy + static_cast<int64_t>(pos[i]) * D + c, left);
     x.add_to(acc);
   }
 }
-__device__ __forceinline__ void add_parts(const float* __restrict__ part, int64_t p0, int64_t p1, int D, int c, int left, float (&acc)[kVec]) {
+template <int N>
+__device__ __forceinline__ void add_parts(const float* __restrict__ part, int64_t p0, int64_t p1, int D, int c, int left, float (&acc)[N]) {
 #pragma unroll 8
   for (int64_t p = p0; p < p1; ++p) {
-    float x[kVec];
-    load8(part + p * D + c, left, x);
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) acc[j] += x[j];
+    Pack<float, N> x;
+    x.load(part + p * D + c, left);
+    x.add_to(acc);
   }
 }
 
@@ -329,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(const T* __restrict__ 
   for (int c = (threadIdx.x % 64) * kVec + blockIdx.y * kCols; c < D; c += gridDim.y * kCols) {
     float acc[kVec] = {};
     add_rows(dy, sorted.pos, p * kPiece, (p + 1) * kPiece, D, c, D - c, acc);
-    store8(part + p * D + c, D - c, acc);
+    Pack<float, kVec>::template store<false>(part + p * D + c, D - c, acc);
   }
 }
 
@@ -389,13 +372,13 @@ __global__ __launch_bounds__(kRunThreads) void runs_kernel(const T* __restrict__
         for (int w = 1; w < kRunWaves; ++w) t += s_sum[w][j * 64 + lane];
         acc[j] = t * scale;
       }
-      store8(dw + static_cast<int64_t>(key) * D + c, left, acc);
+      Pack<Tw, kVec>::template store<false>(dw + static_cast<int64_t>(key) * D + c, left, acc);
     }
     __syncthreads();
   }
 }
 
-template <typename T, typename Tw>
+template <typename T, typename Tw, bool kPast>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ first,
                                                         const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
   const int64_t v0 = (static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
@@ -404,23 +387,24 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy
 #pragma unroll
   for (int q = 0; q <= kRows; ++q) at[q] = first[std::min<int64_t>(v0 + q, V)];
   const int n = at[kRows] - at[0];
-  for (int c = (threadIdx.x % 64) * kVec + blockIdx.y * kCols; c < D; c += gridDim.y * kCols) {
+  constexpr int N = wide_of<Tw>(), kWide = 64 * N;
+  for (int c = (threadIdx.x % 64) * N + blockIdx.y * kWide; c < D; c += gridDim.y * kWide) {
     const int left = D - c;
     Tw* out = dw + v0 * D + c;
-    const auto write = [&](int q, float (&acc)[kVec]) {
+    const auto write = [&](int q, float (&acc)[N]) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) acc[j] *= scale;
-      store8(out + static_cast<int64_t>(q) * D, left, acc);
+      for (int j = 0; j < N; ++j) acc[j] *= scale;
+      Pack<Tw, N>::template store<kPast>(out + static_cast<int64_t>(q) * D, left, acc);
     };
     if (n <= kFew) {
-      Pack<T> x[kFew];
+      Pack<T, N> x[kFew];
 #pragma unroll
       for (int u = 0; u < kFew; ++u)
         if (u < n) x[u].load(dy + static_cast<int64_t>(sorted.pos[at[0] + u]) * D + c, left);
 #pragma unroll
       for (int q = 0; q < kRows; ++q) {
         if (v0 + q >= V) break;
-        float acc[kVec] = {};
+        float acc[N] = {};
 #pragma unroll
         for (int u = 0; u < kFew; ++u)
           if (at[0] + u >= at[q] && at[0] + u < at[q + 1]) x[u].add_to(acc);
@@ -432,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy
         if (v0 + q >= V) break;
         const Run r(first[v0 + q], first[v0 + q + 1]);
         if (r.many()) continue;
-        float acc[kVec] = {};
+        float acc[N] = {};
         if (r.p0 < r.p1) {
           add_rows(dy, sorted.pos, r.i0, r.p0 * kPiece, D, c, left, acc);
           add_parts(part, r.p0, r.p1, D, c, left, acc);
@@ -498,10 +482,13 @@ inline int check_p(const char* fn, const char* name, const void* p, int dt) {
 template <typename Tw, typename Ty>
 void launch_lookup(const Ids& ids, const void* table, void* y, int D, float scale, hipStream_t st) {
   int per = 1;
-  while (per < kThreads && per * kVec < D) per *= 2;
+  while (per < kThreads && per * wide_of<Ty>() < D) per *= 2;
   const int64_t wgs = (ids.N + kThreads / per - 1) / (kThreads / per);
-  hipLaunchKernelGGL((lookup_kernel<Tw, Ty>), dim3(std::min<int64_t>(wgs, 1 << 20)), dim3(kThreads), 0, st, ids, static_cast<const Tw*>(table),
-                     static_cast<Ty*>(y), D, scale, per);
+  const auto go = [&](auto past) {
+    hipLaunchKernelGGL((lookup_kernel<Tw, Ty, decltype(past)::value>), dim3(std::min<int64_t>(wgs, 1 << 20)), dim3(kThreads), 0, st, ids,
+                       static_cast<const Tw*>(table), static_cast<Ty*>(y), D, scale, per);
+  };
+  past_caches(static_cast<Ty*>(y), ids.N, D) ? go(std::true_type{}) : go(std::false_type{});
 }
 
 template <typename T, typename Tw>
@@ -515,8 +502,13 @@ void launch_sums(const void* dy, const Pairs& sorted, const int* first, float* p
     hipLaunchKernelGGL((pieces_kernel<T>), dim3((pieces + kWaves - 1) / kWaves, cols), dim3(kThreads), 0, st, g, sorted, pieces, D, v, part);
   if (pieces > kManyPieces)
     hipLaunchKernelGGL((runs_kernel<T, Tw>), dim3(pieces - kManyPieces, cols), dim3(kRunThreads), 0, st, g, sorted, first, part, w, D, v, scale);
-  hipLaunchKernelGGL((rows_kernel<T, Tw>), dim3((V + kWaves * kRows - 1) / (kWaves * kRows), cols), dim3(kThreads), 0, st, g, sorted, first,
-                     part, w, D, v, scale);
+  constexpr int kWide = 64 * wide_of<Tw>();
+  const auto rows = [&](auto past) {
+    hipLaunchKernelGGL((rows_kernel<T, Tw, decltype(past)::value>),
+                       dim3((V + kWaves * kRows - 1) / (kWaves * kRows), std::min((D + kWide - 1) / kWide, 64)), dim3(kThreads), 0, st, g, sorted,
+                       first, part, w, D, v, scale);
+  };
+  past_caches(w, V, D) ? rows(std::true_type{}) : rows(std::false_type{});
 }
 
 }  // namespace embed_sorted
