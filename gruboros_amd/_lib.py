@@ -116,6 +116,7 @@ SIGNATURES = {
     "mg_distill_workspace_bytes": (_c_size, [_c_i64]),
     "mg_distill": (_c_int, [_c_int, _vp, _c_i64, _c_i64, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, ctypes.c_float, ctypes.c_float,
                             _fp, _vp, _vp, _c_size, _vp]),
+    "mg_capture_id": (ctypes.c_uint64, [_vp]),
     "mg_scale_inplace": (_c_int, [_c_int, _vp, _c_i64, _fp, _vp]),
     "mg_embedding_fwd": (_c_int, [_c_int, _vp, _c_i64, _c_int, _vp, _c_i64, _c_int, ctypes.c_float, _c_int, _vp, _vp]),
     "mg_embedding_sorted_bwd_workspace_bytes": (_c_size, [_c_i64, _c_int, _c_i64]),

@@ -578,6 +578,16 @@ extern "C" int mg_distill(int logits_dtype, const mg_seq* logits, int64_t B, int
   return check_launch(fn);
 }
 
+extern "C" unsigned long long mg_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();  // (the launches that follow report what is wrong with the stream)
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 extern "C" int mg_scale_inplace(int dtype, void* x, int64_t n, const float* factor, void* stream) {
   using namespace distill;
   const char* fn = "mg_scale_inplace";

@@ -1157,7 +1157,8 @@ Tensor scaled_embedding(const Tensor& ids, const Tensor& weight, double scale, b
 // ------------------------------------------------------------------ distillation
 
 // The loss, with the logits' gradient made in the same pass. The backward multiplies that by the loss's gradient in
-// place (a factor of 1 costs nothing) and hands it over; asked a second time, it makes it again.
+// place (a factor of 1 costs nothing) and hands it over; asked a second time, it makes it again. So it does where
+// forward and backward are not in one capture (or both in none): each replay would multiply it once more.
 struct DistillFn : ag::Function<DistillFn> {
   static Tensor launch(const Tensor& logits, const Tensor& ids, const Tensor& top, const Opt& labels, double temperature, double alpha,
                        const Opt& dlogits, int64_t stream) {
@@ -1197,6 +1198,7 @@ struct DistillFn : ag::Function<DistillFn> {
       ctx->save_for_backward({logits, ids, top, plain(labels)});
       auto& d = ctx->saved_data;
       d["dl"] = *dl, d["temperature"] = temperature, d["alpha"] = alpha, d["stream"] = stream;
+      d["capture"] = static_cast<int64_t>(mg_capture_id(st(stream)));
     }
     return loss;
   }
@@ -1206,7 +1208,8 @@ struct DistillFn : ag::Function<DistillFn> {
     Tensor dl;
     const Tensor g = grads[0].to(at::kFloat);
     c10::DeviceGuard guard(g.device());
-    if (d["dl"].isTensor()) {
+    const bool one_capture = d["capture"].toInt() == static_cast<int64_t>(mg_capture_id(st(d["stream"].toInt())));
+    if (d["dl"].isTensor() && one_capture) {
       dl = d["dl"].toTensor();
       d["dl"] = c10::IValue();
     } else {

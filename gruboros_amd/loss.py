@@ -104,7 +104,8 @@ def distillation_loss(logits, top_ids, top_logits, labels=None, temperature=1.0,
     Returns the loss, a float32 scalar. The gradient reaches logits, in their dtype, once and in
     reverse mode; it is made in the forward's pass and kept until the backward, which multiplies it
     by the loss's own gradient (in bfloat16 that rounds a second time, unless it is a power of two),
-    and which makes it again where it is run a second time over a retained graph."""
+    and which makes it again where it is run a second time over a retained graph, or in another
+    captured graph than the forward."""
     require_cuda(logits, top_ids, top_logits, labels)
     dtype_code(logits.dtype)
     dtype_code(top_logits.dtype)

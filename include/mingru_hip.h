@@ -849,11 +849,13 @@ int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N, int dy_dty
  * logits' dtype, rounded to nearest; it must not overlap logits. Sums over
  * rows are in double, in a fixed order. 1e-4 <= temperature <= 1e4.
  * mg_scale_inplace: x *= *factor (read on the stream) over n values; a factor
- * of 1 touches nothing. */
+ * of 1 touches nothing.
+ * mg_capture_id: the capture that the stream is in, 0 where it is in none. */
 size_t mg_distill_workspace_bytes(int64_t N);
 int mg_distill(int logits_dtype, const mg_seq* logits, int64_t B, int64_t T, int V, int id_bytes, const void* ids,
                int top_dtype, const void* top, int K, const int64_t* labels, float temperature, float alpha,
                float* loss, void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+unsigned long long mg_capture_id(void* stream);
 int mg_scale_inplace(int dtype, void* x, int64_t n, const float* factor, void* stream);
 
 #ifdef __cplusplus

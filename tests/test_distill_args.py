@@ -47,6 +47,10 @@ def test_scale():
     assert L.mg_scale_inplace(2, 4096, 5, 4096, None) == DTYPE
 
 
+def test_no_capture():
+    assert _lib.lib().mg_capture_id(None) == 0
+
+
 def test_cpu_tensors_are_refused():
     from gruboros_amd.loss import distillation_loss
 

@@ -279,6 +279,44 @@ def test_streams_and_graphs():
     assert all(torch.equal(a, b) for v, m in zip(want, made) for a, b in zip(m[1], v))
 
 
+def test_backward_captured_without_its_forward():
+    """Each replay gives the gradient once, not multiplied again, and an eager backward leaves a captured forward's alone."""
+    from gruboros_amd.loss import distillation_loss
+
+    ops = [t.to(DEV) for t in _operands((2, 40), 3001, 16, bf16)]
+    z = ops[0].requires_grad_(True)
+    call = lambda: distillation_loss(*ops, 2.0, 0.5)  # noqa: E731
+    up = torch.tensor(0.5, device=DEV)
+    (want,) = torch.autograd.grad(call(), z, up)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        loss = call()
+        torch.autograd.grad(loss, z, up, retain_graph=True)
+        eager = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (first,) = torch.autograd.grad(loss, z, up, retain_graph=True)  # (handed over before)
+        (g,) = torch.autograd.grad(eager, z, up, retain_graph=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(g, want)
+    (again,) = torch.autograd.grad(eager, z, up, retain_graph=True)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, want) and torch.equal(g, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        inside = call()
+    graph.replay()
+    grads = [torch.autograd.grad(inside, z, up, retain_graph=True)[0] for _ in range(2)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for t in grads)
+
+
 def test_values_beyond_32_bit_offsets():
     from gruboros_amd.loss import distillation_loss
 
