@@ -9,12 +9,12 @@
 //   1. Radix sort of (id, token) in passes of up to 10 bits, least digit first. hist_kernel counts a chunk's digits,
 //      scatter_kernel turns the counts of all chunks into first places and moves its chunk's pairs there; a token's
 //      rank among the wave's lanes of its digit comes from one ballot per bit. Up to 4096 tokens one workgroup does
-//      all passes in one launch. Ids without a gradient sort behind the table as id V. places_kernel then searches
-//      every id's first place within its last digit's places.
+//      all passes in one launch. Ids without a gradient sort behind the table as id V.
 //   2. pieces_kernel: every 32 places that are all one id become one row of partial sums, so that an id of many
-//      tokens is not one wave's work; runs_kernel: an id of more than 16 pieces is a workgroup's.
+//      tokens is not one wave's work; beside them, every id's first place is searched within its last digit's places.
 //   3. rows_kernel: a wave has four rows of dw, and where they have few tokens loads those all at once. Else it adds a
-//      row's places before its first piece, its pieces, and those after the last.
+//      row's places before its first piece, its pieces, and those after the last. An id of more than 16 pieces is a
+//      workgroup's.
 // Sums are fp32, rounded once to the table's type.
 //
 // Bound by memory: dy is read once, dw written once.
@@ -31,8 +31,7 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSmall = 4096;       // tokens that one workgroup sorts
 constexpr int kMaxChunks = 256;
 constexpr int kPiece = 32;
-constexpr int kManyPieces = 16;    // an id of more is runs_kernel's
-constexpr int kRunThreads = 512, kRunWaves = kRunThreads / 64;
+constexpr int kManyPieces = 16;    // an id of more is a workgroup's
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kVec = 8, kCols = 64 * kVec;  // columns of a lane and of a wave
 constexpr int kRows = 4;                    // rows of dw per wave
@@ -301,25 +300,9 @@ __device__ __forceinline__ void add_parts(const float* __restrict__ part, int64_
   }
 }
 
-// part[p, :] = the sum of places [32 p, 32 p + 32) where they are all one id of the table; a wave per piece and kCols columns
-template <typename T>
-__global__ __launch_bounds__(kThreads) void pieces_kernel(const T* __restrict__ dy, Pairs sorted, int64_t pieces, int D, uint32_t V,
-                                                          float* __restrict__ part) {
-  const int64_t p = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  if (p >= pieces) return;
-  const uint32_t key = sorted.key[p * kPiece];
-  if (key >= V || key != sorted.key[p * kPiece + kPiece - 1]) return;
-  for (int c = (threadIdx.x % 64) * kVec + blockIdx.y * kCols; c < D; c += gridDim.y * kCols) {
-    float acc[kVec] = {};
-    add_rows(dy, sorted.pos, p * kPiece, (p + 1) * kPiece, D, c, D - c, acc);
-    Pack<float, kVec>::template store<false>(part + p * D + c, D - c, acc);
-  }
-}
-
 // first[v]: the first place of id v, and of V
-__global__ __launch_bounds__(kThreads) void places_kernel(const uint32_t* __restrict__ key, const int* __restrict__ starts, int shift, uint32_t V,
-                                                          int* __restrict__ first) {
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+__device__ __forceinline__ void place(const uint32_t* __restrict__ key, const int* __restrict__ starts, int shift, uint32_t V, int64_t n,
+                                      int* __restrict__ first) {
   if (n > V) return;
   const uint32_t v = static_cast<uint32_t>(n);
   int lo = starts[v >> shift], hi = starts[(v >> shift) + 1];
@@ -333,6 +316,25 @@ __global__ __launch_bounds__(kThreads) void places_kernel(const uint32_t* __rest
   first[v] = lo;
 }
 
+// The first `piece_wgs` workgroups: part[p, :] = the sum of places [32 p, 32 p + 32) where they are all one id of the
+// table, a wave per piece and kCols columns. The others: the ids' first places.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void pieces_kernel(const T* __restrict__ dy, Pairs sorted, int64_t pieces, int piece_wgs, int cols, int D,
+                                                          uint32_t V, float* __restrict__ part, const int* __restrict__ starts, int shift,
+                                                          int* __restrict__ first) {
+  if (blockIdx.x >= static_cast<uint32_t>(piece_wgs))
+    return place(sorted.key, starts, shift, V, static_cast<int64_t>(blockIdx.x - piece_wgs) * kThreads + threadIdx.x, first);
+  const int64_t p = static_cast<int64_t>(blockIdx.x / cols) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (p >= pieces) return;
+  const uint32_t key = sorted.key[p * kPiece];
+  if (key >= V || key != sorted.key[p * kPiece + kPiece - 1]) return;
+  for (int c = (threadIdx.x % 64) * kVec + blockIdx.x % cols * kCols; c < D; c += cols * kCols) {
+    float acc[kVec] = {};
+    add_rows(dy, sorted.pos, p * kPiece, (p + 1) * kPiece, D, c, D - c, acc);
+    Pack<float, kVec>::template store<false>(part + p * D + c, D - c, acc);
+  }
+}
+
 // The pieces of the run [i0, i1): [p0, p1)
 struct Run {
   int64_t i0, i1, p0, p1;
@@ -340,48 +342,53 @@ struct Run {
   __device__ __forceinline__ bool many() const { return p1 - p0 > kManyPieces; }
 };
 
-// Ids of many pieces, a workgroup per piece, of which only the first of such an id's does anything: each wave sums a
-// share of the pieces, the first wave the places before them too, the last those behind, and the shares are added in order
+// An id of many pieces is a workgroup's: each wave sums a share of the pieces, the first wave the places before them
+// too, the last those behind, and the shares are added in order. Such an id has at least one piece whose number is a
+// multiple of kManyPieces; the workgroup of its first such piece has it.
 template <typename T, typename Tw>
-__global__ __launch_bounds__(kRunThreads) void runs_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ first,
-                                                           const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
-  __shared__ float s_sum[kRunWaves][kCols];
-  const int64_t p = blockIdx.x;
+__device__ __forceinline__ void sum_run(const T* __restrict__ dy, const Pairs& sorted, const int* __restrict__ first,
+                                        const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale, int64_t p) {
+  constexpr int N = wide_of<Tw>();
+  __shared__ float s_sum[kWaves][64 * N];
   const uint32_t key = sorted.key[p * kPiece];
   if (key >= V) return;
   const Run r(first[key], first[key + 1]);
-  if (r.p0 != p || !r.many()) return;
+  if (r.p0 > p || r.p0 <= p - kManyPieces || !r.many()) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int64_t share = (r.p1 - r.p0 + kRunWaves - 1) / kRunWaves, q0 = std::min(r.p1, r.p0 + wave * share), q1 = std::min(r.p1, q0 + share);
-  for (int c0 = blockIdx.y * kCols; c0 < D; c0 += gridDim.y * kCols) {
-    const int c = c0 + lane * kVec, left = D - c;
-    float acc[kVec] = {};
+  const int64_t share = (r.p1 - r.p0 + kWaves - 1) / kWaves, q0 = std::min(r.p1, r.p0 + wave * share), q1 = std::min(r.p1, q0 + share);
+  for (int c0 = blockIdx.y * 64 * N; c0 < D; c0 += gridDim.y * 64 * N) {
+    const int c = c0 + lane * N, left = D - c;
+    float acc[N] = {};
     if (left > 0) {
       if (wave == 0) add_rows(dy, sorted.pos, r.i0, r.p0 * kPiece, D, c, left, acc);
       add_parts(part, q0, q1, D, c, left, acc);
-      if (wave == kRunWaves - 1) add_rows(dy, sorted.pos, r.p1 * kPiece, r.i1, D, c, left, acc);
+      if (wave == kWaves - 1) add_rows(dy, sorted.pos, r.p1 * kPiece, r.i1, D, c, left, acc);
     }
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) s_sum[wave][j * 64 + lane] = acc[j];
+    for (int j = 0; j < N; ++j) s_sum[wave][j * 64 + lane] = acc[j];
     __syncthreads();
     if (wave == 0 && left > 0) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
+      for (int j = 0; j < N; ++j) {
         float t = s_sum[0][j * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < kRunWaves; ++w) t += s_sum[w][j * 64 + lane];
+        for (int w = 1; w < kWaves; ++w) t += s_sum[w][j * 64 + lane];
         acc[j] = t * scale;
       }
-      Pack<Tw, kVec>::template store<false>(dw + static_cast<int64_t>(key) * D + c, left, acc);
+      Pack<Tw, N>::template store<false>(dw + static_cast<int64_t>(key) * D + c, left, acc);
     }
     __syncthreads();
   }
 }
 
+// The first `run_wgs` workgroups: ids of many pieces. The others: kRows rows of dw to a wave.
 template <typename T, typename Tw, bool kPast>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const T* __restrict__ dy, Pairs sorted, const int* __restrict__ first,
-                                                        const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale) {
-  const int64_t v0 = (static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
+                                                        const float* __restrict__ part, Tw* __restrict__ dw, int D, uint32_t V, float scale,
+                                                        uint32_t run_wgs) {
+  const uint32_t wg = blockIdx.z * gridDim.x + blockIdx.x;
+  if (wg < run_wgs) return sum_run(dy, sorted, first, part, dw, D, V, scale, static_cast<int64_t>(wg) * kManyPieces);
+  const int64_t v0 = (static_cast<int64_t>(wg - run_wgs) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
   if (v0 >= V) return;
   int at[kRows + 1];
 #pragma unroll
@@ -492,21 +499,21 @@ void launch_lookup(const Ids& ids, const void* table, void* y, int D, float scal
 }
 
 template <typename T, typename Tw>
-void launch_sums(const void* dy, const Pairs& sorted, const int* first, float* part, int64_t pieces, void* dw, int D, int64_t V, float scale,
-                 hipStream_t st) {
-  const int cols = std::min((D + kCols - 1) / kCols, 64);
+void launch_sums(const void* dy, const Pairs& sorted, const int* starts, int shift, int* first, float* part, int64_t pieces, void* dw, int D,
+                 int64_t V, float scale, hipStream_t st) {
+  const int cols = std::min((D + kCols - 1) / kCols, 16);
   const uint32_t v = static_cast<uint32_t>(V);
   const T* g = static_cast<const T*>(dy);
   Tw* w = static_cast<Tw*>(dw);
-  if (pieces)
-    hipLaunchKernelGGL((pieces_kernel<T>), dim3((pieces + kWaves - 1) / kWaves, cols), dim3(kThreads), 0, st, g, sorted, pieces, D, v, part);
-  if (pieces > kManyPieces)
-    hipLaunchKernelGGL((runs_kernel<T, Tw>), dim3(pieces - kManyPieces, cols), dim3(kRunThreads), 0, st, g, sorted, first, part, w, D, v, scale);
+  const int64_t piece_wgs = (pieces + kWaves - 1) / kWaves * cols, place_wgs = (V + kThreads) / kThreads;
+  hipLaunchKernelGGL((pieces_kernel<T>), dim3(piece_wgs + place_wgs), dim3(kThreads), 0, st, g, sorted, pieces, static_cast<int>(piece_wgs), cols, D,
+                     v, part, starts, shift, first);
+  const uint32_t run_wgs = pieces > kManyPieces ? (pieces + kManyPieces - 1) / kManyPieces : 0;
   constexpr int kWide = 64 * wide_of<Tw>();
+  const uint32_t wgs = run_wgs + (v + kWaves * kRows - 1) / (kWaves * kRows), z = (wgs >> 20) + 1;  // (x below 2^32 threads)
   const auto rows = [&](auto past) {
-    hipLaunchKernelGGL((rows_kernel<T, Tw, decltype(past)::value>),
-                       dim3((V + kWaves * kRows - 1) / (kWaves * kRows), std::min((D + kWide - 1) / kWide, 64)), dim3(kThreads), 0, st, g, sorted,
-                       first, part, w, D, v, scale);
+    hipLaunchKernelGGL((rows_kernel<T, Tw, decltype(past)::value>), dim3((wgs + z - 1) / z, std::min((D + kWide - 1) / kWide, 64), z), dim3(kThreads),
+                       0, st, g, sorted, first, part, w, D, v, scale, run_wgs);
   };
   past_caches(w, V, D) ? rows(std::true_type{}) : rows(std::false_type{});
 }
@@ -572,13 +579,12 @@ extern "C" int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N,
     }
   }
   int* first = reinterpret_cast<int*>(ws + l.first);
-  hipLaunchKernelGGL(places_kernel, dim3((V + kThreads) / kThreads), dim3(kThreads), 0, st, sorted.key, starts, (p.passes - 1) * p.digit,
-                     static_cast<uint32_t>(V), first);
+  const int shift = (p.passes - 1) * p.digit;
   if (dy_dtype == MG_BF16)
-    dw_dtype == MG_BF16 ? launch_sums<bf16_t, bf16_t>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st)
-                        : launch_sums<bf16_t, float>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st);
+    dw_dtype == MG_BF16 ? launch_sums<bf16_t, bf16_t>(dy, sorted, starts, shift, first, part, l.pieces, dw, D, V, scale, st)
+                        : launch_sums<bf16_t, float>(dy, sorted, starts, shift, first, part, l.pieces, dw, D, V, scale, st);
   else
-    dw_dtype == MG_BF16 ? launch_sums<float, bf16_t>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st)
-                        : launch_sums<float, float>(dy, sorted, first, part, l.pieces, dw, D, V, scale, st);
+    dw_dtype == MG_BF16 ? launch_sums<float, bf16_t>(dy, sorted, starts, shift, first, part, l.pieces, dw, D, V, scale, st)
+                        : launch_sums<float, float>(dy, sorted, starts, shift, first, part, l.pieces, dw, D, V, scale, st);
   return check_launch(fn);
 }

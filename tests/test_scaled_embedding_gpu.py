@@ -220,6 +220,23 @@ def test_values_beyond_32_bit_offsets():
     assert torch.equal(g, count.unsqueeze(-1).expand(40, 1030).contiguous())
 
 
+def test_the_largest_table():
+    """2^28 - 1 rows: three passes of digits, more rows than one dimension of a launch has threads for."""
+    from gruboros_amd.embed import scaled_embedding
+
+    V = 2 ** 28 - 1
+    ids = torch.randint(0, V, (5000,), generator=torch.Generator().manual_seed(9)).to(DEV)
+    ids[:900] = V - 1
+    ids[900:907] = torch.tensor([0, 2 ** 20 - 1, 2 ** 20, 2 ** 24, 2 ** 27, V, -1], device=DEV)
+    w = torch.ones(V, 1, dtype=bf16, device=DEV).requires_grad_(True)
+    y = scaled_embedding(ids, w, 2.0)
+    outside = (ids < 0) | (ids >= V)
+    assert torch.equal(y.isnan().flatten(), outside) and bool((y[~outside] == 2.0).all())
+    (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    at, count = torch.unique(ids[~outside], return_counts=True)
+    assert torch.equal(g[at, 0], (2 * count).to(bf16)) and int(torch.count_nonzero(g)) == len(at)
+
+
 @pytest.mark.parametrize("grad", [True, False], ids=["grad", "no grad"])
 def test_dual_tensors_are_refused(grad):
     import torch.autograd.forward_ad as fwd
