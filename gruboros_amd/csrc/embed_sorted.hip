@@ -10,7 +10,7 @@
 //      scatter_kernel turns the counts of all chunks into first places and moves its chunk's pairs there; a token's
 //      rank among the wave's lanes of its digit comes from one ballot per bit. Up to 4096 tokens one workgroup does
 //      all passes in one launch. Ids without a gradient sort behind the table as id V.
-//   2. pieces_kernel: every 32 places that are all one id become one row of partial sums, so that an id of many
+//   2. pieces_kernel: every 16 places that are all one id become one row of partial sums, so that an id of many
 //      tokens is not one wave's work; beside them, every id's first place is searched within its last digit's places.
 //   3. rows_kernel: a wave has four rows of dw, and where they have few tokens loads those all at once. Else it adds a
 //      row's places before its first piece, its pieces, and those after the last. An id of more than 16 pieces is a
@@ -30,7 +30,7 @@ constexpr int kDigit = 10, kBins = 1 << kDigit;  // at most
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSmall = 4096;       // tokens that one workgroup sorts
 constexpr int kMaxChunks = 256;
-constexpr int kPiece = 32;
+constexpr int kPiece = 16;
 constexpr int kManyPieces = 16;    // an id of more is a workgroup's
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kVec = 8, kCols = 64 * kVec;  // columns of a lane and of a wave
@@ -178,6 +178,7 @@ __global__ __launch_bounds__(kSortThreads) void hist_kernel(Source src, int64_t 
 struct SortShared {
   int cnt[kSortWaves][kBins];  // of each wave's share of the chunk, then where its tokens of a digit go
   int wave[kSortWaves];
+  int all[kSortThreads], before[kSortThreads];  // a bin's tokens by shares of the chunks
 };
 
 // One pass over a chunk by the whole workgroup. counts: those of all chunks, or null where this is the only one;
@@ -185,17 +186,34 @@ struct SortShared {
 __device__ void scatter(SortShared& s, const Source& src, int64_t n0, int64_t n1, int chunk_i, int chunks, const int* counts, int shift,
                         int digit, const Pairs& out, int* starts) {
   const int bins = 1 << digit, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortThreads) (&s.cnt[0][0])[i] = 0;
-  __syncthreads();
   const int64_t per = (n1 - n0 + kSortWaves - 1) / kSortWaves;
   const int64_t w0 = std::min<int64_t>(n1, n0 + wave * per), w1 = std::min<int64_t>(n1, w0 + per);
-  for (int64_t n = w0 + lane; n < w1; n += 64) atomicAdd(&s.cnt[wave][src.key_of(n) >> shift & (bins - 1)], 1);
+  // all loads at once: the wave's first tokens (up to 262144 tokens in all they are its only ones), and the bin's counts
+  // of all chunks by as many threads as there are for it (one for each bin: 9.1 us at 64 chunks, for 7.9)
+  uint32_t key0 = 0, pos0 = 0;
+  if (w0 + lane < w1) key0 = src.key_of(w0 + lane), pos0 = src.pos_of(w0 + lane);
+  int all = 0, before = 0;
+  if (counts) {
+    const int bin = threadIdx.x & (bins - 1), step = kSortThreads >> digit;
+#pragma unroll 16
+    for (int g = threadIdx.x >> digit; g < chunks; g += step) {
+      const int c = counts[static_cast<int64_t>(g) * bins + bin];
+      all += c;
+      before += g < chunk_i ? c : 0;
+    }
+    s.all[threadIdx.x] = all, s.before[threadIdx.x] = before;
+  }
+  for (int w = 0; w < kSortWaves; ++w)
+    for (int i = threadIdx.x; i < bins; i += kSortThreads) s.cnt[w][i] = 0;
+  __syncthreads();
+  for (int64_t n = w0 + lane; n < w1; n += 64)
+    atomicAdd(&s.cnt[wave][(n == w0 + lane ? key0 : src.key_of(n)) >> shift & (bins - 1)], 1);
   __syncthreads();
   // a thread per bin: the waves' first places within the chunk's tokens of the bin; all tokens of the bin, and those
   // of the chunks before
   const int bin = threadIdx.x;
-  int own = 0, all = 0, before = 0;
   if (bin < bins) {
+    int own = 0;
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       const int c = s.cnt[w][bin];
@@ -203,15 +221,12 @@ __device__ void scatter(SortShared& s, const Source& src, int64_t n0, int64_t n1
       own += c;
     }
     if (counts) {
-#pragma unroll 8
-      for (int g = 0; g < chunks; ++g) {
-        const int c = counts[static_cast<int64_t>(g) * bins + bin];
-        all += c;
-        before += g < chunk_i ? c : 0;
-      }
+      for (int i = bin + bins; i < kSortThreads; i += bins) all += s.all[i], before += s.before[i];
     } else {
       all = own;
     }
+  } else {
+    all = 0;
   }
   // exclusive sums over the bins: within the wave, then over the waves
   int sum = all;
@@ -237,7 +252,8 @@ __device__ void scatter(SortShared& s, const Source& src, int64_t n0, int64_t n1
   for (int64_t base = w0; base < w1; base += 64) {
     const int64_t n = base + lane;
     const bool live = n < w1;
-    const uint32_t key = live ? src.key_of(n) : 0, pos = live ? src.pos_of(n) : 0, d = key >> shift & (bins - 1);
+    const bool again = base > w0 && live;
+    const uint32_t key = again ? src.key_of(n) : key0, pos = again ? src.pos_of(n) : pos0, d = key >> shift & (bins - 1);
     const uint64_t m = peers_of(live, d, digit);
     if (live) {
       const int at = s.cnt[wave][d];
@@ -316,7 +332,7 @@ __device__ __forceinline__ void place(const uint32_t* __restrict__ key, const in
   first[v] = lo;
 }
 
-// The first `piece_wgs` workgroups: part[p, :] = the sum of places [32 p, 32 p + 32) where they are all one id of the
+// The first `piece_wgs` workgroups: part[p, :] = the sum of places [16 p, 16 p + 16) where they are all one id of the
 // table, a wave per piece and kCols columns. The others: the ids' first places.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pieces_kernel(const T* __restrict__ dy, Pairs sorted, int64_t pieces, int piece_wgs, int cols, int D,
