@@ -6,7 +6,7 @@
 //   loss = alpha T^2 mean(KL) + (1 - alpha) mean(CE)
 //   dz = alpha T / n1 (q - sum_k p_k [id_k]) + (1 - alpha) / n2 (softmax(z) - [label])
 // The means are over the n1 rows with an entry that counts (id in [0, V), t not -inf) and the n2 rows with a label in
-// [0, V); a row that is in neither is not read and has a gradient of 0. An id that is listed twice counts twice.
+// [0, V); what a row in neither holds does not matter, its gradient is 0. An id that is listed twice counts twice.
 //
 // A workgroup takes a row and keeps it in registers, as loaded, from its maximum to its sums to its gradient: logits
 // are read once and gradients written once. Rows of more than 64 registers to each of 1024 threads are read twice.
@@ -185,8 +185,9 @@ __device__ __forceinline__ void all_sum(float (&v)[M], float (&red)[M][NT / 64])
   }
 }
 
-// S vectors of a row to each of NT threads, and one of the values behind the last whole vector to the first few;
-// S = 0: rows of any length, read twice. A row that counts for one part alone has a share of 0 of the other's
+// S vectors of a row to each of NT threads, and one of the values before and behind them to the first few; S = 0: rows
+// of any length, read twice. The vectors begin where the row's gradient, which is dense, has a multiple of 16 bytes
+// (with all rows' vectors from their first values, V 50001 took 844 us where V 50000 took 723, 16376 rows). A row that counts for one part alone has a share of 0 of the other's
 // gradient.
 // After a row's gradient (where a row has 16 vectors to a thread and few workgroups share a CU: while it is written,
 // each vector's registers in turn) the next row is loaded, and its entries before that, so that a row begins with all
@@ -207,8 +208,13 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
   __shared__ int s_id[kMaxTop], s_place[kMaxTop];
   __shared__ float s_p[kMaxTop], s_at[kMaxTop], s_put[kMaxTop];
   const int tid = threadIdx.x;
-  const int whole = a.V / kN * kN, last = whole + tid;  // (last: this thread's value behind them, if it has one)
-  const uint32_t whole_bytes = static_cast<uint32_t>(whole) * sizeof(T);
+  // of row n: the values before the vectors, the values in vectors and this thread's value outside of them, if it has one
+  const auto head_of = [&](int64_t n) {
+    const uint32_t off = static_cast<uint32_t>(n) * static_cast<uint32_t>(a.V) % kN;
+    return std::min<int>(off ? kN - off : 0, a.V);
+  };
+  const auto whole_of = [&](int head) { return (a.V - head) / kN * kN; };
+  const auto own_of = [&](int head) { return tid < head ? tid : whole_of(head) + tid; };
   // a thread's first byte of a row, computed anew wherever it is needed (kept from row to row, the places of all S
   // vectors take two registers each)
   const auto here = [](uint32_t t) {
@@ -229,7 +235,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
   if (tid < 2) s_loss[tid] = 0.0;  // (the first thread's)
 
   V16 x[S ? S : 1];
-  // this thread's entries, as loaded, then their ids; the logits there, at the label (-1: none) and behind the vectors
+  // this thread's entries, as loaded, then their ids; the logits there, at the label (-1: none) and beside the vectors
   uint32_t raw_lo[kEntries], raw_hi[kEntries], raw_t[kEntries];
   int id[kEntries], label = -1;
   T at[kEntries], zl, xl;
@@ -252,7 +258,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
     if (kHard) raw_label = a.labels[n];
   };
   const auto teacher = [&](int i) { return __uint_as_float(a.top_bf16 ? raw_t[i] << 16 : raw_t[i]); };
-  const auto fetch_places = [&](const T* z) {
+  const auto fetch_places = [&](const T* z, int head) {
 #pragma unroll
     for (int i = 0; i < kEntries; ++i) {
       id[i] = -1;
@@ -266,7 +272,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
       label = a.inside(raw_label) ? static_cast<int>(raw_label) : -1;
       zl = z[std::max(label, 0)];
     }
-    xl = z[std::min(last, a.V - 1)];
+    xl = z[std::min(own_of(head), a.V - 1)];
     twice = !narrow;
     if (narrow && tid < 64) {  // (while the loads are under way; every entry that is none differs from all)
       const int own = id[0] >= 0 ? id[0] : -1 - tid;
@@ -279,20 +285,21 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
     }
   };
   // a vector that the row does not have is its last one
-  const auto fetch = [&](V16& v, const T* z, uint32_t c) { v.load(at_byte(z, std::min(c, whole_bytes - 16))); };
+  const auto fetch = [&](V16& v, const T* z, uint32_t c, uint32_t whole_bytes) { v.load(at_byte(z, std::min(c, whole_bytes - 16))); };
   int64_t row_b = blockIdx.x / a.T, row_t = blockIdx.x % a.T;
   const int64_t next_b = gridDim.x / a.T, next_t = gridDim.x % a.T;
   const T* z = row_of(row_b, row_t);
-  const auto fetch_row = [&](const T* z, uint32_t step) {
+  const auto fetch_row = [&](const T* z, int head, uint32_t step) {
     if constexpr (S > 0) {
-      const uint32_t c0 = here(tid);
+      const uint32_t c0 = here(tid), bytes = whole_of(head) * static_cast<uint32_t>(sizeof(T));
 #pragma unroll
-      for (int s = 0; s < S; ++s) fetch(x[s], z, c0 + s * step);
+      for (int s = 0; s < S; ++s) fetch(x[s], z + head, c0 + s * step, bytes);
     }
   };
   fetch_entries(blockIdx.x);
-  fetch_row(z, NT * 16);
-  fetch_places(z);
+  int head = head_of(blockIdx.x);
+  fetch_row(z, head, NT * 16);
+  fetch_places(z, head);
   for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
     T* dz = a.dz ? static_cast<T*>(a.dz) + n * a.V : nullptr;
     const bool more_rows = n + gridDim.x < a.N, told = kHard && label >= 0;
@@ -302,6 +309,9 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
       if (row_t >= a.T) row_t -= a.T, ++row_b;
     }
     const T* z_next = row_of(row_b, row_t);
+    const int head_next = head_of(n_next), whole = whole_of(head), own = own_of(head);
+    const uint32_t whole_bytes = static_cast<uint32_t>(whole) * sizeof(T);
+    const uint32_t next_bytes = static_cast<uint32_t>(whole_of(head_next)) * sizeof(T);
     const uint32_t step = more_rows ? NT * 16 : 0;
     // f(vector, its first byte) over the row's whole vectors; `then`: after each of the S, with its number
     const auto each = [&](auto&& f, auto&& then) {
@@ -317,7 +327,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
         }
       } else {
         for (int c = tid * kN; c < whole; c += NT * kN) {
-          x[0].load(z + c);
+          x[0].load(z + head + c);
           f(x[0], static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)));
         }
       }
@@ -335,8 +345,8 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) zm = fmaxf(zm, v.get(j));
     }, nothing);
-    const float behind = last < a.V ? value(&xl) : -INFINITY;
-    zm = fmaxf(zm, behind);
+    const float beside = own < a.V ? value(&xl) : -INFINITY;
+    zm = fmaxf(zm, beside);
     if (const int one = __any(any); tid % 64 == 0) s_any[tid / 64] = one;
     zm = all_max<NT>(zm, s_max);
     bool taught = false;
@@ -408,7 +418,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) add(v.get(j));
     }, nothing);
-    if (last < a.V) add(behind);
+    if (own < a.V) add(beside);
     all_sum<NT>(sum, s_sum);
     const float c1 = uniform(taught ? w1 / sum[0] : 0.0f), c2 = uniform(told ? w2 / sum[kHard ? 1 : 0] : 0.0f);
     const bool counted = taught || told;
@@ -431,7 +441,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
       if (tid == 0 && told) s_loss[1] += kLn2 * (__builtin_amdgcn_logf(sum[kHard ? 1 : 0]) - (zk - zm) * k2);
     }
     if (tid == 0 && taught) s_loss[0] += kLn2 * (teach[1] / teach[0] - __builtin_amdgcn_logf(teach[0]) + __builtin_amdgcn_logf(sum[0]));
-    if (dz && last < a.V) put(dz + last, counted ? slope(behind) : 0.0f);
+    if (dz && own < a.V) put(dz + own, counted ? slope(beside) : 0.0f);
     const int label_place = label;
     fetch_entries(n_next);
     each([&](const V16& v, uint32_t c) {
@@ -441,13 +451,13 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < kN; ++j) d[j] = slope(v.get(j));
       }
-      V16::store(at_byte(dz, c), d);
+      V16::store(at_byte(dz + head, c), d);
     }, [&](V16& v, uint32_t c0, int s) {
-      if constexpr (kAhead) fetch(v, z_next, c0 + s * step);
+      if constexpr (kAhead) fetch(v, z_next + head_next, c0 + s * step, next_bytes);
     });
-    if constexpr (!kAhead) fetch_row(z_next, step);
-    fetch_places(z_next);
-    __syncthreads();  // the row, and what lies behind its vectors, then its places
+    if constexpr (!kAhead) fetch_row(z_next, head_next, step);
+    fetch_places(z_next, head_next);
+    __syncthreads();  // the row, and what lies beside its vectors, then its places
     if (dz) {
 #pragma unroll
       for (int i = 0; i < kEntries; ++i) {
@@ -456,7 +466,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
       }
       if (label_own) put(dz + label_place, label_put);
     }
-    z = z_next;
+    z = z_next, head = head_next;
   }
   if (tid == 0) a.losses[2 * blockIdx.x] = s_loss[0], a.losses[2 * blockIdx.x + 1] = s_loss[1];
 }
@@ -517,7 +527,7 @@ int launch_rows(const Args& a, hipStream_t st) {
     wgs = row_wgs(a.N, wgs_of(NT, S));                                                       \
     hipLaunchKernelGGL((rows_kernel<T, NT, S, kMode>), dim3(wgs), dim3(NT), 0, st, a);       \
   }
-  if (vecs == 0) GO(128, 0)
+  if (a.V < 2 * Vec<T>::kN - 1) GO(128, 0)  // (some row may have no vector)
   else if (vecs <= 512) GO(128, 4)
   else if (vecs <= 1024) GO(128, 8)
   else if (vecs <= 2048) GO(256, 8)

@@ -98,8 +98,8 @@ def distillation_loss(logits, top_ids, top_logits, labels=None, temperature=1.0,
     1 <= K <= 512, labels [...] (an integer type) or None where alpha is 1. The teacher's distribution
     is over its K entries alone; one whose id is outside [0, V) or whose logit is -inf is none, and
     an id that is listed twice counts twice. Rows without an entry, and labels outside [0, V) such as
-    -100, do not count: each mean is over the rows that do, and 0 where none does. A row that counts
-    for neither is not read.
+    -100, do not count: each mean is over the rows that do, and 0 where none does. What a
+    row that counts for neither holds does not matter.
 
     Returns the loss, a float32 scalar. The gradient reaches logits, in their dtype, once and in
     reverse mode; it is made in the forward's pass and kept until the backward, which multiplies it

@@ -841,7 +841,7 @@ int mg_embedding_sorted_bwd(int id_bytes, const void* ids, int64_t N, int dy_dty
  *   loss = alpha temperature^2 mean(KL) + (1 - alpha) mean(CE)
  * An entry with an id outside [0, V) or a t of -inf is none; KL's mean is over
  * the rows with an entry, CE's over those with a label in [0, V); a part that
- * no row is in is 0. A row in neither is not read and has a gradient of 0.
+ * no row is in is 0. A row in neither may hold anything; its gradient is 0.
  * labels NULL or alpha 1: no CE; alpha 0: no KL.
  * logits: element (b, t, v) at p + b sb + t st + v, B T < 2^31 rows, fp32 or
  * bf16, of any alignment. ids [B T, K] int32 or int64, top [B T, K] fp32 or

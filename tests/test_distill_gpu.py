@@ -95,6 +95,17 @@ def test_parity(V, K, dtype):
     _check(*ops[:3], None, 1.0, 1.0)
 
 
+@pytest.mark.parametrize("dtype", [f32, bf16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [2, 6, 7, 8, 9, 13, 14, 15, 16, 17, 23, 31, 513, 514])
+def test_rows_begin_anywhere_in_a_vector(V, dtype):
+    """Nine rows, each at another distance from a multiple of 16 bytes; few values, of which no vector may be full; strides."""
+    ops = _operands((9,), V, 2, dtype)
+    _check(*ops, 2.0, 0.7)
+    _check(*_operands((3, 4), V, 2, dtype, seed=5), 1.0, 0.4)
+    z, ids, top, labels = _operands((3, 4), V, 2, dtype, seed=6)
+    _check(torch.cat([z, z[:, :1] * float("nan")], 1)[:, :-1], ids, top, labels, 4.0, 0.5)
+
+
 @pytest.mark.parametrize("temperature,alpha", [(1.0, 0.5), (0.25, 1.0), (7.0, 0.0), (4.0, 0.9), (1000.0, 0.5)])
 def test_shares_and_temperatures(temperature, alpha):
     for dtype in (f32, bf16):
