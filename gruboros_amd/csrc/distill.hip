@@ -9,13 +9,19 @@
 // [0, V); what a row in neither holds does not matter, its gradient is 0. An id that is listed twice counts twice.
 //
 // A workgroup takes a row and keeps it in registers, as loaded, from its maximum to its sums to its gradient: logits
-// are read once and gradients written once. Rows of more than 64 registers to each of 1024 threads are read twice.
+// are read once and gradients written once. Rows of more than 64 registers to each of 1024 threads (131072 values in bfloat16) are read twice.
 // Everything is in powers of two: with k = log2(e) / T a term is 2^((z - max z) k), in the sums and in the logarithms
 // alike. (The difference first: with a product z k + b the rounding of b = -k max z overflows the power for logits of
 // the type's lowest value.) The few places that an entry or the label changes are
 // written again after the row, by the threads that hold the entries. Losses are summed in double, in a fixed order.
 //
 // A small kernel counts n1 and n2 first; the last adds the workgroups' losses.
+//
+// Bound by memory as long as a row's sums and another's loads overlap: with bfloat16, 16376 rows of 32000 (K 64, labels)
+// take 455 us (2.1 GB, 4.6 TB/s), 2044 rows of 131071 (K 32), of which a CU holds one, 257 us (1.07 GB, 4.2 TB/s). For
+// rows this long a CU's registers are full with one of them, and memory waits while its sums are made; holding the
+// beginning of the next row as well (4 to 8 of 16 vectors) costs registers that are missing elsewhere (278 to 310 us
+// where 283 was the time without).
 
 #include <algorithm>
 
@@ -517,7 +523,9 @@ constexpr int wgs_of(int nt, int s) { return 256 * 4 * 64 * waves_of(nt, s) / nt
 inline int row_wgs(int64_t N, int most) { return static_cast<int>(std::min<int64_t>(N, most)); }
 
 // Few threads and many vectors to each: a row costs each of its waves about the same beyond its vectors (sums over the
-// workgroup, entries). Returns the workgroups
+// workgroup, entries). With half the threads and twice the vectors 16376 rows of V 4001, 8001, 16001 and 32000 take 111,
+// 163, 283 and 481 us, with twice the threads and half the vectors 128, 158, 270 and 747, with these 107, 155, 264 and
+// 470. Returns the workgroups
 template <typename T, int kMode>
 int launch_rows(const Args& a, hipStream_t st) {
   const int64_t vecs = a.V / Vec<T>::kN;

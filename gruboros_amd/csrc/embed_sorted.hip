@@ -17,7 +17,10 @@
 //      workgroup's.
 // Sums are fp32, rounded once to the table's type.
 //
-// Bound by memory: dy is read once, dw written once.
+// Bound by memory (dy is read once, dw written once), and for fewer tokens by the chain of launches. Measured, bfloat16
+// gradients, D 1024, tokens drawn by rank: 16376 tokens, V 32000, fp32 table: lookup 13.5 us, sort 18, pieces 5, rows
+// 30 (131 MB written, 4.4 TB/s); 65528 tokens, V 131071, bfloat16 table: lookup 48, sort 25, pieces 17, rows 89 us (268
+// MB written, 4.5 TB/s with the gradients read).
 
 #include <algorithm>
 
@@ -28,7 +31,9 @@ namespace embed_sorted {
 
 constexpr int kDigit = 10, kBins = 1 << kDigit;  // at most
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kSmall = 4096;       // tokens that one workgroup sorts
+// Tokens that one workgroup sorts (3000 tokens: 50 us either way, in three launches fewer; 5000 and 8000: 69 and 74 us
+// in one workgroup, 46 and 47 in several)
+constexpr int kSmall = 4096;
 constexpr int kMaxChunks = 256;
 constexpr int kPiece = 16;
 constexpr int kManyPieces = 16;    // an id of more is a workgroup's

@@ -20,6 +20,11 @@
 // The order of every sum is fixed, whatever the timing.
 //
 // The state is kept every 8 steps in fp32 for the backward (half a byte per value); the steps between are made again.
+//
+// Bound by memory and, by a fifth, arithmetic. bfloat16, B8 T2047 D1024: forward 40 us (142 MB, 3.5 TB/s; 33 with no
+// arithmetic and no carries, 36 with the carries alone), backward 58 (243 MB, 4.2 TB/s). B2 T16381 D2048, forward: 132
+// us (537 MB, 4.1 TB/s), with resets 148: forgetting also what is not finite takes selects with every value. (Taking
+// them in the waves alone that have a reset: 146, and the registers leave room for fewer waves.)
 
 #include <algorithm>
 

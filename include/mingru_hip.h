@@ -48,8 +48,9 @@ extern "C" {
  * declared in this file (0.2.1 to 0.2.5 add entry points to 0.2.0 and change
  * none; 0.2.6 changes no signature: mg_gemm also splits small bf16 products
  * along K, see mg_gemm, and mg_gemm_f32, mg_gemm_group, mg_gemm_hilo_cols,
- * mg_scan_fwd_pair, mg_delta_*, mg_layernorm_* and mg_dropout are additions
- * under the same number). */
+ * mg_scan_fwd_pair, mg_delta_*, mg_layernorm_*, mg_dropout, mg_recurrence_*,
+ * mg_block_norm_*, mg_embedding_fwd, mg_embedding_sorted_*, mg_distill*,
+ * mg_scale_inplace and mg_capture_id are additions under the same number). */
 int mg_version(void);
 
 /* Message of the last failed call on this thread ("" if none). */
