@@ -31,11 +31,14 @@ namespace mg {
 namespace distill {
 
 constexpr int kMaxTop = 512;
-constexpr int kCountRows = 32, kCountWgs = 256, kRowWgs = 3072;
+constexpr int kCountRows = 32, kCountWgs = 256, kRowWgs = 6144;
 
 // The teacher's part alone; with the labels': an exponential for each, or, at the temperatures 1, 2 and 4, that of the
 // labels' as a power of the teacher's (e^z = (e^{z/T})^T).
 constexpr int kSoft = 0, kBoth = 1, kT1 = 2, kT2 = 3, kT4 = 4;
+
+// Entries that a workgroup has room for
+constexpr int top_of(int nt) { return nt == 64 ? 64 : kMaxTop; }
 
 constexpr bool ahead(int s) { return s >= 16; }
 
@@ -204,15 +207,15 @@ template <typename T, int NT, int S, int kMode>
 __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
   constexpr bool kHard = kMode != kSoft, kAhead = ahead(S);
   using V16 = Vec<T>;
-  constexpr int kN = V16::kN, kEntries = (kMaxTop + NT - 1) / NT;
+  constexpr int kN = V16::kN, kTop = top_of(NT), kEntries = (kTop + NT - 1) / NT;
   constexpr float kLn2 = 0.6931471805599453f;
   __shared__ float s_max[NT / 64], s_teacher[NT / 64], s_sum[kHard ? 2 : 1][NT / 64], s_teach[2][NT / 64];
   __shared__ int s_count[2], s_any[NT / 64], s_mine[NT / 64];
   __shared__ double s_loss[2];
   // of the entries: id (-1: none), unnormalised probability; of those that are the first of their id the place (else
   // -1), the logit there and what the gradient there has beyond the student's
-  __shared__ int s_id[kMaxTop], s_place[kMaxTop];
-  __shared__ float s_p[kMaxTop], s_at[kMaxTop], s_put[kMaxTop];
+  __shared__ int s_id[kTop], s_place[kTop];
+  __shared__ float s_p[kTop], s_at[kTop], s_put[kTop];
   const int tid = threadIdx.x;
   // of row n: the values before the vectors, the values in vectors and this thread's value outside of them, if it has one
   const auto head_of = [&](int64_t n) {
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
   };
   const auto row_of = [&](int64_t b, int64_t t) { return static_cast<const T*>(a.z) + b * a.sb + t * a.st; };
   const int entries = a.soft ? a.K : 0;
-  const bool narrow = a.K <= 64;
+  const bool narrow = kTop == 64 || a.K <= 64;
   all_counts(a, s_count);
   const float w1 = uniform(s_count[0] ? a.alpha * a.temperature / static_cast<float>(s_count[0]) : 0.0f);
   const float w2 = uniform(s_count[1] ? (1.0f - a.alpha) / static_cast<float>(s_count[1]) : 0.0f);
@@ -525,7 +528,8 @@ inline int row_wgs(int64_t N, int most) { return static_cast<int>(std::min<int64
 // Few threads and many vectors to each: a row costs each of its waves about the same beyond its vectors (sums over the
 // workgroup, entries). With half the threads and twice the vectors 16376 rows of V 4001, 8001, 16001 and 32000 take 111,
 // 163, 283 and 481 us, with twice the threads and half the vectors 128, 158, 270 and 747, with these 107, 155, 264 and
-// 470. Returns the workgroups
+// 470. Of up to 64 entries a row of few vectors is one wave's business, which waits for no other: at V 1001 (31000 rows),
+// 2040, 4001, 6001 and 8001, 66, 65, 79, 102 and 142 us, with two waves 99, 86, 98, 131 and 154. Returns the workgroups
 template <typename T, int kMode>
 int launch_rows(const Args& a, hipStream_t st) {
   const int64_t vecs = a.V / Vec<T>::kN;
@@ -536,6 +540,11 @@ int launch_rows(const Args& a, hipStream_t st) {
     hipLaunchKernelGGL((rows_kernel<T, NT, S, kMode>), dim3(wgs), dim3(NT), 0, st, a);       \
   }
   if (a.V < 2 * Vec<T>::kN - 1) GO(128, 0)  // (some row may have no vector)
+  else if (a.K <= 64 && vecs <= 128) GO(64, 2)
+  else if (a.K <= 64 && vecs <= 256) GO(64, 4)
+  else if (a.K <= 64 && vecs <= 512) GO(64, 8)
+  else if (a.K <= 64 && vecs <= 768) GO(64, 12)
+  else if (a.K <= 64 && vecs <= 1024) GO(64, 16)
   else if (vecs <= 512) GO(128, 4)
   else if (vecs <= 1024) GO(128, 8)
   else if (vecs <= 2048) GO(256, 8)

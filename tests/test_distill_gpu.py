@@ -106,6 +106,17 @@ def test_rows_begin_anywhere_in_a_vector(V, dtype):
     _check(torch.cat([z, z[:, :1] * float("nan")], 1)[:, :-1], ids, top, labels, 4.0, 0.5)
 
 
+@pytest.mark.parametrize("dtype", [f32, bf16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V,K", [(515, 64), (1030, 64), (1030, 65), (2056, 7), (2060, 64), (3070, 64), (4100, 64), (4101, 65), (6143, 1), (6150, 64),
+                                 (8191, 64), (8199, 63)])
+def test_up_to_64_entries_and_more(V, K, dtype):
+    """Rows that one wave, two or more have, at the ends of each."""
+    ops = _operands((1, 7), V, K, dtype)
+    _check(*ops, 2.0, 0.7)
+    _check(*ops, 3.0, 0.3)
+    _check(*ops[:3], None, 1.0, 1.0)
+
+
 @pytest.mark.parametrize("temperature,alpha", [(1.0, 0.5), (0.25, 1.0), (7.0, 0.0), (4.0, 0.9), (1000.0, 0.5)])
 def test_shares_and_temperatures(temperature, alpha):
     for dtype in (f32, bf16):
