@@ -23,8 +23,7 @@
 //
 // Bound by memory and, by a fifth, arithmetic. bfloat16, B8 T2047 D1024: forward 40 us (142 MB, 3.5 TB/s; 33 with no
 // arithmetic and no carries, 36 with the carries alone), backward 58 (243 MB, 4.2 TB/s). B2 T16381 D2048, forward: 132
-// us (537 MB, 4.1 TB/s), with resets 148: forgetting also what is not finite takes selects with every value. (Taking
-// them in the waves alone that have a reset: 146, and the registers leave room for fewer waves.)
+// us (537 MB, 4.1 TB/s), with resets 140: forgetting also what is not finite takes selects with every value.
 
 #include <algorithm>
 
@@ -164,16 +163,7 @@ __device__ __forceinline__ void decay_terms(float gate, float crate, float& r, f
   m = __builtin_amdgcn_sqrtf(one_minus(2.0f * l, a));
 }
 
-// The map h -> a h + v after the map h -> A h + V. With kReset an a of 0 forgets what came before, be it finite or not.
-template <bool kReset>
-__device__ __forceinline__ void then(float a, float v, float& A, float& V) {
-  if (kReset && a == 0.0f) {
-    A = 0.0f, V = v;
-  } else {
-    V = __builtin_fmaf(a, V, v);
-    A *= a;
-  }
-}
+// The map h -> a h + v of a run or a tile. With kReset an a of 0 forgets what came before, be it finite or not.
 template <bool kReset>
 __device__ __forceinline__ float apply(float a, float h, float v) {
   return kReset && a == 0.0f ? v : __builtin_fmaf(a, h, v);
@@ -325,10 +315,13 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
     for (int j = 0; j < kVec; ++j) {
       float r, m;
       decay_terms(gr[i].get(j), rate.v[j], r, a[i][j], m);
-      if (kReset && (fresh >> i & 1)) a[i][j] = 0.0f, m = 1.0f;
+      const bool cut = kReset && (fresh >> i & 1);
+      if (cut) m = 1.0f;
       v[i][j] = m * (sigma(gi[i].get(j)) * x[i].get(j));
       if (i >= rows) a[i][j] = 1.0f, v[i][j] = 0.0f;  // past the end nothing changes
-      then<kReset>(a[i][j], v[i][j], A.v[j], V.v[j]);
+      // (the bits themselves, not a made 0 and compared again: B2 T16381 D2048 149 -> 141 us)
+      V.v[j] = cut ? v[i][j] : __builtin_fmaf(a[i][j], V.v[j], v[i][j]);
+      A.v[j] = cut ? 0.0f : A.v[j] * a[i][j];
     }
   }
   const int buf = scan_runs<false, kReset>(s_maps, s, cl, A, V);
@@ -361,7 +354,7 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
 #pragma unroll
   for (int i = 0; i < kFwdRows; ++i) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) h.v[j] = apply<kReset>(a[i][j], h.v[j], v[i][j]);
+    for (int j = 0; j < kVec; ++j) h.v[j] = kReset && (fresh >> i & 1) ? v[i][j] : __builtin_fmaf(a[i][j], h.v[j], v[i][j]);
     if (i < rows) store4_nt(out + static_cast<int64_t>(i) * g.D, h, left);
     if (i + 1 == rows && p.last) store4(p.last + row, h, left);
   }
