@@ -82,6 +82,13 @@ def test_parity(shape, types, form):
     _compare(ops, dres, dy, form[0] or "silu", yt)
 
 
+@pytest.mark.parametrize("shape", [(1, 4500, 260), (1, 1500, 1100), (2, 300, 4100), (1, 530, 8195), (1, 530, 12289)], ids=lambda s: "x".join(map(str, s)))
+def test_more_rows_than_workgroups(shape):
+    """Sums over several rows of one workgroup, of every number of threads to a row, and those kept in LDS."""
+    for types in ((bf16, bf16), (f32, f32)):
+        _compare(*_operands(shape, types[0], True, True), "silu", types[1])
+
+
 def test_views():
     """Columns of wider tensors at odd offsets, transposed batch, weights of other types."""
     ops, dres, dy = _operands((6, 10, 97), bf16, True, True)
