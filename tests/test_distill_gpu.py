@@ -134,6 +134,13 @@ def test_many_rows():
     assert torch.equal(distillation_loss(*a, 2.0, 0.6), distillation_loss(a[0], a[1].int(), a[2], a[3].int(), 2.0, 0.6))
 
 
+@pytest.mark.parametrize("N,V,K,dtype", [(6500, 261, 4, f32), (3300, 71, 70, bf16), (1600, 12001, 9, bf16), (1100, 17003, 5, bf16), (600, 33001, 5, bf16),
+                                         (300, 66001, 5, bf16), (300, 131077, 3, bf16)])
+def test_several_rows_of_one_workgroup(N, V, K, dtype):
+    """Rows that are loaded while the one before is written, with entries, heads and ends of their own."""
+    _check(*_operands((N,), V, K, dtype), 2.0, 0.6)
+
+
 def test_listed_twice_and_labels_among_the_listed():
     z, ids, top, labels = _operands((4, 5), 100, 30, f32, masked=False)
     ids[..., 10:20] = ids[..., :10]
