@@ -18,7 +18,7 @@
 // A small kernel counts n1 and n2 first; the last adds the workgroups' losses.
 //
 // Bound by memory as long as a row's sums and another's loads overlap: with bfloat16, 16376 rows of 32000 (K 64, labels)
-// take 455 us (2.1 GB, 4.6 TB/s), 2044 rows of 131071 (K 32), of which a CU holds one, 257 us (1.07 GB, 4.2 TB/s). For
+// take 455 us (2.1 GB, 4.6 TB/s), 2044 rows of 131071 (K 32), of which a CU holds one, 251 us (1.07 GB, 4.3 TB/s). For
 // rows this long a CU's registers are full with one of them, and memory waits while its sums are made; holding the
 // beginning of the next row as well (4 to 8 of 16 vectors) costs registers that are missing elsewhere (278 to 310 us
 // where 283 was the time without).
@@ -139,15 +139,17 @@ __host__ __device__ __forceinline__ int count_wgs(int64_t N) {
 }
 static_assert(kCountWgs == 256, "a thread of loss_kernel for each");
 
-// (n1, n2), by a whole workgroup
+// (n1, n2), by the first wave (with counters in LDS that every thread adds to, 31000 rows of V 1001 take 61 us, not 52)
 __device__ __forceinline__ void all_counts(const Args& a, int (&s)[2]) {
   const int g = count_wgs(a.N);
-  if (threadIdx.x < 2) s[threadIdx.x] = 0;
-  __syncthreads();
-  int2 c = make_int2(0, 0);
-  for (int i = threadIdx.x; i < g; i += blockDim.x) c.x += a.counts[2 * i], c.y += a.counts[2 * i + 1];
-  atomicAdd(&s[0], c.x);
-  atomicAdd(&s[1], c.y);
+  if (threadIdx.x < 64) {
+    int n1 = 0, n2 = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < g; i += 64) n1 += a.counts[2 * i], n2 += a.counts[2 * i + 1];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n1 += __shfl_xor(n1, o, 64), n2 += __shfl_xor(n2, o, 64);
+    if (threadIdx.x == 0) s[0] = n1, s[1] = n2;
+  }
   __syncthreads();
 }
 
@@ -541,10 +543,10 @@ constexpr int wgs_of(int nt, int s) { return 256 * 4 * 64 * waves_of(nt, s) / nt
 inline int row_wgs(int64_t N, int most) { return static_cast<int>(std::min<int64_t>(N, most)); }
 
 // Few threads and many vectors to each: a row costs each of its waves about the same beyond its vectors (sums over the
-// workgroup, entries). With half the threads and twice the vectors 16376 rows of V 4001, 8001, 16001 and 32000 take 111,
-// 163, 283 and 481 us, with twice the threads and half the vectors 128, 158, 270 and 747, with these 107, 155, 264 and
-// 470. Of up to 64 entries a row of few vectors is one wave's business, which waits for no other: at V 1001 (31000 rows),
-// 2040, 4001, 6001 and 8001, 66, 65, 79, 102 and 142 us, with two waves 99, 86, 98, 131 and 154. Returns the workgroups
+// workgroup, entries). With half the threads and twice the vectors 16376 rows of V 16001 and 32000 take 266 and 469 us,
+// with twice the threads and half the vectors 254 and 731, with these 257 and 470. Of up to 64 entries a row of few
+// vectors is one wave's business, which waits for no other: at V 1001 (31000 rows), 2040, 4001, 6001 and 8001, 55, 51,
+// 67, 91 and 128 us, with two waves 91, 74, 87, 121 and 146. Returns the workgroups
 template <typename T, int kMode>
 int launch_rows(const Args& a, hipStream_t st) {
   const int64_t vecs = a.V / Vec<T>::kN;
