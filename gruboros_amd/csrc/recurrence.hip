@@ -163,10 +163,14 @@ __device__ __forceinline__ void decay_terms(float gate, float crate, float& r, f
   m = __builtin_amdgcn_sqrtf(one_minus(2.0f * l, a));
 }
 
-// The map h -> a h + v of a run or a tile. With kReset an a of 0 forgets what came before, be it finite or not.
+// The map h -> a h + v of a run or a tile. With kReset an a of -0 forgets what came before, be it finite or not: that is
+// what a reset gives, and any product with it. A product of decays that underflows is +0: it forgets finite values, and
+// what is not finite stays so.
+constexpr float kCut = -0.0f;
+__device__ __forceinline__ bool is_cut(float a) { return __float_as_uint(a) == __float_as_uint(kCut); }
 template <bool kReset>
 __device__ __forceinline__ float apply(float a, float h, float v) {
-  return kReset && a == 0.0f ? v : __builtin_fmaf(a, h, v);
+  return kReset && is_cut(a) ? v : __builtin_fmaf(a, h, v);
 }
 
 // ------------------------------------------------------------------ tiles and carries
@@ -189,7 +193,7 @@ __device__ __forceinline__ int scan_runs(Maps& m, int s, int cl, f4 A, f4 V) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         V.v[j] = apply<kReset>(A.v[j], pv.v[j], V.v[j]);
-        A.v[j] = kReset && A.v[j] == 0.0f ? 0.0f : A.v[j] * pa.v[j];
+        A.v[j] = kReset && is_cut(A.v[j]) ? kCut : A.v[j] * pa.v[j];
       }
     }
     buf ^= 1;
@@ -206,6 +210,18 @@ __device__ __forceinline__ int take_tile(const Grid& g, uint32_t* tickets, uint3
   if (threadIdx.x == 0) *s_ticket = atomicAdd(tickets + chain, 1u);
   __syncthreads();
   return static_cast<int>(__builtin_amdgcn_readfirstlane(*s_ticket));
+}
+
+// A tile's map for the tiles after it: of an A without a sign, and the bit that calls that keep their words alternate
+// instead (a NaN has that bit too: then the V beside it is NaN, and forgets or not)
+template <bool kReset>
+__device__ __forceinline__ void publish_map(uint64_t* word, float A, float V) {
+  publish_agg(word, A, V, kReset && is_cut(A));
+}
+template <bool kReset>
+__device__ __forceinline__ float map_of(uint32_t tag) {
+  if (kReset && (tag & kTagParity)) return kCut;
+  return __uint_as_float(tag & ~kTagAggBit);
 }
 
 // What enters tile k of channel c: back (step -1) or on (+1) to the nearest tile whose result is known, then through
@@ -261,7 +277,7 @@ __device__ __forceinline__ float look_back(const uint64_t* words, int64_t BD, in
     for (int q = 0; q < kAt; ++q) {
       if (i == k) continue;
       const uint32_t tag = static_cast<uint32_t>(x[q]);
-      carry = tag == kTagIncl ? value(x[q]) : apply<kReset>(__uint_as_float(tag & ~kTagAggBit), carry, value(x[q]));
+      carry = tag == kTagIncl ? value(x[q]) : apply<kReset>(map_of<kReset>(tag), carry, value(x[q]));
       i -= step;
     }
   }
@@ -321,7 +337,7 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
       if (i >= rows) a[i][j] = 1.0f, v[i][j] = 0.0f;  // past the end nothing changes
       // (the bits themselves, not a made 0 and compared again: B2 T16381 D2048 149 -> 141 us)
       V.v[j] = cut ? v[i][j] : __builtin_fmaf(a[i][j], V.v[j], v[i][j]);
-      A.v[j] = cut ? 0.0f : A.v[j] * a[i][j];
+      A.v[j] = cut ? kCut : A.v[j] * a[i][j];
     }
   }
   const int buf = scan_runs<false, kReset>(s_maps, s, cl, A, V);
@@ -335,7 +351,7 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
     if (k == 0) {
       carry = p.h0 ? p.h0[row + s] : 0.0f;
     } else {
-      publish_agg(words + k * BD, TA, TV, 0);
+      publish_map<kReset>(words + k * BD, TA, TV);
       carry = look_back<kReset>(words, BD, k, -1, 0);
     }
     if (k + 1 < g.tiles) publish_incl(words + k * BD, apply<kReset>(TA, carry, TV), 0);
@@ -421,7 +437,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(B
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       decay_terms(gr[i].get(j), rate.v[j], r[i][j], a[i][j], m[i][j]);
-      if (kReset && (fresh >> i & 1)) a[i][j] = 0.0f, m[i][j] = 1.0f;
+      if (kReset && (fresh >> i & 1)) a[i][j] = kCut, m[i][j] = 1.0f;
       if (i >= rows) a[i][j] = 1.0f, m[i][j] = 0.0f;
       gate[i][j] = sigma(gi[i].get(j));
     }
@@ -440,9 +456,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(B
   for (int i = kRows - 1; i >= 0; --i)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const bool cut = kReset && a[i][j] == 0.0f;
+      const bool cut = kReset && is_cut(a[i][j]);
       M.v[j] = cut ? 0.0f : a[i][j] * (dh[i].get(j) + M.v[j]);
-      A.v[j] = cut ? 0.0f : A.v[j] * a[i][j];
+      A.v[j] = cut ? kCut : A.v[j] * a[i][j];
     }
   const int buf = scan_runs<true, kReset>(s_maps, s, cl, A, M);
 
@@ -456,7 +472,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(B
         // (the steps past the end pass it on unchanged)
         if (p.dlast) carry = p.dlast[row + q];
       } else {
-        publish_agg(words + k * BD, TA, TM, 0);
+        publish_map<kReset>(words + k * BD, TA, TM);
         carry = look_back<kReset>(words, BD, k, 1, g.tiles - 1);
       }
       if (k > 0) publish_incl(words + k * BD, apply<kReset>(TA, carry, TM), 0);
@@ -479,7 +495,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(B
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         lam[i][j] = dh[i].get(j) + mu.v[j];
-        mu.v[j] = kReset && a[i][j] == 0.0f ? 0.0f : a[i][j] * lam[i][j];
+        mu.v[j] = kReset && is_cut(a[i][j]) ? 0.0f : a[i][j] * lam[i][j];
       }
     if (p.dh0 && t0 == 0) store4(p.dh0 + row, mu, left);
     const int64_t out = (static_cast<int64_t>(b) * g.T + t0) * g.D + d;

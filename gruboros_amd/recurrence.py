@@ -53,8 +53,8 @@ def gated_recurrence(x, input_gate, decay_gate, decay, initial_state=None, reset
     Returns h [B, T, D] in x's dtype, or (h, last state float32 [B, D]) with return_state. Gradients
     reach all tensors but reset, once and in reverse mode. Where they are recorded, the state of
     every eighth token is kept in fp32 for the backward, half a byte per value; a decay gate that is
-    shut (its sigmoid is 0 in float32) has no gradient. Without `reset` a value that is not finite
-    spoils what follows it in its row and channel."""
+    shut (its sigmoid is 0 in float32) has no gradient. A value that is not finite
+    spoils what follows it in its row and channel, up to the next reset."""
     _check(x, input_gate, decay_gate, decay, initial_state, "initial_state", 3)
     c = _rate(c)
     if reset is not None:
