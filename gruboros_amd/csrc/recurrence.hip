@@ -147,6 +147,23 @@ __device__ __forceinline__ uint32_t starts(const uint8_t* p, int rows) {
 
 __device__ __forceinline__ float sigma(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_raw(x * -kLog2e)); }
 
+// sigma(x) and 1 - sigma(x), each with all its digits (1 minus the rounded sigma has lost them all at x = 17), in one
+// register: sigma where x is negative, else 1 - sigma with its sign turned. A value k of either kind is sigma or one
+// less, so that the fraction of k is sigma, and that of -k is 1 - sigma; 2^-126 keeps the latter off 0, whose fraction
+// is 0 on both sides. Hidden from the compiler, which would keep both. (A difference instead: B8 T2047 D1024 63 us, not
+// 64, B2 T16381 D2048 packed 259, not 262; both sides by selects 65 and 268.)
+struct Sides {
+  float k;
+  __device__ __forceinline__ float of(float x) {
+    const float e = exp2_raw(x * -kLog2e), s = __builtin_amdgcn_rcpf(1.0f + e);
+    k = x >= 0.0f ? -__builtin_fmaf(e, s, 0x1p-126f) : s;
+    asm volatile("" : "+v"(k));
+    return s;
+  }
+  __device__ __forceinline__ float open() const { return __builtin_amdgcn_fractf(k); }
+  __device__ __forceinline__ float shut() const { return __builtin_amdgcn_fractf(-k); }
+};
+
 __device__ __forceinline__ float softplus(float x) { return log1pf(expf(-fabsf(x))) + fmaxf(x, 0.0f); }
 
 // 1 - e^{-w}, w >= 0, of which a = e^{-w/2} is known
@@ -155,10 +172,8 @@ __device__ __forceinline__ float one_minus(float w, float a) {
   return w <= 0.25f ? s : 1.0f - a * a;
 }
 
-// crate = c softplus(decay): a, m from the decay gate, with r
-__device__ __forceinline__ void decay_terms(float gate, float crate, float& r, float& a, float& m) {
-  r = sigma(gate);
-  const float l = crate * r;  // (-l_t)
+// a, m from l = c softplus(decay) sigma(decay_gate) (-l_t)
+__device__ __forceinline__ void decay_terms(float l, float& a, float& m) {
   a = exp2_raw(l * -kLog2e);
   m = __builtin_amdgcn_sqrtf(one_minus(2.0f * l, a));
 }
@@ -329,8 +344,8 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(Fwd p) {
   for (int i = 0; i < kFwdRows; ++i) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      float r, m;
-      decay_terms(gr[i].get(j), rate.v[j], r, a[i][j], m);
+      float m;
+      decay_terms(rate.v[j] * sigma(gr[i].get(j)), a[i][j], m);
       const bool cut = kReset && (fresh >> i & 1);
       if (cut) m = 1.0f;
       v[i][j] = m * (sigma(gi[i].get(j)) * x[i].get(j));
@@ -431,23 +446,25 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(B
   __syncthreads();
   const f4 rate = *reinterpret_cast<const f4*>(&s_rate[cl * kVec]);
 
-  float a[kRows][kVec], m[kRows][kVec], r[kRows][kVec], gate[kRows][kVec];
+  float a[kRows][kVec], m[kRows][kVec];
+  Sides r[kRows][kVec], gate[kRows][kVec];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      decay_terms(gr[i].get(j), rate.v[j], r[i][j], a[i][j], m[i][j]);
+      decay_terms(rate.v[j] * r[i][j].of(gr[i].get(j)), a[i][j], m[i][j]);
       if (kReset && (fresh >> i & 1)) a[i][j] = kCut, m[i][j] = 1.0f;
       if (i >= rows) a[i][j] = 1.0f, m[i][j] = 0.0f;
-      gate[i][j] = sigma(gi[i].get(j));
+      gate[i][j].of(gi[i].get(j));
     }
+    __builtin_amdgcn_sched_barrier(0);  // (B2 T16381 D2048 packed 267 us, 270 without)
   }
   if (!(s & 1)) {  // the next run's entering state
     f4 e = h;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) e.v[j] = apply<kReset>(a[i][j], e.v[j], m[i][j] * (gate[i][j] * x[i].get(j)));
+      for (int j = 0; j < kVec; ++j) e.v[j] = apply<kReset>(a[i][j], e.v[j], m[i][j] * (gate[i][j].open() * x[i].get(j)));
     s_mid[s / 2][cl] = e;
   }
   // the run as a map of what comes back through it: mu -> A mu + M, mu_t = a_t lam_t
@@ -504,14 +521,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) void bwd_kernel(B
       f4 ox, oi, og;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const float u = gate[i][j] * x[i].get(j), lm = lam[i][j] * m[i][j];
-        ox.v[j] = lm * gate[i][j];
-        oi.v[j] = lm * (u * (1.0f - gate[i][j]));
+        const float u = gate[i][j].open() * x[i].get(j), lm = lam[i][j] * m[i][j];
+        ox.v[j] = lm * gate[i][j].open();
+        oi.v[j] = lm * (u * gate[i][j].shut());
         // l / m is 0 with m, and its square with a
-        const float l = -rate.v[j] * r[i][j], q = l * __builtin_amdgcn_rcpf(fmaxf(m[i][j], 1e-30f));
+        const float l = -rate.v[j] * r[i][j].open(), q = l * __builtin_amdgcn_rcpf(fmaxf(m[i][j], 1e-30f));
         float w = lam[i][j] * (a[i][j] * (h.v[j] * l - u * (a[i][j] * q)));
         if (kReset && (fresh >> i & 1)) w = 0.0f;
-        og.v[j] = w * (1.0f - r[i][j]);
+        og.v[j] = w * r[i][j].shut();
         if (i < rows) sum.v[j] += w;
         h.v[j] = apply<kReset>(a[i][j], h.v[j], m[i][j] * u);
       }
@@ -581,8 +598,8 @@ __global__ __launch_bounds__(64) void step_kernel(Step p) {
     f4 h = load4(sp, left);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float r, a, m;
-      decay_terms(gr.v[j], p.c * softplus(decay.v[j]), r, a, m);
+      float a, m;
+      decay_terms(p.c * softplus(decay.v[j]) * sigma(gr.v[j]), a, m);
       h.v[j] = __builtin_fmaf(a, h.v[j], m * (sigma(gi.v[j]) * x.v[j]));
     }
     store4(sp, h, left);
