@@ -49,17 +49,16 @@ __device__ __forceinline__ int64_t first_row() {
          (TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
 }
 
-__device__ __forceinline__ float sigma(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_raw(x * -kLog2e)); }
-
-// act(g); slope: act'(g). A gate of -inf shuts: silu's 0 there, not -inf 0.
+// act(g); slope: act'(g). A gate of -inf shuts: silu's 0 there, not -inf 0. 1 - sigma is made from the power, since the
+// rounded sigma of an open gate has lost its digits; where the power is infinite, it is 1 (the minimum of a NaN and 1).
 __device__ __forceinline__ float act_of(int act, float g, float& slope) {
-  const float s = sigma(g);
+  const float e = exp2_raw(g * -kLog2e), s = __builtin_amdgcn_rcpf(1.0f + e), rest = fminf(e * s, 1.0f);
   if (act == kSigmoid) {
-    slope = s * (1.0f - s);
+    slope = s * rest;
     return s;
   }
   const float v = s == 0.0f ? 0.0f : g * s;
-  slope = s + v * (1.0f - s);
+  slope = s + v * rest;
   return v;
 }
 

@@ -41,3 +41,21 @@ def test_recurrence(dtype):
         got = torch.autograd.grad(gated_recurrence(*dev), dev, dh.to(DEV))
         for name, g, w in zip(("x", "input_gate", "decay_gate", "decay", "initial_state"), got, want):
             _near(g, w, f"d{name}, decay {decay}")
+
+
+@pytest.mark.parametrize("dtype", [f32, bf16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("activation", ["sigmoid", "silu"])
+def test_block_norm(activation, dtype):
+    from gruboros_amd.norm import add_gated_rms_norm
+
+    n = len(GATES)
+    gen = torch.Generator().manual_seed(1)
+    x, branch, dres = (0.5 + torch.rand(n, n, generator=gen) for _ in range(3))
+    branch, gate, w = branch.to(dtype), GATES.expand(n, n).to(dtype).contiguous(), torch.ones(n)
+    ref = gate.double().requires_grad_(True)
+    f = branch.double()
+    b = f / (f.square().mean(-1, keepdim=True) + 1e-6).sqrt() * torch.sigmoid(ref) * (ref if activation == "silu" else 1.0)
+    (want,) = torch.autograd.grad(b, ref, dres.double())
+    leaf = gate.to(DEV).requires_grad_(True)
+    xn, _ = add_gated_rms_norm(x.to(DEV), branch.to(DEV), w.to(DEV), w.to(DEV), gate=leaf, activation=activation, eps=1e-6)
+    _near(torch.autograd.grad(xn, leaf, dres.to(DEV))[0], want, "dgate")
