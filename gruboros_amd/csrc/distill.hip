@@ -11,8 +11,8 @@
 // A workgroup takes a row and keeps it in registers, as loaded, from its maximum to its sums to its gradient: logits
 // are read once and gradients written once. Rows of more than 64 registers to each of 1024 threads (131072 values in bfloat16) are read twice.
 // Everything is in powers of two: with k = log2(e) / T a term is 2^((z - max z) k), in the sums and in the logarithms
-// alike. (The difference first: with a product z k + b the rounding of b = -k max z overflows the power for logits of
-// the type's lowest value.) The few places that an entry or the label changes are
+// alike, of the student and of the teacher. (The difference first: with a product z k + b the rounding of b = -k max z
+// overflows the power for logits of the type's lowest value.) The few places that an entry or the label changes are
 // written again after the row, by the threads that hold the entries. Losses are summed in double, in a fixed order.
 //
 // A small kernel counts n1 and n2 first; the last adds the workgroups' losses.
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
     bool any = false;
 #pragma unroll
     for (int i = 0; i < kEntries; ++i) {
-      if (id[i] >= 0) tm = fmaxf(tm, teacher(i) * k1), any = true;
+      if (id[i] >= 0) tm = fmaxf(tm, teacher(i)), any = true;
       if (tid + i * NT < entries) s_id[tid + i * NT] = id[i];
     }
     each([&](const V16& v, uint32_t) {
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
       if (k >= entries) continue;
       float p = 0.0f;
       if (id[i] >= 0) {
-        const float u = teacher(i) * k1 - tm, zk = value(&at[i]);
+        const float u = (teacher(i) - tm) * k1, zk = value(&at[i]);
         p = exp2_raw(u);
         teach[0] += p;
         if (p != 0.0f) teach[1] += p * (u - (zk - zm) * k1);
