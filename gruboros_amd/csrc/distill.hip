@@ -214,7 +214,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
   constexpr bool kHard = kMode != kSoft, kAhead = ahead(S);
   using V16 = Vec<T>;
   constexpr int kN = V16::kN, kTop = top_of(NT), kEntries = (kTop + NT - 1) / NT;
-  constexpr float kLn2 = 0.6931471805599453f;
+  constexpr float kLn2 = 0.6931471805599453f, kSmall = 0x1p-24f;
   __shared__ float s_max[NT / 64], s_teacher[NT / 64], s_sum[kHard ? 2 : 1][NT / 64], s_teach[2][NT / 64];
   __shared__ int s_count[2], s_any[NT / 64], s_mine[NT / 64];
   __shared__ double s_loss[2];
@@ -369,7 +369,8 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
     for (int w = 0; w < NT / 64; ++w) taught |= s_any[w] != 0;
     tm = narrow ? wave_max(tm) : all_max<NT>(tm, s_teacher);
 
-    // the teacher's distribution: the sums of 2^u and of 2^u (u - log2 of the student's)
+    // the teacher's distribution: the sums of 2^u and of 2^u (u - log2 of the student's), the latter times kSmall: logits
+    // of the type's lowest value, times k1 and 512 of them, stay finite
     float teach[2] = {};
     bool mine = false;  // the label is one of this thread's entries
 #pragma unroll
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
         const float u = (teacher(i) - tm) * k1, zk = value(&at[i]);
         p = exp2_raw(u);
         teach[0] += p;
-        if (p != 0.0f) teach[1] += p * (u - (zk - zm) * k1);
+        if (p != 0.0f) teach[1] += p * __builtin_fmaf(zm - zk, k1 * kSmall, u * kSmall);
         s_at[k] = zk;
         mine |= told && id[i] == label;
       }
@@ -453,9 +454,11 @@ __global__ __launch_bounds__(NT, waves_of(NT, S)) void rows_kernel(Args a) {
       for (int w = 0; w < NT / 64; ++w) listed |= s_mine[w] != 0;
       label_own = told && !listed && tid == NT - 1;
       label_put = slope(zk) - w2;
-      if (tid == 0 && told) s_loss[1] += kLn2 * (__builtin_amdgcn_logf(sum[kHard ? 1 : 0]) - (zk - zm) * k2);
+      if (tid == 0 && told) s_loss[1] += static_cast<double>(kLn2 * __builtin_amdgcn_logf(sum[kHard ? 1 : 0])) + (zm - zk);
     }
-    if (tid == 0 && taught) s_loss[0] += kLn2 * (teach[1] / teach[0] - __builtin_amdgcn_logf(teach[0]) + __builtin_amdgcn_logf(sum[0]));
+    if (tid == 0 && taught)
+      s_loss[0] += __builtin_fma(teach[1] / teach[0], static_cast<double>(kLn2 / kSmall),
+                                 kLn2 * (__builtin_amdgcn_logf(sum[0]) - __builtin_amdgcn_logf(teach[0])));
     if (dz && own < a.V) put(dz + own, counted ? slope(beside) : 0.0f);
     const int label_place = label;
     fetch_entries(n_next);

@@ -83,3 +83,17 @@ def test_teachers_far_from_zero(temperature):
     z = (-50.0 + temperature * z).clone()
     _check(z, ids, top, None, temperature, 1.0)
     _check(z, ids, top, labels, temperature, 0.9)
+
+
+@TYPES
+@pytest.mark.parametrize("V,K", [(7, 3), (300, 9), (300, 70), (2500, 20)])
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 1.25, 2.0])
+def test_students_masked_with_the_lowest_value(temperature, V, K, dtype):
+    """A listed or labelled token that the student masks costs its logit's size, which a float holds."""
+    z, ids, top, labels = _operands(8, V, K, dtype)
+    z[0, ids[0, 0]] = LOW[dtype]
+    z[1, labels[1]] = LOW[dtype]
+    _check(z, ids, top, None, temperature, 1.0)  # (means over eight rows, which a float holds at these temperatures)
+    _check(z, ids, top, labels, temperature, 0.5)
+    z[2, ids[2]] = LOW[dtype]
+    _check(z, ids, top, labels, temperature, 0.5)
