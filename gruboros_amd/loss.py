@@ -95,11 +95,11 @@ def distillation_loss(logits, top_ids, top_logits, labels=None, temperature=1.0,
 
     logits [N, V] or [B, T, V] (float32 or bfloat16; batch and steps may be strided, as in
     logits[:, :-1]), top_ids (int64 or int32) and top_logits (float32 or bfloat16) [..., K] with
-    1 <= K <= 512, labels [...] (an integer type) or None where alpha is 1. The teacher's distribution
-    is over its K entries alone; one whose id is outside [0, V) or whose logit is -inf is none, and
-    an id that is listed twice counts twice. Rows without an entry, and labels outside [0, V) such as
-    -100, do not count: each mean is over the rows that do, and 0 where none does. What a
-    row that counts for neither holds does not matter.
+    1 <= K <= 512, labels [...] (int64, int32, int16, int8 or uint8) or None where alpha is 1. The
+    teacher's distribution is over its K entries alone; one whose id is outside [0, V) or whose logit
+    is -inf is none, and an id that is listed twice counts twice. Rows without an entry, and labels
+    outside [0, V) such as -100, do not count: each mean is over the rows that do, and 0 where none
+    does. What a row that counts for neither holds does not matter.
 
     Returns the loss, a float32 scalar. The gradient reaches logits, in their dtype, once and in
     reverse mode; it is made in the forward's pass and kept until the backward, which multiplies it
@@ -125,7 +125,7 @@ def distillation_loss(logits, top_ids, top_logits, labels=None, temperature=1.0,
     if labels is None:
         if alpha != 1.0:
             raise ValueError(f"alpha {alpha} gives the labels a share of the loss: labels are needed")
-    elif labels.shape != logits.shape[:-1] or labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+    elif labels.shape != logits.shape[:-1] or labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
         raise ValueError(f"labels must be integers {list(logits.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
     for t in (top_ids, top_logits, labels):
         if t is not None and t.device != logits.device:
