@@ -42,6 +42,7 @@ constexpr int kVec = 8, kCols = 64 * kVec;  // columns of a lane and of a wave
 constexpr int kRows = 4;                    // rows of dw per wave
 constexpr int kFew = 4;                     // tokens of a wave's rows that are loaded at once
 constexpr int64_t kMaxN = 1 << 27, kMaxV = 1 << 28;
+constexpr int kMaxD = 1 << 30;  // (columns of a row are counted in 32 bits, a workgroup's share past the last one too)
 
 struct Pairs {
   uint32_t *key, *pos;
@@ -495,8 +496,8 @@ inline Layout layout_of(int64_t N, int D, int64_t V, const Plan& p) {
 }
 
 inline int check_ids(const char* fn, int id_bytes, const void* ids, int64_t N, int D, int64_t V) {
-  if (N < 1 || N >= kMaxN || D < 1 || V < 1 || V >= kMaxV)
-    return fail(MG_ERR_ARG, "%s: N=%lld, D=%d, V=%lld must be at least 1, N below 2^27, V below 2^28", fn, (long long)N, D, (long long)V);
+  if (N < 1 || N >= kMaxN || D < 1 || D >= kMaxD || V < 1 || V >= kMaxV)
+    return fail(MG_ERR_ARG, "%s: N=%lld, D=%d, V=%lld must be at least 1, N below 2^27, D below 2^30, V below 2^28", fn, (long long)N, D, (long long)V);
   if (id_bytes != 4 && id_bytes != 8) return fail(MG_ERR_DTYPE, "%s: ids of %d bytes", fn, id_bytes);
   if (!ids || !aligned(ids, id_bytes)) return fail(MG_ERR_ARG, "%s: ids NULL or misaligned", fn);
   return MG_OK;
@@ -562,7 +563,7 @@ extern "C" int mg_embedding_fwd(int id_bytes, const void* ids, int64_t N, int ta
 
 extern "C" size_t mg_embedding_sorted_bwd_workspace_bytes(int64_t N, int D, int64_t V) {
   using namespace embed_sorted;
-  if (N < 1 || N >= kMaxN || D < 1 || V < 1 || V >= kMaxV) return 0;
+  if (N < 1 || N >= kMaxN || D < 1 || D >= kMaxD || V < 1 || V >= kMaxV) return 0;
   return layout_of(N, D, V, plan_of(N, V)).total;
 }
 

@@ -63,16 +63,16 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 def scaled_embedding(ids, weight, scale=1.0, out_dtype=None, padding_idx=None):
     """scale * weight[ids] in out_dtype (default weight's), for tables of any size.
 
-    ids: int64 or int32 of any shape; weight [V, D], float32 or bfloat16, V < 2^28; fewer than 2^27
-    ids. The gradient reaches weight, in its dtype, once and in reverse mode: rows are summed in
-    fp32 in the order of the tokens and rounded once, so results repeat bit for bit. An id outside
-    the table (torch's lookup stops the process there) gives a row of NaN and no gradient. The row
-    of padding_idx, which counts from the end where it is negative, gets no gradient."""
+    ids: int64 or int32 of any shape; weight [V, D], float32 or bfloat16, V < 2^28, D < 2^30; fewer
+    than 2^27 ids. The gradient reaches weight, in its dtype, once and in reverse mode: rows are
+    summed in fp32 in the order of the tokens and rounded once, so results repeat bit for bit. An id
+    outside the table (torch's lookup stops the process there) gives a row of NaN and no gradient.
+    The row of padding_idx, which counts from the end where it is negative, gets no gradient."""
     require_cuda(ids, weight)
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
-    if weight.dim() != 2 or not 1 <= weight.shape[0] < 1 << 28:
-        raise ValueError(f"weight must be [V, D] with 1 <= V < 2^28, got {tuple(weight.shape)}")
+    if weight.dim() != 2 or not 1 <= weight.shape[0] < 1 << 28 or weight.shape[1] >= 1 << 30:
+        raise ValueError(f"weight must be [V, D] with 1 <= V < 2^28 and D < 2^30, got {tuple(weight.shape)}")
     if ids.numel() >= 1 << 27:
         raise ValueError(f"{ids.numel()} ids: a call takes fewer than 2^27")
     if ids.device != weight.device:

@@ -824,7 +824,8 @@ int mg_block_norm_bwd(const float* xn, int f_dtype, const void* f, const void* g
  * reads nothing: its row of y is NaN, and dy's adds to no row; nor does that
  * of a token whose id is `padding` (a negative one: none). Every row of dw is
  * written. Sums are fp32, in a fixed order: the same inputs give the same bits.
- * N < 2^27, V < 2^28. The workspace is 256-byte aligned, any contents. */
+ * N < 2^27, V < 2^28, D < 2^30. The workspace is 256-byte aligned, any
+ * contents. */
 int mg_embedding_fwd(int id_bytes, const void* ids, int64_t N, int table_dtype, const void* table, int64_t V, int D,
                      float scale, int y_dtype, void* y, void* stream);
 size_t mg_embedding_sorted_bwd_workspace_bytes(int64_t N, int D, int64_t V);
