@@ -556,6 +556,7 @@ int launch_rows(const Args& a, hipStream_t st) {
   int wgs;
 #define GO(NT, S)                                                                            \
   {                                                                                          \
+    static_assert(wgs_of(NT, S) <= kRowWgs, "a place for each workgroup's losses");          \
     wgs = row_wgs(a.N, wgs_of(NT, S));                                                       \
     hipLaunchKernelGGL((rows_kernel<T, NT, S, kMode>), dim3(wgs), dim3(NT), 0, st, a);       \
   }
