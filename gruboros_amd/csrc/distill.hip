@@ -9,7 +9,8 @@
 // [0, V); what a row in neither holds does not matter, its gradient is 0. An id that is listed twice counts twice.
 //
 // A workgroup takes a row and keeps it in registers, as loaded, from its maximum to its sums to its gradient: logits
-// are read once and gradients written once. Rows of more than 64 registers to each of 1024 threads (131072 values in bfloat16) are read twice.
+// are read once and gradients written once. Rows of more than 64 registers to each of 1024 threads (131072 values in
+// bfloat16, 65536 in fp32) do not stay: they are read for their maximum, for their sums and for their gradient.
 // Everything is in powers of two: with k = log2(e) / T a term is 2^((z - max z) k), in the sums and in the logarithms
 // alike, of the student and of the teacher. (The difference first: with a product z k + b the rounding of b = -k max z
 // overflows the power for logits of the type's lowest value.) The few places that an entry or the label changes are
@@ -18,10 +19,12 @@
 // A small kernel counts n1 and n2 first; the last adds the workgroups' losses.
 //
 // Bound by memory as long as a row's sums and another's loads overlap: with bfloat16, 16376 rows of 32000 (K 64, labels)
-// take 455 us (2.1 GB, 4.6 TB/s), 2044 rows of 131071 (K 32), of which a CU holds one, 251 us (1.07 GB, 4.3 TB/s). For
-// rows this long a CU's registers are full with one of them, and memory waits while its sums are made; holding the
-// beginning of the next row as well (4 to 8 of 16 vectors) costs registers that are missing elsewhere (278 to 310 us
-// where 283 was the time without).
+// take 455 us (2.1 GB, 4.6 TB/s; at a temperature without a power 30 us more), 2044 rows of 131071 (K 32), of which a CU
+// holds one, 251 us (1.07 GB, 4.3 TB/s). Rows beyond the registers, 2044 of 151936 and of 262144 (K 64), whole calls: 395
+// and 690 us, in fp32 128256 648 us, where a read and a write are 233, 402 and 393: the reads from memory again. At
+// 131071 a CU's registers are full with one row, and memory waits while its sums are made; holding the beginning of the
+// next row as well (4 to 8 of 16 vectors) costs registers that are missing elsewhere (278 to 310 us where 283 was the
+// time without).
 
 #include <algorithm>
 
@@ -139,7 +142,8 @@ __host__ __device__ __forceinline__ int count_wgs(int64_t N) {
 }
 static_assert(kCountWgs == 256, "a thread of loss_kernel for each");
 
-// (n1, n2), by the first wave (with counters in LDS that every thread adds to, 31000 rows of V 1001 take 61 us, not 52)
+// (n1, n2), by the first wave (with counters in LDS that every thread adds to, 31000 rows of V 1001 take 61 us, not 52,
+// 2044 of V 131071 264, not 259; 16376 of V 32000 with labels, whose workgroups then start apart, 473, not 480)
 __device__ __forceinline__ void all_counts(const Args& a, int (&s)[2]) {
   const int g = count_wgs(a.N);
   if (threadIdx.x < 64) {
@@ -201,7 +205,7 @@ __device__ __forceinline__ void all_sum(float (&v)[M], float (&red)[M][NT / 64])
 }
 
 // S vectors of a row to each of NT threads, and one of the values before and behind them to the first few; S = 0: rows
-// of any length, read twice. The vectors begin where the row's gradient, which is dense, has a multiple of 16 bytes
+// of any length, read three times (twice without a gradient). The vectors begin where the row's gradient, which is dense, has a multiple of 16 bytes
 // (with all rows' vectors from their first values, V 50001 took 844 us where V 50000 took 723, 16376 rows). A row that counts for one part alone has a share of 0 of the other's
 // gradient.
 // After a row's gradient (where a row has 16 vectors to a thread and few workgroups share a CU: while it is written,

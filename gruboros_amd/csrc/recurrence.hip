@@ -1,6 +1,6 @@
 // Gated linear recurrence over sequences, forward and backward, and for single tokens, for gfx950.
 // Per channel, with sigma the logistic function and rate = softplus(decay):
-//   r_t = sigma(decay_gate_t), i_t = sigma(input_gate_t), l_t = -c rate r_t, a_t = e^{l_t} (0 at a reset)
+//   r_t = sigma(decay_gate_t), i_t = sigma(input_gate_t), l_t = -c rate r_t, a_t = e^{l_t} (at a reset none: -0)
 //   m_t = sqrt(1 - a_t^2),  h_t = a_t h_{t-1} + m_t i_t x_t
 // Backward, with dh the gradient of h:
 //   lam_t = dh_t + a_{t+1} lam_{t+1}
@@ -22,8 +22,8 @@
 // The state is kept every 8 steps in fp32 for the backward (half a byte per value); the steps between are made again.
 //
 // Bound by memory and, by a fifth, arithmetic. bfloat16, B8 T2047 D1024: forward 40 us (142 MB, 3.5 TB/s; 33 with no
-// arithmetic and no carries, 36 with the carries alone), backward 58 (243 MB, 4.2 TB/s). B2 T16381 D2048, forward: 132
-// us (537 MB, 4.1 TB/s), with resets 140: forgetting also what is not finite takes selects with every value.
+// arithmetic and no carries, 36 with the carries alone), backward 60 (243 MB, 4.0 TB/s). B2 T16381 D2048, forward: 132
+// us (537 MB, 4.1 TB/s), with resets 141: forgetting also what is not finite takes selects with every value.
 
 #include <algorithm>
 
