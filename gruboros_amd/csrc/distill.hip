@@ -205,9 +205,9 @@ __device__ __forceinline__ void all_sum(float (&v)[M], float (&red)[M][NT / 64])
 }
 
 // S vectors of a row to each of NT threads, and one of the values before and behind them to the first few; S = 0: rows
-// of any length, read three times (twice without a gradient). The vectors begin where the row's gradient, which is dense, has a multiple of 16 bytes
-// (with all rows' vectors from their first values, V 50001 took 844 us where V 50000 took 723, 16376 rows). A row that counts for one part alone has a share of 0 of the other's
-// gradient.
+// of any length, read three times (twice without a gradient). The vectors begin where the row's gradient, which is
+// dense, has a multiple of 16 bytes (with all rows' vectors from their first values, V 50001 took 844 us where V 50000
+// took 723, 16376 rows). A row that counts for one part alone has a share of 0 of the other's gradient.
 // After a row's gradient (where a row has 16 vectors to a thread and few workgroups share a CU: while it is written,
 // each vector's registers in turn) the next row is loaded, and its entries before that, so that a row begins with all
 // of its loads under way; what is loaded early stays as it comes until it is needed, or the wait for it would come
